@@ -233,10 +233,10 @@ def _plain_step(s):
     b, blocks = tables.shape
     ctx, new, count = s["ctx"].long(), s["new"].long(), s["free_count"].long()
     have, want = (ctx + p - 1) // p, (ctx + new + p - 1) // p
-    need = want - have
-    cum = need.cumsum(0)
     ends = new.cumsum(0)
-    fits = (ctx >= 0) & (new >= 0) & (want <= blocks) & (ends <= t)
+    fits = (want <= blocks) & (ends <= t)
+    need = torch.where(fits, want - have, 0)
+    cum = need.cumsum(0)
     granted = fits & ((need == 0) | (cum <= count))
     # the pages' places in the tables
     j = torch.arange(blocks, device=tables.device)
