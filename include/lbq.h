@@ -293,6 +293,107 @@ int lbq_quantize_act(uint32_t act_type, const float *d_x, int64_t m, int64_t k, 
 int lbq_quantize_weights_f32(uint32_t ggml_type, const float *d_w, int64_t nelem, void *d_out_blocks, void *stream);
 
 /* ---------------------------------------------------------------------------
+ * 8-bit paged key/value cache and attention over it: what a decoder layer does
+ * between its q/k/v projections and its o projection (the reference's
+ * custom_attention.rs:250-671 over src/cache/, in f32; here the cache is held in
+ * 8 bits).  Four calls make a step:
+ *   lbq_kv_step_build    lengths -> block tables, slots and positions, on the device
+ *   lbq_kv_append        rotate q and k, quantise k and v into their pages
+ *   lbq_kv_attention     prompts, single tokens and cross attention over the pages
+ *   lbq_kv_release       pages of finished sequences back to the free ones
+ *
+ * A page holds page_size (16, 32, 64 or 128) consecutive tokens of one sequence; block j
+ * of sequence b, its tokens j * page_size and on, lies in page tables[b][j].  Each
+ * (page, kv head) has one scale for its keys and one for its values; a value is
+ * code * scale.  Codes are int8 (scale = largest magnitude / 127) or e4m3 (OCP; the
+ * power of two that brings the largest magnitude to at most 448).  A scale grows while its
+ * page fills, never falls, and the codes already there are then coded again; a page whose
+ * keys or values are not finite has the scale NaN from then on and reads as NaN.
+ * head_dim is 64, 96, 128, 192 or 256; dtype is LBQ_TYPE_F32, _F16 or _BF16 and is that of
+ * q, k, v and out alike, whose rows [token][head][head_dim] may have any strides (in
+ * elements) but the last, which is 1.  All calls run on the context's device; none of them
+ * uses the context's memory, so calls on different streams need no order among
+ * themselves but that of their own buffers.
+ * ------------------------------------------------------------------------- */
+enum lbq_kv_kind { LBQ_KV_INT8 = 0, LBQ_KV_E4M3 = 1 };
+
+typedef struct lbq_kv_cache {
+    void *d_k;          /* codes [num_pages][kv_heads][page_size][head_dim], 16-byte aligned */
+    void *d_v;          /* codes [num_pages][kv_heads][head_dim][page_size], 16-byte aligned */
+    float *d_k_scales;  /* [num_pages][kv_heads] */
+    float *d_v_scales;  /* [num_pages][kv_heads] */
+    int64_t num_pages;
+    int32_t kind;       /* lbq_kv_kind */
+    int32_t page_size, kv_heads, head_dim;
+} lbq_kv_cache;
+
+typedef struct lbq_kv_step {
+    const int32_t *d_tables;    /* [batch][table_stride]: pages of each sequence's blocks; an entry that is no page: no keys */
+    int64_t table_stride;
+    const int32_t *d_seq_lens;  /* [batch]: tokens of each sequence, the new ones included */
+    const int32_t *d_cu_new;    /* [batch + 1]: rows cu[b] .. cu[b + 1] - 1 are sequence b's new tokens, its last ones */
+    const int64_t *d_slots;     /* [num_tokens]: page * page_size + place of each row, -1: none (append only, else may be NULL) */
+    const int32_t *d_positions; /* [num_tokens], -1: none (append only, else may be NULL) */
+    int64_t num_tokens;         /* rows of q, k, v and out; those from cu[batch] on are padding and are left as they are */
+    int32_t batch;              /* up to 65536 */
+    int32_t max_blocks;         /* blocks of a table row in use, <= table_stride */
+    int32_t max_len;            /* no seq_lens entry is larger; 0: max_blocks * page_size.  Keys beyond it are not seen */
+    int32_t max_new;            /* no sequence has more new tokens; 0: not known.  Rows beyond it are not served */
+} lbq_kv_step;
+
+/* Block tables, slots and positions of a step from the requests' lengths, in one launch.
+ * Sequence b holds ctx_lens[b] tokens and gets new_lens[b]; its rows are cu_new[b] and on.
+ * A sequence is granted its pages if its lengths are not negative, its blocks fit
+ * max_blocks and its rows num_tokens, and if it needs none or the pages that it and those
+ * before it need are no more than *d_free_count; the i-th page taken is
+ * d_free[*d_free_count - 1 - i] and goes into d_tables, whose other entries stay.  Where it is
+ * not granted, granted[b] and seq_lens[b] are 0 and its rows' slots and positions -1.
+ * *d_free_count_out = *d_free_count less the pages taken; the two pointers may be equal
+ * (the step is then taken), in which case d_ticket is a word that is zero before the call and
+ * after it. */
+int lbq_kv_step_build(lbq_ctx *ctx, const int32_t *d_ctx_lens, const int32_t *d_new_lens, int32_t batch,
+                      int32_t *d_tables, int64_t table_stride, int32_t max_blocks, int32_t page_size,
+                      const int32_t *d_free, int64_t num_pages, const int32_t *d_free_count, int32_t *d_free_count_out,
+                      uint32_t *d_ticket, int64_t num_tokens, int32_t *d_seq_lens, int32_t *d_cu_new, int32_t *d_granted,
+                      int64_t *d_slots, int32_t *d_positions, void *stream);
+
+/* The pages that hold the lens[b] tokens of each sequence with which[b] != 0 go back on top of
+ * the free ones, sequence by sequence and block by block, and their table entries become -1
+ * (so a second release of the same sequence frees nothing). */
+int lbq_kv_release(lbq_ctx *ctx, const int32_t *d_lens, const int32_t *d_which, int32_t batch, int32_t *d_tables,
+                   int64_t table_stride, int32_t max_blocks, int32_t page_size, int32_t *d_free, int64_t num_pages,
+                   int32_t *d_free_count, void *stream);
+
+/* k and v [num_tokens][kv_heads][head_dim] into their pages, after the rotation of k's first
+ * rot_dim channels by its row's position where rot_dim > 0; and, where d_q is not NULL, q's
+ * rows rotated likewise into d_q_out [num_tokens][q_heads][head_dim] (contiguous, apart from
+ * q, k and v).  Pairs are the channels (i, i + rot_dim / 2), or neighbours where interleaved;
+ * (a, b) becomes (a cos - b sin, b cos + a sin), with cos and sin [max_pos][rot_dim / 2] f32.
+ * A position from max_pos on gives NaN.  Each page takes new tokens of one sequence only.
+ * Rows whose slot is -1 are passed over. */
+int lbq_kv_append(lbq_ctx *ctx, const lbq_kv_cache *cache, const lbq_kv_step *step, uint32_t dtype, const void *d_k,
+                  int64_t k_token_stride, int64_t k_head_stride, const void *d_v, int64_t v_token_stride,
+                  int64_t v_head_stride, const void *d_q, int64_t q_token_stride, int64_t q_head_stride, int32_t q_heads,
+                  const float *d_cos, const float *d_sin, int64_t max_pos, int32_t rot_dim, int32_t interleaved,
+                  void *d_q_out, void *stream);
+
+/* out[t][h] = sum_j softmax_j(scale * q[t][h] . k[j]) v[j] over the cached tokens j of row t's
+ * sequence, kv head h / (q_heads / kv_heads).  causal: row i of n new ones is at position
+ * seq_len - n + i and sees j <= position, and with a window > 0 only j > position - window.
+ * Not causal (window 0): every row sees the whole sequence -- cross attention, with cu_new of
+ * the decoder's rows and tables and seq_lens of the encoder's states.  A row that sees
+ * nothing is zero.  out is [num_tokens][q_heads][head_dim], contiguous, apart from q.
+ * Sums and softmax are f32; products are formed exactly enough that f32 results are f32's
+ * (about 1e-6 relative).  The work of one sequence is spread over the chip through d_ws:
+ * lbq_kv_attention_workspace gives the bytes that are of use; with less (or NULL) the same
+ * call runs with less of it spread. */
+int lbq_kv_attention_workspace(lbq_ctx *ctx, const lbq_kv_cache *cache, const lbq_kv_step *step, int32_t q_heads,
+                               size_t *bytes);
+int lbq_kv_attention(lbq_ctx *ctx, const lbq_kv_cache *cache, const lbq_kv_step *step, uint32_t dtype, const void *d_q,
+                     int64_t q_token_stride, int64_t q_head_stride, int32_t q_heads, float scale, int32_t causal,
+                     int64_t window, void *d_out, void *d_ws, size_t ws_bytes, void *stream);
+
+/* ---------------------------------------------------------------------------
  * GGUF container (v3, little-endian) and the direct GGUF -> device upload.
  * lbq_gguf_open maps the file and parses it as the reference's parse_gguf does
  * (/root/reference/src/gguf/parser.rs:136-213, reached from Content::read,

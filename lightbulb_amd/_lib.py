@@ -27,6 +27,23 @@ STATUS_NAMES = {
 # name -> (restype, argtypes); must list every function include/lbq.h declares
 _c = ctypes
 _VP, _I64, _U32, _SZ = _c.c_void_p, _c.c_int64, _c.c_uint32, _c.c_size_t
+_I32 = _c.c_int32
+
+
+class KvCacheStruct(ctypes.Structure):
+    """``lbq_kv_cache``"""
+    _fields_ = [("d_k", _VP), ("d_v", _VP), ("d_k_scales", _VP), ("d_v_scales", _VP), ("num_pages", _I64),
+                ("kind", _I32), ("page_size", _I32), ("kv_heads", _I32), ("head_dim", _I32)]
+
+
+class KvStepStruct(ctypes.Structure):
+    """``lbq_kv_step``"""
+    _fields_ = [("d_tables", _VP), ("table_stride", _I64), ("d_seq_lens", _VP), ("d_cu_new", _VP), ("d_slots", _VP),
+                ("d_positions", _VP), ("num_tokens", _I64), ("batch", _I32), ("max_blocks", _I32), ("max_len", _I32),
+                ("max_new", _I32)]
+
+
+_CACHE, _STEP = _c.POINTER(KvCacheStruct), _c.POINTER(KvStepStruct)
 SIGNATURES = {
     "lbq_last_error": (_c.c_char_p, []),
     "lbq_type_block_size": (_c.c_int, [_U32]),
@@ -57,6 +74,14 @@ SIGNATURES = {
     "lbq_embedding_i64_f32": (_c.c_int, [_VP, _VP, _VP, _I64, _VP, _VP]),
     "lbq_quantize_act": (_c.c_int, [_U32, _VP, _I64, _I64, _VP, _VP]),
     "lbq_quantize_weights_f32": (_c.c_int, [_U32, _VP, _I64, _VP, _VP]),
+    "lbq_kv_step_build": (_c.c_int, [_VP, _VP, _VP, _I32, _VP, _I64, _I32, _I32, _VP, _I64, _VP, _VP, _VP, _I64, _VP, _VP,
+                                     _VP, _VP, _VP, _VP]),
+    "lbq_kv_release": (_c.c_int, [_VP, _VP, _VP, _I32, _VP, _I64, _I32, _I32, _VP, _I64, _VP, _VP]),
+    "lbq_kv_append": (_c.c_int, [_VP, _CACHE, _STEP, _U32, _VP, _I64, _I64, _VP, _I64, _I64, _VP, _I64, _I64, _I32, _VP, _VP,
+                                 _I64, _I32, _I32, _VP, _VP]),
+    "lbq_kv_attention_workspace": (_c.c_int, [_VP, _CACHE, _STEP, _I32, _c.POINTER(_SZ)]),
+    "lbq_kv_attention": (_c.c_int, [_VP, _CACHE, _STEP, _U32, _VP, _I64, _I64, _I32, _c.c_float, _I32, _I64, _VP, _VP, _SZ,
+                                    _VP]),
     "lbq_gguf_open": (_c.c_int, [_c.c_char_p, _c.POINTER(_VP)]),
     "lbq_gguf_close": (_c.c_int, [_VP]),
     "lbq_gguf_header": (_c.c_int, [_VP, _c.POINTER(_U32), _c.POINTER(_I64), _c.POINTER(_I64), _c.POINTER(_c.c_uint64),

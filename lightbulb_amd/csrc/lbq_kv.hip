@@ -1,0 +1,391 @@
+// lbq_kv.hip -- block tables and slot maps from request lengths, and appends to the 8-bit
+// paged key/value cache.
+#include "lbq_kv.hpp"
+
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+
+#include <algorithm>
+
+namespace lbq {
+namespace {
+
+constexpr int STEP_THREADS = 256, STEP_PER = 4, STEP_CHUNK = STEP_THREADS * STEP_PER;
+
+// inclusive sums over the workgroup's threads of two values each
+__device__ __forceinline__ void block_scan2(int64_t &a, int64_t &b, int64_t (*sums)[2]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int64_t ua = __shfl_up(a, d), ub = __shfl_up(b, d);
+        if (lane >= d) a += ua, b += ub;
+    }
+    if (lane == 63) sums[wave][0] = a, sums[wave][1] = b;
+    __syncthreads();
+    for (int w = 0; w < wave; w++) a += sums[w][0], b += sums[w][1];
+}
+
+// the last i in [0, n) with v[i] <= x; v never falls and v[0] <= x
+__device__ __forceinline__ int last_at_most(const int32_t *v, int n, int32_t x) {
+    int lo = 0;
+    while (n > 1) {
+        const int h = n / 2;
+        if (v[lo + h] <= x) lo += h, n -= h;
+        else n = h;
+    }
+    return lo;
+}
+
+// Tables, slots and positions of one step.  With n = new_lens, c = ctx_lens, P = page size:
+//   cu[b] = n[0] + .. + n[b - 1]          need[b] = ceil((c + n) / P) - ceil(c / P)
+//   granted[b]: lengths that fit (table, rows), and need[b] = 0 or need[0] + .. + need[b] <= free
+// and the i-th page taken is free_pages[free - 1 - i].  Every workgroup forms the sums over
+// all sequences by itself (1024 at a time; the lengths are a few KB and come out of L2), then
+// writes its share of the tokens and of the tables: no workgroup reads what another writes,
+// so one launch does.  A free count updated in place is written by the last workgroup to
+// take a ticket, after all have read it.
+__global__ __launch_bounds__(STEP_THREADS) void k_kv_step(KvStepBuild a) {
+    __shared__ int64_t sums[STEP_THREADS / 64][2];
+    __shared__ int32_t s_cu[STEP_CHUNK + 1], s_off[STEP_CHUNK + 1], s_ctx[STEP_CHUNK];
+    __shared__ uint8_t s_granted[STEP_CHUNK];
+    __shared__ int64_t carry[2];
+    __shared__ int s_taken;
+    const int tid = threadIdx.x, P = 1 << a.log2_page;
+    const int64_t stride = (int64_t)gridDim.x * STEP_THREADS, first = (int64_t)blockIdx.x * STEP_THREADS + tid;
+    const int32_t count = (int32_t)max((int64_t)0, min((int64_t)*a.free_count, a.num_pages));
+    int64_t before_n = 0, before_need = 0;  // sums over the earlier chunks
+    int taken = 0;
+    if (tid == 0) s_taken = 0;
+    for (int base = 0; base < a.batch; base += STEP_CHUNK) {
+        const int m = min(STEP_CHUNK, a.batch - base);
+        int64_t n[STEP_PER], need[STEP_PER], tn = 0, tneed = 0;
+        int32_t ctx[STEP_PER];
+        bool fits[STEP_PER];
+#pragma unroll
+        for (int j = 0; j < STEP_PER; j++) {
+            const int i = tid * STEP_PER + j;
+            const int32_t c = i < m ? a.ctx_lens[base + i] : 0, w = i < m ? a.new_lens[base + i] : 0;
+            const bool ok = c >= 0 && w >= 0;
+            const int64_t have = ((int64_t)c + P - 1) >> a.log2_page, want = ((int64_t)c + w + P - 1) >> a.log2_page;
+            ctx[j] = c;
+            n[j] = ok ? w : 0;
+            fits[j] = ok && want <= a.max_blocks && (int64_t)c + w <= INT32_MAX;
+            need[j] = fits[j] ? want - have : 0;
+            tn += n[j], tneed += need[j];
+        }
+        // a sequence whose rows do not fit takes no pages: its rows' end is known only
+        // after this sum, so the pages are summed again where that happens
+        int64_t en = tn, eneed = tneed;
+        block_scan2(en, eneed, sums);
+        int64_t run = before_n + en - tn;
+        tneed = 0;
+#pragma unroll
+        for (int j = 0; j < STEP_PER; j++) {
+            run += n[j];
+            if (run > a.num_tokens) fits[j] = false, need[j] = 0;
+            tneed += need[j];
+        }
+        __syncthreads();
+        int64_t again = tn;
+        eneed = tneed;
+        block_scan2(again, eneed, sums);
+        int64_t cn = before_n + en - tn, cneed = before_need + eneed - tneed;
+#pragma unroll
+        for (int j = 0; j < STEP_PER; j++) {
+            const int i = tid * STEP_PER + j;
+            s_cu[i] = (int32_t)min(cn, a.num_tokens);
+            s_off[i] = (int32_t)min(cneed, (int64_t)INT32_MAX);
+            cn += n[j], cneed += need[j];
+            const bool granted = fits[j] && (need[j] == 0 || cneed <= count);
+            s_ctx[i] = ctx[j];
+            s_granted[i] = granted;
+            if (i < m) {
+                if (granted) taken += (int)need[j];
+                if (blockIdx.x == 0) {
+                    a.seq_lens[base + i] = granted ? ctx[j] + (int32_t)n[j] : 0;
+                    a.granted[base + i] = granted;
+                    a.cu[base + i] = s_cu[i];
+                }
+            }
+        }
+        if (tid == STEP_THREADS - 1) {
+            s_cu[STEP_CHUNK] = (int32_t)min(cn, a.num_tokens);
+            s_off[STEP_CHUNK] = (int32_t)min(cneed, (int64_t)INT32_MAX);
+            carry[0] = cn, carry[1] = cneed;
+        }
+        __syncthreads();
+        // (entries from m on are empty: the searches below pass over them)
+        auto page_at = [&](int i, int j) {  // block j of sequence base + i
+            const int have = (int)(((int64_t)s_ctx[i] + P - 1) >> a.log2_page);
+            return j >= have ? a.free_pages[count - 1 - (s_off[i] + j - have)] : a.tables[(base + i) * a.table_stride + j];
+        };
+        const int32_t t_end = s_cu[STEP_CHUNK];
+        // the first of this thread's tokens in the chunk's range
+        const int64_t skip = s_cu[0] > first ? (s_cu[0] - first + stride - 1) / stride : 0;
+        for (int64_t t = first + skip * stride; t < t_end; t += stride) {
+            const int i = last_at_most(s_cu, m, (int32_t)t);
+            int64_t slot = -1;
+            int32_t at = -1;
+            if (s_granted[i]) {
+                at = s_ctx[i] + ((int32_t)t - s_cu[i]);
+                const int32_t page = page_at(i, at >> a.log2_page);
+                if (page >= 0 && page < a.num_pages) slot = ((int64_t)page << a.log2_page) + (at & (P - 1));
+                else at = -1;
+            }
+            a.slots[t] = slot;
+            a.positions[t] = at;
+        }
+        const int32_t p_end = min(s_off[STEP_CHUNK], count);
+        const int64_t skip_p = s_off[0] > first ? (s_off[0] - first + stride - 1) / stride : 0;
+        for (int64_t p = first + skip_p * stride; p < p_end; p += stride) {
+            const int i = last_at_most(s_off, m, (int32_t)p);
+            if (!s_granted[i]) continue;
+            const int have = (int)(((int64_t)s_ctx[i] + P - 1) >> a.log2_page);
+            a.tables[(base + i) * a.table_stride + have + ((int32_t)p - s_off[i])] = a.free_pages[count - 1 - p];
+        }
+        before_n = carry[0], before_need = carry[1];
+        __syncthreads();
+    }
+    // rows behind the last sequence
+    const int64_t total = min(before_n, a.num_tokens), skip = total > first ? (total - first + stride - 1) / stride : 0;
+    for (int64_t t = first + skip * stride; t < a.num_tokens; t += stride) a.slots[t] = -1, a.positions[t] = -1;
+    if (taken) atomicAdd(&s_taken, taken);  // whole numbers: any order
+    __syncthreads();
+    if (tid == 0) {
+        if (blockIdx.x == 0) a.cu[a.batch] = (int32_t)total;
+        if (a.free_count_out != a.free_count) {
+            if (blockIdx.x == 0) *a.free_count_out = count - s_taken;
+        } else {
+            __threadfence();
+            if (gridDim.x == 1 || atomicAdd(a.ticket, 1u) == gridDim.x - 1) {
+                *a.free_count_out = count - s_taken;
+                if (gridDim.x > 1) *a.ticket = 0;
+            }
+        }
+    }
+}
+
+// The pages of the sequences with which[b] != 0 go back on top of the free pages, in the
+// order of the sequences and of their blocks; their table entries become -1.  One
+// workgroup: few sequences end in a step, and the order is then the same every time.
+__global__ __launch_bounds__(1024) void k_kv_release(KvRelease a) {
+    __shared__ int32_t rows[1024];
+    __shared__ int s_rows, s_waves[16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, P = 1 << a.log2_page;
+    int64_t count = max((int64_t)0, min((int64_t)*a.free_count, a.num_pages));
+    // where this thread's entry goes among the workgroup's kept ones, and how many are kept
+    auto place = [&](bool keep, int &all) {
+        const uint64_t b = __ballot(keep);
+        if (lane == 0) s_waves[wave] = __popcll(b);
+        __syncthreads();
+        int at = __popcll(b & ((1ull << lane) - 1));
+        all = 0;
+        for (int w = 0; w < 16; w++) {
+            if (w < wave) at += s_waves[w];
+            all += s_waves[w];
+        }
+        __syncthreads();
+        return at;
+    };
+    for (int base = 0; base < a.batch; base += 1024) {
+        const int b = base + tid;
+        const bool go = b < a.batch && a.which[b] != 0 && a.lens[b] > 0;
+        int found;
+        const int at = place(go, found);
+        if (go) rows[at] = b;
+        if (tid == 0) s_rows = found;
+        __syncthreads();
+        for (int r = 0; r < s_rows; r++) {
+            const int row = rows[r];
+            const int blocks = (int)min((int64_t)a.max_blocks, ((int64_t)a.lens[row] + P - 1) >> a.log2_page);
+            for (int j0 = 0; j0 < blocks; j0 += 1024) {
+                const int j = j0 + tid;
+                int32_t *e = a.tables + row * a.table_stride + j;
+                const int32_t page = j < blocks ? *e : -1;
+                const bool keep = page >= 0 && page < a.num_pages;
+                int kept;
+                const int64_t to = count + place(keep, kept);
+                if (keep && to < a.num_pages) a.free_pages[to] = page;
+                if (j < blocks) *e = -1;
+                count = min(count + kept, a.num_pages);
+            }
+        }
+        __syncthreads();
+    }
+    if (tid == 0) *a.free_count = (int32_t)count;
+}
+
+// ---------------------------------------------------------------------------
+// append
+// ---------------------------------------------------------------------------
+template <int DT>
+__device__ __forceinline__ float load_value(const void *p, int64_t i) {
+    if constexpr (DT == DT_F32) return static_cast<const float *>(p)[i];
+    else if constexpr (DT == DT_F16) return __half2float(static_cast<const __half *>(p)[i]);
+    else return __uint_as_float((uint32_t) static_cast<const uint16_t *>(p)[i] << 16);
+}
+template <int DT>
+__device__ __forceinline__ void store_value(void *p, int64_t i, float v) {
+    if constexpr (DT == DT_F32) static_cast<float *>(p)[i] = v;
+    else if constexpr (DT == DT_F16) static_cast<__half *>(p)[i] = __float2half_rn(v);
+    else static_cast<__hip_bfloat16 *>(p)[i] = __float2bfloat16(v);
+}
+
+// Element d of a row rotated by its position's angles: (a, b) -> (a c - b s, b c + a s) for
+// the pairs (i, i + rot/2), or neighbours.  Both products are exact in 64 bits and their sum
+// is rounded once there and once to 32: one value whatever the order, which the codes need
+// (a last bit moves a code that lies at a tie).  A position outside the table gives NaN.
+template <int DT>
+__device__ __forceinline__ float rotated(const KvAppend &a, const void *row, int64_t d, int64_t pos) {
+    const float x = load_value<DT>(row, d);
+    if (d >= a.rot_dim) return x;
+    if (pos < 0 || pos >= a.max_pos) return __uint_as_float(0x7fc00000u);
+    const int half = a.rot_dim / 2;
+    const int i = a.interleaved ? (int)d / 2 : (int)(d < half ? d : d - half);
+    const bool upper = a.interleaved ? d & 1 : d >= half;
+    const float y = load_value<DT>(row, a.interleaved ? d ^ 1 : upper ? d - half : d + half);
+    const double c = a.cos[pos * half + i], s = a.sin[pos * half + i];
+    float r = (float)(upper ? (double)x * c + (double)y * s : (double)x * c - (double)y * s);
+    asm("" : "+v"(r));  // the compiler would round a 16-bit result from 64 bits at once: another value at some ties
+    return r;
+}
+
+// The scale of a block whose largest magnitude is amax: int8 amax / 127; e4m3 the power of
+// two that brings amax to at most 448 (a floating code loses nothing by it, and x / scale is
+// exact).  Never below the smallest normal number; NaN where a value is not finite.
+__device__ __forceinline__ float block_scale(float amax, int kind) {
+    if (!(amax < INFINITY)) return __uint_as_float(0x7fc00000u);
+    if (amax == 0.f) return 0.f;
+    if (kind == KV_INT8) return fmaxf(amax / 127.f, 0x1p-126f);
+    int e;
+    const float m = frexpf(amax, &e);
+    return ldexpf(1.f, max(m > 0.875f ? e - 8 : e - 9, -126));
+}
+
+// x / s to the nearest code, ties to even, decided as if the quotient were exact; 0 where s is 0 or NaN
+__device__ __forceinline__ uint8_t code_of(float x, float s, int kind) {
+    if (!(s > 0.f)) return 0;
+    if (kind == KV_E4M3) return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(x / s, 0.f, 0, false);
+    // rint of the rounded quotient is the answer or, next to a tie, one beside it; what is
+    // left, x - q s, is exact in f32 (a multiple of the operands' last place no larger than
+    // s), so its comparison with s / 2 decides
+    float q = rintf(x / s);
+    const float left = fmaf(-q, s, x);
+    if (fabsf(left) > 0.5f * s) q += copysignf(1.f, left);
+    else if (fabsf(left) == 0.5f * s && ((int)q & 1)) q += copysignf(1.f, left);
+    return (uint8_t)(int8_t)(int)fminf(fmaxf(q, -127.f), 127.f);
+}
+
+// a code under scale `was`, under the larger scale `now`
+__device__ __forceinline__ uint8_t recode(uint8_t c, float was, float now, int kind) {
+    if (kind == KV_E4M3)  // a power of two: exact up to the one rounding
+        return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(__builtin_amdgcn_cvt_f32_fp8((int)c, 0) * (was / now), 0.f, 0, false);
+    return (uint8_t)(int8_t)(int)rint((double)(int8_t)c * (double)was / (double)now);
+}
+
+constexpr int APPEND_THREADS = 256;
+
+// One workgroup per (run of new tokens in one page, kv head, keys or values); the workgroups
+// behind those rotate queries.  Sequence b has at most cu[b + 1] / P - cu[b] / P + 2 runs, so
+// run r belongs to the sequence with cu[b] / P + 2 b <= r, without a list.  The new values
+// are rotated into LDS while their largest magnitude is found, then coded from there.  A
+// scale never falls while a page fills; where it grows, the codes that are there are
+// recoded.  One workgroup owns a (page, head)'s codes and scale: no atomics.
+template <int DT>
+__global__ __launch_bounds__(APPEND_THREADS) void k_kv_append(KvAppend a, int runs) {
+    extern __shared__ float vals[];
+    __shared__ float s_max[APPEND_THREADS / 64];
+    const int tid = threadIdx.x, D = a.c.head_dim, P = a.c.page_size, H = a.c.kv_heads;
+    int64_t id = blockIdx.x;
+    const int64_t kv_groups = (int64_t)runs * H * 2;
+    if (id >= kv_groups) {
+        const int64_t n = a.s.num_tokens * a.q_heads * D, step = (gridDim.x - kv_groups) * APPEND_THREADS;
+        for (int64_t i = (id - kv_groups) * APPEND_THREADS + tid; i < n; i += step) {
+            const int d = (int)(i % D);
+            const int64_t th = i / D, t = th / a.q_heads, h = th % a.q_heads;
+            const int32_t pos = a.s.positions[t];
+            if (pos < 0) continue;
+            const int64_t at = t * a.q.token_stride + h * a.q.head_stride;
+            constexpr int size = DT == DT_F32 ? 4 : 2;
+            store_value<DT>(a.q_out, i, rotated<DT>(a, static_cast<const char *>(a.q.p) + at * size, d, pos));
+        }
+        return;
+    }
+    const bool is_v = id & 1;
+    const int h = (int)((id >> 1) % H);
+    const int64_t run = (id >> 1) / H;
+    const int b = find_sequence(a.s.batch, run, [&](int i) { return (int64_t)(a.s.cu[i] >> a.c.log2_page) + 2 * (int64_t)i; });
+    const int64_t t0 = a.s.cu[b], t1 = a.s.cu[b + 1], len = a.s.seq_lens[b], ctx = len - (t1 - t0);
+    if (t0 < 0 || t1 > a.s.num_tokens || t1 <= t0 || ctx < 0) return;
+    const int64_t block = (ctx >> a.c.log2_page) + run - ((t0 >> a.c.log2_page) + 2 * (int64_t)b);
+    const int64_t lo = max(block << a.c.log2_page, ctx), hi = min((block + 1) << a.c.log2_page, len);
+    if (lo >= hi) return;
+    const int64_t tok = t0 + (lo - ctx), slot = a.s.slots[tok], page = slot >> a.c.log2_page;
+    const int o = (int)(lo & (P - 1)), count = (int)(hi - lo);
+    if (slot < 0 || page >= a.c.num_pages || (int)(slot & (P - 1)) != o) return;
+
+    const KvRows &rows = is_v ? a.v : a.k;
+    constexpr int size = DT == DT_F32 ? 4 : 2;
+    float amax = 0.f;
+    bool bad = false;
+    for (int i = tid; i < count * D; i += APPEND_THREADS) {
+        const int j = i / D, d = i % D;
+        const void *row = static_cast<const char *>(rows.p) + ((tok + j) * rows.token_stride + h * rows.head_stride) * size;
+        const float x = is_v || !a.rot_dim ? load_value<DT>(row, d) : rotated<DT>(a, row, d, a.s.positions[tok + j]);
+        vals[i] = x;
+        bad |= !(fabsf(x) < INFINITY);
+        amax = fmaxf(amax, fabsf(x));
+    }
+    if (bad) amax = INFINITY;
+#pragma unroll
+    for (int d = 32; d; d /= 2) amax = fmaxf(amax, __shfl_xor(amax, d));
+    if ((tid & 63) == 0) s_max[tid >> 6] = amax;
+    float *const sp = (is_v ? a.c.vs : a.c.ks) + page * H + h;
+    const float was = o ? *sp : 0.f;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < APPEND_THREADS / 64; w++) amax = fmaxf(amax, s_max[w]);
+    const float fresh = block_scale(amax, a.c.kind);
+    const float now = was != was || fresh != fresh ? __uint_as_float(0x7fc00000u) : fmaxf(was, fresh);
+    uint8_t *const codes = (is_v ? a.c.v : a.c.k) + (page * H + h) * (int64_t)P * D;
+    for (int i = tid; i < count * D; i += APPEND_THREADS) {
+        const int j = i / D, d = i % D;
+        codes[is_v ? d * P + o + j : (o + j) * D + d] = code_of(vals[i], now, a.c.kind);
+    }
+    if (now > was && was > 0.f)
+        for (int i = tid; i < o * D; i += APPEND_THREADS) {
+            const int at = is_v ? i / o * P + i % o : i;
+            codes[at] = recode(codes[at], was, now, a.c.kind);
+        }
+    if (tid == 0) *sp = now;
+}
+
+}  // namespace
+
+hipError_t launch_kv_step(const KvStepBuild &a, hipStream_t st) {
+    const int64_t groups = std::max<int64_t>(1, std::min<int64_t>((a.num_tokens + 1023) / 1024, 64));
+    k_kv_step<<<dim3((unsigned)groups), STEP_THREADS, 0, st>>>(a);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv_release(const KvRelease &a, hipStream_t st) {
+    k_kv_release<<<1, 1024, 0, st>>>(a);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv_append(const KvAppend &a, hipStream_t st) {
+    const int64_t runs = std::min<int64_t>((a.s.num_tokens >> a.c.log2_page) + 2 * (int64_t)a.s.batch, INT32_MAX);
+    const int64_t q = a.q.p ? std::min<int64_t>((a.s.num_tokens * a.q_heads * a.c.head_dim + 1023) / 1024, 65536) : 0;
+    const int64_t groups = runs * a.c.kv_heads * 2 + q;
+    const int rows = a.max_new > 0 ? std::min(a.max_new, a.c.page_size) : a.c.page_size;
+    const size_t lds = (size_t)rows * a.c.head_dim * sizeof(float);
+    auto k = a.dtype == DT_F32 ? k_kv_append<DT_F32> : a.dtype == DT_F16 ? k_kv_append<DT_F16> : k_kv_append<DT_BF16>;
+    if (lds > 65536) {
+        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return e;
+    }
+    k<<<dim3((unsigned)groups), APPEND_THREADS, lds, st>>>(a, (int)runs);
+    return hipGetLastError();
+}
+
+}  // namespace lbq
