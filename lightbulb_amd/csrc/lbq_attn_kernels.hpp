@@ -1,0 +1,731 @@
+// lbq_attn_kernels.hpp -- attention over the 8-bit paged key/value cache on the f16 matrix cores.
+//
+// The codes of both kinds are f16 numbers, so a code goes into a matrix instruction exactly and
+// its scale, one per 16 or more keys, into the f32 logit or weight.  f32 queries go in as two f16
+// parts of a power-of-two multiple of their row (22 bits), f32 weights likewise, with the products
+// of both parts in one f32 sum: results of f32's accuracy at twice the matrix work.  f16 and bf16
+// queries are one part, exactly.
+//
+// Products are formed transposed: S^T = K Q^T, then O^T = V^T P^T.  Column n of every tile is
+// query row n, so a row's softmax stays inside a lane and the lanes that share its column, and the
+// accumulator layout of S^T (column = lane mod 16 or 32, rows in registers) is already the operand
+// layout of P^T once the rows of K are taken in the right order.  Weights never leave registers.
+//
+// Weights carry a factor 2^15 (they are at most 1), which keeps both their f16 parts clear of the
+// subnormals; the row's sum carries it too.  Value scales are applied to the weights relative to
+// the largest one so far, rounded up to a power of two (r): weights stay at most 2^15 and the
+// accumulators are rescaled where r grows, as where the running maximum does.
+#pragma once
+#include "lbq_kv.hpp"
+
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+
+namespace lbq {
+
+// the launch's plan, the same in the kernels and in the join
+struct AttnPlan {
+    int splits_short, splits_long;  // parts that a sequence's keys are cut into
+    float *part;                    // [splits][num_q][q_heads][head_dim] outputs of parts
+    float *stat;                    // [splits][num_q][q_heads][2]: running maximum (log2), sum
+    int tiles;                      // 128-row tiles of the long form, an upper bound
+    int group;                      // query heads per kv head
+    int short_rows;                 // rows (queries * group) up to which a sequence takes the short form; 0: none does
+};
+
+namespace attn {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// rows of one kv head's queries that the short form takes: one 16-column tile
+constexpr int SHORT_ROWS = 16;
+constexpr int TILE = 64;  // keys per step of either form
+
+template <int DT>
+__device__ __forceinline__ float load_value(const void *p, int64_t i) {
+    if constexpr (DT == DT_F32) return static_cast<const float *>(p)[i];
+    else if constexpr (DT == DT_F16) return __half2float(static_cast<const __half *>(p)[i]);
+    else return __uint_as_float((uint32_t) static_cast<const uint16_t *>(p)[i] << 16);
+}
+template <int DT>
+__device__ __forceinline__ void store_values4(void *p, int64_t i, const float *v) {
+    if constexpr (DT == DT_F32) {
+        // (a contiguous output's rows of 64 or more values need no more than their own 4-byte alignment)
+        float *o = static_cast<float *>(p) + i;
+        o[0] = v[0], o[1] = v[1], o[2] = v[2], o[3] = v[3];
+    } else if constexpr (DT == DT_F16) {
+        _Float16 *o = static_cast<_Float16 *>(p) + i;
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[j] = (_Float16)v[j];
+    } else {
+        __hip_bfloat16 *o = static_cast<__hip_bfloat16 *>(p) + i;
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[j] = __float2bfloat16(v[j]);
+    }
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+// a maximum as the base of exponents: 0 where nothing was seen, so that no inf - inf is formed
+__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
+
+// four codes of a word as f16, exactly.  int8: the byte + 128 under the exponent of 1024, less 1152.
+template <int KIND>
+__device__ __forceinline__ half4 codes4(uint32_t w) {
+    if constexpr (KIND == KV_INT8) {
+        const uint32_t x = w ^ 0x80808080u;
+        const half2v off = {(_Float16)-1152.f, (_Float16)-1152.f};
+        const half2v a = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u)) + off;
+        const half2v b = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)) + off;
+        return half4{a[0], a[1], b[0], b[1]};
+    } else {
+        const half2v a = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.f, false));
+        const half2v b = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.f, true));
+        return half4{a[0], a[1], b[0], b[1]};
+    }
+}
+template <int KIND>
+__device__ __forceinline__ half8 codes8(uint32_t lo, uint32_t hi) {
+    return __builtin_shufflevector(codes4<KIND>(lo), codes4<KIND>(hi), 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// the first `keep` (0 .. 16) of 16 code bytes, zeros behind them
+__device__ __forceinline__ u32x4 keep_bytes(u32x4 v, int keep) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int n = min(max(keep - 4 * i, 0), 4);
+        v[i] &= n == 4 ? 0xffffffffu : (1u << (8 * n)) - 1u;
+    }
+    return v;
+}
+
+// eight f32 values as one f16 operand, or two that add up to them
+template <int NS>
+__device__ __forceinline__ void parts8(const float *v, half8 *o) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const _Float16 hi = (_Float16)v[j];
+        o[0][j] = hi;
+        if constexpr (NS == 2) o[NS - 1][j] = (_Float16)(v[j] - (float)hi);
+    }
+}
+
+// the exponent e with |max| < 2^e for the parts of a query row: values times 2^(15 - e) fit f16
+__device__ __forceinline__ int row_exponent(float amax) {
+    int e = 0;
+    if (amax > 0.f && amax < INFINITY) (void)frexpf(amax, &e);
+    return e;
+}
+
+// a power of two no smaller than a value scale (and normal, as is its inverse)
+__device__ __forceinline__ float scale_ceiling(float s) {
+    int e = 0;
+    (void)frexpf(s, &e);
+    return ldexpf(1.f, min(max(e, -126), 126));
+}
+
+// what a sequence's rows see, and where its queries lie
+struct Sequence {
+    int64_t t0;      // first query row
+    int n;           // its queries
+    int64_t len;     // keys that can be seen at all
+    int64_t first;   // position of the first query
+};
+__device__ __forceinline__ bool sequence_of(const KvAttention &a, int b, Sequence &s) {
+    const int64_t t0 = a.cu_q[b], t1 = a.cu_q[b + 1];
+    if (t0 < 0 || t1 > a.num_q || t1 <= t0) return false;
+    s.t0 = t0;
+    s.n = (int)(t1 - t0);
+    s.len = min((int64_t)a.s.seq_lens[b], a.max_len);
+    s.first = (int64_t)a.s.seq_lens[b] - s.n;
+    return true;
+}
+
+// keys [lo, hi) that the query at position pos sees
+__device__ __forceinline__ void seen_range(const KvAttention &a, const Sequence &s, int64_t pos, int &lo, int &hi) {
+    hi = (int)max((int64_t)0, a.causal ? min(s.len, pos + 1) : s.len);
+    lo = a.causal && a.window > 0 ? (int)max((int64_t)0, pos - a.window + 1) : 0;
+}
+
+// The join of parts' outputs o_i with maxima m_i and sums l_i: weights l_i 2^(m_i - max).
+__device__ __forceinline__ float part_weight(float m, float l, float top) { return l * exp2_fast(m - base_of(top)); }
+
+// ---------------------------------------------------------------------------
+// Short form: up to 16 query rows of one kv head (a token step: its group of query heads).
+// Bound by reading the cache, 2 head_dim bytes per key: one wave takes 64 keys at a time
+// straight from memory into its operands, the next 64 on their way while it works, with no
+// barrier until the waves' outputs are joined at the end.  16x16x32 products; in S^T lane
+// (c, n) = (lane / 16, lane % 16) holds keys 16 c .. 16 c + 15 of the 64 for row n, which is
+// what the products with V take, and all of one page: one scale per lane.
+// ---------------------------------------------------------------------------
+constexpr int SHORT_WAVES = 4;
+
+template <int D, int KIND, int DT>
+__global__ __launch_bounds__(64 * SHORT_WAVES) void k_attn_short(KvAttention a, AttnPlan plan) {
+    constexpr int NS = DT == DT_F32 ? 2 : 1;
+    constexpr int STEPS = D / 32, DB = D / 16;
+    __shared__ float s_o[SHORT_WAVES][SHORT_ROWS][D + 4];
+    __shared__ float s_m[SHORT_WAVES][SHORT_ROWS], s_l[SHORT_WAVES][SHORT_ROWS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, c = lane >> 4;
+    const int H = a.c.kv_heads, P = a.c.page_size, lp = a.c.log2_page;
+    const int h = blockIdx.x % H, split = blockIdx.x / H % plan.splits_short, b = blockIdx.x / H / plan.splits_short;
+    Sequence sq;
+    if (!sequence_of(a, b, sq) || sq.n * plan.group > plan.short_rows) return;
+    const int rows = sq.n * plan.group;
+    const int tok = n / plan.group, head = h * plan.group + n % plan.group;
+    const bool mine = n < rows;
+    int lo, hi, first_lo, first_hi, last_lo, last_hi;
+    seen_range(a, sq, sq.first + (mine ? tok : 0), lo, hi);
+    seen_range(a, sq, sq.first, first_lo, first_hi);
+    seen_range(a, sq, sq.first + sq.n - 1, last_lo, last_hi);
+    if (!mine) hi = 0;
+    // this part's steps of 64 keys: every SHORT_WAVES-th is this wave's
+    const int t_lo = first_lo / TILE, t_hi = (last_hi + TILE - 1) / TILE;
+    const int per = max(t_hi - t_lo + plan.splits_short - 1, 0) / plan.splits_short;
+    const int begin = t_lo + split * per, end = min(begin + per, t_hi);
+
+    // the row's parts and the factor of its logits (in powers of two)
+    half8 q[STEPS][NS];
+    float factor;
+    {
+        const int64_t at = (sq.t0 + tok) * a.q.token_stride + (int64_t)head * a.q.head_stride + c * (D / 4);
+        float v[STEPS][8], amax = 0.f;
+#pragma unroll
+        for (int s = 0; s < STEPS; s++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                v[s][j] = mine ? load_value<DT>(a.q.p, at + 8 * s + j) : 0.f;
+                amax = fmaxf(amax, fabsf(v[s][j]));
+            }
+        amax = fmaxf(amax, __shfl_xor(amax, 16));
+        amax = fmaxf(amax, __shfl_xor(amax, 32));
+        const int e = row_exponent(amax);
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[s][j] = ldexpf(v[s][j], 15 - e);
+            parts8<NS>(v[s], q[s]);
+        }
+        factor = ldexpf(a.scale * 1.44269504088896340736f, e - 15);
+    }
+
+    f32x4 o[DB];
+#pragma unroll
+    for (int i = 0; i < DB; i++) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f, r = 0.f;
+
+    const int32_t *table = a.s.tables + b * a.s.table_stride;
+    const int64_t page_bytes = (int64_t)P * D;
+    const int kg = (lane & 15) >> 2;  // the 16-key group of this lane's rows of K
+    // pages of 16-key group g of step t; -1 where there is none to see
+    auto page_of = [&](int t, int g) {
+        const int key = t * TILE + 16 * g;
+        int32_t p = -1;
+        if (t < end && key < last_hi) p = table[key >> lp];
+        return p >= 0 && p < a.c.num_pages ? p : -1;
+    };
+    struct Loaded {
+        uint32_t k[4][D / 16];
+        u32x4 v[DB];
+        float ks, vs;
+    };
+    auto load = [&](Loaded &x, int t, int32_t kp, int32_t vp) {
+        const int key = t * TILE;
+        {
+            const uint8_t *p = a.c.k + ((int64_t)max(kp, 0) * H + h) * page_bytes + c * (D / 4);
+            const int at = (key + 16 * kg) & (P - 1);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint8_t *row = p + (at + 4 * i + (lane & 3)) * D;
+                if constexpr (D % 64 == 0) {
+#pragma unroll
+                    for (int j = 0; j < D / 64; j++) {
+                        const u32x4 w = reinterpret_cast<const u32x4 *>(row)[j];
+                        x.k[i][4 * j] = w[0], x.k[i][4 * j + 1] = w[1], x.k[i][4 * j + 2] = w[2], x.k[i][4 * j + 3] = w[3];
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < D / 32; j++) {
+                        const u32x2 w = reinterpret_cast<const u32x2 *>(row)[j];
+                        x.k[i][2 * j] = w[0], x.k[i][2 * j + 1] = w[1];
+                    }
+                }
+            }
+        }
+        const int64_t vh = (int64_t)max(vp, 0) * H + h;
+        const uint8_t *p = a.c.v + vh * page_bytes + n * P + ((key + 16 * c) & (P - 1));
+#pragma unroll
+        for (int i = 0; i < DB; i++) x.v[i] = *reinterpret_cast<const u32x4 *>(p + i * 16 * P);
+        x.ks = a.c.ks[vh];
+        x.vs = vp >= 0 ? a.c.vs[vh] : 0.f;
+    };
+
+    int t = begin + wave;
+    Loaded cur;
+    int32_t vp = page_of(t, c), kp = page_of(t, kg);
+    if (t < end) load(cur, t, kp, vp);
+    int32_t vp_next = page_of(t + SHORT_WAVES, c), kp_next = page_of(t + SHORT_WAVES, kg);
+    for (; t < end; t += SHORT_WAVES) {
+        Loaded next;
+        const bool more = t + SHORT_WAVES < end;
+        if (more) load(next, t + SHORT_WAVES, kp_next, vp_next);
+        const int32_t vp_far = page_of(t + 2 * SHORT_WAVES, c), kp_far = page_of(t + 2 * SHORT_WAVES, kg);
+
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < STEPS; j++) {
+                const half8 k8 = codes8<KIND>(cur.k[i][2 * j], cur.k[i][2 * j + 1]);
+#pragma unroll
+                for (int u = NS - 1; u >= 0; u--) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, q[j][u], s, 0, 0, 0);
+            }
+            const float f = cur.ks * factor;
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[4 * i + j] = s[j] * f;
+        }
+        // keys that some row does not see, or that are not there
+        const int key = t * TILE;
+        const bool edge = key < last_lo || key + TILE > first_hi || __any(vp < 0);
+        uint32_t unseen = 0;
+        if (edge) {
+            const int from = lo - (key + 16 * c), to = vp >= 0 ? hi - (key + 16 * c) : 0;
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const bool seen = j >= from && j < to;
+                x[j] = seen ? x[j] : -INFINITY;
+                unseen |= seen ? 0u : 1u << j;
+            }
+        }
+        float top = x[0];
+#pragma unroll
+        for (int j = 1; j < 16; j++) top = fmaxf(top, x[j]);
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), m);
+        float vmax = fmaxf(cur.vs, __shfl_xor(cur.vs, 16));
+        vmax = fmaxf(vmax, __shfl_xor(vmax, 32));
+        float grown = 1.f;
+        if (vmax > r) {  // (the same in every lane)
+            const float rn = scale_ceiling(vmax);
+            grown = r / rn;
+            r = rn;
+        }
+        if (__any(top > m) || grown != 1.f) {
+            const float alpha = exp2_fast(m - base_of(top));
+            l *= alpha;
+            const float f = alpha * grown;
+#pragma unroll
+            for (int i = 0; i < DB; i++) o[i] *= f;
+            m = top;
+        }
+        const float base = base_of(m) - 15.f, vr = r > 0.f ? cur.vs / r : 0.f;
+        float w[16];
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            w[j] = exp2_fast(x[j] - base);
+            l += w[j];
+            w[j] *= vr;
+        }
+        if (edge) {  // (a weight of 0 under a scale of NaN)
+#pragma unroll
+            for (int j = 0; j < 16; j++) w[j] = unseen >> j & 1 ? 0.f : w[j];
+            const int keep = vp >= 0 ? min(max((int)sq.len - (key + 16 * c), 0), 16) : 0;
+#pragma unroll
+            for (int i = 0; i < DB; i++) cur.v[i] = keep_bytes(cur.v[i], keep);
+        }
+        half8 p[2][NS];
+        parts8<NS>(w, p[0]);
+        parts8<NS>(w + 8, p[1]);
+#pragma unroll
+        for (int i = 0; i < DB; i++)
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const half8 v8 = codes8<KIND>(cur.v[i][2 * u], cur.v[i][2 * u + 1]);
+#pragma unroll
+                for (int z = NS - 1; z >= 0; z--) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, p[u][z], o[i], 0, 0, 0);
+            }
+        cur = next;
+        vp = vp_next, kp = kp_next;
+        vp_next = vp_far, kp_next = kp_far;
+    }
+
+    // the waves' parts, then theirs joined: channel by channel
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    const float inv = l == 0.f ? 0.f : 1.f / l;  // (apart from r: their quotient can be subnormal)
+#pragma unroll
+    for (int i = 0; i < DB; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) s_o[wave][n][16 * i + 4 * c + j] = l == 0.f ? 0.f : o[i][j] * inv * r;
+    if (c == 0) s_m[wave][n] = m, s_l[wave][n] = l;
+    __syncthreads();
+    const int64_t all = a.num_q * a.q_heads;
+    for (int i = threadIdx.x; i < rows * (D / 4); i += 64 * SHORT_WAVES) {
+        const int row = i / (D / 4), d = i % (D / 4) * 4;
+        float top = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < SHORT_WAVES; w++) top = fmaxf(top, s_m[w][row]);
+#pragma unroll
+        for (int w = 0; w < SHORT_WAVES; w++) {
+            const float f = part_weight(s_m[w][row], s_l[w][row], top);
+            sum += f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = fmaf(f, s_o[w][row][d + j], v[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = sum == 0.f ? 0.f : v[j] / sum;
+        const int64_t out = (sq.t0 + row / plan.group) * a.q_heads + h * plan.group + row % plan.group;
+        if (plan.splits_short == 1) {
+            store_values4<DT>(a.out, out * D + d, v);
+        } else {
+            const int64_t at = split * all + out;
+            *reinterpret_cast<f32x4 *>(plan.part + at * D + d) = f32x4{v[0], v[1], v[2], v[3]};
+            if (d == 0) plan.stat[2 * at] = top, plan.stat[2 * at + 1] = sum;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Long form: 128 query rows of one kv head (row i * group + head: neighbouring tokens see
+// nearly the same keys), 32 for each of four waves.  Bound by the matrix cores and by the
+// exponentials.  64 keys at a time are turned into f16 once for all four waves and kept in
+// LDS, two buffers, the next step's codes on their way from memory meanwhile.  32x32x16
+// products; rows of K lie in LDS in the order in which lane (half, n) then holds keys
+// 16 u + 8 half + j of its row n, what the products with V take.  Both LDS arrays have rows of
+// an odd number of 16-byte chunks, so that eight lanes' reads of one column use all banks.
+// ---------------------------------------------------------------------------
+constexpr int LONG_ROWS = 128, LONG_WAVES = 4;
+
+template <int D>
+constexpr int long_lds_halves() { return TILE * (D + 8) + D * (TILE + 8); }
+
+template <int D, int KIND, int DT>
+__global__ __launch_bounds__(64 * LONG_WAVES, D <= 128 ? 2 : 1) void k_attn_long(KvAttention a, AttnPlan plan) {
+    constexpr int NS = DT == DT_F32 ? 2 : 1;
+    constexpr int STEPS = D / 16, DB = D / 32;
+    constexpr int KROW = D + 8, VROW = TILE + 8;
+    constexpr int CHUNKS = TILE * D / 16, PER = (CHUNKS + 64 * LONG_WAVES - 1) / (64 * LONG_WAVES);  // 16-code chunks, of K and of V
+    extern __shared__ _Float16 lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, hf = lane >> 5;
+    const int H = a.c.kv_heads, P = a.c.page_size, lp = a.c.log2_page;
+    const int h = blockIdx.x % H;
+    // the tiles with most keys (a sequence's last) first
+    const int tile = plan.tiles - 1 - blockIdx.x / H, split = blockIdx.y;
+    const int b = find_sequence(a.s.batch, tile, [&](int i) { return (int64_t)a.cu_q[i] * plan.group / LONG_ROWS + i; });
+    Sequence sq;
+    if (!sequence_of(a, b, sq) || sq.n * plan.group <= plan.short_rows) return;
+    const int rows = sq.n * plan.group;
+    const int row0 = (int)(tile - (sq.t0 * plan.group / LONG_ROWS + b)) * LONG_ROWS;
+    if (row0 < 0 || row0 >= rows) return;
+    const int row = row0 + 32 * wave + n;
+    const bool mine = row < rows;
+    const int tok = (mine ? row : rows - 1) / plan.group, head = h * plan.group + (mine ? row : rows - 1) % plan.group;
+    int lo, hi, first_lo, first_hi, last_lo, last_hi, w_first_lo, w_first_hi, w_last_lo, w_last_hi;
+    seen_range(a, sq, sq.first + tok, lo, hi);
+    seen_range(a, sq, sq.first + row0 / plan.group, first_lo, first_hi);
+    seen_range(a, sq, sq.first + (min(row0 + LONG_ROWS, rows) - 1) / plan.group, last_lo, last_hi);
+    seen_range(a, sq, sq.first + min(row0 + 32 * wave, rows - 1) / plan.group, w_first_lo, w_first_hi);
+    seen_range(a, sq, sq.first + min(row0 + 32 * wave + 31, rows - 1) / plan.group, w_last_lo, w_last_hi);
+    const int t_lo = first_lo / TILE, t_hi = (last_hi + TILE - 1) / TILE;
+    const int per = max(t_hi - t_lo + plan.splits_long - 1, 0) / plan.splits_long;
+    const int begin = t_lo + split * per, end = min(begin + per, t_hi);
+
+    half8 q[STEPS][NS];
+    float factor;
+    {
+        const int64_t at = (sq.t0 + tok) * a.q.token_stride + (int64_t)head * a.q.head_stride + 8 * hf;
+        float amax = 0.f;
+#pragma unroll
+        for (int s = 0; s < STEPS; s++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) amax = fmaxf(amax, fabsf(load_value<DT>(a.q.p, at + 16 * s + j)));
+        amax = fmaxf(amax, __shfl_xor(amax, 32));
+        const int e = row_exponent(amax);
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = ldexpf(load_value<DT>(a.q.p, at + 16 * s + j), 15 - e);
+            parts8<NS>(v, q[s]);
+        }
+        factor = ldexpf(a.scale * 1.44269504088896340736f, e - 15);
+    }
+
+    f32x16 o[DB];
+#pragma unroll
+    for (int i = 0; i < DB; i++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) o[i][j] = 0.f;
+    float m = -INFINITY, l = 0.f, r = 0.f;
+
+    const int32_t *table = a.s.tables + b * a.s.table_stride;
+    const int64_t page_bytes = (int64_t)P * D;
+    struct Pages {
+        int32_t p[4];  // of the step's four 16-key groups; -1: none to see
+    };
+    auto pages_of = [&](int t) {
+        Pages g;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int key = t * TILE + 16 * i;
+            int32_t p = -1;
+            if (t < end && key < last_hi) p = table[key >> lp];
+            g.p[i] = p >= 0 && p < a.c.num_pages ? p : -1;
+        }
+        return g;
+    };
+    auto pick = [](const Pages &g, int i) { return i & 2 ? (i & 1 ? g.p[3] : g.p[2]) : (i & 1 ? g.p[1] : g.p[0]); };
+    u32x4 kc[PER], vc[PER];
+    float ks[4], vs[4];
+    auto load = [&](int t, const Pages &g) {
+        const int key = t * TILE;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int id = tid + 64 * LONG_WAVES * i;
+            if (CHUNKS % (64 * LONG_WAVES) == 0 || id < CHUNKS) {
+                const int kt = id / (D / 16), kd = id % (D / 16) * 16;
+                const uint8_t *kp = a.c.k + ((int64_t)max(pick(g, kt >> 4), 0) * H + h) * page_bytes;
+                kc[i] = *reinterpret_cast<const u32x4 *>(kp + ((key + kt) & (P - 1)) * D + kd);
+                const int vg = id & 3, vd = id >> 2;
+                const uint8_t *vp = a.c.v + ((int64_t)max(pick(g, vg), 0) * H + h) * page_bytes;
+                vc[i] = *reinterpret_cast<const u32x4 *>(vp + vd * P + ((key + 16 * vg) & (P - 1)));
+            }
+        }
+    };
+    auto scales = [&](const Pages &g) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int64_t at = (int64_t)max(g.p[i], 0) * H + h;
+            ks[i] = a.c.ks[at];
+            vs[i] = g.p[i] >= 0 ? a.c.vs[at] : 0.f;
+        }
+    };
+    // codes -> f16 in LDS; values behind the sequence's end, or of no page, as zeros
+    auto stage = [&](int t, const Pages &g, _Float16 *buf) {
+        _Float16 *const kb = buf, *const vb = buf + TILE * KROW;
+        const bool partial = (t + 1) * TILE > sq.len || g.p[0] < 0 || g.p[1] < 0 || g.p[2] < 0 || g.p[3] < 0;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int id = tid + 64 * LONG_WAVES * i;
+            if (CHUNKS % (64 * LONG_WAVES) == 0 || id < CHUNKS) {
+                const int kt = id / (D / 16), kd = id % (D / 16) * 16;
+                // key 32 b + 16 a1 + 8 half + 4 a0 + j is row 32 b + 16 a1 + 8 a0 + 4 half + j
+                const int kr = (kt & 0x33) | (kt & 8) >> 1 | (kt & 4) << 1;
+                half8 *const ko = reinterpret_cast<half8 *>(kb + kr * KROW + kd);
+                ko[0] = codes8<KIND>(kc[i][0], kc[i][1]);
+                ko[1] = codes8<KIND>(kc[i][2], kc[i][3]);
+                const int vg = id & 3, vd = id >> 2;
+                if (partial) vc[i] = keep_bytes(vc[i], pick(g, vg) >= 0 ? min(max((int)sq.len - (t * TILE + 16 * vg), 0), 16) : 0);
+                half8 *const vo = reinterpret_cast<half8 *>(vb + vd * VROW + 16 * vg);
+                vo[0] = codes8<KIND>(vc[i][0], vc[i][1]);
+                vo[1] = codes8<KIND>(vc[i][2], vc[i][3]);
+            }
+        }
+    };
+
+    Pages now = pages_of(begin), next = pages_of(begin + 1);
+    int buf = 0;
+    if (begin < end) {
+        load(begin, now);
+        stage(begin, now, lds);
+    }
+    __syncthreads();
+    for (int t = begin; t < end; t++, buf ^= 1) {
+        scales(now);
+        if (t + 1 < end) load(t + 1, next);
+        const Pages far = pages_of(t + 2);
+        const _Float16 *const kb = lds + buf * long_lds_halves<D>(), *const vb = kb + TILE * KROW;
+        const int key = t * TILE;
+        if (key < w_last_hi && key + TILE > w_first_lo) {  // (else no row of this wave sees any of it)
+            f32x16 s[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+#pragma unroll
+                for (int j = 0; j < 16; j++) s[i][j] = 0.f;
+#pragma unroll
+                for (int j = 0; j < STEPS; j++) {
+                    const half8 k8 = *reinterpret_cast<const half8 *>(kb + (32 * i + n) * KROW + 16 * j + 8 * hf);
+#pragma unroll
+                    for (int u = NS - 1; u >= 0; u--) s[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, q[j][u], s[i], 0, 0, 0);
+                }
+            }
+            // s[i][j] is key 16 u + 8 hf + 4 (j / 4 % 2) + j % 4 of the step, u = 2 i + j / 8
+            const bool there = now.p[0] >= 0 && now.p[1] >= 0 && now.p[2] >= 0 && now.p[3] >= 0;
+            const bool edge = key < w_last_lo || key + TILE > w_first_hi || !there;
+            uint32_t unseen = 0;
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) s[i][j] *= ks[2 * i + j / 8] * factor;
+            if (edge) {
+                const int from = lo - (key + 8 * hf), to = hi - (key + 8 * hf);
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int j = 0; j < 16; j++) {
+                        const int at = 16 * (2 * i + j / 8) + j % 8;
+                        const bool seen = at >= from && at < to && now.p[2 * i + j / 8] >= 0;
+                        s[i][j] = seen ? s[i][j] : -INFINITY;
+                        unseen |= seen ? 0u : 1u << (16 * i + j);
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) top = fmaxf(top, s[i][j]);
+            top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), m);
+            const float vmax = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+            float grown = 1.f;
+            if (vmax > r) {
+                const float rn = scale_ceiling(vmax);
+                grown = r / rn;
+                r = rn;
+            }
+            if (__any(top > m) || grown != 1.f) {
+                const float alpha = exp2_fast(m - base_of(top));
+                l *= alpha;
+                const float f = alpha * grown;
+#pragma unroll
+                for (int i = 0; i < DB; i++)
+#pragma unroll
+                    for (int j = 0; j < 16; j++) o[i][j] *= f;
+                m = top;
+            }
+            const float base = base_of(m) - 15.f;
+            float vr[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) vr[i] = r > 0.f ? vs[i] / r : 0.f;
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                float w[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    w[j] = exp2_fast(s[u / 2][8 * (u % 2) + j] - base);
+                    l += w[j];
+                    w[j] *= vr[u];
+                }
+                if (edge)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) w[j] = unseen >> (8 * u + j) & 1 ? 0.f : w[j];
+                half8 p[NS];
+                parts8<NS>(w, p);
+#pragma unroll
+                for (int i = 0; i < DB; i++) {
+                    const half8 v8 = *reinterpret_cast<const half8 *>(vb + (32 * i + n) * VROW + 16 * u + 8 * hf);
+#pragma unroll
+                    for (int z = NS - 1; z >= 0; z--) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, p[z], o[i], 0, 0, 0);
+                }
+            }
+        }
+        if (t + 1 < end) stage(t + 1, next, lds + (buf ^ 1) * long_lds_halves<D>());
+        now = next;
+        next = far;
+        __syncthreads();
+    }
+
+    l += __shfl_xor(l, 32);
+    const float inv = l == 0.f ? 0.f : 1.f / l;  // (apart from r: their quotient can be subnormal)
+    if (!mine) return;
+    const int64_t out = (sq.t0 + tok) * a.q_heads + head, at = split * a.num_q * a.q_heads + out;
+    if (plan.splits_long > 1 && hf == 0) plan.stat[2 * at] = m, plan.stat[2 * at + 1] = l;
+#pragma unroll
+    for (int i = 0; i < DB; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            float v[4];
+#pragma unroll
+            for (int z = 0; z < 4; z++) v[z] = l == 0.f ? 0.f : o[i][4 * j + z] * inv * r;
+            const int d = 32 * i + 8 * j + 4 * hf;
+            if (plan.splits_long == 1) store_values4<DT>(a.out, out * D + d, v);
+            else *reinterpret_cast<f32x4 *>(plan.part + at * D + d) = f32x4{v[0], v[1], v[2], v[3]};
+        }
+}
+
+// The join of a row's parts, one wave per (row, head): a lane's channels over the parts in
+// order.  Rows whose form did not cut its keys were written by it.
+template <int D, int DT>
+__global__ __launch_bounds__(64) void k_attn_join(KvAttention a, AttnPlan plan) {
+    const int lane = threadIdx.x;
+    const int64_t t = blockIdx.x / a.q_heads, row = blockIdx.x;
+    const int b = find_sequence(a.s.batch, t, [&](int i) { return (int64_t)a.cu_q[i]; });
+    Sequence sq;
+    if (!sequence_of(a, b, sq) || t < sq.t0 || t >= sq.t0 + sq.n) return;
+    const int splits = sq.n * plan.group <= plan.short_rows ? plan.splits_short : plan.splits_long;
+    if (splits <= 1) return;
+    const int64_t all = a.num_q * a.q_heads;
+    float top = -INFINITY;
+    for (int i = lane; i < splits; i += 64) top = fmaxf(top, plan.stat[2 * (i * all + row)]);
+#pragma unroll
+    for (int d = 32; d; d /= 2) top = fmaxf(top, __shfl_xor(top, d));
+    float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+    const int d0 = 4 * lane;
+    for (int i = 0; i < splits; i++) {
+        const float l = plan.stat[2 * (i * all + row) + 1];
+        if (l == 0.f) continue;
+        const float f = part_weight(plan.stat[2 * (i * all + row)], l, top);
+        sum += f;
+        if (d0 < D) {
+            const f32x4 o = *reinterpret_cast<const f32x4 *>(plan.part + (i * all + row) * D + d0);
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = fmaf(f, o[j], v[j]);
+        }
+    }
+    if (d0 >= D) return;
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = sum == 0.f ? 0.f : v[j] / sum;
+    store_values4<DT>(a.out, row * D + d0, v);
+}
+
+template <int D, int KIND, int DT>
+hipError_t launch_typed(const KvAttention &a, const AttnPlan &plan, bool any_short, bool any_long, hipStream_t st) {
+    if (any_long) {
+        const size_t lds = 2 * sizeof(_Float16) * long_lds_halves<D>();
+        auto k = k_attn_long<D, KIND, DT>;
+        if (lds > 65536) {
+            hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+            if (e != hipSuccess) return e;
+        }
+        k<<<dim3((unsigned)(plan.tiles * a.c.kv_heads), (unsigned)plan.splits_long), 64 * LONG_WAVES, lds, st>>>(a, plan);
+        hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    if (any_short) {
+        k_attn_short<D, KIND, DT><<<dim3((unsigned)(plan.splits_short * a.c.kv_heads * a.s.batch)), 64 * SHORT_WAVES, 0, st>>>(a, plan);
+        hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    if ((any_long && plan.splits_long > 1) || (any_short && plan.splits_short > 1))
+        k_attn_join<D, DT><<<dim3((unsigned)(a.num_q * a.q_heads)), 64, 0, st>>>(a, plan);
+    return hipGetLastError();
+}
+
+template <int D>
+hipError_t launch_dim(const KvAttention &a, const AttnPlan &plan, bool any_short, bool any_long, hipStream_t st) {
+    const bool i8 = a.c.kind == KV_INT8;
+    switch (a.dtype) {
+        case DT_F32:
+            return i8 ? launch_typed<D, KV_INT8, DT_F32>(a, plan, any_short, any_long, st) : launch_typed<D, KV_E4M3, DT_F32>(a, plan, any_short, any_long, st);
+        case DT_F16:
+            return i8 ? launch_typed<D, KV_INT8, DT_F16>(a, plan, any_short, any_long, st) : launch_typed<D, KV_E4M3, DT_F16>(a, plan, any_short, any_long, st);
+        default:
+            return i8 ? launch_typed<D, KV_INT8, DT_BF16>(a, plan, any_short, any_long, st) : launch_typed<D, KV_E4M3, DT_BF16>(a, plan, any_short, any_long, st);
+    }
+}
+
+}  // namespace attn
+
+// one translation unit per head size (lbq_attn_d*.hip)
+hipError_t launch_attn_d64(const KvAttention &a, const AttnPlan &plan, bool any_short, bool any_long, hipStream_t st);
+hipError_t launch_attn_d96(const KvAttention &a, const AttnPlan &plan, bool any_short, bool any_long, hipStream_t st);
+hipError_t launch_attn_d128(const KvAttention &a, const AttnPlan &plan, bool any_short, bool any_long, hipStream_t st);
+hipError_t launch_attn_d192(const KvAttention &a, const AttnPlan &plan, bool any_short, bool any_long, hipStream_t st);
+hipError_t launch_attn_d256(const KvAttention &a, const AttnPlan &plan, bool any_short, bool any_long, hipStream_t st);
+
+}  // namespace lbq

@@ -228,6 +228,8 @@ static int attention_args(const lbq_kv_cache *cache, const lbq_kv_step *step, in
     a->max_len = step->max_len ? std::min<int64_t>(step->max_len, held) : held;
     if (a->max_len > INT32_MAX - 65536) return fail(LBQ_ERR_LIMIT, "sequences of %lld tokens", (long long)a->max_len);
     a->max_new = step->max_new;
+    if (step->num_tokens * q_heads > INT32_MAX)
+        return fail(LBQ_ERR_LIMIT, "%lld tokens of %d heads in one call", (long long)step->num_tokens, q_heads);
     return LBQ_OK;
 }
 

@@ -101,12 +101,13 @@ def append(k_codes, v_codes, k_scales, v_scales, kind, k, v, slots, page):
 
 
 def attention(q, k_codes, v_codes, k_scales, v_scales, tables, seq_lens, cu, scale, causal=True, window=0):
-    """(out, sum_j p_j |v_j|, largest sum_d |q_d k_d| scale) in 64 bits, over codes given as values;
-    rows no sequence owns are zero."""
+    """(out, sum_j p_j |v_j|, largest |v|, largest sum_d |q_d k_d| scale) in 64 bits, over codes given as
+    values; the largest |v| is over the keys that a row's sequence shows to any of its rows.  Rows no
+    sequence owns are zero."""
     page, dev = k_codes.shape[2], q.device
     heads, kv = q.shape[1], k_codes.shape[1]
     out = torch.zeros(q.shape, dtype=F64, device=dev)
-    mag = torch.zeros_like(out)
+    mag, most = torch.zeros_like(out), torch.zeros_like(out)
     reach = 0.0
     for b in range(len(seq_lens)):
         t0, t1, n = cu[b], cu[b + 1], seq_lens[b]
@@ -137,22 +138,30 @@ def attention(q, k_codes, v_codes, k_scales, v_scales, tables, seq_lens, cu, sca
             vz = torch.where(seen.any(0)[:, None], vs, 0.0)
             out[t0:t1, h * g:(h + 1) * g] = w @ vz
             mag[t0:t1, h * g:(h + 1) * g] = w @ vz.abs()
+            most[t0:t1, h * g:(h + 1) * g] = torch.nan_to_num(vz).abs().max()
             big = (rows.abs() @ torch.where(seen.any(0)[:, None], ks, 0.0).abs().t()) * abs(scale)
             reach = max(reach, torch.nan_to_num(big).max().item())
-    return out, mag, reach
+    return out, mag, most, reach
 
 
-def attention_bound(dtype, mag, out, reach, keys):
+def attention_bound(dtype, mag, most, out, reach, keys):
     """How far an output may be from the 64-bit one, element by element.
 
     f32: a logit is a sum of dim products whose operands are held to 2^-22 of the row's largest and
     whose running sum is rounded at most 20 times, so it is off by (2^-22 + 20 * 2^-24) sum |q k| scale;
     a weight by twice that (its own logit and the sum's) and the exponential's few last bits (16 * 2^-24);
     the weighted sum over the keys is rounded once per 16 keys and per join, 2^-24 each.  16-bit types:
-    the weights are rounded to f16 (half a step: 2^-11) and the result to its type."""
+    the weights are rounded to f16 (half a step: 2^-11) and the result to its type.
+
+    All types: a weight goes into the product as f16 parts of 2^15 w s / r, w at most 1 (the row's
+    largest is 1, so the weights' sum is at least 1), s its page's scale and r the power of two next above the largest
+    scale so far.  The parts are off by half the smallest f16 step, 2^-25, whatever the weight's size:
+    2^-40 r |code| of the result for each key, and r |code| < 2 s_max |code|_max.  s_max |code|_max is at
+    most 127 (448 for e4m3) s_max, which the tests' blocks of random codes reach to within a factor of 2:
+    2^-40 * 4 * the largest |v|, for each key."""
     rel = 2 * (2.0 ** -22 + 20 * 2.0 ** -24) * reach + (16 + keys / 16 + 64) * 2.0 ** -24
     step_half = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[dtype]
     if dtype != torch.float32:
         rel += 2.0 ** -11
     tiny = {torch.float32: 0.0, torch.float16: 2.0 ** -25, torch.bfloat16: 0.0}[dtype]
-    return rel * mag + step_half * out.abs() + tiny + 1e-37
+    return rel * mag + keys * 2.0 ** -38 * most + step_half * out.abs() + tiny + 1e-37
