@@ -21,6 +21,8 @@
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
+#include <algorithm>
+
 namespace lbq {
 
 // the launch's plan, the same in the kernels and in the join
@@ -38,6 +40,7 @@ namespace attn {
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -108,10 +111,17 @@ __device__ __forceinline__ u32x4 keep_bytes(u32x4 v, int keep) {
 template <int NS>
 __device__ __forceinline__ void parts8(const float *v, half8 *o) {
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const _Float16 hi = (_Float16)v[j];
-        o[0][j] = hi;
-        if constexpr (NS == 2) o[NS - 1][j] = (_Float16)(v[j] - (float)hi);
+    for (int j = 0; j < 8; j += 2) {
+        const half2v hi = __builtin_convertvector((f32x2){v[j], v[j + 1]}, half2v);
+        o[0][j] = hi[0], o[0][j + 1] = hi[1];
+        if constexpr (NS == 2) {
+            // v - hi, exactly, taking the f16 as it is (the compiler widens it first)
+            float d0, d1;
+            asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(d0) : "v"(hi), "v"(v[j]));
+            asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d1) : "v"(hi), "v"(v[j + 1]));
+            const half2v lo = __builtin_convertvector((f32x2){d0, d1}, half2v);
+            o[NS - 1][j] = lo[0], o[NS - 1][j + 1] = lo[1];
+        }
     }
 }
 
@@ -122,12 +132,8 @@ __device__ __forceinline__ int row_exponent(float amax) {
     return e;
 }
 
-// a power of two no smaller than a value scale (and normal, as is its inverse)
-__device__ __forceinline__ float scale_ceiling(float s) {
-    int e = 0;
-    (void)frexpf(s, &e);
-    return ldexpf(1.f, min(max(e, -126), 126));
-}
+// the exponent of a power of two no smaller than a value scale (and normal, as is its inverse)
+__device__ __forceinline__ int scale_ceiling(float s) { return min(max(__builtin_amdgcn_frexp_expf(s), -126), 126); }
 
 // what a sequence's rows see, and where its queries lie
 struct Sequence {
@@ -152,6 +158,21 @@ __device__ __forceinline__ void seen_range(const KvAttention &a, const Sequence 
     lo = a.causal && a.window > 0 ? (int)max((int64_t)0, pos - a.window + 1) : 0;
 }
 
+// The weights' factor for a value scale s, relative to r and in powers of two.  Below 2^-45 a
+// weight of at most 2^15 is less than half the smallest f16 step whatever it is, so that the
+// bound changes nothing, and keeps the inverse finite for a scale of 0.
+// (The last term is 0, or NaN for a scale that is.)
+__device__ __forceinline__ float scale_log(float s, float inv_r) {
+    return fmaf(s, 0.f, fmaxf(__builtin_amdgcn_logf(s * inv_r), -45.f));
+}
+
+// The factor of a key scale's products.  Not negative (the largest product has the largest logit),
+// and not 0, so that a product of -infinity, which stands for a key that is not seen, stays one.
+__device__ __forceinline__ float logit_factor(float scale, float factor) {
+    const float f = scale * factor;
+    return f == 0.f ? 0x1p-126f : f;
+}
+
 // The join of parts' outputs o_i with maxima m_i and sums l_i: weights l_i 2^(m_i - max).
 __device__ __forceinline__ float part_weight(float m, float l, float top) { return l * exp2_fast(m - base_of(top)); }
 
@@ -166,12 +187,12 @@ __device__ __forceinline__ float part_weight(float m, float l, float top) { retu
 constexpr int SHORT_WAVES = 4;
 
 template <int D, int KIND, int DT>
-__global__ __launch_bounds__(64 * SHORT_WAVES) void k_attn_short(KvAttention a, AttnPlan plan) {
+__global__ __launch_bounds__(64 * SHORT_WAVES, D <= 128 ? 2 : 1) void k_attn_short(KvAttention a, AttnPlan plan) {
     constexpr int NS = DT == DT_F32 ? 2 : 1;
     constexpr int STEPS = D / 32, DB = D / 16;
     __shared__ float s_o[SHORT_WAVES][SHORT_ROWS][D + 4];
     __shared__ float s_m[SHORT_WAVES][SHORT_ROWS], s_l[SHORT_WAVES][SHORT_ROWS];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, c = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, c = lane >> 4;
     const int H = a.c.kv_heads, P = a.c.page_size, lp = a.c.log2_page;
     const int h = blockIdx.x % H, split = blockIdx.x / H % plan.splits_short, b = blockIdx.x / H / plan.splits_short;
     Sequence sq;
@@ -208,16 +229,16 @@ __global__ __launch_bounds__(64 * SHORT_WAVES) void k_attn_short(KvAttention a, 
 #pragma unroll
         for (int s = 0; s < STEPS; s++) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[s][j] = ldexpf(v[s][j], 15 - e);
+            for (int j = 0; j < 8; j++) v[s][j] = copysignf(1.f, a.scale) * ldexpf(v[s][j], 15 - e);
             parts8<NS>(v[s], q[s]);
         }
-        factor = ldexpf(a.scale * 1.44269504088896340736f, e - 15);
+        factor = ldexpf(fabsf(a.scale) * 1.44269504088896340736f, e - 15);
     }
 
     f32x4 o[DB];
 #pragma unroll
     for (int i = 0; i < DB; i++) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f, r = 0.f;
+    float m = -INFINITY, l = 0.f, r = 0.f, inv_r = 1.f;
 
     const int32_t *table = a.s.tables + b * a.s.table_stride;
     const int64_t page_bytes = (int64_t)P * D;
@@ -276,6 +297,7 @@ __global__ __launch_bounds__(64 * SHORT_WAVES) void k_attn_short(KvAttention a, 
         if (more) load(next, t + SHORT_WAVES, kp_next, vp_next);
         const int32_t vp_far = page_of(t + 2 * SHORT_WAVES, c), kp_far = page_of(t + 2 * SHORT_WAVES, kg);
 
+        const int key = t * TILE;
         float x[16];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -286,59 +308,50 @@ __global__ __launch_bounds__(64 * SHORT_WAVES) void k_attn_short(KvAttention a, 
 #pragma unroll
                 for (int u = NS - 1; u >= 0; u--) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, q[j][u], s, 0, 0, 0);
             }
-            const float f = cur.ks * factor;
 #pragma unroll
-            for (int j = 0; j < 4; j++) x[4 * i + j] = s[j] * f;
+            for (int j = 0; j < 4; j++) x[4 * i + j] = s[j];
         }
-        // keys that some row does not see, or that are not there
-        const int key = t * TILE;
-        const bool edge = key < last_lo || key + TILE > first_hi || __any(vp < 0);
-        uint32_t unseen = 0;
-        if (edge) {
+        float vmax = fmaxf(cur.vs, __shfl_xor(cur.vs, 16));
+        vmax = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(fmaxf(vmax, __shfl_xor(vmax, 32)))));
+        float grown = 1.f;
+        if (vmax > r) {
+            const int e = scale_ceiling(vmax);
+            inv_r = ldexpf(1.f, -e);
+            grown = r * inv_r;
+            r = ldexpf(1.f, e);
+        }
+        float f = logit_factor(cur.ks, factor), lv = scale_log(cur.vs, inv_r), back = exp2_fast(-lv);
+        if (key < last_lo || key + TILE > first_hi || __any(vp < 0)) {
+            // some row does not see some of these keys, or they are not there
             const int from = lo - (key + 16 * c), to = vp >= 0 ? hi - (key + 16 * c) : 0;
 #pragma unroll
-            for (int j = 0; j < 16; j++) {
-                const bool seen = j >= from && j < to;
-                x[j] = seen ? x[j] : -INFINITY;
-                unseen |= seen ? 0u : 1u << j;
-            }
-        }
-        float top = x[0];
-#pragma unroll
-        for (int j = 1; j < 16; j++) top = fmaxf(top, x[j]);
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), m);
-        float vmax = fmaxf(cur.vs, __shfl_xor(cur.vs, 16));
-        vmax = fmaxf(vmax, __shfl_xor(vmax, 32));
-        float grown = 1.f;
-        if (vmax > r) {  // (the same in every lane)
-            const float rn = scale_ceiling(vmax);
-            grown = r / rn;
-            r = rn;
-        }
-        if (__any(top > m) || grown != 1.f) {
-            const float alpha = exp2_fast(m - base_of(top));
-            l *= alpha;
-            const float f = alpha * grown;
-#pragma unroll
-            for (int i = 0; i < DB; i++) o[i] *= f;
-            m = top;
-        }
-        const float base = base_of(m) - 15.f, vr = r > 0.f ? cur.vs / r : 0.f;
-        float w[16];
-#pragma unroll
-        for (int j = 0; j < 16; j++) {
-            w[j] = exp2_fast(x[j] - base);
-            l += w[j];
-            w[j] *= vr;
-        }
-        if (edge) {  // (a weight of 0 under a scale of NaN)
-#pragma unroll
-            for (int j = 0; j < 16; j++) w[j] = unseen >> j & 1 ? 0.f : w[j];
+            for (int j = 0; j < 16; j++) x[j] = j >= from && j < to ? x[j] : -INFINITY;
+            if (max(from, 0) >= min(to, 16)) f = 1.f, lv = 0.f, back = 1.f;  // none of them, so neither their scales
             const int keep = vp >= 0 ? min(max((int)sq.len - (key + 16 * c), 0), 16) : 0;
 #pragma unroll
             for (int i = 0; i < DB; i++) cur.v[i] = keep_bytes(cur.v[i], keep);
         }
+        float top = x[0];
+#pragma unroll
+        for (int j = 1; j < 16; j++) top = fmaxf(top, x[j]);
+        top *= f;
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), m);
+        if (grown != 1.f || __any(top > m)) {
+            const float alpha = exp2_fast(m - base_of(top)), g = alpha * grown;
+            l *= alpha;
+#pragma unroll
+            for (int i = 0; i < DB; i++) o[i] *= g;
+            m = top;
+        }
+        const float base = base_of(m) - 15.f - lv;
+        float w[16], sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            w[j] = exp2_fast(fmaf(x[j], f, -base));
+            sum += w[j];
+        }
+        l = fmaf(sum, back, l);
         half8 p[2][NS];
         parts8<NS>(w, p[0]);
         parts8<NS>(w + 8, p[1]);
@@ -412,7 +425,7 @@ __global__ __launch_bounds__(64 * LONG_WAVES, D <= 128 ? 2 : 1) void k_attn_long
     constexpr int KROW = D + 8, VROW = TILE + 8;
     constexpr int CHUNKS = TILE * D / 16, PER = (CHUNKS + 64 * LONG_WAVES - 1) / (64 * LONG_WAVES);  // 16-code chunks, of K and of V
     extern __shared__ _Float16 lds[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, hf = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, hf = lane >> 5;
     const int H = a.c.kv_heads, P = a.c.page_size, lp = a.c.log2_page;
     const int h = blockIdx.x % H;
     // the tiles with most keys (a sequence's last) first
@@ -451,10 +464,10 @@ __global__ __launch_bounds__(64 * LONG_WAVES, D <= 128 ? 2 : 1) void k_attn_long
         for (int s = 0; s < STEPS; s++) {
             float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = ldexpf(load_value<DT>(a.q.p, at + 16 * s + j), 15 - e);
+            for (int j = 0; j < 8; j++) v[j] = copysignf(1.f, a.scale) * ldexpf(load_value<DT>(a.q.p, at + 16 * s + j), 15 - e);
             parts8<NS>(v, q[s]);
         }
-        factor = ldexpf(a.scale * 1.44269504088896340736f, e - 15);
+        factor = ldexpf(fabsf(a.scale) * 1.44269504088896340736f, e - 15);
     }
 
     f32x16 o[DB];
@@ -462,27 +475,27 @@ __global__ __launch_bounds__(64 * LONG_WAVES, D <= 128 ? 2 : 1) void k_attn_long
     for (int i = 0; i < DB; i++)
 #pragma unroll
         for (int j = 0; j < 16; j++) o[i][j] = 0.f;
-    float m = -INFINITY, l = 0.f, r = 0.f;
+    float m = -INFINITY, l = 0.f, r = 0.f, inv_r = 1.f;
 
     const int32_t *table = a.s.tables + b * a.s.table_stride;
     const int64_t page_bytes = (int64_t)P * D;
-    struct Pages {
-        int32_t p[4];  // of the step's four 16-key groups; -1: none to see
-    };
-    auto pages_of = [&](int t) {
-        Pages g;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int key = t * TILE + 16 * i;
-            int32_t p = -1;
-            if (t < end && key < last_hi) p = table[key >> lp];
-            g.p[i] = p >= 0 && p < a.c.num_pages ? p : -1;
+    struct Pages {  // of the step's four 16-key groups; -1: none to see
+        int32_t p0, p1, p2, p3;
+        __device__ int32_t of(int i) const {
+            const int32_t a0 = p0, a1 = p1, a2 = p2, a3 = p3;  // (values: a choice of members would be one of addresses)
+            const int32_t lo = i & 1 ? a1 : a0, hi = i & 1 ? a3 : a2;
+            return i & 2 ? hi : lo;
         }
-        return g;
+        __device__ bool all() const { return p0 >= 0 && p1 >= 0 && p2 >= 0 && p3 >= 0; }
     };
-    auto pick = [](const Pages &g, int i) { return i & 2 ? (i & 1 ? g.p[3] : g.p[2]) : (i & 1 ? g.p[1] : g.p[0]); };
+    auto page_of = [&](int t, int g) {
+        const int key = t * TILE + 16 * g;
+        int32_t p = -1;
+        if (t < end && key < last_hi) p = table[key >> lp];
+        return p >= 0 && p < a.c.num_pages ? p : -1;
+    };
+    auto pages_of = [&](int t) { return Pages{page_of(t, 0), page_of(t, 1), page_of(t, 2), page_of(t, 3)}; };
     u32x4 kc[PER], vc[PER];
-    float ks[4], vs[4];
     auto load = [&](int t, const Pages &g) {
         const int key = t * TILE;
 #pragma unroll
@@ -490,26 +503,28 @@ __global__ __launch_bounds__(64 * LONG_WAVES, D <= 128 ? 2 : 1) void k_attn_long
             const int id = tid + 64 * LONG_WAVES * i;
             if (CHUNKS % (64 * LONG_WAVES) == 0 || id < CHUNKS) {
                 const int kt = id / (D / 16), kd = id % (D / 16) * 16;
-                const uint8_t *kp = a.c.k + ((int64_t)max(pick(g, kt >> 4), 0) * H + h) * page_bytes;
+                const uint8_t *kp = a.c.k + ((int64_t)max(g.of(kt >> 4), 0) * H + h) * page_bytes;
                 kc[i] = *reinterpret_cast<const u32x4 *>(kp + ((key + kt) & (P - 1)) * D + kd);
                 const int vg = id & 3, vd = id >> 2;
-                const uint8_t *vp = a.c.v + ((int64_t)max(pick(g, vg), 0) * H + h) * page_bytes;
+                const uint8_t *vp = a.c.v + ((int64_t)max(g.of(vg), 0) * H + h) * page_bytes;
                 vc[i] = *reinterpret_cast<const u32x4 *>(vp + vd * P + ((key + 16 * vg) & (P - 1)));
             }
         }
     };
-    auto scales = [&](const Pages &g) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int64_t at = (int64_t)max(g.p[i], 0) * H + h;
-            ks[i] = a.c.ks[at];
-            vs[i] = g.p[i] >= 0 ? a.c.vs[at] : 0.f;
-        }
+    // lane i holds the scales of group i mod 4
+    struct Scales {
+        float k, v;
     };
+    auto scales_of = [&](const Pages &g) {
+        const int32_t p = g.of(lane & 3);
+        const int64_t at = (int64_t)max(p, 0) * H + h;
+        return Scales{a.c.ks[at], p >= 0 ? a.c.vs[at] : 0.f};
+    };
+    auto from_lane = [](float x, int i) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), i)); };
     // codes -> f16 in LDS; values behind the sequence's end, or of no page, as zeros
     auto stage = [&](int t, const Pages &g, _Float16 *buf) {
         _Float16 *const kb = buf, *const vb = buf + TILE * KROW;
-        const bool partial = (t + 1) * TILE > sq.len || g.p[0] < 0 || g.p[1] < 0 || g.p[2] < 0 || g.p[3] < 0;
+        const bool partial = (t + 1) * TILE > sq.len || !g.all();
 #pragma unroll
         for (int i = 0; i < PER; i++) {
             const int id = tid + 64 * LONG_WAVES * i;
@@ -521,7 +536,7 @@ __global__ __launch_bounds__(64 * LONG_WAVES, D <= 128 ? 2 : 1) void k_attn_long
                 ko[0] = codes8<KIND>(kc[i][0], kc[i][1]);
                 ko[1] = codes8<KIND>(kc[i][2], kc[i][3]);
                 const int vg = id & 3, vd = id >> 2;
-                if (partial) vc[i] = keep_bytes(vc[i], pick(g, vg) >= 0 ? min(max((int)sq.len - (t * TILE + 16 * vg), 0), 16) : 0);
+                if (partial) vc[i] = keep_bytes(vc[i], g.of(vg) >= 0 ? min(max((int)sq.len - (t * TILE + 16 * vg), 0), 16) : 0);
                 half8 *const vo = reinterpret_cast<half8 *>(vb + vd * VROW + 16 * vg);
                 vo[0] = codes8<KIND>(vc[i][0], vc[i][1]);
                 vo[1] = codes8<KIND>(vc[i][2], vc[i][3]);
@@ -530,6 +545,7 @@ __global__ __launch_bounds__(64 * LONG_WAVES, D <= 128 ? 2 : 1) void k_attn_long
     };
 
     Pages now = pages_of(begin), next = pages_of(begin + 1);
+    Scales sc = scales_of(now);
     int buf = 0;
     if (begin < end) {
         load(begin, now);
@@ -537,8 +553,8 @@ __global__ __launch_bounds__(64 * LONG_WAVES, D <= 128 ? 2 : 1) void k_attn_long
     }
     __syncthreads();
     for (int t = begin; t < end; t++, buf ^= 1) {
-        scales(now);
         if (t + 1 < end) load(t + 1, next);
+        const Scales sc_next = scales_of(next);
         const Pages far = pages_of(t + 2);
         const _Float16 *const kb = lds + buf * long_lds_halves<D>(), *const vb = kb + TILE * KROW;
         const int key = t * TILE;
@@ -556,64 +572,67 @@ __global__ __launch_bounds__(64 * LONG_WAVES, D <= 128 ? 2 : 1) void k_attn_long
                 }
             }
             // s[i][j] is key 16 u + 8 hf + 4 (j / 4 % 2) + j % 4 of the step, u = 2 i + j / 8
-            const bool there = now.p[0] >= 0 && now.p[1] >= 0 && now.p[2] >= 0 && now.p[3] >= 0;
-            const bool edge = key < w_last_lo || key + TILE > w_first_hi || !there;
-            uint32_t unseen = 0;
-            float top = -INFINITY;
+            const float vmax = fmaxf(fmaxf(from_lane(sc.v, 0), from_lane(sc.v, 1)), fmaxf(from_lane(sc.v, 2), from_lane(sc.v, 3)));
+            float grown = 1.f;
+            if (__any(vmax > r)) {
+                const int e = scale_ceiling(vmax);
+                inv_r = ldexpf(1.f, -e);
+                grown = r * inv_r;
+                r = ldexpf(1.f, e);
+            }
+            float f[4], lv[4], back[4];
+            {
+                const float mine_lv = scale_log(sc.v, inv_r), mine_back = exp2_fast(-mine_lv);
 #pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int j = 0; j < 16; j++) s[i][j] *= ks[2 * i + j / 8] * factor;
-            if (edge) {
+                for (int u = 0; u < 4; u++) {
+                    f[u] = logit_factor(from_lane(sc.k, u), factor);
+                    lv[u] = from_lane(mine_lv, u);
+                    back[u] = from_lane(mine_back, u);
+                }
+            }
+            if (key < w_last_lo || key + TILE > w_first_hi || !now.all()) {
+                // some row does not see some of these keys, or they are not there
                 const int from = lo - (key + 8 * hf), to = hi - (key + 8 * hf);
 #pragma unroll
-                for (int i = 0; i < 2; i++)
+                for (int u = 0; u < 4; u++) {
+                    const int a0 = max(from - 16 * u, 0), a1 = now.of(u) >= 0 ? min(to - 16 * u, 8) : 0;
 #pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        const int at = 16 * (2 * i + j / 8) + j % 8;
-                        const bool seen = at >= from && at < to && now.p[2 * i + j / 8] >= 0;
-                        s[i][j] = seen ? s[i][j] : -INFINITY;
-                        unseen |= seen ? 0u : 1u << (16 * i + j);
+                    for (int j = 0; j < 8; j++) {
+                        const float x = s[u / 2][8 * (u % 2) + j];
+                        s[u / 2][8 * (u % 2) + j] = j >= a0 && j < a1 ? x : -INFINITY;
                     }
+                    if (a0 >= a1) f[u] = 1.f, lv[u] = 0.f, back[u] = 1.f;  // none of the group, so neither its scales
+                }
             }
+            float top = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 2; i++)
+            for (int u = 0; u < 4; u++) {
+                float x = s[u / 2][8 * (u % 2)];
 #pragma unroll
-                for (int j = 0; j < 16; j++) top = fmaxf(top, s[i][j]);
+                for (int j = 1; j < 8; j++) x = fmaxf(x, s[u / 2][8 * (u % 2) + j]);
+                top = fmaxf(top, x * f[u]);
+            }
             top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), m);
-            const float vmax = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
-            float grown = 1.f;
-            if (vmax > r) {
-                const float rn = scale_ceiling(vmax);
-                grown = r / rn;
-                r = rn;
-            }
-            if (__any(top > m) || grown != 1.f) {
-                const float alpha = exp2_fast(m - base_of(top));
+            if (grown != 1.f || __any(top > m)) {
+                const float alpha = exp2_fast(m - base_of(top)), g = alpha * grown;
                 l *= alpha;
-                const float f = alpha * grown;
 #pragma unroll
                 for (int i = 0; i < DB; i++)
 #pragma unroll
-                    for (int j = 0; j < 16; j++) o[i][j] *= f;
+                    for (int j = 0; j < 16; j++) o[i][j] *= g;
                 m = top;
             }
             const float base = base_of(m) - 15.f;
-            float vr[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) vr[i] = r > 0.f ? vs[i] / r : 0.f;
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                float w[8];
+                const float at = base - lv[u];
+                float w[8], sum = 0.f;
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    w[j] = exp2_fast(s[u / 2][8 * (u % 2) + j] - base);
-                    l += w[j];
-                    w[j] *= vr[u];
+                    w[j] = exp2_fast(fmaf(s[u / 2][8 * (u % 2) + j], f[u], -at));
+                    sum += w[j];
                 }
-                if (edge)
-#pragma unroll
-                    for (int j = 0; j < 8; j++) w[j] = unseen >> (8 * u + j) & 1 ? 0.f : w[j];
+                l = fmaf(sum, back[u], l);
                 half8 p[NS];
                 parts8<NS>(w, p);
 #pragma unroll
@@ -627,6 +646,7 @@ __global__ __launch_bounds__(64 * LONG_WAVES, D <= 128 ? 2 : 1) void k_attn_long
         if (t + 1 < end) stage(t + 1, next, lds + (buf ^ 1) * long_lds_halves<D>());
         now = next;
         next = far;
+        sc = sc_next;
         __syncthreads();
     }
 
@@ -648,39 +668,58 @@ __global__ __launch_bounds__(64 * LONG_WAVES, D <= 128 ? 2 : 1) void k_attn_long
         }
 }
 
-// The join of a row's parts, one wave per (row, head): a lane's channels over the parts in
-// order.  Rows whose form did not cut its keys were written by it.
-template <int D, int DT>
-__global__ __launch_bounds__(64) void k_attn_join(KvAttention a, AttnPlan plan) {
-    const int lane = threadIdx.x;
-    const int64_t t = blockIdx.x / a.q_heads, row = blockIdx.x;
-    const int b = find_sequence(a.s.batch, t, [&](int i) { return (int64_t)a.cu_q[i]; });
+// The join of a row's parts, D / 4 threads a row: few parts, a row for each group of threads; many,
+// a workgroup for one row, whose groups take every JOIN_GROUPS-th part and are added in order.
+// Rows whose form did not cut its keys were written by it.
+constexpr int JOIN_THREADS = 256;
+template <int D>
+constexpr int JOIN_GROUPS = JOIN_THREADS / (D / 4);
+
+template <int D, int DT, bool ONE>
+__global__ __launch_bounds__(JOIN_THREADS) void k_attn_join(KvAttention a, AttnPlan plan) {
+    constexpr int G = JOIN_GROUPS<D>;
+    __shared__ f32x4 s_v[ONE ? G : 1][D / 4];
+    __shared__ float s_sum[ONE ? G : 1];
+    const int g = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
+    const int64_t all = a.num_q * a.q_heads, row = ONE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * G + g;
+    if (g >= G || row >= all) return;
+    const int64_t t = row / a.q_heads;
+    int b = 0;
+    for (int n = a.s.batch; n > 1;) {  // the last sequence that begins at or before t
+        const int half = n / 2;
+        const bool up = a.cu_q[b + half] <= t;
+        b += up ? half : 0;
+        n = up ? n - half : half;
+    }
     Sequence sq;
     if (!sequence_of(a, b, sq) || t < sq.t0 || t >= sq.t0 + sq.n) return;
     const int splits = sq.n * plan.group <= plan.short_rows ? plan.splits_short : plan.splits_long;
     if (splits <= 1) return;
-    const int64_t all = a.num_q * a.q_heads;
+    const float *const stat = plan.stat + 2 * row;
+    const float *const part = plan.part + row * D + d;
     float top = -INFINITY;
-    for (int i = lane; i < splits; i += 64) top = fmaxf(top, plan.stat[2 * (i * all + row)]);
-#pragma unroll
-    for (int d = 32; d; d /= 2) top = fmaxf(top, __shfl_xor(top, d));
-    float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-    const int d0 = 4 * lane;
-    for (int i = 0; i < splits; i++) {
-        const float l = plan.stat[2 * (i * all + row) + 1];
-        if (l == 0.f) continue;
-        const float f = part_weight(plan.stat[2 * (i * all + row)], l, top);
+#pragma unroll 8
+    for (int i = 0; i < splits; i++) top = fmaxf(top, stat[2 * i * all]);
+    float sum = 0.f;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = ONE ? g : 0; i < splits; i += ONE ? G : 1) {
+        const float f = part_weight(stat[2 * i * all], stat[2 * i * all + 1], top);
         sum += f;
-        if (d0 < D) {
-            const f32x4 o = *reinterpret_cast<const f32x4 *>(plan.part + (i * all + row) * D + d0);
-#pragma unroll
-            for (int j = 0; j < 4; j++) v[j] = fmaf(f, o[j], v[j]);
-        }
+        v += f * *reinterpret_cast<const f32x4 *>(part + i * all * D);  // (a part that saw nothing is zero)
     }
-    if (d0 >= D) return;
+    if constexpr (ONE) {
+        s_v[g][d / 4] = v;
+        if (d == 0) s_sum[g] = sum;
+        __syncthreads();
+        if (g) return;
 #pragma unroll
-    for (int j = 0; j < 4; j++) v[j] = sum == 0.f ? 0.f : v[j] / sum;
-    store_values4<DT>(a.out, row * D + d0, v);
+        for (int i = 1; i < G; i++) v += s_v[i][d / 4], sum += s_sum[i];
+    }
+    float o[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) o[j] = sum == 0.f ? 0.f : v[j] / sum;
+    store_values4<DT>(a.out, row * D + d, o);
 }
 
 template <int D, int KIND, int DT>
@@ -701,8 +740,10 @@ hipError_t launch_typed(const KvAttention &a, const AttnPlan &plan, bool any_sho
         hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    if ((any_long && plan.splits_long > 1) || (any_short && plan.splits_short > 1))
-        k_attn_join<D, DT><<<dim3((unsigned)(a.num_q * a.q_heads)), 64, 0, st>>>(a, plan);
+    const int splits = std::max(any_long ? plan.splits_long : 1, any_short ? plan.splits_short : 1);
+    const int64_t rows = a.num_q * a.q_heads;
+    if (splits > JOIN_GROUPS<D>) k_attn_join<D, DT, true><<<dim3((unsigned)rows), JOIN_THREADS, 0, st>>>(a, plan);
+    else if (splits > 1) k_attn_join<D, DT, false><<<dim3((unsigned)((rows + JOIN_GROUPS<D> - 1) / JOIN_GROUPS<D>)), JOIN_THREADS, 0, st>>>(a, plan);
     return hipGetLastError();
 }
 
