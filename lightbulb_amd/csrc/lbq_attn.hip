@@ -14,29 +14,29 @@ struct Layout {
     size_t part_bytes;  // per split
 };
 
-// Which forms a call needs and into how many parts each cuts a sequence's keys: as many as
-// give every CU two workgroups of four waves, while a part keeps a step of 64 keys for each
-// wave (short form) or four steps (long form, whose parts pay for their queries and outputs).
-// The batch's real lengths are on the device: the counts go by the bounds that the caller gave.
+// Which forms a call needs and into how many parts each cuts a sequence's keys.  The batch's real
+// lengths are on the device: the counts go by the bounds that the caller gave.
 Layout layout(const KvAttention &a) {
     Layout l = {};
     const int64_t group = a.q_heads / a.c.kv_heads, t = a.s.num_tokens;
     const int64_t most = a.max_new ? std::min<int64_t>(a.max_new, t) : t;
     l.plan.group = (int)group;
-    // one form serves every sequence where all have the same number of rows, or there is one;
-    // else each takes its own (a launch that finds none of its kind costs about 2 us, a single
-    // token in the long form a tile of 128 rows)
-    const bool same = a.s.batch == 1 || (a.max_new && most * a.s.batch == t);
-    l.any_short = group <= attn::SHORT_ROWS && !(same && most * group > attn::SHORT_ROWS);
+    // the short form takes sequences of up to 16 rows, unless all have more (the long form then
+    // takes whatever is there)
+    const bool same = a.max_new && most * a.s.batch == t;
     l.any_long = most * group > attn::SHORT_ROWS;
+    l.any_short = group <= attn::SHORT_ROWS && !(same && l.any_long);
     l.plan.short_rows = l.any_short ? attn::SHORT_ROWS : 0;
     l.plan.tiles = (int)(t * group / attn::LONG_ROWS + a.s.batch);
-    const int64_t want = 2 * num_cus(), steps = (a.max_len + attn::TILE - 1) / attn::TILE;
-    auto splits = [&](int64_t groups, int64_t least) {
+    const int64_t cus = num_cus(), steps = (a.max_len + attn::TILE - 1) / attn::TILE;
+    const auto splits = [&](int64_t groups, int64_t want, int64_t least) {
         return (int)std::max<int64_t>(1, std::min({(want + groups - 1) / groups, steps / least, (int64_t)128}));
     };
-    l.plan.splits_short = l.any_short ? splits(std::min<int64_t>(a.s.batch, t) * a.c.kv_heads, attn::SHORT_WAVES) : 1;
-    l.plan.splits_long = l.any_long ? splits((t * group / attn::LONG_ROWS + 1) * a.c.kv_heads, 4) : 1;
+    const int64_t rows = std::min<int64_t>(a.s.batch, t) * a.c.kv_heads;
+    const int waves = l.any_long ? attn::LONG_WAVES : a.c.head_dim <= 128 ? 8 : 4, per_cu = a.c.head_dim <= 128 ? 8 / waves : 1;
+    l.plan.splits_short = l.any_short ? splits(rows, per_cu * cus, 2 * waves) : 1;
+    const int64_t tiles = (t * group / attn::LONG_ROWS + 1) * a.c.kv_heads;
+    l.plan.splits_long = l.any_long && tiles < cus ? splits(tiles, 2 * cus, 4) : 1;
     l.part_bytes = (size_t)t * a.q_heads * (a.c.head_dim + 2) * sizeof(float);
     return l;
 }

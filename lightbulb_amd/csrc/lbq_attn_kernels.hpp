@@ -184,17 +184,20 @@ __device__ __forceinline__ float part_weight(float m, float l, float top) { retu
 // (c, n) = (lane / 16, lane % 16) holds keys 16 c .. 16 c + 15 of the 64 for row n, which is
 // what the products with V take, and all of one page: one scale per lane.
 // ---------------------------------------------------------------------------
-constexpr int SHORT_WAVES = 4;
+template <int D, int WAVES>
+constexpr size_t short_lds() { return sizeof(float) * WAVES * SHORT_ROWS * (D + 4 + 2); }
 
-template <int D, int KIND, int DT>
-__global__ __launch_bounds__(64 * SHORT_WAVES, D <= 128 ? 2 : 1) void k_attn_short(KvAttention a, AttnPlan plan) {
+// group: its place among the form's workgroups (parts * kv heads * sequences); lds: short_lds bytes
+template <int D, int KIND, int DT, int WAVES>
+__device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan &plan, int group, float *lds) {
     constexpr int NS = DT == DT_F32 ? 2 : 1;
     constexpr int STEPS = D / 32, DB = D / 16;
-    __shared__ float s_o[SHORT_WAVES][SHORT_ROWS][D + 4];
-    __shared__ float s_m[SHORT_WAVES][SHORT_ROWS], s_l[SHORT_WAVES][SHORT_ROWS];
+    float(*const s_o)[SHORT_ROWS][D + 4] = reinterpret_cast<float(*)[SHORT_ROWS][D + 4]>(lds);
+    float(*const s_m)[SHORT_ROWS] = reinterpret_cast<float(*)[SHORT_ROWS]>(lds + WAVES * SHORT_ROWS * (D + 4));
+    float(*const s_l)[SHORT_ROWS] = s_m + WAVES;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, c = lane >> 4;
     const int H = a.c.kv_heads, P = a.c.page_size, lp = a.c.log2_page;
-    const int h = blockIdx.x % H, split = blockIdx.x / H % plan.splits_short, b = blockIdx.x / H / plan.splits_short;
+    const int h = group % H, split = group / H % plan.splits_short, b = group / H / plan.splits_short;
     Sequence sq;
     if (!sequence_of(a, b, sq) || sq.n * plan.group > plan.short_rows) return;
     const int rows = sq.n * plan.group;
@@ -205,7 +208,7 @@ __global__ __launch_bounds__(64 * SHORT_WAVES, D <= 128 ? 2 : 1) void k_attn_sho
     seen_range(a, sq, sq.first, first_lo, first_hi);
     seen_range(a, sq, sq.first + sq.n - 1, last_lo, last_hi);
     if (!mine) hi = 0;
-    // this part's steps of 64 keys: every SHORT_WAVES-th is this wave's
+    // this part's steps of 64 keys: every WAVES-th is this wave's
     const int t_lo = first_lo / TILE, t_hi = (last_hi + TILE - 1) / TILE;
     const int per = max(t_hi - t_lo + plan.splits_short - 1, 0) / plan.splits_short;
     const int begin = t_lo + split * per, end = min(begin + per, t_hi);
@@ -290,12 +293,12 @@ __global__ __launch_bounds__(64 * SHORT_WAVES, D <= 128 ? 2 : 1) void k_attn_sho
     Loaded cur;
     int32_t vp = page_of(t, c), kp = page_of(t, kg);
     if (t < end) load(cur, t, kp, vp);
-    int32_t vp_next = page_of(t + SHORT_WAVES, c), kp_next = page_of(t + SHORT_WAVES, kg);
-    for (; t < end; t += SHORT_WAVES) {
+    int32_t vp_next = page_of(t + WAVES, c), kp_next = page_of(t + WAVES, kg);
+    for (; t < end; t += WAVES) {
         Loaded next;
-        const bool more = t + SHORT_WAVES < end;
-        if (more) load(next, t + SHORT_WAVES, kp_next, vp_next);
-        const int32_t vp_far = page_of(t + 2 * SHORT_WAVES, c), kp_far = page_of(t + 2 * SHORT_WAVES, kg);
+        const bool more = t + WAVES < end;
+        if (more) load(next, t + WAVES, kp_next, vp_next);
+        const int32_t vp_far = page_of(t + 2 * WAVES, c), kp_far = page_of(t + 2 * WAVES, kg);
 
         const int key = t * TILE;
         float x[16];
@@ -379,13 +382,13 @@ __global__ __launch_bounds__(64 * SHORT_WAVES, D <= 128 ? 2 : 1) void k_attn_sho
     if (c == 0) s_m[wave][n] = m, s_l[wave][n] = l;
     __syncthreads();
     const int64_t all = a.num_q * a.q_heads;
-    for (int i = threadIdx.x; i < rows * (D / 4); i += 64 * SHORT_WAVES) {
+    for (int i = threadIdx.x; i < rows * (D / 4); i += 64 * WAVES) {
         const int row = i / (D / 4), d = i % (D / 4) * 4;
         float top = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < SHORT_WAVES; w++) top = fmaxf(top, s_m[w][row]);
+        for (int w = 0; w < WAVES; w++) top = fmaxf(top, s_m[w][row]);
 #pragma unroll
-        for (int w = 0; w < SHORT_WAVES; w++) {
+        for (int w = 0; w < WAVES; w++) {
             const float f = part_weight(s_m[w][row], s_l[w][row], top);
             sum += f;
 #pragma unroll
@@ -404,6 +407,17 @@ __global__ __launch_bounds__(64 * SHORT_WAVES, D <= 128 ? 2 : 1) void k_attn_sho
     }
 }
 
+// Waves of a workgroup where all sequences are short: as many as the registers allow on a CU, so
+// that most batches need no parts and no join.
+template <int D>
+constexpr int SHORT_WAVES = D <= 128 ? 8 : 4;
+
+template <int D, int KIND, int DT>
+__global__ __launch_bounds__(64 * SHORT_WAVES<D>, D <= 128 ? 2 : 1) void k_attn_short(KvAttention a, AttnPlan plan) {
+    extern __shared__ __align__(16) float lds_f[];
+    attn_short<D, KIND, DT, SHORT_WAVES<D>>(a, plan, blockIdx.x, lds_f);
+}
+
 // ---------------------------------------------------------------------------
 // Long form: 128 query rows of one kv head (row i * group + head: neighbouring tokens see
 // nearly the same keys), 32 for each of four waves.  Bound by the matrix cores and by the
@@ -418,18 +432,17 @@ constexpr int LONG_ROWS = 128, LONG_WAVES = 4;
 template <int D>
 constexpr int long_lds_halves() { return TILE * (D + 8) + D * (TILE + 8); }
 
+// group: its place among the form's workgroups (tiles * kv heads * parts); lds: two buffers of long_lds_halves
 template <int D, int KIND, int DT>
-__global__ __launch_bounds__(64 * LONG_WAVES, D <= 128 ? 2 : 1) void k_attn_long(KvAttention a, AttnPlan plan) {
+__device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &plan, int group, _Float16 *lds) {
     constexpr int NS = DT == DT_F32 ? 2 : 1;
     constexpr int STEPS = D / 16, DB = D / 32;
     constexpr int KROW = D + 8, VROW = TILE + 8;
     constexpr int CHUNKS = TILE * D / 16, PER = (CHUNKS + 64 * LONG_WAVES - 1) / (64 * LONG_WAVES);  // 16-code chunks, of K and of V
-    extern __shared__ _Float16 lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, hf = lane >> 5;
     const int H = a.c.kv_heads, P = a.c.page_size, lp = a.c.log2_page;
-    const int h = blockIdx.x % H;
     // the tiles with most keys (a sequence's last) first
-    const int tile = plan.tiles - 1 - blockIdx.x / H, split = blockIdx.y;
+    const int h = group % H, split = group / H % plan.splits_long, tile = plan.tiles - 1 - group / H / plan.splits_long;
     const int b = find_sequence(a.s.batch, tile, [&](int i) { return (int64_t)a.cu_q[i] * plan.group / LONG_ROWS + i; });
     Sequence sq;
     if (!sequence_of(a, b, sq) || sq.n * plan.group <= plan.short_rows) return;
@@ -561,15 +574,28 @@ __global__ __launch_bounds__(64 * LONG_WAVES, D <= 128 ? 2 : 1) void k_attn_long
         if (key < w_last_hi && key + TILE > w_first_lo) {  // (else no row of this wave sees any of it)
             f32x16 s[2];
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
+            for (int i = 0; i < 2; i++)
 #pragma unroll
                 for (int j = 0; j < 16; j++) s[i][j] = 0.f;
+            // Four operands at a time, the next four read before the products of the last: left to
+            // itself the compiler reads each right before its product and waits for it.
+            half8 k8[2][4];
+            auto read_keys = [&](int g) {  // k dimension 2 g and 2 g + 1, both blocks of 32 keys
 #pragma unroll
-                for (int j = 0; j < STEPS; j++) {
-                    const half8 k8 = *reinterpret_cast<const half8 *>(kb + (32 * i + n) * KROW + 16 * j + 8 * hf);
+                for (int z = 0; z < 4; z++)
+                    k8[g & 1][z] = *reinterpret_cast<const half8 *>(kb + (32 * (z & 1) + n) * KROW + 16 * (2 * g + z / 2) + 8 * hf);
+            };
+            read_keys(0);
 #pragma unroll
-                    for (int u = NS - 1; u >= 0; u--) s[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, q[j][u], s[i], 0, 0, 0);
-                }
+            for (int g = 0; g < STEPS / 2; g++) {
+                if (g + 1 < STEPS / 2) read_keys(g + 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int z = 0; z < 4; z++)
+#pragma unroll
+                    for (int u = NS - 1; u >= 0; u--)
+                        s[z & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[g & 1][z], q[2 * g + z / 2][u], s[z & 1], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
             }
             // s[i][j] is key 16 u + 8 hf + 4 (j / 4 % 2) + j % 4 of the step, u = 2 i + j / 8
             const float vmax = fmaxf(fmaxf(from_lane(sc.v, 0), from_lane(sc.v, 1)), fmaxf(from_lane(sc.v, 2), from_lane(sc.v, 3)));
@@ -623,8 +649,10 @@ __global__ __launch_bounds__(64 * LONG_WAVES, D <= 128 ? 2 : 1) void k_attn_long
                 m = top;
             }
             const float base = base_of(m) - 15.f;
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
+            // The weights of one group of keys are formed between the products of the one before,
+            // whose operands are read a group ahead.
+            half8 p[2][NS], v8[2][DB];
+            auto weigh = [&](int u) {
                 const float at = base - lv[u];
                 float w[8], sum = 0.f;
 #pragma unroll
@@ -633,14 +661,32 @@ __global__ __launch_bounds__(64 * LONG_WAVES, D <= 128 ? 2 : 1) void k_attn_long
                     sum += w[j];
                 }
                 l = fmaf(sum, back[u], l);
-                half8 p[NS];
-                parts8<NS>(w, p);
+                parts8<NS>(w, p[u & 1]);
+            };
+            auto read_values = [&](int u) {
 #pragma unroll
-                for (int i = 0; i < DB; i++) {
-                    const half8 v8 = *reinterpret_cast<const half8 *>(vb + (32 * i + n) * VROW + 16 * u + 8 * hf);
+                for (int i = 0; i < DB; i++) v8[u & 1][i] = *reinterpret_cast<const half8 *>(vb + (32 * i + n) * VROW + 16 * u + 8 * hf);
+            };
+            read_values(0);
+            weigh(0);
 #pragma unroll
-                    for (int z = NS - 1; z >= 0; z--) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, p[z], o[i], 0, 0, 0);
+            for (int u = 0; u < 4; u++) {
+                if (u < 3) read_values(u + 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int z = NS - 1; z >= 0; z--)
+#pragma unroll
+                    for (int i = 0; i < DB; i++) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[u & 1][i], p[u & 1][z], o[i], 0, 0, 0);
+                if (u < 3) {
+                    weigh(u + 1);
+                    constexpr int MFMA = 0x8, VALU = 0x2, TRANS = 0x400;
+#pragma unroll
+                    for (int i = 0; i < DB * NS; i++) {
+                        __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(VALU | TRANS, 32 / (DB * NS) + 1, 0);
+                    }
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
         if (t + 1 < end) stage(t + 1, next, lds + (buf ^ 1) * long_lds_halves<D>());
@@ -666,6 +712,15 @@ __global__ __launch_bounds__(64 * LONG_WAVES, D <= 128 ? 2 : 1) void k_attn_long
             if (plan.splits_long == 1) store_values4<DT>(a.out, out * D + d, v);
             else *reinterpret_cast<f32x4 *>(plan.part + at * D + d) = f32x4{v[0], v[1], v[2], v[3]};
         }
+}
+
+// Both forms in one launch, each sequence in its own: short_groups workgroups of the short form,
+// which are the first to start (a long context's single token takes longest), then the long form's.
+template <int D, int KIND, int DT>
+__global__ __launch_bounds__(64 * LONG_WAVES, D <= 128 ? 2 : 1) void k_attn_mixed(KvAttention a, AttnPlan plan, int short_groups) {
+    extern __shared__ __align__(16) _Float16 lds_h[];
+    if ((int)blockIdx.x < short_groups) attn_short<D, KIND, DT, LONG_WAVES>(a, plan, blockIdx.x, reinterpret_cast<float *>(lds_h));
+    else attn_long<D, KIND, DT>(a, plan, blockIdx.x - short_groups, lds_h);
 }
 
 // The join of a row's parts, D / 4 threads a row: few parts, a row for each group of threads; many,
@@ -724,22 +779,22 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_attn_join(KvAttention a, AttnP
 
 template <int D, int KIND, int DT>
 hipError_t launch_typed(const KvAttention &a, const AttnPlan &plan, bool any_short, bool any_long, hipStream_t st) {
-    if (any_long) {
-        const size_t lds = 2 * sizeof(_Float16) * long_lds_halves<D>();
-        auto k = k_attn_long<D, KIND, DT>;
+    const int short_groups = any_short ? plan.splits_short * a.c.kv_heads * a.s.batch : 0;
+    const auto launch = [&](auto k, int groups, int threads, size_t lds, auto... more) {
         if (lds > 65536) {
             hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
             if (e != hipSuccess) return e;
         }
-        k<<<dim3((unsigned)(plan.tiles * a.c.kv_heads), (unsigned)plan.splits_long), 64 * LONG_WAVES, lds, st>>>(a, plan);
-        hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-    }
-    if (any_short) {
-        k_attn_short<D, KIND, DT><<<dim3((unsigned)(plan.splits_short * a.c.kv_heads * a.s.batch)), 64 * SHORT_WAVES, 0, st>>>(a, plan);
-        hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-    }
+        k<<<dim3((unsigned)groups), threads, lds, st>>>(a, plan, more...);
+        return hipGetLastError();
+    };
+    hipError_t e = hipSuccess;
+    if (any_long)
+        e = launch(k_attn_mixed<D, KIND, DT>, short_groups + plan.tiles * a.c.kv_heads * plan.splits_long, 64 * LONG_WAVES,
+                   std::max(2 * sizeof(_Float16) * long_lds_halves<D>(), short_lds<D, LONG_WAVES>()), short_groups);
+    else if (any_short)
+        e = launch(k_attn_short<D, KIND, DT>, short_groups, 64 * SHORT_WAVES<D>, short_lds<D, SHORT_WAVES<D>>());
+    if (e != hipSuccess) return e;
     const int splits = std::max(any_long ? plan.splits_long : 1, any_short ? plan.splits_short : 1);
     const int64_t rows = a.num_q * a.q_heads;
     if (splits > JOIN_GROUPS<D>) k_attn_join<D, DT, true><<<dim3((unsigned)rows), JOIN_THREADS, 0, st>>>(a, plan);
