@@ -492,22 +492,28 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
 
     const int32_t *table = a.s.tables + b * a.s.table_stride;
     const int64_t page_bytes = (int64_t)P * D;
-    struct Pages {  // of the step's four 16-key groups; -1: none to see
+    // Pages of the step's four 16-key groups, -1: none to see.  Read by lanes (lane i that of group
+    // i mod 4) and not by the scalar unit, whose loads come back in no order among the LDS
+    // reads: every wait for an operand would wait for them too.
+    struct Pages {
         int32_t p0, p1, p2, p3;
         __device__ int32_t of(int i) const {
             const int32_t a0 = p0, a1 = p1, a2 = p2, a3 = p3;  // (values: a choice of members would be one of addresses)
             const int32_t lo = i & 1 ? a1 : a0, hi = i & 1 ? a3 : a2;
             return i & 2 ? hi : lo;
         }
-        __device__ bool all() const { return p0 >= 0 && p1 >= 0 && p2 >= 0 && p3 >= 0; }
+        __device__ bool all() const { return (p0 | p1 | p2 | p3) >= 0; }
     };
-    auto page_of = [&](int t, int g) {
-        const int key = t * TILE + 16 * g;
+    auto page_of_lane = [&](int t) {
+        const int key = t * TILE + 16 * (lane & 3);
         int32_t p = -1;
         if (t < end && key < last_hi) p = table[key >> lp];
         return p >= 0 && p < a.c.num_pages ? p : -1;
     };
-    auto pages_of = [&](int t) { return Pages{page_of(t, 0), page_of(t, 1), page_of(t, 2), page_of(t, 3)}; };
+    auto pages_of = [](int32_t lanes) {
+        return Pages{__builtin_amdgcn_readlane(lanes, 0), __builtin_amdgcn_readlane(lanes, 1), __builtin_amdgcn_readlane(lanes, 2),
+                     __builtin_amdgcn_readlane(lanes, 3)};
+    };
     u32x4 kc[PER], vc[PER];
     auto load = [&](int t, const Pages &g) {
         const int key = t * TILE;
@@ -528,8 +534,7 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
     struct Scales {
         float k, v;
     };
-    auto scales_of = [&](const Pages &g) {
-        const int32_t p = g.of(lane & 3);
+    auto scales_of = [&](int32_t p) {
         const int64_t at = (int64_t)max(p, 0) * H + h;
         return Scales{a.c.ks[at], p >= 0 ? a.c.vs[at] : 0.f};
     };
@@ -557,8 +562,10 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
         }
     };
 
-    Pages now = pages_of(begin), next = pages_of(begin + 1);
-    Scales sc = scales_of(now);
+    int32_t next_lane = page_of_lane(begin);
+    Pages now = pages_of(next_lane);
+    Scales sc = scales_of(next_lane);
+    next_lane = page_of_lane(begin + 1);
     int buf = 0;
     if (begin < end) {
         load(begin, now);
@@ -566,9 +573,10 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
     }
     __syncthreads();
     for (int t = begin; t < end; t++, buf ^= 1) {
+        const Pages next = pages_of(next_lane);
         if (t + 1 < end) load(t + 1, next);
-        const Scales sc_next = scales_of(next);
-        const Pages far = pages_of(t + 2);
+        const Scales sc_next = scales_of(next_lane);
+        next_lane = page_of_lane(t + 2);
         const _Float16 *const kb = lds + buf * long_lds_halves<D>(), *const vb = kb + TILE * KROW;
         const int key = t * TILE;
         if (key < w_last_hi && key + TILE > w_first_lo) {  // (else no row of this wave sees any of it)
@@ -691,7 +699,6 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
         }
         if (t + 1 < end) stage(t + 1, next, lds + (buf ^ 1) * long_lds_halves<D>());
         now = next;
-        next = far;
         sc = sc_next;
         __syncthreads();
     }
