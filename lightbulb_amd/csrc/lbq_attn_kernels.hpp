@@ -30,7 +30,8 @@ struct AttnPlan {
     int splits_short, splits_long;  // parts that a sequence's keys are cut into
     float *part;                    // [splits][num_q][q_heads][head_dim] outputs of parts
     float *stat;                    // [splits][num_q][q_heads][2]: running maximum (log2), sum
-    int tiles;                      // 128-row tiles of the long form, an upper bound
+    int long_waves;                 // waves of the long form's workgroups, 32 rows each: 4 or 8
+    int tiles;                      // tiles of the long form, an upper bound
     int group;                      // query heads per kv head
     int short_rows;                 // rows (queries * group) up to which a sequence takes the short form; 0: none does
 };
@@ -419,35 +420,35 @@ __global__ __launch_bounds__(64 * SHORT_WAVES<D>, D <= 128 ? 2 : 1) void k_attn_
 }
 
 // ---------------------------------------------------------------------------
-// Long form: 128 query rows of one kv head (row i * group + head: neighbouring tokens see
-// nearly the same keys), 32 for each of four waves.  Bound by the matrix cores and by the
-// exponentials.  64 keys at a time are turned into f16 once for all four waves and kept in
+// Long form: 128 or 256 query rows of one kv head (row i * group + head: neighbouring tokens see
+// nearly the same keys), 32 for each of four or eight waves.  Bound by the matrix cores and by the
+// exponentials.  64 keys at a time are turned into f16 once for all waves and kept in
 // LDS, two buffers, the next step's codes on their way from memory meanwhile.  32x32x16
 // products; rows of K lie in LDS in the order in which lane (half, n) then holds keys
 // 16 u + 8 half + j of its row n, what the products with V take.  Both LDS arrays have rows of
 // an odd number of 16-byte chunks, so that eight lanes' reads of one column use all banks.
 // ---------------------------------------------------------------------------
-constexpr int LONG_ROWS = 128, LONG_WAVES = 4;
+constexpr int WAVE_ROWS = 32;
 
 template <int D>
 constexpr int long_lds_halves() { return TILE * (D + 8) + D * (TILE + 8); }
 
 // group: its place among the form's workgroups (tiles * kv heads * parts); lds: two buffers of long_lds_halves
-template <int D, int KIND, int DT>
+template <int D, int KIND, int DT, int WAVES>
 __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &plan, int group, _Float16 *lds) {
-    constexpr int NS = DT == DT_F32 ? 2 : 1;
+    constexpr int NS = DT == DT_F32 ? 2 : 1, ROWS = WAVE_ROWS * WAVES;
     constexpr int STEPS = D / 16, DB = D / 32;
     constexpr int KROW = D + 8, VROW = TILE + 8;
-    constexpr int CHUNKS = TILE * D / 16, PER = (CHUNKS + 64 * LONG_WAVES - 1) / (64 * LONG_WAVES);  // 16-code chunks, of K and of V
+    constexpr int CHUNKS = TILE * D / 16, PER = (CHUNKS + 64 * WAVES - 1) / (64 * WAVES);  // 16-code chunks, of K and of V
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, hf = lane >> 5;
     const int H = a.c.kv_heads, P = a.c.page_size, lp = a.c.log2_page;
     // the tiles with most keys (a sequence's last) first
     const int h = group % H, split = group / H % plan.splits_long, tile = plan.tiles - 1 - group / H / plan.splits_long;
-    const int b = find_sequence(a.s.batch, tile, [&](int i) { return (int64_t)a.cu_q[i] * plan.group / LONG_ROWS + i; });
+    const int b = find_sequence(a.s.batch, tile, [&](int i) { return (int64_t)a.cu_q[i] * plan.group / ROWS + i; });
     Sequence sq;
     if (!sequence_of(a, b, sq) || sq.n * plan.group <= plan.short_rows) return;
     const int rows = sq.n * plan.group;
-    const int row0 = (int)(tile - (sq.t0 * plan.group / LONG_ROWS + b)) * LONG_ROWS;
+    const int row0 = (int)(tile - (sq.t0 * plan.group / ROWS + b)) * ROWS;
     if (row0 < 0 || row0 >= rows) return;
     const int row = row0 + 32 * wave + n;
     const bool mine = row < rows;
@@ -455,7 +456,7 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
     int lo, hi, first_lo, first_hi, last_lo, last_hi, w_first_lo, w_first_hi, w_last_lo, w_last_hi;
     seen_range(a, sq, sq.first + tok, lo, hi);
     seen_range(a, sq, sq.first + row0 / plan.group, first_lo, first_hi);
-    seen_range(a, sq, sq.first + (min(row0 + LONG_ROWS, rows) - 1) / plan.group, last_lo, last_hi);
+    seen_range(a, sq, sq.first + (min(row0 + ROWS, rows) - 1) / plan.group, last_lo, last_hi);
     seen_range(a, sq, sq.first + min(row0 + 32 * wave, rows - 1) / plan.group, w_first_lo, w_first_hi);
     seen_range(a, sq, sq.first + min(row0 + 32 * wave + 31, rows - 1) / plan.group, w_last_lo, w_last_hi);
     const int t_lo = first_lo / TILE, t_hi = (last_hi + TILE - 1) / TILE;
@@ -519,8 +520,8 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
         const int key = t * TILE;
 #pragma unroll
         for (int i = 0; i < PER; i++) {
-            const int id = tid + 64 * LONG_WAVES * i;
-            if (CHUNKS % (64 * LONG_WAVES) == 0 || id < CHUNKS) {
+            const int id = tid + 64 * WAVES * i;
+            if (CHUNKS % (64 * WAVES) == 0 || id < CHUNKS) {
                 const int kt = id / (D / 16), kd = id % (D / 16) * 16;
                 const uint8_t *kp = a.c.k + ((int64_t)max(g.of(kt >> 4), 0) * H + h) * page_bytes;
                 kc[i] = *reinterpret_cast<const u32x4 *>(kp + ((key + kt) & (P - 1)) * D + kd);
@@ -545,8 +546,8 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
         const bool partial = (t + 1) * TILE > sq.len || !g.all();
 #pragma unroll
         for (int i = 0; i < PER; i++) {
-            const int id = tid + 64 * LONG_WAVES * i;
-            if (CHUNKS % (64 * LONG_WAVES) == 0 || id < CHUNKS) {
+            const int id = tid + 64 * WAVES * i;
+            if (CHUNKS % (64 * WAVES) == 0 || id < CHUNKS) {
                 const int kt = id / (D / 16), kd = id % (D / 16) * 16;
                 // key 32 b + 16 a1 + 8 half + 4 a0 + j is row 32 b + 16 a1 + 8 a0 + 4 half + j
                 const int kr = (kt & 0x33) | (kt & 8) >> 1 | (kt & 4) << 1;
@@ -723,11 +724,11 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
 
 // Both forms in one launch, each sequence in its own: short_groups workgroups of the short form,
 // which are the first to start (a long context's single token takes longest), then the long form's.
-template <int D, int KIND, int DT>
-__global__ __launch_bounds__(64 * LONG_WAVES, D <= 128 ? 2 : 1) void k_attn_mixed(KvAttention a, AttnPlan plan, int short_groups) {
+template <int D, int KIND, int DT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void k_attn_mixed(KvAttention a, AttnPlan plan, int short_groups) {
     extern __shared__ __align__(16) _Float16 lds_h[];
-    if ((int)blockIdx.x < short_groups) attn_short<D, KIND, DT, LONG_WAVES>(a, plan, blockIdx.x, reinterpret_cast<float *>(lds_h));
-    else attn_long<D, KIND, DT>(a, plan, blockIdx.x - short_groups, lds_h);
+    if ((int)blockIdx.x < short_groups) attn_short<D, KIND, DT, WAVES>(a, plan, blockIdx.x, reinterpret_cast<float *>(lds_h));
+    else attn_long<D, KIND, DT, WAVES>(a, plan, blockIdx.x - short_groups, lds_h);
 }
 
 // The join of a row's parts, D / 4 threads a row: few parts, a row for each group of threads; many,
@@ -796,10 +797,16 @@ hipError_t launch_typed(const KvAttention &a, const AttnPlan &plan, bool any_sho
         return hipGetLastError();
     };
     hipError_t e = hipSuccess;
-    if (any_long)
-        e = launch(k_attn_mixed<D, KIND, DT>, short_groups + plan.tiles * a.c.kv_heads * plan.splits_long, 64 * LONG_WAVES,
-                   std::max(2 * sizeof(_Float16) * long_lds_halves<D>(), short_lds<D, LONG_WAVES>()), short_groups);
-    else if (any_short)
+    const auto mixed = [&](auto k, int waves, size_t short_bytes) {
+        return launch(k, short_groups + plan.tiles * a.c.kv_heads * plan.splits_long, 64 * waves,
+                      std::max(2 * sizeof(_Float16) * long_lds_halves<D>(), short_bytes), short_groups);
+    };
+    if (any_long) {
+        if constexpr (D <= 128)
+            e = plan.long_waves == 8 ? mixed(k_attn_mixed<D, KIND, DT, 8>, 8, short_lds<D, 8>()) : mixed(k_attn_mixed<D, KIND, DT, 4>, 4, short_lds<D, 4>());
+        else
+            e = mixed(k_attn_mixed<D, KIND, DT, 4>, 4, short_lds<D, 4>());
+    } else if (any_short)
         e = launch(k_attn_short<D, KIND, DT>, short_groups, 64 * SHORT_WAVES<D>, short_lds<D, SHORT_WAVES<D>>());
     if (e != hipSuccess) return e;
     const int splits = std::max(any_long ? plan.splits_long : 1, any_short ? plan.splits_short : 1);
