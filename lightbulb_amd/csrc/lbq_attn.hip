@@ -27,21 +27,18 @@ Layout layout(const KvAttention &a) {
     l.any_long = most * group > attn::SHORT_ROWS;
     l.any_short = group <= attn::SHORT_ROWS && !(same && l.any_long);
     l.plan.short_rows = l.any_short ? attn::SHORT_ROWS : 0;
-    // Eight waves share the codes' conversion where a sequence's rows fill more than four
-    // (and the registers allow it)
-    const bool small = a.c.head_dim <= 128;
-    l.plan.long_waves = small && t * group > (int64_t)a.s.batch * 4 * attn::WAVE_ROWS ? 8 : 4;
-    const int64_t tile_rows = attn::WAVE_ROWS * l.plan.long_waves;
+    // waves of a workgroup, in either form and also all that a CU holds
+    const int waves = a.c.head_dim <= 128 ? 8 : 4;
+    const int64_t tile_rows = attn::WAVE_ROWS * waves;
     l.plan.tiles = (int)(t * group / tile_rows + a.s.batch);
+    // parts: enough workgroups for every CU, while a part keeps `least` steps of 64 keys
     const int64_t cus = num_cus(), steps = (a.max_len + attn::TILE - 1) / attn::TILE;
-    const auto splits = [&](int64_t groups, int64_t want, int64_t least) {
-        return (int)std::max<int64_t>(1, std::min({(want + groups - 1) / groups, steps / least, (int64_t)128}));
+    const auto splits = [&](int64_t groups, int64_t least) {
+        return (int)std::max<int64_t>(1, std::min({(cus + groups - 1) / groups, steps / least, (int64_t)128}));
     };
-    const int64_t rows = std::min<int64_t>(a.s.batch, t) * a.c.kv_heads;
-    const int waves = l.any_long ? l.plan.long_waves : small ? 8 : 4, slots = small ? 8 : 4;  // of a CU
-    l.plan.splits_short = l.any_short ? splits(rows, slots / waves * cus, (l.any_long ? 8 : 2) * waves) : 1;
-    const int64_t tiles = (t * group / tile_rows + 1) * a.c.kv_heads, fill = slots / l.plan.long_waves * cus;
-    l.plan.splits_long = l.any_long && 2 * tiles < fill ? splits(tiles, fill, 4) : 1;
+    l.plan.splits_short = l.any_short ? splits(std::min<int64_t>(a.s.batch, t) * a.c.kv_heads, (l.any_long ? 8 : 2) * waves) : 1;
+    const int64_t tiles = (t * group / tile_rows + 1) * a.c.kv_heads;
+    l.plan.splits_long = l.any_long && 2 * tiles < cus ? splits(tiles, 4) : 1;
     l.part_bytes = (size_t)t * a.q_heads * (a.c.head_dim + 2) * sizeof(float);
     return l;
 }

@@ -11,10 +11,11 @@
 // accumulator layout of S^T (column = lane mod 16 or 32, rows in registers) is already the operand
 // layout of P^T once the rows of K are taken in the right order.  Weights never leave registers.
 //
-// Weights carry a factor 2^15 (they are at most 1), which keeps both their f16 parts clear of the
-// subnormals; the row's sum carries it too.  Value scales are applied to the weights relative to
-// the largest one so far, rounded up to a power of two (r): weights stay at most 2^15 and the
-// accumulators are rescaled where r grows, as where the running maximum does.
+// Weights are exponentials relative to a base that follows the running maximum and is moved only
+// when the maximum is 2^6 above it (moving it multiplies all accumulators).  They carry a factor 2^9,
+// so that they stay below 2^15 and both their f16 parts of those that matter clear of the
+// subnormals; the row's sum carries it too.  Value scales are applied to the weights, inside the
+// exponential, relative to a power of two r that no scale seen so far exceeds.
 #pragma once
 #include "lbq_kv.hpp"
 
@@ -30,7 +31,6 @@ struct AttnPlan {
     int splits_short, splits_long;  // parts that a sequence's keys are cut into
     float *part;                    // [splits][num_q][q_heads][head_dim] outputs of parts
     float *stat;                    // [splits][num_q][q_heads][2]: running maximum (log2), sum
-    int long_waves;                 // waves of the long form's workgroups, 32 rows each: 4 or 8
     int tiles;                      // tiles of the long form, an upper bound
     int group;                      // query heads per kv head
     int short_rows;                 // rows (queries * group) up to which a sequence takes the short form; 0: none does
@@ -73,6 +73,9 @@ __device__ __forceinline__ void store_values4(void *p, int64_t i, const float *v
         for (int j = 0; j < 4; j++) o[j] = __float2bfloat16(v[j]);
     }
 }
+
+// weights carry 2^WEIGHT_LOG2, and their base is moved when the maximum is LAZY_LOG2 above it
+constexpr float WEIGHT_LOG2 = 9.f, LAZY_LOG2 = 6.f;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 // a maximum as the base of exponents: 0 where nothing was seen, so that no inf - inf is formed
@@ -138,25 +141,33 @@ __device__ __forceinline__ int scale_ceiling(float s) { return min(max(__builtin
 
 // what a sequence's rows see, and where its queries lie
 struct Sequence {
-    int64_t t0;      // first query row
-    int n;           // its queries
-    int64_t len;     // keys that can be seen at all
-    int64_t first;   // position of the first query
+    int t0;     // first query row
+    int n;      // its queries
+    int len;    // keys that can be seen at all
+    int first;  // position of the first query
 };
 __device__ __forceinline__ bool sequence_of(const KvAttention &a, int b, Sequence &s) {
-    const int64_t t0 = a.cu_q[b], t1 = a.cu_q[b + 1];
+    const int t0 = a.cu_q[b], t1 = a.cu_q[b + 1];
     if (t0 < 0 || t1 > a.num_q || t1 <= t0) return false;
     s.t0 = t0;
-    s.n = (int)(t1 - t0);
-    s.len = min((int64_t)a.s.seq_lens[b], a.max_len);
-    s.first = (int64_t)a.s.seq_lens[b] - s.n;
+    s.n = t1 - t0;
+    const int len = max(a.s.seq_lens[b], 0);
+    s.len = min(len, a.max_len);
+    s.first = len - s.n;
     return true;
 }
 
 // keys [lo, hi) that the query at position pos sees
-__device__ __forceinline__ void seen_range(const KvAttention &a, const Sequence &s, int64_t pos, int &lo, int &hi) {
-    hi = (int)max((int64_t)0, a.causal ? min(s.len, pos + 1) : s.len);
-    lo = a.causal && a.window > 0 ? (int)max((int64_t)0, pos - a.window + 1) : 0;
+__device__ __forceinline__ void seen_range(const KvAttention &a, const Sequence &s, int pos, int &lo, int &hi) {
+    hi = a.causal ? max(min(s.len, pos + 1), 0) : s.len;
+    lo = a.causal && a.window > 0 ? max(pos - a.window + 1, 0) : 0;
+}
+
+// x, or -infinity where j is outside [from, to).  On the vector unit alone: compares would hold a
+// pair of scalar registers for each value, and there are none left.
+__device__ __forceinline__ float seen_or_not(float x, int j, int from, int to) {
+    const uint32_t out = (uint32_t)(((j - from) | (to - 1 - j)) >> 31);
+    return __uint_as_float((out & 0xff800000u) | (~out & __float_as_uint(x)));
 }
 
 // The weights' factor for a value scale s, relative to r and in powers of two.  Below 2^-45 a
@@ -167,12 +178,9 @@ __device__ __forceinline__ float scale_log(float s, float inv_r) {
     return fmaf(s, 0.f, fmaxf(__builtin_amdgcn_logf(s * inv_r), -45.f));
 }
 
-// The factor of a key scale's products.  Not negative (the largest product has the largest logit),
-// and not 0, so that a product of -infinity, which stands for a key that is not seen, stays one.
-__device__ __forceinline__ float logit_factor(float scale, float factor) {
-    const float f = scale * factor;
-    return f == 0.f ? 0x1p-126f : f;
-}
+// A logit's factor where products of -infinity stand for keys that are not seen: not 0, which
+// would make them NaN.  (What it multiplies besides is below 2^33.)
+__device__ __forceinline__ float not_zero(float f) { return f == 0.f ? 0x1p-126f : f; }
 
 // The join of parts' outputs o_i with maxima m_i and sums l_i: weights l_i 2^(m_i - max).
 __device__ __forceinline__ float part_weight(float m, float l, float top) { return l * exp2_fast(m - base_of(top)); }
@@ -324,14 +332,15 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
             grown = r * inv_r;
             r = ldexpf(1.f, e);
         }
-        float f = logit_factor(cur.ks, factor), lv = scale_log(cur.vs, inv_r), back = exp2_fast(-lv);
+        float f = cur.ks * factor, lv = scale_log(cur.vs, inv_r), back = exp2_fast(-lv);  // f >= 0: the largest product has the largest logit
         if (key < last_lo || key + TILE > first_hi || __any(vp < 0)) {
             // some row does not see some of these keys, or they are not there
             const int from = lo - (key + 16 * c), to = vp >= 0 ? hi - (key + 16 * c) : 0;
 #pragma unroll
-            for (int j = 0; j < 16; j++) x[j] = j >= from && j < to ? x[j] : -INFINITY;
+            for (int j = 0; j < 16; j++) x[j] = seen_or_not(x[j], j, from, to);
+            f = not_zero(f);
             if (max(from, 0) >= min(to, 16)) f = 1.f, lv = 0.f, back = 1.f;  // none of them, so neither their scales
-            const int keep = vp >= 0 ? min(max((int)sq.len - (key + 16 * c), 0), 16) : 0;
+            const int keep = vp >= 0 ? min(max(sq.len - (key + 16 * c), 0), 16) : 0;
 #pragma unroll
             for (int i = 0; i < DB; i++) cur.v[i] = keep_bytes(cur.v[i], keep);
         }
@@ -341,14 +350,14 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
         top *= f;
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), m);
-        if (grown != 1.f || __any(top > m)) {
+        if (grown != 1.f || __any(top > m + LAZY_LOG2)) {
             const float alpha = exp2_fast(m - base_of(top)), g = alpha * grown;
             l *= alpha;
 #pragma unroll
             for (int i = 0; i < DB; i++) o[i] *= g;
             m = top;
         }
-        const float base = base_of(m) - 15.f - lv;
+        const float base = base_of(m) - WEIGHT_LOG2 - lv;
         float w[16], sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 16; j++) {
@@ -420,26 +429,39 @@ __global__ __launch_bounds__(64 * SHORT_WAVES<D>, D <= 128 ? 2 : 1) void k_attn_
 }
 
 // ---------------------------------------------------------------------------
-// Long form: 128 or 256 query rows of one kv head (row i * group + head: neighbouring tokens see
-// nearly the same keys), 32 for each of four or eight waves.  Bound by the matrix cores and by the
-// exponentials.  64 keys at a time are turned into f16 once for all waves and kept in
-// LDS, two buffers, the next step's codes on their way from memory meanwhile.  32x32x16
-// products; rows of K lie in LDS in the order in which lane (half, n) then holds keys
-// 16 u + 8 half + j of its row n, what the products with V take.  Both LDS arrays have rows of
-// an odd number of 16-byte chunks, so that eight lanes' reads of one column use all banks.
+// Long form: query rows of one kv head (row i * group + head: neighbouring tokens see nearly the
+// same keys), 32 for each wave.  Bound by the matrix cores and by the exponentials.  64 keys at a
+// time are turned into f16 once for all waves and kept in LDS, the next steps' codes on their
+// way from memory meanwhile.  32x32x16 products; rows of K lie in LDS in the order in which lane
+// (half, n) then holds keys 16 u + 8 half + j of its row n, what the products with V take.
+// LDS rows are an odd number of 16-byte chunks long, so that eight lanes' reads of one column
+// use all banks.
+//
+// Pages and scales of up to 256 steps are looked up at once, by all threads, and kept in LDS: offsets
+// of the pages' codes, key scales, value scales as they enter the exponential.  (Looked up step by
+// step they took a quarter of a step's time, most of it address arithmetic.)
+//
+// Up to 128 channels the registers allow two waves on a SIMD, and one's products run while the
+// other forms weights.  Above that there is one, and four in a workgroup.  In either case the
+// weights of 16 keys are formed between the products of the 16 before.
 // ---------------------------------------------------------------------------
 constexpr int WAVE_ROWS = 32;
+template <int D>
+constexpr int LONG_WAVES = D <= 128 ? 8 : 4;
+constexpr int TABLE_STEPS = 256, GROUPS = TILE / 16;  // steps looked up at once; groups of 16 keys in a step
 
 template <int D>
-constexpr int long_lds_halves() { return TILE * (D + 8) + D * (TILE + 8); }
+constexpr int buffer_halves() { return TILE * (D + 8) + D * (TILE + 8); }  // f16 of one step's K and V
+template <int D>
+constexpr size_t long_lds() { return 2 * sizeof(_Float16) * buffer_halves<D>() + TABLE_STEPS * GROUPS * (sizeof(uint64_t) + 3 * sizeof(float)); }
 
-// group: its place among the form's workgroups (tiles * kv heads * parts); lds: two buffers of long_lds_halves
-template <int D, int KIND, int DT, int WAVES>
+// group: its place among the form's workgroups (tiles * kv heads * parts); lds: long_lds bytes
+template <int D, int KIND, int DT>
 __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &plan, int group, _Float16 *lds) {
-    constexpr int NS = DT == DT_F32 ? 2 : 1, ROWS = WAVE_ROWS * WAVES;
+    constexpr int NS = DT == DT_F32 ? 2 : 1, WAVES = LONG_WAVES<D>, ROWS = WAVE_ROWS * WAVES, THREADS = 64 * WAVES;
     constexpr int STEPS = D / 16, DB = D / 32;
     constexpr int KROW = D + 8, VROW = TILE + 8;
-    constexpr int CHUNKS = TILE * D / 16, PER = (CHUNKS + 64 * WAVES - 1) / (64 * WAVES);  // 16-code chunks, of K and of V
+    constexpr int CHUNKS = TILE * D / 16, PER = (CHUNKS + THREADS - 1) / THREADS;  // 16-code chunks, of K and of V
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, hf = lane >> 5;
     const int H = a.c.kv_heads, P = a.c.page_size, lp = a.c.log2_page;
     // the tiles with most keys (a sequence's last) first
@@ -450,18 +472,30 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
     const int rows = sq.n * plan.group;
     const int row0 = (int)(tile - (sq.t0 * plan.group / ROWS + b)) * ROWS;
     if (row0 < 0 || row0 >= rows) return;
-    const int row = row0 + 32 * wave + n;
+    const int row = row0 + WAVE_ROWS * wave + n;
     const bool mine = row < rows;
     const int tok = (mine ? row : rows - 1) / plan.group, head = h * plan.group + (mine ? row : rows - 1) % plan.group;
-    int lo, hi, first_lo, first_hi, last_lo, last_hi, w_first_lo, w_first_hi, w_last_lo, w_last_hi;
+    int lo, hi;  // keys that this lane's row sees
     seen_range(a, sq, sq.first + tok, lo, hi);
-    seen_range(a, sq, sq.first + row0 / plan.group, first_lo, first_hi);
-    seen_range(a, sq, sq.first + (min(row0 + ROWS, rows) - 1) / plan.group, last_lo, last_hi);
-    seen_range(a, sq, sq.first + min(row0 + 32 * wave, rows - 1) / plan.group, w_first_lo, w_first_hi);
-    seen_range(a, sq, sq.first + min(row0 + 32 * wave + 31, rows - 1) / plan.group, w_last_lo, w_last_hi);
-    const int t_lo = first_lo / TILE, t_hi = (last_hi + TILE - 1) / TILE;
-    const int per = max(t_hi - t_lo + plan.splits_long - 1, 0) / plan.splits_long;
-    const int begin = t_lo + split * per, end = min(begin + per, t_hi);
+    int begin, end;  // steps of this part
+    {
+        int first_lo, first_hi, last_lo, last_hi;
+        seen_range(a, sq, sq.first + row0 / plan.group, first_lo, first_hi);
+        seen_range(a, sq, sq.first + (min(row0 + ROWS, rows) - 1) / plan.group, last_lo, last_hi);
+        const int t_lo = first_lo / TILE, t_hi = (last_hi + TILE - 1) / TILE;
+        const int per = max(t_hi - t_lo + plan.splits_long - 1, 0) / plan.splits_long;
+        begin = t_lo + split * per, end = min(begin + per, t_hi);
+    }
+    int see_lo, see_hi, all_lo, all_hi;  // steps of which any row of this wave sees a key; of which every row sees all
+    {
+        const int w0 = row0 + WAVE_ROWS * wave, w1 = min(w0 + WAVE_ROWS, rows) - 1;
+        int first_lo, first_hi, last_lo, last_hi;
+        seen_range(a, sq, sq.first + min(w0, rows - 1) / plan.group, first_lo, first_hi);
+        seen_range(a, sq, sq.first + w1 / plan.group, last_lo, last_hi);
+        see_lo = first_lo / TILE, see_hi = w0 < rows ? min((last_hi + TILE - 1) / TILE, end) : 0;
+        all_lo = (last_lo + TILE - 1) / TILE, all_hi = first_hi / TILE;
+    }
+    auto visible = [&](int t) { return t >= see_lo && t < see_hi; };
 
     half8 q[STEPS][NS];
     float factor;
@@ -469,239 +503,276 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
         const int64_t at = (sq.t0 + tok) * a.q.token_stride + (int64_t)head * a.q.head_stride + 8 * hf;
         float amax = 0.f;
 #pragma unroll
-        for (int s = 0; s < STEPS; s++)
+        for (int i = 0; i < STEPS; i++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) amax = fmaxf(amax, fabsf(load_value<DT>(a.q.p, at + 16 * s + j)));
+            for (int j = 0; j < 8; j++) amax = fmaxf(amax, fabsf(load_value<DT>(a.q.p, at + 16 * i + j)));
         amax = fmaxf(amax, __shfl_xor(amax, 32));
         const int e = row_exponent(amax);
 #pragma unroll
-        for (int s = 0; s < STEPS; s++) {
+        for (int i = 0; i < STEPS; i++) {
             float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = copysignf(1.f, a.scale) * ldexpf(load_value<DT>(a.q.p, at + 16 * s + j), 15 - e);
-            parts8<NS>(v, q[s]);
+            for (int j = 0; j < 8; j++) v[j] = copysignf(1.f, a.scale) * ldexpf(load_value<DT>(a.q.p, at + 16 * i + j), 15 - e);
+            parts8<NS>(v, q[i]);
         }
         factor = ldexpf(fabsf(a.scale) * 1.44269504088896340736f, e - 15);
     }
 
-    f32x16 o[DB];
+    f32x16 o[DB], s[2];
 #pragma unroll
     for (int i = 0; i < DB; i++)
 #pragma unroll
         for (int j = 0; j < 16; j++) o[i][j] = 0.f;
     float m = -INFINITY, l = 0.f, r = 0.f, inv_r = 1.f;
 
-    const int32_t *table = a.s.tables + b * a.s.table_stride;
-    const int64_t page_bytes = (int64_t)P * D;
-    // Pages of the step's four 16-key groups, -1: none to see.  Read by lanes (lane i that of group
-    // i mod 4) and not by the scalar unit, whose loads come back in no order among the LDS
-    // reads: every wait for an operand would wait for them too.
-    struct Pages {
-        int32_t p0, p1, p2, p3;
-        __device__ int32_t of(int i) const {
-            const int32_t a0 = p0, a1 = p1, a2 = p2, a3 = p3;  // (values: a choice of members would be one of addresses)
-            const int32_t lo = i & 1 ? a1 : a0, hi = i & 1 ? a3 : a2;
-            return i & 2 ? hi : lo;
+    // ---- the steps' pages and scales
+    _Float16 *const buffers = lds;
+    uint64_t *const s_at = reinterpret_cast<uint64_t *>(lds + 2 * buffer_halves<D>());  // bytes from the cache's start to the group's page
+    float *const s_k = reinterpret_cast<float *>(s_at + TABLE_STEPS * GROUPS);          // key scales, -1: the group is not there
+    float *const s_lv = s_k + TABLE_STEPS * GROUPS, *const s_back = s_lv + TABLE_STEPS * GROUPS;  // scale_log of value scales, and 2^-that
+    __shared__ float s_max[WAVES];
+    const int32_t *const table = a.s.tables + b * a.s.table_stride;
+    const int seen_end = min(end * TILE, sq.len);
+    // the entries of steps c0 .. c1 - 1; grown: r's growth, which the accumulators have to follow
+    auto look_up = [&](int c0, int c1, float &grown) {
+        const int n = (c1 - c0) * GROUPS;
+        float vmax = 0.f;
+        for (int i = tid; i < n; i += THREADS) {
+            const int key = c0 * TILE + 16 * i;
+            const int page = key < seen_end ? table[key >> lp] : -1;
+            const bool there = page >= 0 && page < a.c.num_pages;
+            const int64_t at = there ? (int64_t)page * H + h : 0;
+            const float v = there ? a.c.vs[at] : 0.f;
+            s_at[i] = at * (uint64_t)(P * D);
+            s_k[i] = there ? a.c.ks[at] : -1.f;
+            s_lv[i] = v;
+            vmax = fmaxf(vmax, v);
         }
-        __device__ bool all() const { return (p0 | p1 | p2 | p3) >= 0; }
+#pragma unroll
+        for (int d = 32; d; d /= 2) vmax = fmaxf(vmax, __shfl_xor(vmax, d));
+        if (lane == 0) s_max[wave] = vmax;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < WAVES; i++) vmax = fmaxf(vmax, s_max[i]);
+        grown = 1.f;
+        if (vmax > r) {  // (the same in every thread)
+            const int e = scale_ceiling(vmax);
+            inv_r = ldexpf(1.f, -e);
+            grown = r * inv_r;
+            r = ldexpf(1.f, e);
+        }
+        for (int i = tid; i < n; i += THREADS) {
+            const float lv = scale_log(s_lv[i], inv_r);
+            s_lv[i] = lv;
+            s_back[i] = exp2_fast(-lv);
+        }
+        __syncthreads();
     };
-    auto page_of_lane = [&](int t) {
-        const int key = t * TILE + 16 * (lane & 3);
-        int32_t p = -1;
-        if (t < end && key < last_hi) p = table[key >> lp];
-        return p >= 0 && p < a.c.num_pages ? p : -1;
+
+    // ---- codes on their way.  A thread has the same chunks of 16 codes in every step: of K key `kt`
+    // of the step, channels kd and on; of V channel `vd`, keys 16 vg and on.
+    struct Chunk {
+        int kt, kd, vg, vd;
+        bool on;
     };
-    auto pages_of = [](int32_t lanes) {
-        return Pages{__builtin_amdgcn_readlane(lanes, 0), __builtin_amdgcn_readlane(lanes, 1), __builtin_amdgcn_readlane(lanes, 2),
-                     __builtin_amdgcn_readlane(lanes, 3)};
+    auto chunk = [&](int i) {
+        const int id = tid + THREADS * i;
+        return Chunk{id / (D / 16), id % (D / 16) * 16, id & 3, id >> 2, CHUNKS % THREADS == 0 || id < CHUNKS};
     };
     u32x4 kc[PER], vc[PER];
-    auto load = [&](int t, const Pages &g) {
-        const int key = t * TILE;
+    uint64_t k_at[PER], v_at[PER];  // of the step to load next
+    auto read_places = [&](int i) {  // entry i of the table
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int id = tid + 64 * WAVES * i;
-            if (CHUNKS % (64 * WAVES) == 0 || id < CHUNKS) {
-                const int kt = id / (D / 16), kd = id % (D / 16) * 16;
-                const uint8_t *kp = a.c.k + ((int64_t)max(g.of(kt >> 4), 0) * H + h) * page_bytes;
-                kc[i] = *reinterpret_cast<const u32x4 *>(kp + ((key + kt) & (P - 1)) * D + kd);
-                const int vg = id & 3, vd = id >> 2;
-                const uint8_t *vp = a.c.v + ((int64_t)max(g.of(vg), 0) * H + h) * page_bytes;
-                vc[i] = *reinterpret_cast<const u32x4 *>(vp + vd * P + ((key + 16 * vg) & (P - 1)));
+        for (int j = 0; j < PER; j++) {
+            k_at[j] = s_at[GROUPS * i + (chunk(j).kt >> 4 & 3)];
+            v_at[j] = s_at[GROUPS * i + chunk(j).vg];
+        }
+    };
+    auto load = [&](int t) {
+        const int in_page = t * TILE & (P - 1);  // (pages of 128: the step is one half of one)
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const Chunk c = chunk(j);
+            if (c.on) {
+                kc[j] = *reinterpret_cast<const u32x4 *>(a.c.k + k_at[j] + ((in_page + (c.kt & (P - 1))) * D + c.kd));
+                vc[j] = *reinterpret_cast<const u32x4 *>(a.c.v + v_at[j] + (c.vd * P + in_page + (16 * c.vg & (P - 1))));
             }
         }
     };
-    // lane i holds the scales of group i mod 4
-    struct Scales {
-        float k, v;
-    };
-    auto scales_of = [&](int32_t p) {
-        const int64_t at = (int64_t)max(p, 0) * H + h;
-        return Scales{a.c.ks[at], p >= 0 ? a.c.vs[at] : 0.f};
-    };
-    auto from_lane = [](float x, int i) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), i)); };
-    // codes -> f16 in LDS; values behind the sequence's end, or of no page, as zeros
-    auto stage = [&](int t, const Pages &g, _Float16 *buf) {
-        _Float16 *const kb = buf, *const vb = buf + TILE * KROW;
-        const bool partial = (t + 1) * TILE > sq.len || !g.all();
+    // codes -> f16 in buffer `buf`.  Values behind the sequence's end, or of no page, as zeros: their
+    // weights are 0, but a code can be NaN.
+    auto stage = [&](int t, int i, int buf) {
+        _Float16 *const kb = buffers + buf * buffer_halves<D>(), *const vb = kb + TILE * KROW;
+        bool whole = (t + 1) * TILE <= sq.len;
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int id = tid + 64 * WAVES * i;
-            if (CHUNKS % (64 * WAVES) == 0 || id < CHUNKS) {
-                const int kt = id / (D / 16), kd = id % (D / 16) * 16;
+        for (int g = 0; g < GROUPS; g++) whole = whole && !(s_k[GROUPS * i + g] < 0.f);
+        if (!whole) {
+#pragma unroll
+            for (int j = 0; j < PER; j++) {
+                const int vg = chunk(j).vg;
+                vc[j] = keep_bytes(vc[j], s_k[GROUPS * i + vg] < 0.f ? 0 : min(max(sq.len - (t * TILE + 16 * vg), 0), 16));
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const Chunk c = chunk(j);
+            if (c.on) {
                 // key 32 b + 16 a1 + 8 half + 4 a0 + j is row 32 b + 16 a1 + 8 a0 + 4 half + j
-                const int kr = (kt & 0x33) | (kt & 8) >> 1 | (kt & 4) << 1;
-                half8 *const ko = reinterpret_cast<half8 *>(kb + kr * KROW + kd);
-                ko[0] = codes8<KIND>(kc[i][0], kc[i][1]);
-                ko[1] = codes8<KIND>(kc[i][2], kc[i][3]);
-                const int vg = id & 3, vd = id >> 2;
-                if (partial) vc[i] = keep_bytes(vc[i], g.of(vg) >= 0 ? min(max((int)sq.len - (t * TILE + 16 * vg), 0), 16) : 0);
-                half8 *const vo = reinterpret_cast<half8 *>(vb + vd * VROW + 16 * vg);
-                vo[0] = codes8<KIND>(vc[i][0], vc[i][1]);
-                vo[1] = codes8<KIND>(vc[i][2], vc[i][3]);
+                const int kr = (c.kt & 0x33) | (c.kt & 8) >> 1 | (c.kt & 4) << 1;
+                half8 *const ko = reinterpret_cast<half8 *>(kb + kr * KROW + c.kd);
+                ko[0] = codes8<KIND>(kc[j][0], kc[j][1]);
+                ko[1] = codes8<KIND>(kc[j][2], kc[j][3]);
+                half8 *const vo = reinterpret_cast<half8 *>(vb + c.vd * VROW + 16 * c.vg);
+                vo[0] = codes8<KIND>(vc[j][0], vc[j][1]);
+                vo[1] = codes8<KIND>(vc[j][2], vc[j][3]);
             }
         }
     };
 
-    int32_t next_lane = page_of_lane(begin);
-    Pages now = pages_of(next_lane);
-    Scales sc = scales_of(next_lane);
-    next_lane = page_of_lane(begin + 1);
-    int buf = 0;
-    if (begin < end) {
-        load(begin, now);
-        stage(begin, now, lds);
-    }
-    __syncthreads();
-    for (int t = begin; t < end; t++, buf ^= 1) {
-        const Pages next = pages_of(next_lane);
-        if (t + 1 < end) load(t + 1, next);
-        const Scales sc_next = scales_of(next_lane);
-        next_lane = page_of_lane(t + 2);
-        const _Float16 *const kb = lds + buf * long_lds_halves<D>(), *const vb = kb + TILE * KROW;
-        const int key = t * TILE;
-        if (key < w_last_hi && key + TILE > w_first_lo) {  // (else no row of this wave sees any of it)
-            f32x16 s[2];
+    // ---- products.  Operands in groups of up to four, the next group read before the products of
+    // the last: left to itself the compiler reads each right before its product and waits for it.
+    half8 fr[2][4], p[4][NS];
+    auto read_keys = [&](int g, const _Float16 *kb) {  // k dimensions 2 g and 2 g + 1, both blocks of 32 keys
 #pragma unroll
-            for (int i = 0; i < 2; i++)
+        for (int z = 0; z < 4; z++) fr[g & 1][z] = *reinterpret_cast<const half8 *>(kb + (32 * (z & 1) + n) * KROW + 16 * (2 * g + z / 2) + 8 * hf);
+    };
+    auto key_products = [&](const _Float16 *kb) {
 #pragma unroll
-                for (int j = 0; j < 16; j++) s[i][j] = 0.f;
-            // Four operands at a time, the next four read before the products of the last: left to
-            // itself the compiler reads each right before its product and waits for it.
-            half8 k8[2][4];
-            auto read_keys = [&](int g) {  // k dimension 2 g and 2 g + 1, both blocks of 32 keys
+        for (int i = 0; i < 2; i++)
 #pragma unroll
-                for (int z = 0; z < 4; z++)
-                    k8[g & 1][z] = *reinterpret_cast<const half8 *>(kb + (32 * (z & 1) + n) * KROW + 16 * (2 * g + z / 2) + 8 * hf);
-            };
-            read_keys(0);
+            for (int j = 0; j < 16; j++) s[i][j] = 0.f;
+        read_keys(0, kb);
 #pragma unroll
-            for (int g = 0; g < STEPS / 2; g++) {
-                if (g + 1 < STEPS / 2) read_keys(g + 1);
-                __builtin_amdgcn_sched_barrier(0);
+        for (int g = 0; g < STEPS / 2; g++) {
+            if (g + 1 < STEPS / 2) read_keys(g + 1, kb);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int z = 0; z < 4; z++)
+            for (int z = 0; z < 4; z++)
 #pragma unroll
-                    for (int u = NS - 1; u >= 0; u--)
-                        s[z & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[g & 1][z], q[2 * g + z / 2][u], s[z & 1], 0, 0, 0);
-                __builtin_amdgcn_sched_barrier(0);
+                for (int u = NS - 1; u >= 0; u--)
+                    s[z & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fr[g & 1][z], q[2 * g + z / 2][u], s[z & 1], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    constexpr int VG = DB <= 4 ? DB : DB / 2, VGROUPS = 4 * DB / VG;  // channel blocks in a group of operands of V
+    auto read_values = [&](int g, const _Float16 *vb) {
+#pragma unroll
+        for (int i = 0; i < VG; i++)
+            fr[g & 1][i] = *reinterpret_cast<const half8 *>(vb + (32 * (g % (DB / VG) * VG + i) + n) * VROW + 16 * (g / (DB / VG)) + 8 * hf);
+    };
+    auto value_products = [&](int g) {
+#pragma unroll
+        for (int z = NS - 1; z >= 0; z--)
+#pragma unroll
+            for (int i = 0; i < VG; i++) {
+                f32x16 &to = o[g % (DB / VG) * VG + i];
+                to = __builtin_amdgcn_mfma_f32_32x32x16_f16(fr[g & 1][i], p[g / (DB / VG)][z], to, 0, 0, 0);
             }
-            // s[i][j] is key 16 u + 8 hf + 4 (j / 4 % 2) + j % 4 of the step, u = 2 i + j / 8
-            const float vmax = fmaxf(fmaxf(from_lane(sc.v, 0), from_lane(sc.v, 1)), fmaxf(from_lane(sc.v, 2), from_lane(sc.v, 3)));
-            float grown = 1.f;
-            if (__any(vmax > r)) {
-                const int e = scale_ceiling(vmax);
-                inv_r = ldexpf(1.f, -e);
-                grown = r * inv_r;
-                r = ldexpf(1.f, e);
-            }
-            float f[4], lv[4], back[4];
-            {
-                const float mine_lv = scale_log(sc.v, inv_r), mine_back = exp2_fast(-mine_lv);
+    };
+
+    // ---- weights.  s[i][j] is key 16 u + 8 hf + 4 (j / 4 % 2) + j % 4 of the step, u = 2 i + j / 8
+    auto scale_outputs = [&](float by) {
 #pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    f[u] = logit_factor(from_lane(sc.k, u), factor);
-                    lv[u] = from_lane(mine_lv, u);
-                    back[u] = from_lane(mine_back, u);
-                }
-            }
-            if (key < w_last_lo || key + TILE > w_first_hi || !now.all()) {
-                // some row does not see some of these keys, or they are not there
-                const int from = lo - (key + 8 * hf), to = hi - (key + 8 * hf);
+        for (int i = 0; i < DB; i++)
 #pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    const int a0 = max(from - 16 * u, 0), a1 = now.of(u) >= 0 ? min(to - 16 * u, 8) : 0;
+            for (int j = 0; j < 16; j++) o[i][j] *= by;
+    };
+    float f[4], lv[4], back[4];
+    auto start_weights = [&](int t, int i) {  // entry i of the table
+        const f32x4 k4 = *reinterpret_cast<const f32x4 *>(s_k + GROUPS * i), lv4 = *reinterpret_cast<const f32x4 *>(s_lv + GROUPS * i);
+        const f32x4 back4 = *reinterpret_cast<const f32x4 *>(s_back + GROUPS * i);
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const float x = s[u / 2][8 * (u % 2) + j];
-                        s[u / 2][8 * (u % 2) + j] = j >= a0 && j < a1 ? x : -INFINITY;
-                    }
-                    if (a0 >= a1) f[u] = 1.f, lv[u] = 0.f, back[u] = 1.f;  // none of the group, so neither its scales
-                }
-            }
-            float top = -INFINITY;
+        for (int u = 0; u < 4; u++) {
+            f[u] = k4[u] * factor;  // not negative where a key is seen: the largest product has the largest logit
+            lv[u] = lv4[u];
+            back[u] = back4[u];
+        }
+        if (t < all_lo || t >= all_hi || __any(fminf(fminf(k4[0], k4[1]), fminf(k4[2], k4[3])) < 0.f)) {
+            // some row does not see some of these keys, or they are not there
+            const int from = lo - (t * TILE + 8 * hf), to = hi - (t * TILE + 8 * hf);
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                float x = s[u / 2][8 * (u % 2)];
-#pragma unroll
-                for (int j = 1; j < 8; j++) x = fmaxf(x, s[u / 2][8 * (u % 2) + j]);
-                top = fmaxf(top, x * f[u]);
-            }
-            top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), m);
-            if (grown != 1.f || __any(top > m)) {
-                const float alpha = exp2_fast(m - base_of(top)), g = alpha * grown;
-                l *= alpha;
-#pragma unroll
-                for (int i = 0; i < DB; i++)
-#pragma unroll
-                    for (int j = 0; j < 16; j++) o[i][j] *= g;
-                m = top;
-            }
-            const float base = base_of(m) - 15.f;
-            // The weights of one group of keys are formed between the products of the one before,
-            // whose operands are read a group ahead.
-            half8 p[2][NS], v8[2][DB];
-            auto weigh = [&](int u) {
-                const float at = base - lv[u];
-                float w[8], sum = 0.f;
+                const int a0 = max(from - 16 * u, 0), a1 = k4[u] < 0.f ? 0 : min(to - 16 * u, 8);
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    w[j] = exp2_fast(fmaf(s[u / 2][8 * (u % 2) + j], f[u], -at));
-                    sum += w[j];
+                    const float x = s[u / 2][8 * (u % 2) + j];
+                    s[u / 2][8 * (u % 2) + j] = seen_or_not(x, j, a0, a1);
                 }
-                l = fmaf(sum, back[u], l);
-                parts8<NS>(w, p[u & 1]);
-            };
-            auto read_values = [&](int u) {
-#pragma unroll
-                for (int i = 0; i < DB; i++) v8[u & 1][i] = *reinterpret_cast<const half8 *>(vb + (32 * i + n) * VROW + 16 * u + 8 * hf);
-            };
-            read_values(0);
-            weigh(0);
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                if (u < 3) read_values(u + 1);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int z = NS - 1; z >= 0; z--)
-#pragma unroll
-                    for (int i = 0; i < DB; i++) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[u & 1][i], p[u & 1][z], o[i], 0, 0, 0);
-                if (u < 3) {
-                    weigh(u + 1);
-                    constexpr int MFMA = 0x8, VALU = 0x2, TRANS = 0x400;
-#pragma unroll
-                    for (int i = 0; i < DB * NS; i++) {
-                        __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
-                        __builtin_amdgcn_sched_group_barrier(VALU | TRANS, 32 / (DB * NS) + 1, 0);
-                    }
-                }
-                __builtin_amdgcn_sched_barrier(0);
+                f[u] = not_zero(f[u]);
+                if (a0 >= a1) f[u] = 1.f, lv[u] = 0.f, back[u] = 1.f;  // none of the group, so neither its scales
             }
         }
-        if (t + 1 < end) stage(t + 1, next, lds + (buf ^ 1) * long_lds_halves<D>());
-        now = next;
-        sc = sc_next;
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            float x = s[u / 2][8 * (u % 2)];
+#pragma unroll
+            for (int j = 1; j < 8; j++) x = fmaxf(x, s[u / 2][8 * (u % 2) + j]);
+            top = fmaxf(top, x * f[u]);
+        }
+        top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), m);
+        if (__any(top > m + LAZY_LOG2)) {
+            const float alpha = exp2_fast(m - base_of(top));
+            l *= alpha;
+            scale_outputs(alpha);
+            m = top;
+        }
+    };
+    auto weigh = [&](int u) {
+        const float at = base_of(m) - WEIGHT_LOG2 - lv[u];
+        float w[8], sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            w[j] = exp2_fast(fmaf(s[u / 2][8 * (u % 2) + j], f[u], -at));
+            sum += w[j];
+        }
+        l = fmaf(sum, back[u], l);
+        parts8<NS>(w, p[u]);
+    };
+
+    for (int c0 = begin; c0 < end; c0 += TABLE_STEPS) {
+        const int n = min(end - c0, TABLE_STEPS);
+        float grown;
+        look_up(c0, c0 + n, grown);
+        if (grown != 1.f) scale_outputs(grown);
+        read_places(0);
+        load(c0);
+        read_places(min(1, n - 1));
+        stage(c0, 0, 0);
         __syncthreads();
+        for (int i = 0; i < n; i++) {
+            const int t = c0 + i, buf = i & 1;
+            if (i + 1 < n) load(t + 1);
+            if (visible(t)) {
+                const _Float16 *const kb = buffers + buf * buffer_halves<D>(), *const vb = kb + TILE * KROW;
+                key_products(kb);
+                start_weights(t, i);
+                read_values(0, vb);
+                weigh(0);
+#pragma unroll
+                for (int g = 0; g < VGROUPS; g++) {
+                    if (g + 1 < VGROUPS) read_values(g + 1, vb);
+                    __builtin_amdgcn_sched_barrier(0);
+                    value_products(g);
+                    const int u = g / (DB / VG) + 1;
+                    if (g % (DB / VG) == 0 && u < 4) {
+                        weigh(u);
+                        constexpr int MFMA = 0x8, VALU = 0x2, TRANS = 0x400;
+#pragma unroll
+                        for (int j = 0; j < VG * NS; j++) {
+                            __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+                            __builtin_amdgcn_sched_group_barrier(VALU | TRANS, 32 / (VG * NS) + 1, 0);
+                        }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            if (i + 1 < n) {
+                stage(t + 1, i + 1, buf ^ 1);
+                read_places(min(i + 2, n - 1));
+            }
+            __syncthreads();
+        }
     }
 
     l += __shfl_xor(l, 32);
@@ -724,11 +795,11 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
 
 // Both forms in one launch, each sequence in its own: short_groups workgroups of the short form,
 // which are the first to start (a long context's single token takes longest), then the long form's.
-template <int D, int KIND, int DT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void k_attn_mixed(KvAttention a, AttnPlan plan, int short_groups) {
+template <int D, int KIND, int DT>
+__global__ __launch_bounds__(64 * LONG_WAVES<D>, D <= 128 ? 2 : 1) void k_attn_mixed(KvAttention a, AttnPlan plan, int short_groups) {
     extern __shared__ __align__(16) _Float16 lds_h[];
-    if ((int)blockIdx.x < short_groups) attn_short<D, KIND, DT, WAVES>(a, plan, blockIdx.x, reinterpret_cast<float *>(lds_h));
-    else attn_long<D, KIND, DT, WAVES>(a, plan, blockIdx.x - short_groups, lds_h);
+    if ((int)blockIdx.x < short_groups) attn_short<D, KIND, DT, LONG_WAVES<D>>(a, plan, blockIdx.x, reinterpret_cast<float *>(lds_h));
+    else attn_long<D, KIND, DT>(a, plan, blockIdx.x - short_groups, lds_h);
 }
 
 // The join of a row's parts, D / 4 threads a row: few parts, a row for each group of threads; many,
@@ -797,16 +868,10 @@ hipError_t launch_typed(const KvAttention &a, const AttnPlan &plan, bool any_sho
         return hipGetLastError();
     };
     hipError_t e = hipSuccess;
-    const auto mixed = [&](auto k, int waves, size_t short_bytes) {
-        return launch(k, short_groups + plan.tiles * a.c.kv_heads * plan.splits_long, 64 * waves,
-                      std::max(2 * sizeof(_Float16) * long_lds_halves<D>(), short_bytes), short_groups);
-    };
-    if (any_long) {
-        if constexpr (D <= 128)
-            e = plan.long_waves == 8 ? mixed(k_attn_mixed<D, KIND, DT, 8>, 8, short_lds<D, 8>()) : mixed(k_attn_mixed<D, KIND, DT, 4>, 4, short_lds<D, 4>());
-        else
-            e = mixed(k_attn_mixed<D, KIND, DT, 4>, 4, short_lds<D, 4>());
-    } else if (any_short)
+    if (any_long)
+        e = launch(k_attn_mixed<D, KIND, DT>, short_groups + plan.tiles * a.c.kv_heads * plan.splits_long, 64 * LONG_WAVES<D>,
+                   std::max(long_lds<D>(), short_lds<D, LONG_WAVES<D>>()), short_groups);
+    else if (any_short)
         e = launch(k_attn_short<D, KIND, DT>, short_groups, 64 * SHORT_WAVES<D>, short_lds<D, SHORT_WAVES<D>>());
     if (e != hipSuccess) return e;
     const int splits = std::max(any_long ? plan.splits_long : 1, any_short ? plan.splits_short : 1);

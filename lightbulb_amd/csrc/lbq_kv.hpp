@@ -90,8 +90,8 @@ struct KvAttention {
     void *out;                // [num_q][q_heads][head_dim]
     float scale;
     int causal;
-    int64_t window;           // 0: none
-    int64_t max_len;          // no sequence is longer
+    int window;               // 0: none
+    int max_len;              // no sequence is longer
     int max_new;              // no sequence has more queries; 0: not known
     void *ws;
     size_t ws_bytes;

@@ -49,6 +49,7 @@ bool aligned(const void *p, unsigned a) { return (reinterpret_cast<uintptr_t>(p)
 constexpr int MAX_BATCH = 65536;
 constexpr int64_t MAX_TOKENS = (int64_t)1 << 24;
 constexpr int MAX_HEADS = 1024;
+constexpr int64_t MAX_LEN = (int64_t)1 << 30;
 
 int log2_of_page(int page_size) {
     return page_size == 16 ? 4 : page_size == 32 ? 5 : page_size == 64 ? 6 : page_size == 128 ? 7 : -1;
@@ -225,8 +226,9 @@ static int attention_args(const lbq_kv_cache *cache, const lbq_kv_step *step, in
     if (int e = check_query_heads(q_heads, a->c.kv_heads)) return e;
     a->q_heads = q_heads;
     const int64_t held = (int64_t)a->s.max_blocks * a->c.page_size;
-    a->max_len = step->max_len ? std::min<int64_t>(step->max_len, held) : held;
-    if (a->max_len > INT32_MAX - 65536) return fail(LBQ_ERR_LIMIT, "sequences of %lld tokens", (long long)a->max_len);
+    const int64_t longest = step->max_len ? std::min<int64_t>(step->max_len, held) : held;
+    if (longest > MAX_LEN) return fail(LBQ_ERR_LIMIT, "sequences of %lld tokens", (long long)longest);
+    a->max_len = (int)longest;
     a->max_new = step->max_new;
     if (step->num_tokens * q_heads > INT32_MAX)
         return fail(LBQ_ERR_LIMIT, "%lld tokens of %d heads in one call", (long long)step->num_tokens, q_heads);
@@ -264,7 +266,7 @@ int lbq_kv_attention(lbq_ctx *ctx, const lbq_kv_cache *cache, const lbq_kv_step 
     a.out = d_out;
     a.scale = scale;
     a.causal = causal != 0;
-    a.window = window;
+    a.window = (int)std::min(window, MAX_LEN);  // (as wide as any sequence)
     a.ws = d_ws;
     a.ws_bytes = d_ws ? ws_bytes : 0;
     return launched(ctx, "attention launch", [&] { return lbq::launch_kv_attention(a, static_cast<hipStream_t>(stream)); });
