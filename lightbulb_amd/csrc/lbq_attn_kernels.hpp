@@ -453,7 +453,7 @@ constexpr int TABLE_STEPS = 256, GROUPS = TILE / 16;  // steps looked up at once
 template <int D>
 constexpr int buffer_halves() { return TILE * (D + 8) + D * (TILE + 8); }  // f16 of one step's K and V
 template <int D>
-constexpr size_t long_lds() { return 2 * sizeof(_Float16) * buffer_halves<D>() + TABLE_STEPS * GROUPS * (sizeof(uint64_t) + 3 * sizeof(float)); }
+constexpr size_t long_lds() { return 2 * sizeof(_Float16) * buffer_halves<D>() + TABLE_STEPS * GROUPS * (sizeof(uint64_t) + 2 * sizeof(float)); }
 
 // group: its place among the form's workgroups (tiles * kv heads * parts); lds: long_lds bytes
 template <int D, int KIND, int DT>
@@ -529,14 +529,17 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
     _Float16 *const buffers = lds;
     uint64_t *const s_at = reinterpret_cast<uint64_t *>(lds + 2 * buffer_halves<D>());  // bytes from the cache's start to the group's page
     float *const s_k = reinterpret_cast<float *>(s_at + TABLE_STEPS * GROUPS);          // key scales, -1: the group is not there
-    float *const s_lv = s_k + TABLE_STEPS * GROUPS, *const s_back = s_lv + TABLE_STEPS * GROUPS;  // scale_log of value scales, and 2^-that
+    float *const s_lv = s_k + TABLE_STEPS * GROUPS;  // scale_log of value scales
     __shared__ float s_max[WAVES];
+    __shared__ int s_missing[WAVES];
+    bool missing = false;  // whether a group that a row could see is not there
     const int32_t *const table = a.s.tables + b * a.s.table_stride;
     const int seen_end = min(end * TILE, sq.len);
     // the entries of steps c0 .. c1 - 1; grown: r's growth, which the accumulators have to follow
     auto look_up = [&](int c0, int c1, float &grown) {
         const int n = (c1 - c0) * GROUPS;
         float vmax = 0.f;
+        bool lacks = false;
         for (int i = tid; i < n; i += THREADS) {
             const int key = c0 * TILE + 16 * i;
             const int page = key < seen_end ? table[key >> lp] : -1;
@@ -547,13 +550,17 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
             s_k[i] = there ? a.c.ks[at] : -1.f;
             s_lv[i] = v;
             vmax = fmaxf(vmax, v);
+            lacks |= key < seen_end && !there;
         }
 #pragma unroll
         for (int d = 32; d; d /= 2) vmax = fmaxf(vmax, __shfl_xor(vmax, d));
-        if (lane == 0) s_max[wave] = vmax;
+        const bool any = __any(lacks);
+        if (lane == 0) s_max[wave] = vmax, s_missing[wave] = any;
         __syncthreads();
+        missing = false;
 #pragma unroll
-        for (int i = 0; i < WAVES; i++) vmax = fmaxf(vmax, s_max[i]);
+        for (int i = 0; i < WAVES; i++) vmax = fmaxf(vmax, s_max[i]), missing |= s_missing[i] != 0;
+        missing = __any(missing);
         grown = 1.f;
         if (vmax > r) {  // (the same in every thread)
             const int e = scale_ceiling(vmax);
@@ -561,11 +568,7 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
             grown = r * inv_r;
             r = ldexpf(1.f, e);
         }
-        for (int i = tid; i < n; i += THREADS) {
-            const float lv = scale_log(s_lv[i], inv_r);
-            s_lv[i] = lv;
-            s_back[i] = exp2_fast(-lv);
-        }
+        for (int i = tid; i < n; i += THREADS) s_lv[i] = scale_log(s_lv[i], inv_r);
         __syncthreads();
     };
 
@@ -603,10 +606,7 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
     // weights are 0, but a code can be NaN.
     auto stage = [&](int t, int i, int buf) {
         _Float16 *const kb = buffers + buf * buffer_halves<D>(), *const vb = kb + TILE * KROW;
-        bool whole = (t + 1) * TILE <= sq.len;
-#pragma unroll
-        for (int g = 0; g < GROUPS; g++) whole = whole && !(s_k[GROUPS * i + g] < 0.f);
-        if (!whole) {
+        if (missing || (t + 1) * TILE > sq.len) {
 #pragma unroll
             for (int j = 0; j < PER; j++) {
                 const int vg = chunk(j).vg;
@@ -677,17 +677,15 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
 #pragma unroll
             for (int j = 0; j < 16; j++) o[i][j] *= by;
     };
-    float f[4], lv[4], back[4];
+    float f[4], lv[4];
     auto start_weights = [&](int t, int i) {  // entry i of the table
         const f32x4 k4 = *reinterpret_cast<const f32x4 *>(s_k + GROUPS * i), lv4 = *reinterpret_cast<const f32x4 *>(s_lv + GROUPS * i);
-        const f32x4 back4 = *reinterpret_cast<const f32x4 *>(s_back + GROUPS * i);
 #pragma unroll
         for (int u = 0; u < 4; u++) {
             f[u] = k4[u] * factor;  // not negative where a key is seen: the largest product has the largest logit
             lv[u] = lv4[u];
-            back[u] = back4[u];
         }
-        if (t < all_lo || t >= all_hi || __any(fminf(fminf(k4[0], k4[1]), fminf(k4[2], k4[3])) < 0.f)) {
+        if (missing || t < all_lo || t >= all_hi) {
             // some row does not see some of these keys, or they are not there
             const int from = lo - (t * TILE + 8 * hf), to = hi - (t * TILE + 8 * hf);
 #pragma unroll
@@ -699,7 +697,7 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
                     s[u / 2][8 * (u % 2) + j] = seen_or_not(x, j, a0, a1);
                 }
                 f[u] = not_zero(f[u]);
-                if (a0 >= a1) f[u] = 1.f, lv[u] = 0.f, back[u] = 1.f;  // none of the group, so neither its scales
+                if (a0 >= a1) f[u] = 1.f, lv[u] = 0.f;  // none of the group, so neither its scales
             }
         }
         float top = -INFINITY;
@@ -726,7 +724,7 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
             w[j] = exp2_fast(fmaf(s[u / 2][8 * (u % 2) + j], f[u], -at));
             sum += w[j];
         }
-        l = fmaf(sum, back[u], l);
+        l = fmaf(sum, exp2_fast(-lv[u]), l);
         parts8<NS>(w, p[u]);
     };
 
@@ -745,10 +743,14 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
             if (i + 1 < n) load(t + 1);
             if (visible(t)) {
                 const _Float16 *const kb = buffers + buf * buffer_halves<D>(), *const vb = kb + TILE * KROW;
+                // (a wave's products go before the other's weights where both could go)
+                __builtin_amdgcn_s_setprio(1);
                 key_products(kb);
+                __builtin_amdgcn_s_setprio(0);
                 start_weights(t, i);
                 read_values(0, vb);
                 weigh(0);
+                __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                 for (int g = 0; g < VGROUPS; g++) {
                     if (g + 1 < VGROUPS) read_values(g + 1, vb);
@@ -766,6 +768,7 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
+                __builtin_amdgcn_s_setprio(0);
             }
             if (i + 1 < n) {
                 stage(t + 1, i + 1, buf ^ 1);

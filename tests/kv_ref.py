@@ -153,15 +153,15 @@ def attention_bound(dtype, mag, most, out, reach, keys):
     the weighted sum over the keys is rounded once per 16 keys and per join, 2^-24 each.  16-bit types:
     the weights are rounded to f16 (half a step: 2^-11) and the result to its type.
 
-    All types: a weight goes into the product as f16 parts of 2^15 w s / r, w at most 1 (the row's
-    largest is 1, so the weights' sum is at least 1), s its page's scale and r the power of two next above the largest
-    scale so far.  The parts are off by half the smallest f16 step, 2^-25, whatever the weight's size:
-    2^-40 r |code| of the result for each key, and r |code| < 2 s_max |code|_max.  s_max |code|_max is at
-    most 127 (448 for e4m3) s_max, which the tests' blocks of random codes reach to within a factor of 2:
-    2^-40 * 4 * the largest |v|, for each key."""
+    All types: a weight goes into the product as f16 parts of 2^9 w s / r, where w is relative to a base
+    that the row's largest logit is at or up to 6 above (so the weights' sum is at least 1 and w at most
+    2^6), s its page's scale and r the power of two next above the largest scale so far.  The parts are
+    off by half the smallest f16 step, 2^-25, whatever the weight's size: 2^-34 r |code| of the result for
+    each key, and r |code| < 2 s_max |code|_max.  s_max |code|_max is at most 127 (448 for e4m3) s_max, which
+    the tests' blocks of random codes reach to within a factor of 2: 2^-34 * 4 * the largest |v|, for each key."""
     rel = 2 * (2.0 ** -22 + 20 * 2.0 ** -24) * reach + (16 + keys / 16 + 64) * 2.0 ** -24
     step_half = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[dtype]
     if dtype != torch.float32:
         rel += 2.0 ** -11
     tiny = {torch.float32: 0.0, torch.float16: 2.0 ** -25, torch.bfloat16: 0.0}[dtype]
-    return rel * mag + keys * 2.0 ** -38 * most + step_half * out.abs() + tiny + 1e-37
+    return rel * mag + keys * 2.0 ** -32 * most + step_half * out.abs() + tiny + 1e-37
