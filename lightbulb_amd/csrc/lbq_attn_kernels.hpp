@@ -222,31 +222,19 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
     const int per = max(t_hi - t_lo + plan.splits_short - 1, 0) / plan.splits_short;
     const int begin = t_lo + split * per, end = min(begin + per, t_hi);
 
-    // the row's parts and the factor of its logits (in powers of two)
-    half8 q[STEPS][NS];
-    float factor;
+    // The channels that lane group c takes in k step s are 8 of its 16 in channels 64 (s / 2) and on (of 32,
+    // 8 in the last step, where head_dim is no multiple of 64): a load of 16 codes by all lanes is then
+    // 64 whole bytes of each of 16 keys.
+    auto channel = [&](int s) { return s / 2 < D / 64 ? 64 * (s / 2) + 16 * c + 8 * (s % 2) : 64 * (D / 64) + 8 * c; };
+    // (the first keys are asked for before the row is looked at: each waits for memory once)
+    float raw[STEPS][8];
     {
-        const int64_t at = (sq.t0 + tok) * a.q.token_stride + (int64_t)head * a.q.head_stride + c * (D / 4);
-        float v[STEPS][8], amax = 0.f;
+        const int64_t at = (sq.t0 + (mine ? tok : 0)) * a.q.token_stride + (int64_t)(mine ? head : h * plan.group) * a.q.head_stride;
 #pragma unroll
         for (int s = 0; s < STEPS; s++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                v[s][j] = mine ? load_value<DT>(a.q.p, at + 8 * s + j) : 0.f;
-                amax = fmaxf(amax, fabsf(v[s][j]));
-            }
-        amax = fmaxf(amax, __shfl_xor(amax, 16));
-        amax = fmaxf(amax, __shfl_xor(amax, 32));
-        const int e = row_exponent(amax);
-#pragma unroll
-        for (int s = 0; s < STEPS; s++) {
-#pragma unroll
-            for (int j = 0; j < 8; j++) v[s][j] = copysignf(1.f, a.scale) * ldexpf(v[s][j], 15 - e);
-            parts8<NS>(v[s], q[s]);
-        }
-        factor = ldexpf(fabsf(a.scale) * 1.44269504088896340736f, e - 15);
+            for (int j = 0; j < 8; j++) raw[s][j] = load_value<DT>(a.q.p, at + channel(s) + j);
     }
-
     f32x4 o[DB];
 #pragma unroll
     for (int i = 0; i < DB; i++) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -270,23 +258,19 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
     auto load = [&](Loaded &x, int t, int32_t kp, int32_t vp) {
         const int key = t * TILE;
         {
-            const uint8_t *p = a.c.k + ((int64_t)max(kp, 0) * H + h) * page_bytes + c * (D / 4);
+            const uint8_t *p = a.c.k + ((int64_t)max(kp, 0) * H + h) * page_bytes;
             const int at = (key + 16 * kg) & (P - 1);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const uint8_t *row = p + (at + 4 * i + (lane & 3)) * D;
-                if constexpr (D % 64 == 0) {
 #pragma unroll
-                    for (int j = 0; j < D / 64; j++) {
-                        const u32x4 w = reinterpret_cast<const u32x4 *>(row)[j];
-                        x.k[i][4 * j] = w[0], x.k[i][4 * j + 1] = w[1], x.k[i][4 * j + 2] = w[2], x.k[i][4 * j + 3] = w[3];
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < D / 32; j++) {
-                        const u32x2 w = reinterpret_cast<const u32x2 *>(row)[j];
-                        x.k[i][2 * j] = w[0], x.k[i][2 * j + 1] = w[1];
-                    }
+                for (int j = 0; j < D / 64; j++) {
+                    const u32x4 w = *reinterpret_cast<const u32x4 *>(row + channel(2 * j));
+                    x.k[i][4 * j] = w[0], x.k[i][4 * j + 1] = w[1], x.k[i][4 * j + 2] = w[2], x.k[i][4 * j + 3] = w[3];
+                }
+                if constexpr (D % 64 != 0) {
+                    const u32x2 w = *reinterpret_cast<const u32x2 *>(row + channel(STEPS - 1));
+                    x.k[i][2 * STEPS - 2] = w[0], x.k[i][2 * STEPS - 1] = w[1];
                 }
             }
         }
@@ -301,8 +285,28 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
     int t = begin + wave;
     Loaded cur;
     int32_t vp = page_of(t, c), kp = page_of(t, kg);
-    if (t < end) load(cur, t, kp, vp);
     int32_t vp_next = page_of(t + WAVES, c), kp_next = page_of(t + WAVES, kg);
+    if (t < end) load(cur, t, kp, vp);
+    // the row's parts and the factor of its logits (in powers of two)
+    half8 q[STEPS][NS];
+    float factor;
+    {
+        float amax = 0.f;
+#pragma unroll
+        for (int s = 0; s < STEPS; s++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) amax = fmaxf(amax, fabsf(raw[s][j]));
+        amax = fmaxf(amax, __shfl_xor(amax, 16));
+        amax = fmaxf(amax, __shfl_xor(amax, 32));
+        const int e = row_exponent(amax);
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) raw[s][j] = copysignf(1.f, a.scale) * ldexpf(raw[s][j], 15 - e);
+            parts8<NS>(raw[s], q[s]);
+        }
+        factor = ldexpf(fabsf(a.scale) * 1.44269504088896340736f, e - 15);
+    }
     for (; t < end; t += WAVES) {
         Loaded next;
         const bool more = t + WAVES < end;
