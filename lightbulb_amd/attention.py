@@ -69,9 +69,6 @@ class Step:
             raise ValueError("num_tokens, max_len and max_new must not be negative")
         if page_size not in PAGE_SIZES:
             raise ValueError(f"page_size {page_size} is none of {PAGE_SIZES}")
-        self._set(tables, seq_lens, cu_new, slots, positions, page_size, num_tokens, max_len, max_new, granted, free_count)
-
-    def _set(self, tables, seq_lens, cu_new, slots, positions, page_size, num_tokens, max_len, max_new, granted, free_count):
         self.tables, self.seq_lens, self.cu_new, self.slots, self.positions = tables, seq_lens, cu_new, slots, positions
         self.page_size, self.num_tokens, self.max_len, self.max_new = page_size, num_tokens, max_len, max_new
         self.granted, self.free_count = granted, free_count
@@ -122,6 +119,9 @@ class PageTable:
         self.device = tables.device
         self._ctx = context(self.device)
         self._ticket = torch.zeros(1, dtype=torch.int32, device=self.device)
+        # (what a call would ask the tensors for each time: 2 us of a token step's 13)
+        self._rows, self._blocks = tables.shape
+        self._places = (tables.data_ptr(), tables.stride(0), self._blocks, page_size, free.data_ptr(), free.numel())
 
     def step(self, ctx_lens: torch.Tensor, new_lens: torch.Tensor, num_tokens: int, *, commit: bool = True, max_len: int = 0,
              max_new: int = 0) -> Step:
@@ -130,25 +130,33 @@ class PageTable:
         and v hold the sequences' new tokens in order; what is left over is padding.  A sequence that
         does not fit the free pages, its table row or ``num_tokens`` has ``granted`` 0 and sees nothing.
         ``commit=False`` works the step out without taking the pages."""
-        b = ctx_lens.numel()
-        _expect("ctx_lens", ctx_lens, torch.int32, self.device)
-        _expect("new_lens", new_lens, torch.int32, self.device, b)
-        if not 1 <= b <= self.tables.shape[0]:
-            raise ValueError(f"a batch of {b} sequences over {self.tables.shape[0]} table rows")
-        if min(num_tokens, max_len, max_new) < 0:
+        b, dev = ctx_lens.numel(), self.device
+        _expect("ctx_lens", ctx_lens, torch.int32, dev)
+        _expect("new_lens", new_lens, torch.int32, dev, b)
+        if not 1 <= b <= self._rows:
+            raise ValueError(f"a batch of {b} sequences over {self._rows} table rows")
+        if num_tokens < 0 or max_len < 0 or max_new < 0:
             raise ValueError("num_tokens, max_len and max_new must not be negative")
-        slots = torch.empty(num_tokens, dtype=torch.int64, device=self.device)
-        ints = torch.empty(3 * b + 2 + num_tokens, dtype=torch.int32, device=self.device)
+        slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
+        ints = torch.empty(3 * b + 2 + num_tokens, dtype=torch.int32, device=dev)
         seq_lens, cu, granted, positions, left = ints.split((b, b + 1, b, num_tokens, 1))
+        p_lens, p_slots = ints.data_ptr(), slots.data_ptr()
+        p_cu = p_lens + 4 * b
+        p_granted = p_cu + 4 * (b + 1)
+        p_pos = p_granted + 4 * b
+        p_count = self.free_count.data_ptr()
         if commit:
-            left = self.free_count
-        tables = self.tables if b == self.tables.shape[0] else self.tables[:b]
+            left, p_left = self.free_count, p_count
+        else:
+            p_left = p_pos + 4 * num_tokens
         _lib.check(_lib.lib().lbq_kv_step_build(
-            self._ctx, ctx_lens.data_ptr(), new_lens.data_ptr(), b, tables.data_ptr(), tables.stride(0), tables.shape[1], self.page_size,
-            self.free.data_ptr(), self.free.numel(), self.free_count.data_ptr(), left.data_ptr(), self._ticket.data_ptr(), num_tokens,
-            seq_lens.data_ptr(), cu.data_ptr(), granted.data_ptr(), slots.data_ptr(), positions.data_ptr(), _stream(self.device)))
+            self._ctx, ctx_lens.data_ptr(), new_lens.data_ptr(), b, *self._places, p_count, p_left, self._ticket.data_ptr(), num_tokens,
+            p_lens, p_cu, p_granted, p_slots, p_pos, _stream(dev)))
         s = Step.__new__(Step)
-        s._set(tables, seq_lens, cu, slots, positions, self.page_size, num_tokens, max_len, max_new, granted, left)
+        s.tables, s.seq_lens, s.cu_new, s.slots, s.positions = self.tables if b == self._rows else self.tables[:b], seq_lens, cu, slots, positions
+        s.page_size, s.num_tokens, s.max_len, s.max_new = self.page_size, num_tokens, max_len, max_new
+        s.granted, s.free_count, s.device = granted, left, dev
+        s._struct = _lib.KvStepStruct(self._places[0], self._places[1], p_lens, p_cu, p_slots, p_pos, num_tokens, b, self._blocks, max_len, max_new)
         return s
 
     def release(self, lens: torch.Tensor, which: torch.Tensor) -> None:
@@ -157,11 +165,10 @@ class PageTable:
         b = lens.numel()
         _expect("lens", lens, torch.int32, self.device)
         _expect("which", which, torch.int32, self.device, b)
-        if not 1 <= b <= self.tables.shape[0]:
-            raise ValueError(f"a batch of {b} sequences over {self.tables.shape[0]} table rows")
-        _lib.check(_lib.lib().lbq_kv_release(
-            self._ctx, lens.data_ptr(), which.data_ptr(), b, self.tables.data_ptr(), self.tables.stride(0), self.tables.shape[1],
-            self.page_size, self.free.data_ptr(), self.free.numel(), self.free_count.data_ptr(), _stream(self.device)))
+        if not 1 <= b <= self._rows:
+            raise ValueError(f"a batch of {b} sequences over {self._rows} table rows")
+        _lib.check(_lib.lib().lbq_kv_release(self._ctx, lens.data_ptr(), which.data_ptr(), b, *self._places, self.free_count.data_ptr(),
+                                             _stream(self.device)))
 
 
 class Rotary:

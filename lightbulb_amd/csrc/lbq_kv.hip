@@ -231,23 +231,98 @@ __device__ __forceinline__ void store_value(void *p, int64_t i, float v) {
     else static_cast<__hip_bfloat16 *>(p)[i] = __float2bfloat16(v);
 }
 
-// Element d of a row rotated by its position's angles: (a, b) -> (a c - b s, b c + a s) for
-// the pairs (i, i + rot/2), or neighbours.  Both products are exact in 64 bits and their sum
-// is rounded once there and once to 32: one value whatever the order, which the codes need
-// (a last bit moves a code that lies at a tie).  A position outside the table gives NaN.
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// four neighbouring values, at an address that is a multiple of their size
 template <int DT>
-__device__ __forceinline__ float rotated(const KvAppend &a, const void *row, int64_t d, int64_t pos) {
-    const float x = load_value<DT>(row, d);
-    if (d >= a.rot_dim) return x;
-    if (pos < 0 || pos >= a.max_pos) return __uint_as_float(0x7fc00000u);
+__device__ __forceinline__ f32x4 load4(const void *p, int64_t i) {
+    if constexpr (DT == DT_F32) {
+        return *reinterpret_cast<const f32x4 *>(static_cast<const float *>(p) + i);
+    } else {
+        const u32x2 w = *reinterpret_cast<const u32x2 *>(static_cast<const uint16_t *>(p) + i);
+        f32x4 v;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint16_t h = (uint16_t)(w[j / 2] >> (16 * (j % 2)));
+            v[j] = load_value<DT>(&h, 0);
+        }
+        return v;
+    }
+}
+template <int DT>
+__device__ __forceinline__ void store4(void *p, int64_t i, f32x4 v) {
+    if constexpr (DT == DT_F32) {
+        *reinterpret_cast<f32x4 *>(static_cast<float *>(p) + i) = v;
+    } else {
+        uint16_t h[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) store_value<DT>(h, j, v[j]);
+        *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(p) + i) = u32x2{h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16};
+    }
+}
+
+// The pair (x, y) rotated: (x c - y s, y c + x s).  Both products are exact in 64 bits and their sum
+// is rounded once there and once to 32: one value whatever the order, which the codes need (a
+// last bit moves a code that lies at a tie).
+__device__ __forceinline__ void rotate_pair(float x, float y, float c, float s, float &u, float &w) {
+    u = (float)((double)x * c - (double)y * s);
+    w = (float)((double)y * c + (double)x * s);
+    // (the compiler would round a 16-bit result from 64 bits at once: another value at some ties)
+    asm("" : "+v"(u), "+v"(w));
+}
+
+// Eight channels of a row, rotated where they are among the first rot_dim: `at` gets the first channel
+// of each four of them.  Unit u of a row is channels 8 u and on; where pairs lie half a row apart, the
+// rotated ones' units are four channels of either half.  A position outside the table gives NaN.
+template <int DT, bool VEC>
+__device__ __forceinline__ void load_unit(const KvAppend &a, const void *row, int u, int64_t pos, bool turn, f32x4 v[2], int at[2]) {
     const int half = a.rot_dim / 2;
-    const int i = a.interleaved ? (int)d / 2 : (int)(d < half ? d : d - half);
-    const bool upper = a.interleaved ? d & 1 : d >= half;
-    const float y = load_value<DT>(row, a.interleaved ? d ^ 1 : upper ? d - half : d + half);
-    const double c = a.cos[pos * half + i], s = a.sin[pos * half + i];
-    float r = (float)(upper ? (double)x * c + (double)y * s : (double)x * c - (double)y * s);
-    asm("" : "+v"(r));  // the compiler would round a 16-bit result from 64 bits at once: another value at some ties
-    return r;
+    at[0] = 8 * u, at[1] = 8 * u + 4;
+    if constexpr (VEC) {
+        const bool mine = turn && u < a.rot_dim / 8;
+        if (mine && !a.interleaved) at[0] = 4 * u, at[1] = 4 * u + half;
+        const f32x4 x = load4<DT>(row, at[0]), y = load4<DT>(row, at[1]);
+        v[0] = x, v[1] = y;
+        if (!mine) return;
+        if (pos < 0 || pos >= a.max_pos) {
+            v[0] = v[1] = f32x4{1.f, 1.f, 1.f, 1.f} * __uint_as_float(0x7fc00000u);
+            return;
+        }
+        const f32x4 c = *reinterpret_cast<const f32x4 *>(a.cos + pos * half + 4 * u), s = *reinterpret_cast<const f32x4 *>(a.sin + pos * half + 4 * u);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            float p, q;
+            if (a.interleaved) {
+                const f32x4 &z = j < 2 ? x : y;
+                rotate_pair(z[2 * (j % 2)], z[2 * (j % 2) + 1], c[j], s[j], p, q);
+                v[j / 2][2 * (j % 2)] = p, v[j / 2][2 * (j % 2) + 1] = q;
+            } else {
+                rotate_pair(x[j], y[j], c[j], s[j], p, q);
+                v[0][j] = p, v[1][j] = q;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int d = 8 * u + j;
+            float x = load_value<DT>(row, d);
+            if (turn && d < a.rot_dim) {
+                if (pos < 0 || pos >= a.max_pos) {
+                    x = __uint_as_float(0x7fc00000u);
+                } else {
+                    const int i = a.interleaved ? d / 2 : d < half ? d : d - half;
+                    const bool second = a.interleaved ? d & 1 : d >= half;
+                    const float y = load_value<DT>(row, a.interleaved ? d ^ 1 : second ? d - half : d + half);
+                    float p, q;
+                    rotate_pair(second ? y : x, second ? x : y, a.cos[pos * half + i], a.sin[pos * half + i], p, q);
+                    x = second ? q : p;
+                }
+            }
+            v[j / 4][j % 4] = x;
+        }
+    }
 }
 
 // The scale of a block whose largest magnitude is amax: int8 amax / 127; e4m3 the power of
@@ -262,18 +337,17 @@ __device__ __forceinline__ float block_scale(float amax, int kind) {
     return ldexpf(1.f, max(m > 0.875f ? e - 8 : e - 9, -126));
 }
 
-// x / s to the nearest code, ties to even, decided as if the quotient were exact; 0 where s is 0 or NaN
-__device__ __forceinline__ uint8_t code_of(float x, float s, int kind) {
-    if (!(s > 0.f)) return 0;
-    if (kind == KV_E4M3) return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(x / s, 0.f, 0, false);
-    // rint of the rounded quotient is the answer or, next to a tie, one beside it; what is
-    // left, x - q s, is exact in f32 (a multiple of the operands' last place no larger than
-    // s), so its comparison with s / 2 decides
-    float q = rintf(x / s);
-    const float left = fmaf(-q, s, x);
-    if (fabsf(left) > 0.5f * s) q += copysignf(1.f, left);
-    else if (fabsf(left) == 0.5f * s && ((int)q & 1)) q += copysignf(1.f, left);
-    return (uint8_t)(int8_t)(int)fminf(fmaxf(q, -127.f), 127.f);
+// x / s to the nearest code, ties to even, decided as if the quotient were exact; 0 where s is 0
+// or NaN.  inv: 1 / s.
+__device__ __forceinline__ uint32_t code_of(float x, float s, float inv, int kind) {
+    if (kind == KV_E4M3) return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x * inv, 0.f, 0, false) & 0xffu;  // (a power of two: exact)
+    // rint of the product is the answer or, next to a tie, one beside it; what is left, x - q s, is
+    // exact in f32 (a multiple of the operands' last place no larger than about s), so its
+    // comparison with s / 2 decides
+    const float q = rintf(x * inv), left = fmaf(-q, s, x), most = 0.5f * s;
+    const int i = (int)q;
+    const bool move = fabsf(left) > most || (fabsf(left) == most && (i & 1));
+    return (uint32_t)(move ? left > 0.f ? i + 1 : i - 1 : i) & 0xffu;
 }
 
 // a code under scale `was`, under the larger scale `now`
@@ -286,28 +360,43 @@ __device__ __forceinline__ uint8_t recode(uint8_t c, float was, float now, int k
 constexpr int APPEND_THREADS = 256;
 
 // One workgroup per (run of new tokens in one page, kv head, keys or values); the workgroups
-// behind those rotate queries.  Sequence b has at most cu[b + 1] / P - cu[b] / P + 2 runs, so
-// run r belongs to the sequence with cu[b] / P + 2 b <= r, without a list.  The new values
-// are rotated into LDS while their largest magnitude is found, then coded from there.  A
-// scale never falls while a page fills; where it grows, the codes that are there are
-// recoded.  One workgroup owns a (page, head)'s codes and scale: no atomics.
-template <int DT>
+// behind those rotate queries.  Bound by reading q, k and v and writing q: eight channels of a
+// row per thread at a time, in 16-byte accesses where the tensors allow (VEC).
+//
+// Sequence b has at most cu[b + 1] / P - cu[b] / P + 2 runs, so run r belongs to the sequence with
+// cu[b] / P + 2 b <= r, without a list.  The new values are rotated into LDS while their largest
+// magnitude is found, then coded from there, 16 codes per store: keys along the channels, values
+// along the tokens.  A scale never falls while a page fills; where it grows, the codes that are
+// there are coded again, through a table of all 256.  One workgroup owns a (page, head)'s
+// codes and scale: no atomics.
+template <int DT, bool VEC>
 __global__ __launch_bounds__(APPEND_THREADS) void k_kv_append(KvAppend a, int runs) {
-    extern __shared__ float vals[];
+    extern __shared__ __align__(16) float vals[];
     __shared__ float s_max[APPEND_THREADS / 64];
-    const int tid = threadIdx.x, D = a.c.head_dim, P = a.c.page_size, H = a.c.kv_heads;
-    int64_t id = blockIdx.x;
-    const int64_t kv_groups = (int64_t)runs * H * 2;
+    __shared__ uint8_t s_again[256];
+    const int tid = threadIdx.x, threads = blockDim.x, D = a.c.head_dim, P = a.c.page_size, H = a.c.kv_heads;
+    constexpr int size = DT == DT_F32 ? 4 : 2;
+    const int units = D / 8, u = tid % units, step = threads / units, first = tid / units;  // (threads from step * units on: idle)
+    const int64_t id = blockIdx.x, kv_groups = (int64_t)runs * H * 2;
     if (id >= kv_groups) {
-        const int64_t n = a.s.num_tokens * a.q_heads * D, step = (gridDim.x - kv_groups) * APPEND_THREADS;
-        for (int64_t i = (id - kv_groups) * APPEND_THREADS + tid; i < n; i += step) {
-            const int d = (int)(i % D);
-            const int64_t th = i / D, t = th / a.q_heads, h = th % a.q_heads;
+        const int64_t n = a.s.num_tokens * a.q_heads, stride = (gridDim.x - kv_groups) * step;
+        if (first >= step) return;
+        for (int64_t row = (id - kv_groups) * step + first; row < n; row += stride) {
+            const uint32_t t = (uint32_t)row / (uint32_t)a.q_heads, h = (uint32_t)row % (uint32_t)a.q_heads;
             const int32_t pos = a.s.positions[t];
             if (pos < 0) continue;
-            const int64_t at = t * a.q.token_stride + h * a.q.head_stride;
-            constexpr int size = DT == DT_F32 ? 4 : 2;
-            store_value<DT>(a.q_out, i, rotated<DT>(a, static_cast<const char *>(a.q.p) + at * size, d, pos));
+            f32x4 v[2];
+            int at[2];
+            load_unit<DT, VEC>(a, static_cast<const char *>(a.q.p) + (t * a.q.token_stride + h * a.q.head_stride) * size, u, pos, a.rot_dim > 0, v, at);
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                if constexpr (VEC) {
+                    store4<DT>(a.q_out, row * D + at[j], v[j]);
+                } else {
+#pragma unroll
+                    for (int z = 0; z < 4; z++) store_value<DT>(a.q_out, row * D + at[j] + z, v[j][z]);
+                }
+            }
         }
         return;
     }
@@ -317,6 +406,7 @@ __global__ __launch_bounds__(APPEND_THREADS) void k_kv_append(KvAppend a, int ru
     const int b = find_sequence(a.s.batch, run, [&](int i) { return (int64_t)(a.s.cu[i] >> a.c.log2_page) + 2 * (int64_t)i; });
     const int64_t t0 = a.s.cu[b], t1 = a.s.cu[b + 1], len = a.s.seq_lens[b], ctx = len - (t1 - t0);
     if (t0 < 0 || t1 > a.s.num_tokens || t1 <= t0 || ctx < 0) return;
+    if (a.max_new > 0 && t1 - t0 > a.max_new) return;  // (LDS is for no more)
     const int64_t block = (ctx >> a.c.log2_page) + run - ((t0 >> a.c.log2_page) + 2 * (int64_t)b);
     const int64_t lo = max(block << a.c.log2_page, ctx), hi = min((block + 1) << a.c.log2_page, len);
     if (lo >= hi) return;
@@ -325,38 +415,91 @@ __global__ __launch_bounds__(APPEND_THREADS) void k_kv_append(KvAppend a, int ru
     if (slot < 0 || page >= a.c.num_pages || (int)(slot & (P - 1)) != o) return;
 
     const KvRows &rows = is_v ? a.v : a.k;
-    constexpr int size = DT == DT_F32 ? 4 : 2;
+    float *const sp = (is_v ? a.c.vs : a.c.ks) + page * H + h;
+    const float was = o ? *sp : 0.f;
     float amax = 0.f;
     bool bad = false;
-    for (int i = tid; i < count * D; i += APPEND_THREADS) {
-        const int j = i / D, d = i % D;
-        const void *row = static_cast<const char *>(rows.p) + ((tok + j) * rows.token_stride + h * rows.head_stride) * size;
-        const float x = is_v || !a.rot_dim ? load_value<DT>(row, d) : rotated<DT>(a, row, d, a.s.positions[tok + j]);
-        vals[i] = x;
-        bad |= !(fabsf(x) < INFINITY);
-        amax = fmaxf(amax, fabsf(x));
-    }
+    if (first < step)
+        for (int j = first; j < count; j += step) {
+            const void *row = static_cast<const char *>(rows.p) + ((tok + j) * rows.token_stride + h * rows.head_stride) * size;
+            const bool turn = !is_v && a.rot_dim > 0;
+            f32x4 v[2];
+            int at[2];
+            load_unit<DT, VEC>(a, row, u, turn ? a.s.positions[tok + j] : 0, turn, v, at);
+#pragma unroll
+            for (int z = 0; z < 2; z++) {
+                *reinterpret_cast<f32x4 *>(vals + j * D + at[z]) = v[z];
+#pragma unroll
+                for (int y = 0; y < 4; y++) {
+                    bad |= !(fabsf(v[z][y]) < INFINITY);
+                    amax = fmaxf(amax, fabsf(v[z][y]));
+                }
+            }
+        }
     if (bad) amax = INFINITY;
 #pragma unroll
     for (int d = 32; d; d /= 2) amax = fmaxf(amax, __shfl_xor(amax, d));
     if ((tid & 63) == 0) s_max[tid >> 6] = amax;
-    float *const sp = (is_v ? a.c.vs : a.c.ks) + page * H + h;
-    const float was = o ? *sp : 0.f;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < APPEND_THREADS / 64; w++) amax = fmaxf(amax, s_max[w]);
+    for (int w = 0; w < threads / 64; w++) amax = fmaxf(amax, s_max[w]);
     const float fresh = block_scale(amax, a.c.kind);
     const float now = was != was || fresh != fresh ? __uint_as_float(0x7fc00000u) : fmaxf(was, fresh);
     uint8_t *const codes = (is_v ? a.c.v : a.c.k) + (page * H + h) * (int64_t)P * D;
-    for (int i = tid; i < count * D; i += APPEND_THREADS) {
-        const int j = i / D, d = i % D;
-        codes[is_v ? d * P + o + j : (o + j) * D + d] = code_of(vals[i], now, a.c.kind);
-    }
-    if (now > was && was > 0.f)
-        for (int i = tid; i < o * D; i += APPEND_THREADS) {
-            const int at = is_v ? i / o * P + i % o : i;
-            codes[at] = recode(codes[at], was, now, a.c.kind);
+    if (now > was && was > 0.f) {  // (the same in every thread)
+        for (int i = tid; i < 256; i += threads) s_again[i] = recode((uint8_t)i, was, now, a.c.kind);
+        __syncthreads();
+        // whole 16-byte pieces that hold a code from before; what else is in one stays, or is
+        // written below
+        const int pieces = is_v ? D * ((o + 15) / 16) : o * D / 16, per_row = (o + 15) / 16;
+        for (int i = tid; i < pieces; i += threads) {
+            u32x4 *const to = reinterpret_cast<u32x4 *>(codes + (is_v ? i / per_row * P + i % per_row * 16 : i * 16));
+            const int keep = is_v ? o - i % per_row * 16 : 16;
+            u32x4 w = *to;
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const uint32_t c = w[j / 4] >> (8 * (j % 4)) & 0xffu;
+                if (j < keep) w[j / 4] = (w[j / 4] & ~(0xffu << (8 * (j % 4)))) | (uint32_t)s_again[c] << (8 * (j % 4));
+            }
+            *to = w;
         }
+        __syncthreads();
+    }
+    const bool none = !(now > 0.f);  // a scale of 0 or NaN: all codes are 0
+    const float inv = none ? 0.f : 1.f / now, s = none ? 0.f : now;
+    if (!is_v) {
+        for (int i = tid; i < count * D / 16; i += threads) {
+            u32x4 w;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const f32x4 x = *reinterpret_cast<const f32x4 *>(vals + 16 * i + 4 * j);
+                w[j] = none ? 0u
+                            : code_of(x[0], s, inv, a.c.kind) | code_of(x[1], s, inv, a.c.kind) << 8 | code_of(x[2], s, inv, a.c.kind) << 16 |
+                                  code_of(x[3], s, inv, a.c.kind) << 24;
+            }
+            *reinterpret_cast<u32x4 *>(codes + o * D + 16 * i) = w;
+        }
+    } else {
+        // channel i mod D, places 16 (o / 16 + i / D) and on: a lane's neighbours read neighbours of one token
+        const int g0 = o / 16, groups = (o + count + 15) / 16 - g0;
+        for (int i = tid; i < groups * D; i += threads) {
+            const int d = i % D, at = 16 * (g0 + i / D);
+            const int from = max(o - at, 0), to = min(o + count - at, 16);
+            uint8_t *const out = codes + d * P + at;
+            if (from == 0 && to == 16) {
+                u32x4 w;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    uint32_t c = 0;
+#pragma unroll
+                    for (int z = 0; z < 4; z++) c |= code_of(vals[(at - o + 4 * j + z) * D + d], s, inv, a.c.kind) << (8 * z);
+                    w[j] = none ? 0u : c;
+                }
+                *reinterpret_cast<u32x4 *>(out) = w;
+            } else {
+                for (int j = from; j < to; j++) out[j] = none ? 0 : (uint8_t)code_of(vals[(at - o + j) * D + d], s, inv, a.c.kind);
+            }
+        }
+    }
     if (tid == 0) *sp = now;
 }
 
@@ -374,17 +517,26 @@ hipError_t launch_kv_release(const KvRelease &a, hipStream_t st) {
 }
 
 hipError_t launch_kv_append(const KvAppend &a, hipStream_t st) {
+    const int D = a.c.head_dim;
     const int64_t runs = std::min<int64_t>((a.s.num_tokens >> a.c.log2_page) + 2 * (int64_t)a.s.batch, INT32_MAX);
-    const int64_t q = a.q.p ? std::min<int64_t>((a.s.num_tokens * a.q_heads * a.c.head_dim + 1023) / 1024, 65536) : 0;
-    const int64_t groups = runs * a.c.kv_heads * 2 + q;
     const int rows = a.max_new > 0 ? std::min(a.max_new, a.c.page_size) : a.c.page_size;
-    const size_t lds = (size_t)rows * a.c.head_dim * sizeof(float);
-    auto k = a.dtype == DT_F32 ? k_kv_append<DT_F32> : a.dtype == DT_F16 ? k_kv_append<DT_F16> : k_kv_append<DT_BF16>;
-    if (lds > 65536) {
+    // one wave where the largest run has no work for more
+    const int threads = rows * (D / 8) <= 64 ? 64 : APPEND_THREADS, step = threads / (D / 8);
+    const int64_t q = a.q.p ? std::min<int64_t>((a.s.num_tokens * a.q_heads + 2 * step - 1) / (2 * step), 65536) : 0;  // two rows a thread
+    const size_t lds = (size_t)rows * D * sizeof(float);
+    const unsigned align = a.dtype == DT_F32 ? 16 : 8;
+    auto whole = [&](const KvRows &r) { return !r.p || (reinterpret_cast<uintptr_t>(r.p) % align == 0 && r.token_stride % 4 == 0 && r.head_stride % 4 == 0); };
+    const bool vec = whole(a.q) && whole(a.k) && whole(a.v) && reinterpret_cast<uintptr_t>(a.q_out) % align == 0 && a.rot_dim % 8 == 0 &&
+                     reinterpret_cast<uintptr_t>(a.cos) % 16 == 0 && reinterpret_cast<uintptr_t>(a.sin) % 16 == 0;
+    auto pick = [&](auto with, auto without) { return vec ? with : without; };
+    auto k = a.dtype == DT_F32   ? pick(k_kv_append<DT_F32, true>, k_kv_append<DT_F32, false>)
+             : a.dtype == DT_F16 ? pick(k_kv_append<DT_F16, true>, k_kv_append<DT_F16, false>)
+                                 : pick(k_kv_append<DT_BF16, true>, k_kv_append<DT_BF16, false>);
+    if (lds > 65536 - 1024) {
         hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
     }
-    k<<<dim3((unsigned)groups), APPEND_THREADS, lds, st>>>(a, (int)runs);
+    k<<<dim3((unsigned)(runs * a.c.kv_heads * 2 + q)), threads, lds, st>>>(a, (int)runs);
     return hipGetLastError();
 }
 

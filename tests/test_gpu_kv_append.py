@@ -182,15 +182,27 @@ def test_sequences_without_slots_leave_the_cache(dev):
         assert all(same(a, b) for a, b in zip(values(cache), before)), cu
 
 
+def test_more_tokens_than_the_bound(dev):
+    # max_new is the caller's word: a sequence that breaks it is not served, and nothing else is touched
+    table, cache = at.PageTable(8, 16, 2, 4, dev), at.KvCache(8, 16, 1, 64, "int8", dev)
+    step = table.step(i32([0, 0], dev), i32([30, 2], dev), 32, max_new=2)
+    x = torch.randn(32, 1, 64, device=dev)
+    cache.append(x, x, step)
+    first, second = table.tables[0, :2].long(), table.tables[1, :1].long()
+    assert (cache.k_scales[first] == 0).all() and (cache.k[first] == 0).all()
+    want = kv_ref.block_scale(x[30:, 0].cpu(), "int8")
+    assert cache.k_scales[second].item() == cache.v_scales[second].item() == want
+
+
 def test_pages_behind_four_gib(dev):
     # codes whose offsets pass 32 bits
     pages, page, h, dim = 70000, 64, 8, 128
     cache = at.KvCache.wrap(torch.empty(pages, h, page, dim, dtype=torch.int8, device=dev), torch.empty(pages, h, dim, page, dtype=torch.int8, device=dev),
                             torch.zeros(pages, h, device=dev), torch.zeros(pages, h, device=dev))
-    table = at.PageTable.wrap(torch.full((1, 4), -1, dtype=torch.int32, device=dev), i32([5, pages - 1, 40000], dev), i32([3], dev), page)
+    # (the pool is the cache's: three of its pages are free)
+    free = torch.cat([i32([5, pages - 1, 40000], dev), i32([0] * (pages - 3), dev)])
+    table = at.PageTable.wrap(torch.full((1, 4), -1, dtype=torch.int32, device=dev), free, i32([3], dev), page)
     x = torch.randn(130, h, dim, device=dev)
-    # (the pool is the cache's: its list here holds three of its pages)
-    table.free = torch.cat([table.free, i32([0] * (pages - 3), dev)])
     cache.append(x, x, table.step(i32([0], dev), i32([130], dev), 130))
     gen = table.tables[0, :3].tolist()
     assert gen == [40000, pages - 1, 5]
