@@ -51,6 +51,13 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 constexpr int SHORT_ROWS = 16;
 constexpr int TILE = 64;  // keys per step of either form
 
+// f16 parts of a query value and of a weight.  f16 outputs take weights of two parts too: one
+// part's rounding is as large as the output's own, and would leave it 1.4 times as far off.
+template <int DT>
+constexpr int QUERY_PARTS = DT == DT_F32 ? 2 : 1;
+template <int DT>
+constexpr int WEIGHT_PARTS = DT == DT_BF16 ? 1 : 2;
+
 template <int DT>
 __device__ __forceinline__ float load_value(const void *p, int64_t i) {
     if constexpr (DT == DT_F32) return static_cast<const float *>(p)[i];
@@ -199,7 +206,7 @@ constexpr size_t short_lds() { return sizeof(float) * WAVES * SHORT_ROWS * (D + 
 // group: its place among the form's workgroups (parts * kv heads * sequences); lds: short_lds bytes
 template <int D, int KIND, int DT, int WAVES>
 __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan &plan, int group, float *lds) {
-    constexpr int NS = DT == DT_F32 ? 2 : 1;
+    constexpr int NS = QUERY_PARTS<DT>, NW = WEIGHT_PARTS<DT>;
     constexpr int STEPS = D / 32, DB = D / 16;
     float(*const s_o)[SHORT_ROWS][D + 4] = reinterpret_cast<float(*)[SHORT_ROWS][D + 4]>(lds);
     float(*const s_m)[SHORT_ROWS] = reinterpret_cast<float(*)[SHORT_ROWS]>(lds + WAVES * SHORT_ROWS * (D + 4));
@@ -307,6 +314,8 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
         }
         factor = ldexpf(fabsf(a.scale) * 1.44269504088896340736f, e - 15);
     }
+    // (the older wave of a SIMD goes first where both could, and would be done long before the other)
+    if (wave >= 4) __builtin_amdgcn_s_setprio(1);
     for (; t < end; t += WAVES) {
         Loaded next;
         const bool more = t + WAVES < end;
@@ -369,16 +378,16 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
             sum += w[j];
         }
         l = fmaf(sum, back, l);
-        half8 p[2][NS];
-        parts8<NS>(w, p[0]);
-        parts8<NS>(w + 8, p[1]);
+        half8 p[2][NW];
+        parts8<NW>(w, p[0]);
+        parts8<NW>(w + 8, p[1]);
 #pragma unroll
         for (int i = 0; i < DB; i++)
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 const half8 v8 = codes8<KIND>(cur.v[i][2 * u], cur.v[i][2 * u + 1]);
 #pragma unroll
-                for (int z = NS - 1; z >= 0; z--) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, p[u][z], o[i], 0, 0, 0);
+                for (int z = NW - 1; z >= 0; z--) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, p[u][z], o[i], 0, 0, 0);
             }
         cur = next;
         vp = vp_next, kp = kp_next;
@@ -462,7 +471,7 @@ constexpr size_t long_lds() { return 2 * sizeof(_Float16) * buffer_halves<D>() +
 // group: its place among the form's workgroups (tiles * kv heads * parts); lds: long_lds bytes
 template <int D, int KIND, int DT>
 __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &plan, int group, _Float16 *lds) {
-    constexpr int NS = DT == DT_F32 ? 2 : 1, WAVES = LONG_WAVES<D>, ROWS = WAVE_ROWS * WAVES, THREADS = 64 * WAVES;
+    constexpr int NS = QUERY_PARTS<DT>, NW = WEIGHT_PARTS<DT>, WAVES = LONG_WAVES<D>, ROWS = WAVE_ROWS * WAVES, THREADS = 64 * WAVES;
     constexpr int STEPS = D / 16, DB = D / 32;
     constexpr int KROW = D + 8, VROW = TILE + 8;
     constexpr int CHUNKS = TILE * D / 16, PER = (CHUNKS + THREADS - 1) / THREADS;  // 16-code chunks, of K and of V
@@ -635,7 +644,7 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
 
     // ---- products.  Operands in groups of up to four, the next group read before the products of
     // the last: left to itself the compiler reads each right before its product and waits for it.
-    half8 fr[2][4], p[4][NS];
+    half8 fr[2][4], p[4][NW];
     auto read_keys = [&](int g, const _Float16 *kb) {  // k dimensions 2 g and 2 g + 1, both blocks of 32 keys
 #pragma unroll
         for (int z = 0; z < 4; z++) fr[g & 1][z] = *reinterpret_cast<const half8 *>(kb + (32 * (z & 1) + n) * KROW + 16 * (2 * g + z / 2) + 8 * hf);
@@ -666,7 +675,7 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
     };
     auto value_products = [&](int g) {
 #pragma unroll
-        for (int z = NS - 1; z >= 0; z--)
+        for (int z = NW - 1; z >= 0; z--)
 #pragma unroll
             for (int i = 0; i < VG; i++) {
                 f32x16 &to = o[g % (DB / VG) * VG + i];
@@ -729,7 +738,7 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
             sum += w[j];
         }
         l = fmaf(sum, exp2_fast(-lv[u]), l);
-        parts8<NS>(w, p[u]);
+        parts8<NW>(w, p[u]);
     };
 
     for (int c0 = begin; c0 < end; c0 += TABLE_STEPS) {
@@ -765,9 +774,9 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
                         weigh(u);
                         constexpr int MFMA = 0x8, VALU = 0x2, TRANS = 0x400;
 #pragma unroll
-                        for (int j = 0; j < VG * NS; j++) {
+                        for (int j = 0; j < VG * NW; j++) {
                             __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
-                            __builtin_amdgcn_sched_group_barrier(VALU | TRANS, 32 / (VG * NS) + 1, 0);
+                            __builtin_amdgcn_sched_group_barrier(VALU | TRANS, 32 / (VG * NW) + 1, 0);
                         }
                     }
                     __builtin_amdgcn_sched_barrier(0);
