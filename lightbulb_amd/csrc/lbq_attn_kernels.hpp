@@ -29,8 +29,14 @@ namespace lbq {
 // the launch's plan, the same in the kernels and in the join
 struct AttnPlan {
     int splits_short, splits_long;  // parts that a sequence's keys are cut into
-    float *part;                    // [splits][num_q][q_heads][head_dim] outputs of parts
-    float *stat;                    // [splits][num_q][q_heads][2]: running maximum (log2), sum
+    // Rows of parts: [splits_short][short_tokens][q_heads] of the short form from row 0, then
+    // [splits_long][num_q][q_heads] of the long form from row long_row on.  A short sequence's tokens
+    // are those of the batch, or short_per for each sequence where that is fewer (a prompt's rows have
+    // no place among the parts of a single token's long context).
+    float *part;                    // [rows][head_dim]: outputs of parts
+    float *stat;                    // [rows][2]: running maximum (log2), sum
+    int64_t short_tokens, long_row;
+    int short_per;                  // 0: the batch's tokens
     int tiles;                      // tiles of the long form, an upper bound
     int group;                      // query heads per kv head
     int short_rows;                 // rows (queries * group) up to which a sequence takes the short form; 0: none does
@@ -404,7 +410,6 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
         for (int j = 0; j < 4; j++) s_o[wave][n][16 * i + 4 * c + j] = l == 0.f ? 0.f : o[i][j] * inv * r;
     if (c == 0) s_m[wave][n] = m, s_l[wave][n] = l;
     __syncthreads();
-    const int64_t all = a.num_q * a.q_heads;
     for (int i = threadIdx.x; i < rows * (D / 4); i += 64 * WAVES) {
         const int row = i / (D / 4), d = i % (D / 4) * 4;
         float top = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
@@ -419,11 +424,11 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
         }
 #pragma unroll
         for (int j = 0; j < 4; j++) v[j] = sum == 0.f ? 0.f : v[j] / sum;
-        const int64_t out = (sq.t0 + row / plan.group) * a.q_heads + h * plan.group + row % plan.group;
+        const int tok = row / plan.group, head = h * plan.group + row % plan.group;
         if (plan.splits_short == 1) {
-            store_values4<DT>(a.out, out * D + d, v);
+            store_values4<DT>(a.out, ((int64_t)(sq.t0 + tok) * a.q_heads + head) * D + d, v);
         } else {
-            const int64_t at = split * all + out;
+            const int64_t unit = plan.short_per ? b * plan.short_per + tok : sq.t0 + tok, at = (split * plan.short_tokens + unit) * a.q_heads + head;
             *reinterpret_cast<f32x4 *>(plan.part + at * D + d) = f32x4{v[0], v[1], v[2], v[3]};
             if (d == 0) plan.stat[2 * at] = top, plan.stat[2 * at + 1] = sum;
         }
@@ -794,7 +799,7 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
     l += __shfl_xor(l, 32);
     const float inv = l == 0.f ? 0.f : 1.f / l;  // (apart from r: their quotient can be subnormal)
     if (!mine) return;
-    const int64_t out = (sq.t0 + tok) * a.q_heads + head, at = split * a.num_q * a.q_heads + out;
+    const int64_t out = (sq.t0 + tok) * a.q_heads + head, at = plan.long_row + split * a.num_q * a.q_heads + out;
     if (plan.splits_long > 1 && hf == 0) plan.stat[2 * at] = m, plan.stat[2 * at + 1] = l;
 #pragma unroll
     for (int i = 0; i < DB; i++)
@@ -820,7 +825,7 @@ __global__ __launch_bounds__(64 * LONG_WAVES<D>, D <= 128 ? 2 : 1) void k_attn_m
 
 // The join of a row's parts, D / 4 threads a row: few parts, a row for each group of threads; many,
 // a workgroup for one row, whose groups take every JOIN_GROUPS-th part and are added in order.
-// Rows whose form did not cut its keys were written by it.
+// The rows are the short form's, if it cut its sequences, and then the long form's, if that did.
 constexpr int JOIN_THREADS = 256;
 template <int D>
 constexpr int JOIN_GROUPS = JOIN_THREADS / (D / 4);
@@ -831,22 +836,32 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_attn_join(KvAttention a, AttnP
     __shared__ f32x4 s_v[ONE ? G : 1][D / 4];
     __shared__ float s_sum[ONE ? G : 1];
     const int g = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
-    const int64_t all = a.num_q * a.q_heads, row = ONE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * G + g;
-    if (g >= G || row >= all) return;
-    const int64_t t = row / a.q_heads;
+    const int64_t id = ONE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * G + g;
+    const int64_t short_rows = plan.splits_short > 1 ? plan.short_tokens * a.q_heads : 0, long_rows = plan.splits_long > 1 ? a.num_q * a.q_heads : 0;
+    if (g >= G || id >= short_rows + long_rows) return;
+    const bool is_short = id < short_rows;
+    const int64_t row = is_short ? id : id - short_rows;  // (token, head) in its form's order
+    int64_t t = row / a.q_heads;
     int b = 0;
-    for (int n = a.s.batch; n > 1;) {  // the last sequence that begins at or before t
-        const int half = n / 2;
-        const bool up = a.cu_q[b + half] <= t;
-        b += up ? half : 0;
-        n = up ? n - half : half;
-    }
     Sequence sq;
-    if (!sequence_of(a, b, sq) || t < sq.t0 || t >= sq.t0 + sq.n) return;
-    const int splits = sq.n * plan.group <= plan.short_rows ? plan.splits_short : plan.splits_long;
-    if (splits <= 1) return;
-    const float *const stat = plan.stat + 2 * row;
-    const float *const part = plan.part + row * D + d;
+    if (is_short && plan.short_per) {
+        b = (int)(t / plan.short_per);
+        if (!sequence_of(a, b, sq)) return;
+        t += sq.t0 - (int64_t)b * plan.short_per;
+    } else {
+        for (int n = a.s.batch; n > 1;) {  // the last sequence that begins at or before t
+            const int half = n / 2;
+            const bool up = a.cu_q[b + half] <= t;
+            b += up ? half : 0;
+            n = up ? n - half : half;
+        }
+        if (!sequence_of(a, b, sq)) return;
+    }
+    if (t < sq.t0 || t >= sq.t0 + sq.n || (sq.n * plan.group <= plan.short_rows) != is_short) return;
+    const int splits = is_short ? plan.splits_short : plan.splits_long;
+    const int64_t all = is_short ? short_rows : long_rows, at = row + (is_short ? 0 : plan.long_row);
+    const float *const stat = plan.stat + 2 * at;
+    const float *const part = plan.part + at * D + d;
     float top = -INFINITY;
 #pragma unroll 8
     for (int i = 0; i < splits; i++) top = fmaxf(top, stat[2 * i * all]);
@@ -869,7 +884,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_attn_join(KvAttention a, AttnP
     float o[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) o[j] = sum == 0.f ? 0.f : v[j] / sum;
-    store_values4<DT>(a.out, row * D + d, o);
+    store_values4<DT>(a.out, (t * a.q_heads + row % a.q_heads) * D + d, o);
 }
 
 template <int D, int KIND, int DT>
@@ -890,8 +905,8 @@ hipError_t launch_typed(const KvAttention &a, const AttnPlan &plan, bool any_sho
     else if (any_short)
         e = launch(k_attn_short<D, KIND, DT>, short_groups, 64 * SHORT_WAVES<D>, short_lds<D, SHORT_WAVES<D>>());
     if (e != hipSuccess) return e;
-    const int splits = std::max(any_long ? plan.splits_long : 1, any_short ? plan.splits_short : 1);
-    const int64_t rows = a.num_q * a.q_heads;
+    const int splits = std::max(plan.splits_long, plan.splits_short);
+    const int64_t rows = (plan.splits_short > 1 ? plan.short_tokens * a.q_heads : 0) + (plan.splits_long > 1 ? a.num_q * a.q_heads : 0);
     if (splits > JOIN_GROUPS<D>) k_attn_join<D, DT, true><<<dim3((unsigned)rows), JOIN_THREADS, 0, st>>>(a, plan);
     else if (splits > 1) k_attn_join<D, DT, false><<<dim3((unsigned)((rows + JOIN_GROUPS<D> - 1) / JOIN_GROUPS<D>)), JOIN_THREADS, 0, st>>>(a, plan);
     return hipGetLastError();

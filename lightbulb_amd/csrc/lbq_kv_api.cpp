@@ -232,6 +232,9 @@ static int attention_args(const lbq_kv_cache *cache, const lbq_kv_step *step, in
     a->max_new = step->max_new;
     if (step->num_tokens * q_heads > INT32_MAX)
         return fail(LBQ_ERR_LIMIT, "%lld tokens of %d heads in one call", (long long)step->num_tokens, q_heads);
+    // (tiles of at least 128 rows, and one more for each sequence)
+    if (step->num_tokens * q_heads / 128 + (int64_t)a->s.batch * a->c.kv_heads > lbq::MAX_GROUPS)
+        return fail(LBQ_ERR_LIMIT, "%d sequences of %d heads and %lld tokens in one call", a->s.batch, a->c.kv_heads, (long long)step->num_tokens);
     return LBQ_OK;
 }
 

@@ -1,5 +1,6 @@
 """Attention over the 8-bit cache against the definition in 64 bits, with bounds from the arithmetic
 (kv_ref.attention_bound), and the operators together as a layer runs them."""
+import ctypes
 import math
 import random
 
@@ -248,6 +249,41 @@ def test_without_workspace(dev, lbq):
         assert lbq.lbq_kv_attention(cache._ctx, cache._struct, step._struct, 0, q.data_ptr(), q.stride(0), q.stride(1), 4, 128 ** -0.5, 1, 0,
                                     out.data_ptr(), ws.data_ptr() if n else None, n, torch.cuda.current_stream(dev).cuda_stream) == 0
         check(q, cache, step, got=out)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [128, 192])
+def test_long_contexts_beside_a_prompt(dev, dtype, dim):
+    # single tokens' keys cut into parts whose rows are not the prompt's
+    cache, step, q = setup(dev, "int8", dtype, 64, dim, 1, 4, [0, 30000, 9000, 50, 10], [700, 1, 2, 0, 4], slack=20)
+    check(q, cache, step)
+    hinted = at.Step(step.tables, step.seq_lens, step.cu_new, None, None, page_size=64, num_tokens=step.num_tokens, max_len=30001, max_new=700)
+    check(q, cache, hinted)
+
+
+def test_workspace_is_not_the_prompts(dev, lbq):
+    # (parts of all 16000 tokens would be 4 GiB)
+    cache, step, _ = setup(dev, "int8", torch.float32, 64, 128, 8, 4, [0, 100, 100], [16000 - 2, 1, 1], pad=0)
+    wide = at.Step(step.tables, step.seq_lens, step.cu_new, None, None, page_size=64, num_tokens=16000)
+    wide._struct.max_blocks = wide._struct.table_stride = 2048  # sequences of up to 131072 tokens; nothing is read
+    n = ctypes.c_size_t()
+    assert lbq.lbq_kv_attention_workspace(cache._ctx, cache._struct, wide._struct, 32, n) == 0
+    assert 0 < n.value < 32 << 20
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind,dim", [("int8", 64), ("e4m3", 128), ("int8", 256)])
+def test_more_steps_than_are_looked_up_at_once(dev, lbq, dtype, kind, dim):
+    # 33000 keys in one part, value scales that grow late, pages that are not there
+    cache, step, q = setup(dev, kind, dtype, 64, dim, 1, 4, [33000 - 40], [40], pad=0)
+    page = step.tables[0]
+    cache.v_scales[page[300:520].long()] *= 1000
+    page[270], page[400] = -1, cache.k.shape[0]
+    out = torch.empty_like(q)
+    assert lbq.lbq_kv_attention(cache._ctx, cache._struct, step._struct, at._DTYPES[dtype], q.data_ptr(), q.stride(0), q.stride(1), 4, dim ** -0.5,
+                                1, 0, out.data_ptr(), None, 0, torch.cuda.current_stream(dev).cuda_stream) == 0
+    check(q, cache, step, got=out)
+    check(q, cache, step)
 
 
 def test_same_bits_every_time(dev):

@@ -78,6 +78,8 @@ def test_attention_arguments(lbq):
     assert attend(lbq, cache(), step(), out=D + 4 * (2 * 128 + 64)) == INVALID  # the last row of q
     assert attend(lbq, cache(), step(), ws=D + 8) == INVALID
     assert attend(lbq, cache(), step(max_blocks=1 << 30, table_stride=1 << 30)) == LIMIT
+    assert attend(lbq, cache(kv_heads=1024), step(batch=65536), heads=1024) == LIMIT
+    assert attend(lbq, cache(), step(num_tokens=1 << 24), heads=1024) == LIMIT
     assert attend(lbq, cache(), step(num_tokens=0), q=None, out=None) == 0  # nothing to do
 
 
