@@ -91,6 +91,8 @@ __device__ __forceinline__ void store_values4(void *p, int64_t i, const float *v
 constexpr float WEIGHT_LOG2 = 9.f, LAZY_LOG2 = 6.f;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+// the larger of two, one instruction (fmaxf of values whose origin the compiler does not know takes three)
+__device__ __forceinline__ float larger(float x, float y) { return __builtin_amdgcn_fmed3f(x, y, INFINITY); }
 // a maximum as the base of exponents: 0 where nothing was seen, so that no inf - inf is formed
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
 
@@ -363,13 +365,13 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
 #pragma unroll
             for (int i = 0; i < DB; i++) cur.v[i] = keep_bytes(cur.v[i], keep);
         }
-        float top = x[0];
+        float top = larger(x[0], x[1]);
 #pragma unroll
-        for (int j = 1; j < 16; j++) top = fmaxf(top, x[j]);
-        top *= f;
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), m);
+        for (int j = 2; j < 16; j++) top = fmaxf(top, x[j]);
+        top *= f;  // of this lane's keys; the row's only where the base has to move
         if (grown != 1.f || __any(top > m + LAZY_LOG2)) {
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), m);
             const float alpha = exp2_fast(m - base_of(top)), g = alpha * grown;
             l *= alpha;
 #pragma unroll
@@ -721,13 +723,13 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
         float top = -INFINITY;
 #pragma unroll
         for (int u = 0; u < 4; u++) {
-            float x = s[u / 2][8 * (u % 2)];
+            float x = larger(s[u / 2][8 * (u % 2)], s[u / 2][8 * (u % 2) + 1]);
 #pragma unroll
-            for (int j = 1; j < 8; j++) x = fmaxf(x, s[u / 2][8 * (u % 2) + j]);
+            for (int j = 2; j < 8; j++) x = fmaxf(x, s[u / 2][8 * (u % 2) + j]);
             top = fmaxf(top, x * f[u]);
         }
-        top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), m);
-        if (__any(top > m + LAZY_LOG2)) {
+        if (__any(top > m + LAZY_LOG2)) {  // (this lane's keys; the row's only where the base has to move)
+            top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), m);
             const float alpha = exp2_fast(m - base_of(top));
             l *= alpha;
             scale_outputs(alpha);
