@@ -506,7 +506,7 @@ __global__ __launch_bounds__(APPEND_THREADS) void k_kv_append(KvAppend a, int ru
 }  // namespace
 
 hipError_t launch_kv_step(const KvStepBuild &a, hipStream_t st) {
-    const int64_t groups = std::max<int64_t>(1, std::min<int64_t>((a.num_tokens + 1023) / 1024, 64));
+    const int64_t groups = std::max<int64_t>(1, std::min<int64_t>((a.num_tokens + STEP_THREADS - 1) / STEP_THREADS, 256));
     k_kv_step<<<dim3((unsigned)groups), STEP_THREADS, 0, st>>>(a);
     return hipGetLastError();
 }
