@@ -306,7 +306,7 @@ int lbq_quantize_weights_f32(uint32_t ggml_type, const float *d_w, int64_t nelem
  * of sequence b, its tokens j * page_size and on, lies in page tables[b][j].  Each
  * (page, kv head) has one scale for its keys and one for its values; a value is
  * code * scale.  Codes are int8 (scale = largest magnitude / 127) or e4m3 (OCP; the
- * power of two that brings the largest magnitude to at most 448).  A scale grows while its
+ * power of two that brings the largest magnitude to at most 448); scales are not negative.  A scale grows while its
  * page fills, never falls, and the codes already there are then coded again; a page whose
  * keys or values are not finite has the scale NaN from then on and reads as NaN.
  * head_dim is 64, 96, 128, 192 or 256; dtype is LBQ_TYPE_F32, _F16 or _BF16 and is that of
@@ -359,7 +359,9 @@ int lbq_kv_step_build(lbq_ctx *ctx, const int32_t *d_ctx_lens, const int32_t *d_
 
 /* The pages that hold the lens[b] tokens of each sequence with which[b] != 0 go back on top of
  * the free ones, sequence by sequence and block by block, and their table entries become -1
- * (so a second release of the same sequence frees nothing). */
+ * (so a second release of the same sequence frees nothing).  A page that stands in two released
+ * tables goes back twice: sequences that share pages are released with all but one of the shared
+ * entries at -1. */
 int lbq_kv_release(lbq_ctx *ctx, const int32_t *d_lens, const int32_t *d_which, int32_t batch, int32_t *d_tables,
                    int64_t table_stride, int32_t max_blocks, int32_t page_size, int32_t *d_free, int64_t num_pages,
                    int32_t *d_free_count, void *stream);
@@ -369,8 +371,10 @@ int lbq_kv_release(lbq_ctx *ctx, const int32_t *d_lens, const int32_t *d_which, 
  * rows rotated likewise into d_q_out [num_tokens][q_heads][head_dim] (contiguous, apart from
  * q, k and v).  Pairs are the channels (i, i + rot_dim / 2), or neighbours where interleaved;
  * (a, b) becomes (a cos - b sin, b cos + a sin), with cos and sin [max_pos][rot_dim / 2] f32.
- * A position from max_pos on gives NaN.  Each page takes new tokens of one sequence only.
- * Rows whose slot is -1 are passed over. */
+ * A position from max_pos on gives NaN.  Each page takes new tokens of one sequence only; the first of
+ * a sequence's new rows in a page gives the page (its slot), and where that is -1 or not the place
+ * that seq_lens and cu_new say, none of them is written.  Rows of q whose position is -1 are passed
+ * over. */
 int lbq_kv_append(lbq_ctx *ctx, const lbq_kv_cache *cache, const lbq_kv_step *step, uint32_t dtype, const void *d_k,
                   int64_t k_token_stride, int64_t k_head_stride, const void *d_v, int64_t v_token_stride,
                   int64_t v_head_stride, const void *d_q, int64_t q_token_stride, int64_t q_head_stride, int32_t q_heads,

@@ -161,7 +161,8 @@ class PageTable:
 
     def release(self, lens: torch.Tensor, which: torch.Tensor) -> None:
         """The pages of the sequences b with ``which[b] != 0``, which hold ``lens[b]`` tokens, are free
-        again (int32 [batch] on the GPU)."""
+        again (int32 [batch] on the GPU).  Entries of pages that another sequence still holds are set
+        to -1 by the caller first."""
         b = lens.numel()
         _expect("lens", lens, torch.int32, self.device)
         _expect("which", which, torch.int32, self.device, b)
@@ -259,7 +260,7 @@ class KvCache:
                q: torch.Tensor | None = None) -> torch.Tensor | None:
         """Writes the step's keys and values ([num_tokens, kv_heads, head_dim]) into their pages, keys
         rotated by ``rotary`` first, and gives ``q`` [num_tokens, heads, head_dim] rotated likewise.
-        Rows without a slot are passed over (their rotated queries are left unset)."""
+        Pages that are not there take nothing, and rows of ``q`` without a position are left unset."""
         self._fits(step)
         t = _rows("k", k, self.kv_heads, self.head_dim, step)
         if _rows("v", v, self.kv_heads, self.head_dim, step) != t:

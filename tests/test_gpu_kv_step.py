@@ -147,6 +147,27 @@ def test_release_of_many(dev):
     assert one.free.tolist() == list(range(5000)) and one.free_count.item() == 5000
 
 
+def test_release_of_long_and_empty_sequences(dev):
+    # rows of more entries than a workgroup has threads, rows without any between them, entries that are no pages
+    rows, blocks, page = 1030, 1500, 16
+    lens = [(0, 0, 1500 * 16, 1, 0, 24000 - 1, 0, 16 * 1100)[i % 8] if i < 24 or i > 1020 else 0 for i in range(rows)]
+    which = [int(i % 5 != 2) for i in range(rows)]
+    tables = torch.arange(rows * blocks, dtype=torch.int32).view(rows, blocks)
+    tables[:, 7] = -1
+    tables[:, 9] = rows * blocks
+    p = at.PageTable.wrap(tables.to(dev), torch.full((rows * blocks,), -5, dtype=torch.int32, device=dev), i32([3], dev), page)
+    p.release(i32(lens, dev), i32(which, dev))
+    want = torch.cat([tables[b, : -(-lens[b] // page)] for b in range(rows) if which[b]])
+    want = want[(want >= 0) & (want < rows * blocks)]
+    assert p.free_count.item() == 3 + len(want)
+    assert torch.equal(p.free[3: 3 + len(want)].cpu(), want) and (p.free[3 + len(want):] == -5).all() and (p.free[:3] == -5).all()
+    left = tables.clone()
+    for b in range(rows):
+        if which[b]:
+            left[b, : -(-lens[b] // page)] = -1
+    assert torch.equal(p.tables.cpu(), left)
+
+
 def test_replays_take_pages_each_time(dev):
     p = at.PageTable(64, 16, 4, 16, dev)
     lens, new = i32([0, 0, 0, 0], dev), i32([16, 1, 0, 33], dev)
