@@ -2,9 +2,9 @@
 //
 // The codes of both kinds are f16 numbers, so a code goes into a matrix instruction exactly and
 // its scale, one per 16 or more keys, into the f32 logit or weight.  f32 queries go in as two f16
-// parts of a power-of-two multiple of their row (22 bits), f32 weights likewise, with the products
-// of both parts in one f32 sum: results of f32's accuracy at twice the matrix work.  f16 and bf16
-// queries are one part, exactly.
+// parts of a power-of-two multiple of their row (22 bits); f16 and bf16 queries are one part, exactly.
+// Weights go in as two f16 parts, for bf16 as one.  The products of both parts go into one f32 sum:
+// results of f32's accuracy at twice the matrix work.
 //
 // Products are formed transposed: S^T = K Q^T, then O^T = V^T P^T.  Column n of every tile is
 // query row n, so a row's softmax stays inside a lane and the lanes that share its column, and the
@@ -204,7 +204,12 @@ __device__ __forceinline__ float part_weight(float m, float l, float top) { retu
 // Short form: up to 16 query rows of one kv head (a token step: its group of query heads).
 // Bound by reading the cache, 2 head_dim bytes per key: one wave takes 64 keys at a time
 // straight from memory into its operands, the next 64 on their way while it works, with no
-// barrier until the waves' outputs are joined at the end.  16x16x32 products; in S^T lane
+// barrier until the waves' outputs are joined at the end.  32 tokens of 8 heads with ragged contexts
+// of up to 4096 keys of 128 channels, 202.7 MB: 49 us, 4.1 TB/s (a read stream reaches 5.7; here 256
+// workgroups of unlike length start and end apart).  131071 keys of one sequence, 268 MB: 54 us, 5.0 TB/s,
+// and 5 to join 32 parts.  One workgroup takes about 3.3 us for a
+// step of its eight waves (4000 keys: 33 us), and 7 for launch, bounds, pages and the first codes: a
+// short context's time (1000 keys: 13 us).  16x16x32 products; in S^T lane
 // (c, n) = (lane / 16, lane % 16) holds keys 16 c .. 16 c + 15 of the 64 for row n, which is
 // what the products with V take, and all of one page: one scale per lane.
 // ---------------------------------------------------------------------------
@@ -450,7 +455,8 @@ __global__ __launch_bounds__(64 * SHORT_WAVES<D>, D <= 128 ? 2 : 1) void k_attn_
 
 // ---------------------------------------------------------------------------
 // Long form: query rows of one kv head (row i * group + head: neighbouring tokens see nearly the
-// same keys), 32 for each wave.  Bound by the matrix cores and by the exponentials.  64 keys at a
+// same keys), 32 for each wave.  Bound by the matrix cores and by the vector unit's weights
+// (seven instructions each), which hardly run at once within a wave.  64 keys at a
 // time are turned into f16 once for all waves and kept in LDS, the next steps' codes on their
 // way from memory meanwhile.  32x32x16 products; rows of K lie in LDS in the order in which lane
 // (half, n) then holds keys 16 u + 8 half + j of its row n, what the products with V take.
@@ -464,6 +470,14 @@ __global__ __launch_bounds__(64 * SHORT_WAVES<D>, D <= 128 ? 2 : 1) void k_attn_
 // Up to 128 channels the registers allow two waves on a SIMD, and one's products run while the
 // other forms weights.  Above that there is one, and four in a workgroup.  In either case the
 // weights of 16 keys are formed between the products of the 16 before.
+//
+// A prompt of 8000 tokens in bf16, 32 heads of 128 channels, window 5000, 450.6 GFLOP: 463 to 479 us,
+// 0.94 to 0.97 PFLOP/s (a large library product: 1.14); the matrix cores are busy in 43 % of the cycles, the vector
+// unit in 49 %, at 2.0 GHz: the power limit.  Four chunks of 512 over contexts of 1500 in f32, 38.7 GFLOP and
+// twice the products: 97 us.  220 rows a head over 1500 states of 64 channels in f16: 44 us on 160 CUs, the
+// vector unit's time (per key and row as much as at 128 channels, for half the products).  Measured and no
+// better: steps of 128 keys (64 channels: -3 %, causal prompts +2 %), codes two steps ahead, four waves a workgroup
+// (618 us for the prompt), three buffers with the waves half a step apart (665), sums by dot products.
 // ---------------------------------------------------------------------------
 constexpr int WAVE_ROWS = 32;
 template <int D>
@@ -825,10 +839,13 @@ __global__ __launch_bounds__(64 * LONG_WAVES<D>, D <= 128 ? 2 : 1) void k_attn_m
     else attn_long<D, KIND, DT>(a, plan, blockIdx.x - short_groups, lds_h);
 }
 
-// The join of a row's parts, D / 4 threads a row: few parts, a row for each group of threads; many,
-// a workgroup for one row, whose groups take every JOIN_GROUPS-th part and are added in order.
+// The join of a row's parts, D / 4 threads a row.  Few rows: a workgroup for one row, whose groups take
+// every JOIN_GROUPS-th part and are added in order.  Many: a row for each group of threads.  Bound by
+// latency: rows' bounds, the parts' maxima, the parts; 4.5 to 5 us for 32 rows of 32 parts.  From the
+// call's time: 32 rows of 15 parts 17.2 us with a workgroup a row, 18.5 with a group of threads; 128 rows of
+// 7 parts 17.0 and 18.1; 3200 rows of 15 parts 46.7 and 45.1; 16384 rows of 4 parts 68.1 and 52.6.
 // The rows are the short form's, if it cut its sequences, and then the long form's, if that did.
-constexpr int JOIN_THREADS = 256;
+constexpr int JOIN_THREADS = 256, JOIN_ROWS = 1024;  // rows up to which each has a workgroup
 template <int D>
 constexpr int JOIN_GROUPS = JOIN_THREADS / (D / 4);
 
@@ -907,10 +924,10 @@ hipError_t launch_typed(const KvAttention &a, const AttnPlan &plan, bool any_sho
     else if (any_short)
         e = launch(k_attn_short<D, KIND, DT>, short_groups, 64 * SHORT_WAVES<D>, short_lds<D, SHORT_WAVES<D>>());
     if (e != hipSuccess) return e;
-    const int splits = std::max(plan.splits_long, plan.splits_short);
+    if (plan.splits_short == 1 && plan.splits_long == 1) return hipSuccess;
     const int64_t rows = (plan.splits_short > 1 ? plan.short_tokens * a.q_heads : 0) + (plan.splits_long > 1 ? a.num_q * a.q_heads : 0);
-    if (splits > JOIN_GROUPS<D>) k_attn_join<D, DT, true><<<dim3((unsigned)rows), JOIN_THREADS, 0, st>>>(a, plan);
-    else if (splits > 1) k_attn_join<D, DT, false><<<dim3((unsigned)((rows + JOIN_GROUPS<D> - 1) / JOIN_GROUPS<D>)), JOIN_THREADS, 0, st>>>(a, plan);
+    if (rows <= JOIN_ROWS) k_attn_join<D, DT, true><<<dim3((unsigned)rows), JOIN_THREADS, 0, st>>>(a, plan);
+    else k_attn_join<D, DT, false><<<dim3((unsigned)((rows + JOIN_GROUPS<D> - 1) / JOIN_GROUPS<D>)), JOIN_THREADS, 0, st>>>(a, plan);
     return hipGetLastError();
 }
 
