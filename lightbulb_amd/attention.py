@@ -119,7 +119,8 @@ class PageTable:
         self.device = tables.device
         self._ctx = context(self.device)
         self._ticket = torch.zeros(1, dtype=torch.int32, device=self.device)
-        # (what a call would ask the tensors for each time: 2 us of a token step's 13)
+        self._longs = torch.empty(0, dtype=torch.int64, device=self.device)
+        # (what a call would ask the tensors for each time: 2 us of a token step's 12)
         self._rows, self._blocks = tables.shape
         self._places = (tables.data_ptr(), tables.stride(0), self._blocks, page_size, free.data_ptr(), free.numel())
 
@@ -137,9 +138,9 @@ class PageTable:
             raise ValueError(f"a batch of {b} sequences over {self._rows} table rows")
         if num_tokens < 0 or max_len < 0 or max_new < 0:
             raise ValueError("num_tokens, max_len and max_new must not be negative")
-        slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
-        ints = torch.empty(3 * b + 2 + num_tokens, dtype=torch.int32, device=dev)
-        seq_lens, cu, granted, positions, left = ints.split((b, b + 1, b, num_tokens, 1))
+        slots = self._longs.new_empty(num_tokens)
+        ints = ctx_lens.new_empty(3 * b + 2 + num_tokens)
+        seq_lens, cu, granted, positions, left = ints.split_with_sizes((b, b + 1, b, num_tokens, 1))
         p_lens, p_slots = ints.data_ptr(), slots.data_ptr()
         p_cu = p_lens + 4 * b
         p_granted = p_cu + 4 * (b + 1)
@@ -273,7 +274,7 @@ class KvCache:
             if _rows("q", q, None, self.head_dim, step) != t:
                 raise ValueError(f"k is {k.dtype}, q {q.dtype}")
             heads = q.shape[1]
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = q.new_empty(q.shape)
             qp, qs, op = q.data_ptr(), q.stride(), out.data_ptr()
         if rotary is None:
             cos = sin = None
@@ -308,7 +309,7 @@ def paged_attention(q: torch.Tensor, cache: KvCache, step: Step, *, scale: float
     if window < 0 or (window and not causal):
         raise ValueError(f"a window of {window} needs a causal mask")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(q.shape)
     elif out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous() or out.device != q.device:
         raise ValueError(f"out must be a contiguous {q.dtype} tensor {tuple(q.shape)} on {q.device}")
     if step.num_tokens:
