@@ -350,7 +350,8 @@ class Attention:
         return out
 
     def forward(self, xs: torch.Tensor, cache: KvCache, step: Step) -> torch.Tensor:
-        """``xs`` [.., hidden], ``step.num_tokens`` rows: the step's new tokens in order."""
+        """``xs`` [.., hidden], ``step.num_tokens`` rows: the step's new tokens in order.  Rows behind the
+        last sequence's come out unset."""
         n = step.num_tokens
         q, k, v = (y.view(n, h, self.head_dim) for y, h in zip(self._project(xs), (self.heads, self.kv_heads, self.kv_heads)))
         if self.rotary is None:

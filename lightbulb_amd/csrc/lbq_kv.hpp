@@ -96,8 +96,8 @@ struct KvAttention {
     void *ws;
     size_t ws_bytes;
 };
-// workgroups of either form that a launch may have (of up to 512 threads; both stay below 2^32)
-constexpr int64_t MAX_GROUPS = (int64_t)1 << 22;
+// workgroups of either form that a launch may have (of up to 512 threads: both together below 2^32)
+constexpr int64_t MAX_GROUPS = ((int64_t)1 << 22) - 1;
 size_t kv_attention_workspace(const KvAttention &a);
 hipError_t launch_kv_attention(const KvAttention &a, hipStream_t st);
 

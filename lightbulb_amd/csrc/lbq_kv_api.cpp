@@ -215,7 +215,7 @@ int lbq_kv_append(lbq_ctx *ctx, const lbq_kv_cache *cache, const lbq_kv_step *st
     a.interleaved = interleaved != 0;
     a.max_new = step->max_new;
     const int64_t runs = (a.s.num_tokens >> a.c.log2_page) + 2 * (int64_t)a.s.batch;
-    if (runs * a.c.kv_heads * 2 + 65536 > INT32_MAX)
+    if (runs * a.c.kv_heads * 2 + 65536 >= (int64_t)1 << 24)  // (workgroups of 256 threads: below 2^32)
         return fail(LBQ_ERR_LIMIT, "%lld pages by %d heads in one append", (long long)runs, a.c.kv_heads);
     return launched(ctx, "append launch", [&] { return lbq::launch_kv_append(a, static_cast<hipStream_t>(stream)); });
 }

@@ -353,6 +353,46 @@ def test_captured_beside_eager_calls(dev):
         assert all(torch.equal(a, b) for a, b in zip((*outs, eager), want))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_bounds_that_do_not_hold(dev, dtype):
+    # max_len below a length: the keys behind it are not seen (a single token then sees what a step of that
+    # length shows to all its rows)
+    cache, step, q = setup(dev, "int8", dtype, 16, 64, 2, 4, [300, 20, 2500], [1, 1, 1], pad=0)
+    for most in (10, 130, 2000):
+        low = at.Step(step.tables, step.seq_lens, step.cu_new, None, None, page_size=16, num_tokens=3, max_len=most, max_new=1)
+        cut = at.Step(step.tables, step.seq_lens.clamp(max=most), step.cu_new, None, None, page_size=16, num_tokens=3)
+        check(q, cache, cut, causal=False, got=at.paged_attention(q, cache, low))
+    # max_new below a sequence's rows: the others' are right, and nothing else is touched
+    cache, step, q = setup(dev, "int8", dtype, 16, 64, 2, 4, [300, 20, 100], [4, 40, 3], pad=2)
+    few = at.Step(step.tables, step.seq_lens, step.cu_new, None, None, page_size=16, num_tokens=49, max_new=4)
+    out = torch.full(q.shape, 7.0, dtype=dtype, device=dev)
+    at.paged_attention(q, cache, few, out=out)
+    rest = at.Step(step.tables[[0, 2]], step.seq_lens[[0, 2]], i32([0, 4, 7], dev), None, None, page_size=16, num_tokens=7)
+    check(torch.cat([q[:4], q[44:47]]), cache, rest, got=torch.cat([out[:4], out[44:47]]))
+    assert (out[4:44] == 7.0).all() and (out[47:] == 7.0).all()
+
+
+@pytest.mark.parametrize("new", [[1, 3, 2], [70, 3, 50]])
+def test_queries_of_stride_zero(dev, new):
+    # one query for all heads, one row for all tokens
+    cache, step, q = setup(dev, "int8", torch.float32, 16, 64, 2, 4, [30, 200, 5], new, pad=0)
+    for part in (q[:, :1].expand(q.shape), q[:1].expand(q.shape), q[:1, :1].expand(q.shape)):
+        assert torch.equal(at.paged_attention(part, cache, step), at.paged_attention(part.contiguous(), cache, step))
+
+
+def test_most_sequences(dev):
+    # 65536 rows of a table, most of them idle
+    batch, page, dim = 65536, 16, 64
+    small, one, q = setup(dev, "int8", torch.float32, page, dim, 1, 2, [30, 5, 90], [1, 2, 20], pad=0)
+    tables = torch.full((batch, one.tables.shape[1]), -1, dtype=torch.int32, device=dev)
+    lens, new = torch.zeros(batch, dtype=torch.int32, device=dev), torch.zeros(batch, dtype=torch.int32, device=dev)
+    at_ = torch.tensor([0, 40000, 65535], device=dev)
+    tables[at_], lens[at_], new[at_] = one.tables, one.seq_lens, i32([1, 2, 20], dev)
+    cu = torch.cat([i32([0], dev), new.cumsum(0).to(torch.int32)])
+    step = at.Step(tables, lens, cu, None, None, page_size=page, num_tokens=23)
+    check(q, small, one, got=at.paged_attention(q, small, step))
+
+
 def test_refusals(dev):
     cache, step, q = setup(dev, "int8", torch.float32, 16, 64, 2, 2, [3], [1], pad=0)
     for bad in (q[:, :3], q.double(), q[..., :32], q[0], q.cpu(), torch.cat([q, q])):
@@ -445,3 +485,27 @@ def test_layer_captured(dev):
         torch.cuda.synchronize()
         assert torch.equal(y, want[i]), i
     assert torch.equal(cache.k, cache2.k) and torch.equal(cache.v_scales, cache2.v_scales) and torch.equal(table.tables, table2.tables)
+
+
+def test_layer_of_dense_and_biased_projections(dev):
+    # f16 weights, regular weights with a bias, padding, and a step without tokens
+    hidden, heads, kv, dim, page = 128, 4, 2, 64, 16
+    g = torch.Generator(device=dev).manual_seed(5)
+    rotary = at.Rotary.from_theta(dim, 200, device=dev)
+    w = [torch.randn(n, hidden if i < 3 else heads * dim, generator=g, device=dev) * 0.1 for i, n in enumerate((heads * dim, kv * dim, kv * dim, hidden))]
+    bias = [torch.randn(x.shape[0], generator=g, device=dev) for x in w]
+    dense = [qz.QuantizableLinear.from_qmatmul(qz.QMatMul.from_qtensor(qz.QTensor(x.half().view(torch.uint8).reshape(-1), qz.GgmlDType.F16, tuple(x.shape)))) for x in w[:3]]
+    regular = [qz.QuantizableLinear.from_linear(x, b) for x, b in zip(w, bias)]
+    for projs in ([*dense, regular[3]], regular):
+        layer = at.Attention(*projs, heads, kv, dim, rotary)
+        table, cache, other = at.PageTable(20, page, 2, 8, dev), at.KvCache(20, page, kv, dim, device=dev), at.KvCache(20, page, kv, dim, device=dev)
+        step = table.step(i32([0, 0], dev), i32([21, 3], dev), 30)
+        x = torch.randn(1, 30, hidden, generator=g, device=dev)
+        y = layer(x, cache, step)
+        q, k, v = (p.forward(x).view(30, -1, dim) for p in projs[:3])
+        q = other.append(k, v, step, rotary=rotary, q=q)
+        want = projs[3].forward(at.paged_attention(q, other, step).view(1, 30, heads * dim))
+        assert y.shape == (1, 30, hidden) and torch.allclose(y[:, :24], want[:, :24], rtol=1e-4, atol=1e-4)
+        assert torch.equal(cache.k, other.k) and torch.equal(cache.v_scales, other.v_scales)
+        none = table.step(i32([21, 3], dev), i32([0, 0], dev), 0)
+        assert layer(x[:, :0], cache, none).shape == (1, 0, hidden)

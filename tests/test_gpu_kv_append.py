@@ -182,6 +182,21 @@ def test_sequences_without_slots_leave_the_cache(dev):
         assert all(same(a, b) for a, b in zip(values(cache), before)), cu
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 96])
+def test_rows_of_stride_zero(dev, dtype, dim):
+    # one head's keys for all heads, one token's values for all tokens
+    table, cache = at.PageTable(9, 32, 2, 4, dev), at.KvCache(9, 32, 3, dim, "int8", dev)
+    step = table.step(i32([0, 0], dev), i32([70, 5], dev), 75)
+    k = torch.randn(75, 1, dim, device=dev).to(dtype).expand(75, 3, dim)
+    v = torch.randn(1, 3, dim, device=dev).to(dtype).expand(75, 3, dim)
+    rotary = at.Rotary.from_theta(dim, 80, device=dev)
+    got = cache.append(k, v, step, rotary=rotary, q=k)
+    other = at.KvCache(9, 32, 3, dim, "int8", dev)
+    want = other.append(k.contiguous(), v.contiguous(), step, rotary=rotary, q=k.contiguous())
+    assert torch.equal(got, want) and all(same(a, b) for a, b in zip(values(cache), values(other)))
+
+
 def test_more_tokens_than_the_bound(dev):
     # max_new is the caller's word: a sequence that breaks it is not served, and nothing else is touched
     table, cache = at.PageTable(8, 16, 2, 4, dev), at.KvCache(8, 16, 1, 64, "int8", dev)

@@ -97,6 +97,7 @@ def test_append_arguments(lbq):
     for other in ("q", "k", "v"):
         assert append(lbq, cache(), step(), **{"q": 1 << 22, other: (1 << 20) + 64}) == INVALID
     assert append(lbq, cache(), step(), strides=(128, -1)) == SHAPE
+    assert append(lbq, cache(kv_heads=1024), step(batch=65536)) == LIMIT
     assert append(lbq, cache(), step(num_tokens=0, d_slots=None, d_positions=None), k=None, v=None) == 0
 
 
