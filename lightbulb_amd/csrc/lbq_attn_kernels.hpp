@@ -270,43 +270,47 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
         if (t < end && key < last_hi) p = table[key >> lp];
         return p >= 0 && p < a.c.num_pages ? p : -1;
     };
-    struct Loaded {
-        uint32_t k[4][D / 16];
-        u32x4 v[DB];
-        float ks, vs;
-    };
-    auto load = [&](Loaded &x, int t, int32_t kp, int32_t vp) {
-        const int key = t * TILE;
-        {
-            const uint8_t *p = a.c.k + ((int64_t)max(kp, 0) * H + h) * page_bytes;
-            const int at = (key + 16 * kg) & (P - 1);
+    // one step's codes: keys are asked for when the last step's keys have gone into their products, values
+    // likewise (with registers for two steps' codes the wave copied a ninth of its instructions)
+    uint32_t kc[4][D / 16];
+    u32x4 vc[DB];
+    auto load_keys = [&](int t, int32_t kp) {
+        const uint8_t *p = a.c.k + ((int64_t)max(kp, 0) * H + h) * page_bytes;
+        const int at = (t * TILE + 16 * kg) & (P - 1);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint8_t *row = p + (at + 4 * i + (lane & 3)) * D;
+        for (int i = 0; i < 4; i++) {
+            const uint8_t *row = p + (at + 4 * i + (lane & 3)) * D;
 #pragma unroll
-                for (int j = 0; j < D / 64; j++) {
-                    const u32x4 w = *reinterpret_cast<const u32x4 *>(row + channel(2 * j));
-                    x.k[i][4 * j] = w[0], x.k[i][4 * j + 1] = w[1], x.k[i][4 * j + 2] = w[2], x.k[i][4 * j + 3] = w[3];
-                }
-                if constexpr (D % 64 != 0) {
-                    const u32x2 w = *reinterpret_cast<const u32x2 *>(row + channel(STEPS - 1));
-                    x.k[i][2 * STEPS - 2] = w[0], x.k[i][2 * STEPS - 1] = w[1];
-                }
+            for (int j = 0; j < D / 64; j++) {
+                const u32x4 w = *reinterpret_cast<const u32x4 *>(row + channel(2 * j));
+                kc[i][4 * j] = w[0], kc[i][4 * j + 1] = w[1], kc[i][4 * j + 2] = w[2], kc[i][4 * j + 3] = w[3];
+            }
+            if constexpr (D % 64 != 0) {
+                const u32x2 w = *reinterpret_cast<const u32x2 *>(row + channel(STEPS - 1));
+                kc[i][2 * STEPS - 2] = w[0], kc[i][2 * STEPS - 1] = w[1];
             }
         }
-        const int64_t vh = (int64_t)max(vp, 0) * H + h;
-        const uint8_t *p = a.c.v + vh * page_bytes + n * P + ((key + 16 * c) & (P - 1));
+    };
+    auto load_values = [&](int t, int32_t vp) {
+        const uint8_t *p = a.c.v + ((int64_t)max(vp, 0) * H + h) * page_bytes + n * P + ((t * TILE + 16 * c) & (P - 1));
 #pragma unroll
-        for (int i = 0; i < DB; i++) x.v[i] = *reinterpret_cast<const u32x4 *>(p + i * 16 * P);
-        x.ks = a.c.ks[vh];
-        x.vs = vp >= 0 ? a.c.vs[vh] : 0.f;
+        for (int i = 0; i < DB; i++) vc[i] = *reinterpret_cast<const u32x4 *>(p + i * 16 * P);
+    };
+    auto load_scales = [&](int32_t vp, float &k, float &v) {
+        const int64_t vh = (int64_t)max(vp, 0) * H + h;
+        k = a.c.ks[vh];
+        v = vp >= 0 ? a.c.vs[vh] : 0.f;
     };
 
     int t = begin + wave;
-    Loaded cur;
     int32_t vp = page_of(t, c), kp = page_of(t, kg);
     int32_t vp_next = page_of(t + WAVES, c), kp_next = page_of(t + WAVES, kg);
-    if (t < end) load(cur, t, kp, vp);
+    float ks = 0.f, vs = 0.f;
+    if (t < end) {
+        load_keys(t, kp);
+        load_scales(vp, ks, vs);
+        load_values(t, vp);
+    }
     // the row's parts and the factor of its logits (in powers of two)
     half8 q[STEPS][NS];
     float factor;
@@ -330,9 +334,7 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
     // (the older wave of a SIMD goes first where both could, and would be done long before the other)
     if (wave >= 4) __builtin_amdgcn_s_setprio(1);
     for (; t < end; t += WAVES) {
-        Loaded next;
         const bool more = t + WAVES < end;
-        if (more) load(next, t + WAVES, kp_next, vp_next);
         const int32_t vp_far = page_of(t + 2 * WAVES, c), kp_far = page_of(t + 2 * WAVES, kg);
 
         const int key = t * TILE;
@@ -342,14 +344,19 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
             f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int j = 0; j < STEPS; j++) {
-                const half8 k8 = codes8<KIND>(cur.k[i][2 * j], cur.k[i][2 * j + 1]);
+                const half8 k8 = codes8<KIND>(kc[i][2 * j], kc[i][2 * j + 1]);
 #pragma unroll
                 for (int u = NS - 1; u >= 0; u--) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, q[j][u], s, 0, 0, 0);
             }
 #pragma unroll
             for (int j = 0; j < 4; j++) x[4 * i + j] = s[j];
         }
-        float vmax = fmaxf(cur.vs, __shfl_xor(cur.vs, 16));
+        float ks_next = 0.f, vs_next = 0.f;
+        if (more) {
+            load_keys(t + WAVES, kp_next);
+            load_scales(vp_next, ks_next, vs_next);
+        }
+        float vmax = fmaxf(vs, __shfl_xor(vs, 16));
         vmax = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(fmaxf(vmax, __shfl_xor(vmax, 32)))));
         float grown = 1.f;
         if (vmax > r) {
@@ -358,7 +365,7 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
             grown = r * inv_r;
             r = ldexpf(1.f, e);
         }
-        float f = cur.ks * factor, lv = scale_log(cur.vs, inv_r), back = exp2_fast(-lv);  // f >= 0: the largest product has the largest logit
+        float f = ks * factor, lv = scale_log(vs, inv_r), back = exp2_fast(-lv);  // f >= 0: the largest product has the largest logit
         if (key < last_lo || key + TILE > first_hi || __any(vp < 0)) {
             // some row does not see some of these keys, or they are not there
             const int from = lo - (key + 16 * c), to = vp >= 0 ? hi - (key + 16 * c) : 0;
@@ -368,7 +375,7 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
             if (max(from, 0) >= min(to, 16)) f = 1.f, lv = 0.f, back = 1.f;  // none of them, so neither their scales
             const int keep = vp >= 0 ? min(max(sq.len - (key + 16 * c), 0), 16) : 0;
 #pragma unroll
-            for (int i = 0; i < DB; i++) cur.v[i] = keep_bytes(cur.v[i], keep);
+            for (int i = 0; i < DB; i++) vc[i] = keep_bytes(vc[i], keep);
         }
         float top = larger(x[0], x[1]);
 #pragma unroll
@@ -398,11 +405,12 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
         for (int i = 0; i < DB; i++)
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                const half8 v8 = codes8<KIND>(cur.v[i][2 * u], cur.v[i][2 * u + 1]);
+                const half8 v8 = codes8<KIND>(vc[i][2 * u], vc[i][2 * u + 1]);
 #pragma unroll
                 for (int z = NW - 1; z >= 0; z--) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, p[u][z], o[i], 0, 0, 0);
             }
-        cur = next;
+        if (more) load_values(t + WAVES, vp_next);
+        ks = ks_next, vs = vs_next;
         vp = vp_next, kp = kp_next;
         vp_next = vp_far, kp_next = kp_far;
     }
