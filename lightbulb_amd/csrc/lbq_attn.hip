@@ -18,20 +18,22 @@ struct Layout {
 // lengths are on the device: the counts go by the bounds that the caller gave.
 //
 // Forms: a sequence of up to 16 rows (queries of one kv head's group) is one 16-column tile and takes
-// the short form: 32 single tokens at 4000 keys 47 us, in the long form 111; one at 131071 keys 52 and
+// the short form: 32 single tokens at 4000 keys 45 us, in the long form 111; one at 131071 keys 50 and
 // 117.  More rows would be read once per tile of 16; the long form reads 256 (128 above 128 channels) once.
 //
 // Parts: as many as leave every CU one workgroup.  Up to there each part is so much less work in a
 // row; beyond, a second round costs more than it brings (12 tokens at 8000 keys, 96 workgroups: 2
-// parts 43 us, 3 parts 61; 40 tokens at 4000, 320 workgroups: whole 81, 2 parts 83, 3 parts 89; 1200
-// rows over 4000 keys, 40 tiles: 6 parts 63, 7 parts 83, whole 176).  Parts are joined by a launch of
-// 5 us, so short contexts are left whole: a part has at least one step of 64 keys for each wave in the
-// short form and a context 3 parts' (one token at 8000 keys 17 us, with 2 steps a wave 20, 4 28; at 1000
-// keys 13.0 whole and 12.9 in 2 parts), and 2 steps in the long form and a context 8 (160 rows over 1000
-// keys: 2 steps 23.6 us, 4 27.4, 8 36, whole 51; 400 rows over 200 keys: whole 20.3, 2 parts 22.8).
-// Beside the long form single tokens wait less for their own work than for CUs: 3 steps a wave
-// (a prompt of 200 with two tokens at 8000: 29 us, 1 step 43, 8 steps 64; a prompt of 4000 with four at
-// 4000: 247, 248, 240).
+// parts 40 us, 3 parts 55; 40 tokens at 4000, 320 workgroups: whole 76, 2 parts 76, 3 parts 80; 1200
+// rows over 4000 keys, 40 tiles: 6 parts 60, 7 parts 82, whole 176).  Parts are joined by a launch of
+// 4 to 5 us, so that short contexts are left whole: in the short form up to 2 steps a wave of 64 keys of 128
+// channels (1100 keys: whole 13.3 us, parts 11.8 to 12.3; 800: 11.7, 11.8; at 64 channels 1100: 9.5, 11.9), in
+// the long form up to 7 steps (400 rows over 200 keys: whole 20.3, 2 parts 22.8).  A part has at
+// least 2 steps (short form, 8000 keys of one head: 62 parts 11.9 us, 125 14.1, 31 13.2, 15 14.8; long form, 160 rows
+// over 1000 keys: 2 steps 23.6 us, 4 27.4, 8 36, whole 51).  Beside the long form single tokens get
+// the CUs that it leaves, and parts of 2 steps a wave (a prompt of 100 with eight tokens at 3000 keys:
+// 24 us, 3 steps 30; of 200 with two at 8000: 34, 29, without limit 35); and parts of no more than 16
+// steps a wave where it leaves none (a prompt of 4000 with one token at 131071 keys: 279 us,
+// 8 steps 300, 32 286, whole 797).
 Layout layout(const KvAttention &a) {
     Layout l = {};
     const int64_t group = a.q_heads / a.c.kv_heads, t = a.s.num_tokens;
@@ -46,16 +48,19 @@ Layout layout(const KvAttention &a) {
     const int waves = a.c.head_dim <= 128 ? 8 : 4;
     const int64_t tile_rows = attn::WAVE_ROWS * waves;
     l.plan.tiles = (int)(t * group / tile_rows + a.s.batch);
-    const int64_t cus = num_cus(), steps = (a.max_len + attn::TILE - 1) / attn::TILE;
+    // keys that any of a sequence's rows sees
+    const int64_t seen = a.causal && a.window > 0 ? std::min<int64_t>(a.max_len, a.window + most) : a.max_len;
+    const int64_t cus = num_cus(), steps = (seen + attn::TILE - 1) / attn::TILE;
     const auto splits = [&](int64_t wanted, int64_t least, int64_t launched) {
         return (int)std::max<int64_t>(1, std::min({wanted, steps / least, (int64_t)128, MAX_GROUPS / launched}));
     };
     const int64_t sequences = std::min<int64_t>(a.s.batch, t);
-    const int64_t groups = sequences * a.c.kv_heads, least = (l.any_long ? 3 : 1) * waves;
-    l.plan.splits_short = l.any_short && steps >= 3 * waves ? splits(cus / groups, least, (int64_t)a.s.batch * a.c.kv_heads) : 1;
     // (ragged sequences: the last tile of each is half full in the mean)
     const int64_t tiles = (same ? a.s.batch * ((most * group + tile_rows - 1) / tile_rows) : t * group / tile_rows + (sequences + 1) / 2) * a.c.kv_heads;
     l.plan.splits_long = l.any_long && steps >= 8 ? splits(cus / tiles, 2, (int64_t)l.plan.tiles * a.c.kv_heads) : 1;
+    const int64_t groups = sequences * a.c.kv_heads, least = l.any_long ? 2 * waves : 2;
+    const int64_t wanted = l.any_long ? std::max((cus - tiles) / groups, steps / (16 * waves)) : cus / groups;
+    l.plan.splits_short = l.any_short && steps * a.c.head_dim > 256 * waves ? splits(wanted, least, (int64_t)a.s.batch * a.c.kv_heads) : 1;
     const int64_t per = attn::SHORT_ROWS / group;
     l.plan.short_per = l.any_short && per * a.s.batch < t ? (int)per : 0;
     l.plan.short_tokens = l.plan.short_per ? per * a.s.batch : t;

@@ -205,11 +205,11 @@ __device__ __forceinline__ float part_weight(float m, float l, float top) { retu
 // Bound by reading the cache, 2 head_dim bytes per key: one wave takes 64 keys at a time
 // straight from memory into its operands, the next 64 on their way while it works, with no
 // barrier until the waves' outputs are joined at the end.  32 tokens of 8 heads with ragged contexts
-// of up to 4096 keys of 128 channels, 202.7 MB: 49 us, 4.1 TB/s (a read stream reaches 5.7; here 256
-// workgroups of unlike length start and end apart).  131071 keys of one sequence, 268 MB: 54 us, 5.0 TB/s,
-// and 5 to join 32 parts.  One workgroup takes about 3.3 us for a
-// step of its eight waves (4000 keys: 33 us), and 7 for launch, bounds, pages and the first codes: a
-// short context's time (1000 keys: 13 us).  16x16x32 products; in S^T lane
+// of up to 4096 keys of 128 channels, 202.7 MB: 46 us, 4.4 TB/s (a read stream reaches 5.7; here 256
+// workgroups of unlike length start and end apart).  131071 keys of one sequence, 268 MB: 51 us, 5.3 TB/s,
+// and 4 to join 32 parts.  One workgroup takes about 3 us for a step of its eight waves, half of it the
+// codes' way to f16, and 7 for launch, bounds, pages and the first codes: a short context's time (1000
+// keys: 12 us).  16x16x32 products; in S^T lane
 // (c, n) = (lane / 16, lane % 16) holds keys 16 c .. 16 c + 15 of the 64 for row n, which is
 // what the products with V take, and all of one page: one scale per lane.
 // ---------------------------------------------------------------------------
@@ -849,69 +849,134 @@ __global__ __launch_bounds__(64 * LONG_WAVES<D>, D <= 128 ? 2 : 1) void k_attn_m
 
 // The join of a row's parts, D / 4 threads a row.  Few rows: a workgroup for one row, whose groups take
 // every JOIN_GROUPS-th part and are added in order.  Many: a row for each group of threads.  Bound by
-// latency: rows' bounds, the parts' maxima, the parts; 4.5 to 5 us for 32 rows of 32 parts.  From the
-// call's time: 32 rows of 15 parts 17.2 us with a workgroup a row, 18.5 with a group of threads; 128 rows of
-// 7 parts 17.0 and 18.1; 3200 rows of 15 parts 46.7 and 45.1; 16384 rows of 4 parts 68.1 and 52.6.
+// latency: a row's workgroup asks for maxima, parts and the row's bounds at once (one after the
+// other 8000 keys in 62 parts took 15.7 us, now 11.9).  From the call's time: 32 rows of 15 parts 16.8 us
+// with a workgroup a row, 18.5 with a group of threads; 128 rows of 7 parts 16.8 and 18.0; 3200 rows of 15
+// parts 47.8 and 46.0; 16384 rows of 4 parts 67.4 and 52.
 // The rows are the short form's, if it cut its sequences, and then the long form's, if that did.
 constexpr int JOIN_THREADS = 256, JOIN_ROWS = 1024;  // rows up to which each has a workgroup
 template <int D>
 constexpr int JOIN_GROUPS = JOIN_THREADS / (D / 4);
 
-template <int D, int DT, bool ONE>
-__global__ __launch_bounds__(JOIN_THREADS) void k_attn_join(KvAttention a, AttnPlan plan) {
-    constexpr int G = JOIN_GROUPS<D>;
-    __shared__ f32x4 s_v[ONE ? G : 1][D / 4];
-    __shared__ float s_sum[ONE ? G : 1];
-    const int g = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
-    const int64_t id = ONE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * G + g;
-    const int64_t short_rows = plan.splits_short > 1 ? plan.short_tokens * a.q_heads : 0, long_rows = plan.splits_long > 1 ? a.num_q * a.q_heads : 0;
-    if (g >= G || id >= short_rows + long_rows) return;
-    const bool is_short = id < short_rows;
-    const int64_t row = is_short ? id : id - short_rows;  // (token, head) in its form's order
-    int64_t t = row / a.q_heads;
-    int b = 0;
+// a row of the parts: whose it is, without the sequence's bounds
+struct PartRow {
+    bool is_short;
+    int splits;
+    int64_t row, all, at;  // (token, head) in its form's order; rows of one part; its place in the first part
+};
+__device__ __forceinline__ PartRow part_row(const KvAttention &a, const AttnPlan &plan, int64_t id) {
+    const int64_t short_rows = plan.splits_short > 1 ? plan.short_tokens * a.q_heads : 0;
+    PartRow r;
+    r.is_short = id < short_rows;
+    r.splits = r.is_short ? plan.splits_short : plan.splits_long;
+    r.row = r.is_short ? id : id - short_rows;
+    r.all = r.is_short ? short_rows : a.num_q * a.q_heads;
+    r.at = r.row + (r.is_short ? 0 : plan.long_row);
+    return r;
+}
+// the batch's token t of a row, given sequence b that begins at or before t; false where no sequence has it in this form
+template <class Find>
+__device__ __forceinline__ bool part_token(const KvAttention &a, const AttnPlan &plan, const PartRow &r, Find find, int64_t &t) {
+    t = r.row / a.q_heads;
+    const bool own = r.is_short && plan.short_per;
+    const int b = own ? (int)(t / plan.short_per) : find(t);
     Sequence sq;
-    if (is_short && plan.short_per) {
-        b = (int)(t / plan.short_per);
-        if (!sequence_of(a, b, sq)) return;
-        t += sq.t0 - (int64_t)b * plan.short_per;
-    } else {
-        for (int n = a.s.batch; n > 1;) {  // the last sequence that begins at or before t
+    if (!sequence_of(a, b, sq)) return false;
+    if (own) t += sq.t0 - (int64_t)b * plan.short_per;
+    return t >= sq.t0 && t < sq.t0 + sq.n && (sq.n * plan.group <= plan.short_rows) == r.is_short;
+}
+
+template <int D, int DT>
+__global__ __launch_bounds__(JOIN_THREADS) void k_attn_join_row(KvAttention a, AttnPlan plan) {
+    constexpr int G = JOIN_GROUPS<D>, AHEAD = 8;
+    __shared__ f32x4 s_v[G][D / 4];
+    __shared__ float s_f[JOIN_THREADS], s_top[JOIN_THREADS / 64], s_sum[JOIN_THREADS / 64];
+    const int tid = threadIdx.x, wave = tid >> 6, g = tid / (D / 4), d = tid % (D / 4) * 4;
+    const PartRow r = part_row(a, plan, blockIdx.x);
+    // everything is asked for before the row's sequence is known
+    float m = -INFINITY, l = 0.f;
+    if (tid < r.splits) {
+        const float *const stat = plan.stat + 2 * (r.at + tid * r.all);
+        m = stat[0], l = stat[1];
+    }
+    const float *const part = plan.part + r.at * D + d;
+    f32x4 x[AHEAD];
+#pragma unroll
+    for (int z = 0; z < AHEAD; z++)
+        x[z] = g < G && g + z * G < r.splits ? *reinterpret_cast<const f32x4 *>(part + (g + z * G) * r.all * D) : f32x4{0.f, 0.f, 0.f, 0.f};
+    int64_t t;
+    if (!part_token(a, plan, r, [&](int64_t at) { return find_sequence(a.s.batch, at, [&](int i) { return (int64_t)a.cu_q[i]; }); }, t)) return;
+    float top = m;
+#pragma unroll
+    for (int i = 32; i; i /= 2) top = fmaxf(top, __shfl_xor(top, i));
+    if ((tid & 63) == 0) s_top[wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < JOIN_THREADS / 64; i++) top = fmaxf(top, s_top[i]);
+    const float f = part_weight(m, l, top);
+    s_f[tid] = f;
+    float sum = f;
+#pragma unroll
+    for (int i = 32; i; i /= 2) sum += __shfl_xor(sum, i);
+    if ((tid & 63) == 0) s_sum[wave] = sum;
+    __syncthreads();
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};  // (a part that saw nothing is zero)
+    if (g < G) {
+#pragma unroll
+        for (int z = 0; z < AHEAD; z++)
+            if (g + z * G < r.splits) v += s_f[g + z * G] * x[z];
+        for (int i = g + AHEAD * G; i < r.splits; i += G) v += s_f[i] * *reinterpret_cast<const f32x4 *>(part + i * r.all * D);
+        s_v[g][d / 4] = v;
+    }
+    __syncthreads();
+    if (g) return;
+#pragma unroll
+    for (int i = 1; i < G; i++) v += s_v[i][d / 4];
+    sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < JOIN_THREADS / 64; i++) sum += s_sum[i];
+    float o[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) o[j] = sum == 0.f ? 0.f : v[j] / sum;
+    store_values4<DT>(a.out, (t * a.q_heads + r.row % a.q_heads) * D + d, o);
+}
+
+template <int D, int DT>
+__global__ __launch_bounds__(JOIN_THREADS) void k_attn_join(KvAttention a, AttnPlan plan, int64_t rows) {
+    constexpr int G = JOIN_GROUPS<D>;
+    const int g = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
+    const int64_t id = (int64_t)blockIdx.x * G + g;
+    if (g >= G || id >= rows) return;
+    const PartRow r = part_row(a, plan, id);
+    int64_t t;
+    const auto find = [&](int64_t at) {
+        int b = 0;
+        for (int n = a.s.batch; n > 1;) {  // the last sequence that begins at or before the token
             const int half = n / 2;
-            const bool up = a.cu_q[b + half] <= t;
+            const bool up = a.cu_q[b + half] <= at;
             b += up ? half : 0;
             n = up ? n - half : half;
         }
-        if (!sequence_of(a, b, sq)) return;
-    }
-    if (t < sq.t0 || t >= sq.t0 + sq.n || (sq.n * plan.group <= plan.short_rows) != is_short) return;
-    const int splits = is_short ? plan.splits_short : plan.splits_long;
-    const int64_t all = is_short ? short_rows : long_rows, at = row + (is_short ? 0 : plan.long_row);
-    const float *const stat = plan.stat + 2 * at;
-    const float *const part = plan.part + at * D + d;
+        return b;
+    };
+    if (!part_token(a, plan, r, find, t)) return;
+    const float *const stat = plan.stat + 2 * r.at;
+    const float *const part = plan.part + r.at * D + d;
     float top = -INFINITY;
 #pragma unroll 8
-    for (int i = 0; i < splits; i++) top = fmaxf(top, stat[2 * i * all]);
+    for (int i = 0; i < r.splits; i++) top = fmaxf(top, stat[2 * i * r.all]);
     float sum = 0.f;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int i = ONE ? g : 0; i < splits; i += ONE ? G : 1) {
-        const float f = part_weight(stat[2 * i * all], stat[2 * i * all + 1], top);
+    for (int i = 0; i < r.splits; i++) {
+        const float f = part_weight(stat[2 * i * r.all], stat[2 * i * r.all + 1], top);
         sum += f;
-        v += f * *reinterpret_cast<const f32x4 *>(part + i * all * D);  // (a part that saw nothing is zero)
-    }
-    if constexpr (ONE) {
-        s_v[g][d / 4] = v;
-        if (d == 0) s_sum[g] = sum;
-        __syncthreads();
-        if (g) return;
-#pragma unroll
-        for (int i = 1; i < G; i++) v += s_v[i][d / 4], sum += s_sum[i];
+        v += f * *reinterpret_cast<const f32x4 *>(part + i * r.all * D);  // (a part that saw nothing is zero)
     }
     float o[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) o[j] = sum == 0.f ? 0.f : v[j] / sum;
-    store_values4<DT>(a.out, (t * a.q_heads + row % a.q_heads) * D + d, o);
+    store_values4<DT>(a.out, (t * a.q_heads + r.row % a.q_heads) * D + d, o);
 }
 
 template <int D, int KIND, int DT>
@@ -934,8 +999,8 @@ hipError_t launch_typed(const KvAttention &a, const AttnPlan &plan, bool any_sho
     if (e != hipSuccess) return e;
     if (plan.splits_short == 1 && plan.splits_long == 1) return hipSuccess;
     const int64_t rows = (plan.splits_short > 1 ? plan.short_tokens * a.q_heads : 0) + (plan.splits_long > 1 ? a.num_q * a.q_heads : 0);
-    if (rows <= JOIN_ROWS) k_attn_join<D, DT, true><<<dim3((unsigned)rows), JOIN_THREADS, 0, st>>>(a, plan);
-    else k_attn_join<D, DT, false><<<dim3((unsigned)((rows + JOIN_GROUPS<D> - 1) / JOIN_GROUPS<D>)), JOIN_THREADS, 0, st>>>(a, plan);
+    if (rows <= JOIN_ROWS) k_attn_join_row<D, DT><<<dim3((unsigned)rows), JOIN_THREADS, 0, st>>>(a, plan);
+    else k_attn_join<D, DT><<<dim3((unsigned)((rows + JOIN_GROUPS<D> - 1) / JOIN_GROUPS<D>)), JOIN_THREADS, 0, st>>>(a, plan, rows);
     return hipGetLastError();
 }
 
