@@ -50,6 +50,7 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
@@ -144,6 +145,18 @@ __device__ __forceinline__ void parts8(const float *v, half8 *o) {
     }
 }
 
+// Four values |v| <= 2^22 as whole numbers of three signed digits to the base of 256: o[i] has digit i of
+// each (256^2 o[2] + 256 o[1] + o[0]).  Adding 1.5 * 2^23 leaves a whole number in a float's last bits.
+__device__ __forceinline__ void digits4(const float *v, uint32_t *o) {
+    uint32_t w[4];  // the number + 128 in each digit
+#pragma unroll
+    for (int j = 0; j < 4; j++) w[j] = __float_as_uint(v[j] + 12582912.f) - 0x4b400000u + 0x808080u;
+    const uint32_t ab = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), cd = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
+    o[0] = __builtin_amdgcn_perm(cd, ab, 0x05040100u) ^ 0x80808080u;
+    o[1] = __builtin_amdgcn_perm(cd, ab, 0x07060302u) ^ 0x80808080u;
+    o[2] = (__builtin_amdgcn_perm(w[1], w[0], 0x0c0c0602u) | __builtin_amdgcn_perm(w[3], w[2], 0x06020c0cu)) ^ 0x80808080u;
+}
+
 // the exponent e with |max| < 2^e for the parts of a query row: values times 2^(15 - e) fit f16
 __device__ __forceinline__ int row_exponent(float amax) {
     int e = 0;
@@ -194,7 +207,7 @@ __device__ __forceinline__ float scale_log(float s, float inv_r) {
 }
 
 // A logit's factor where products of -infinity stand for keys that are not seen: not 0, which
-// would make them NaN.  (What it multiplies besides is below 2^33.)
+// would make them NaN.  (What it multiplies besides is below 2^39.)
 __device__ __forceinline__ float not_zero(float f) { return f == 0.f ? 0x1p-126f : f; }
 
 // The join of parts' outputs o_i with maxima m_i and sums l_i: weights l_i 2^(m_i - max).
@@ -205,11 +218,11 @@ __device__ __forceinline__ float part_weight(float m, float l, float top) { retu
 // Bound by reading the cache, 2 head_dim bytes per key: one wave takes 64 keys at a time
 // straight from memory into its operands, the next 64 on their way while it works, with no
 // barrier until the waves' outputs are joined at the end.  32 tokens of 8 heads with ragged contexts
-// of up to 4096 keys of 128 channels, 202.7 MB: 46 us, 4.4 TB/s (a read stream reaches 5.7; here 256
+// of up to 4096 keys of 128 channels, 202.7 MB: 45 us, 4.5 TB/s (a read stream reaches 5.7; here 256
 // workgroups of unlike length start and end apart).  131071 keys of one sequence, 268 MB: 51 us, 5.3 TB/s,
-// and 4 to join 32 parts.  One workgroup takes about 3 us for a step of its eight waves, half of it the
-// codes' way to f16, and 7 for launch, bounds, pages and the first codes: a short context's time (1000
-// keys: 12 us).  16x16x32 products; in S^T lane
+// and 4 to join 32 parts.  One workgroup takes 2.5 us for a step of its eight waves, most of it the
+// values' way to f16 and the weights, and 7 for launch, bounds, pages and the first codes: a short context's
+// time (1000 keys: 11.8 us).  16x16x32 products; in S^T lane
 // (c, n) = (lane / 16, lane % 16) holds keys 16 c .. 16 c + 15 of the 64 for row n, which is
 // what the products with V take, and all of one page: one scale per lane.
 // ---------------------------------------------------------------------------
@@ -221,6 +234,9 @@ template <int D, int KIND, int DT, int WAVES>
 __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan &plan, int group, float *lds) {
     constexpr int NS = QUERY_PARTS<DT>, NW = WEIGHT_PARTS<DT>;
     constexpr int STEPS = D / 32, DB = D / 16;
+    // int8 keys need not go to f16: with the row as whole numbers of three digits the products are
+    // whole too, and exact (32 tokens: 45.2 us, with f16 keys 46.3; at 500 keys 9.2 and 9.7)
+    constexpr bool DIGITS = KIND == KV_INT8;
     float(*const s_o)[SHORT_ROWS][D + 4] = reinterpret_cast<float(*)[SHORT_ROWS][D + 4]>(lds);
     float(*const s_m)[SHORT_ROWS] = reinterpret_cast<float(*)[SHORT_ROWS]>(lds + WAVES * SHORT_ROWS * (D + 4));
     float(*const s_l)[SHORT_ROWS] = s_m + WAVES;
@@ -311,25 +327,38 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
         load_scales(vp, ks, vs);
         load_values(t, vp);
     }
-    // the row's parts and the factor of its logits (in powers of two)
-    half8 q[STEPS][NS];
+    // the row's parts or digits, and the factor of its logits (in powers of two)
+    half8 q[DIGITS ? 1 : STEPS][NS];
+    uint32_t qd[3][DIGITS ? D / 16 : 1];
     float factor;
     {
-        float amax = 0.f;
+        uint32_t most = 0;  // (as whole numbers: what is not finite is the largest)
 #pragma unroll
         for (int s = 0; s < STEPS; s++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) amax = fmaxf(amax, fabsf(raw[s][j]));
-        amax = fmaxf(amax, __shfl_xor(amax, 16));
-        amax = fmaxf(amax, __shfl_xor(amax, 32));
-        const int e = row_exponent(amax);
+            for (int j = 0; j < 8; j++) most = max(most, __float_as_uint(fabsf(raw[s][j])));
+        most = max(most, (uint32_t)__shfl_xor((int)most, 16));
+        most = max(most, (uint32_t)__shfl_xor((int)most, 32));
+        constexpr int BITS = DIGITS ? 22 : 15;
+        const int e = row_exponent(__uint_as_float(most));
 #pragma unroll
         for (int s = 0; s < STEPS; s++) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) raw[s][j] = copysignf(1.f, a.scale) * ldexpf(raw[s][j], 15 - e);
-            parts8<NS>(raw[s], q[s]);
+            for (int j = 0; j < 8; j++) raw[s][j] = copysignf(1.f, a.scale) * ldexpf(raw[s][j], BITS - e);
+            if constexpr (DIGITS) {
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    uint32_t d[3];
+                    digits4(raw[s] + 4 * j, d);
+#pragma unroll
+                    for (int i = 0; i < 3; i++) qd[i][2 * s + j] = d[i];
+                }
+            } else {
+                parts8<NS>(raw[s], q[s]);
+            }
         }
-        factor = ldexpf(fabsf(a.scale) * 1.44269504088896340736f, e - 15);
+        factor = ldexpf(fabsf(a.scale) * 1.44269504088896340736f, e - BITS);
+        if (DIGITS && most >= 0x7f800000u) factor = __uint_as_float(0x7fc00000u);  // (digits cannot say so)
     }
     // (the older wave of a SIMD goes first where both could, and would be done long before the other)
     if (wave >= 4) __builtin_amdgcn_s_setprio(1);
@@ -341,15 +370,32 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
         float x[16];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            f32x4 s = {0.f, 0.f, 0.f, 0.f};
+            if constexpr (DIGITS) {
+                i32x4 s[3] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
-            for (int j = 0; j < STEPS; j++) {
-                const half8 k8 = codes8<KIND>(kc[i][2 * j], kc[i][2 * j + 1]);
+                for (int u = 0; u < 3; u++) {
 #pragma unroll
-                for (int u = NS - 1; u >= 0; u--) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, q[j][u], s, 0, 0, 0);
+                    for (int j = 0; j < D / 64; j++)
+                        s[u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
+                            (i32x4){(int)kc[i][4 * j], (int)kc[i][4 * j + 1], (int)kc[i][4 * j + 2], (int)kc[i][4 * j + 3]},
+                            (i32x4){(int)qd[u][4 * j], (int)qd[u][4 * j + 1], (int)qd[u][4 * j + 2], (int)qd[u][4 * j + 3]}, s[u], 0, 0, 0);
+                    if constexpr (D % 64 != 0)  // (the last 32 channels, and zeros)
+                        s[u] = __builtin_amdgcn_mfma_i32_16x16x64_i8((i32x4){(int)kc[i][D / 16 - 2], (int)kc[i][D / 16 - 1], 0, 0},
+                                                                    (i32x4){(int)qd[u][D / 16 - 2], (int)qd[u][D / 16 - 1], 0, 0}, s[u], 0, 0, 0);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++) x[4 * i + j] = fmaf((float)s[2][j], 65536.f, (float)(256 * s[1][j] + s[0][j]));
+            } else {
+                f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < STEPS; j++) {
+                    const half8 k8 = codes8<KIND>(kc[i][2 * j], kc[i][2 * j + 1]);
+#pragma unroll
+                    for (int u = NS - 1; u >= 0; u--) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, q[j][u], s, 0, 0, 0);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++) x[4 * i + j] = s[j];
             }
-#pragma unroll
-            for (int j = 0; j < 4; j++) x[4 * i + j] = s[j];
         }
         float ks_next = 0.f, vs_next = 0.f;
         if (more) {
