@@ -145,12 +145,13 @@ __device__ __forceinline__ void parts8(const float *v, half8 *o) {
     }
 }
 
-// Four values |v| <= 2^22 as whole numbers of three signed digits to the base of 256: o[i] has digit i of
-// each (256^2 o[2] + 256 o[1] + o[0]).  Adding 1.5 * 2^23 leaves a whole number in a float's last bits.
+// Four values as whole numbers of three signed digits to the base of 256: o[i] has digit i of each
+// (256^2 o[2] + 256 o[1] + o[0]).
+constexpr float MOST_DIGITS = 127 * 65536 + 127 * 256 + 127;
 __device__ __forceinline__ void digits4(const float *v, uint32_t *o) {
     uint32_t w[4];  // the number + 128 in each digit
 #pragma unroll
-    for (int j = 0; j < 4; j++) w[j] = __float_as_uint(v[j] + 12582912.f) - 0x4b400000u + 0x808080u;
+    for (int j = 0; j < 4; j++) w[j] = (uint32_t)(int)rintf(v[j]) + 0x808080u;
     const uint32_t ab = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), cd = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
     o[0] = __builtin_amdgcn_perm(cd, ab, 0x05040100u) ^ 0x80808080u;
     o[1] = __builtin_amdgcn_perm(cd, ab, 0x07060302u) ^ 0x80808080u;
@@ -339,8 +340,9 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
             for (int j = 0; j < 8; j++) most = max(most, __float_as_uint(fabsf(raw[s][j])));
         most = max(most, (uint32_t)__shfl_xor((int)most, 16));
         most = max(most, (uint32_t)__shfl_xor((int)most, 32));
-        constexpr int BITS = DIGITS ? 22 : 15;
-        const int e = row_exponent(__uint_as_float(most));
+        constexpr int BITS = DIGITS ? 23 : 15;
+        int e = row_exponent(__uint_as_float(most));
+        if (DIGITS && ldexpf(__uint_as_float(most), BITS - e) > MOST_DIGITS) e++;
 #pragma unroll
         for (int s = 0; s < STEPS; s++) {
 #pragma unroll
