@@ -76,6 +76,7 @@ class Step:
         self._struct = _lib.KvStepStruct(
             tables.data_ptr(), tables.stride(0), seq_lens.data_ptr(), cu_new.data_ptr(), slots.data_ptr() if slots is not None else None,
             positions.data_ptr() if positions is not None else None, num_tokens, tables.shape[0], tables.shape[1], max_len, max_new)
+        self._ws: dict = {}  # bytes of workspace by heads and head_dim: every layer asks
 
     def across(self, source: "Step") -> "Step":
         """This step's rows over ``source``'s sequences: cross attention of a decoder's queries
@@ -158,6 +159,7 @@ class PageTable:
         s.page_size, s.num_tokens, s.max_len, s.max_new = self.page_size, num_tokens, max_len, max_new
         s.granted, s.free_count, s.device = granted, left, dev
         s._struct = _lib.KvStepStruct(self._places[0], self._places[1], p_lens, p_cu, p_slots, p_pos, num_tokens, b, self._blocks, max_len, max_new)
+        s._ws = {}
         return s
 
     def release(self, lens: torch.Tensor, which: torch.Tensor) -> None:
@@ -313,13 +315,16 @@ def paged_attention(q: torch.Tensor, cache: KvCache, step: Step, *, scale: float
     elif out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous() or out.device != q.device:
         raise ValueError(f"out must be a contiguous {q.dtype} tensor {tuple(q.shape)} on {q.device}")
     if step.num_tokens:
-        lib, n = _lib.lib(), ctypes.c_size_t()
-        _lib.check(lib.lbq_kv_attention_workspace(cache._ctx, cache._struct, step._struct, heads, n))
-        ws = torch.empty(n.value, dtype=torch.uint8, device=q.device) if n.value else None
+        lib, size = _lib.lib(), step._ws.get((heads, kv, dim))
+        if size is None:
+            n = ctypes.c_size_t()
+            _lib.check(lib.lbq_kv_attention_workspace(cache._ctx, cache._struct, step._struct, heads, n))
+            size = step._ws[heads, kv, dim] = n.value
+        ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
         qs = q.stride()
         _lib.check(lib.lbq_kv_attention(
             cache._ctx, cache._struct, step._struct, t, q.data_ptr(), qs[0], qs[1], heads, dim ** -0.5 if scale is None else scale, causal,
-            window, out.data_ptr(), ws.data_ptr() if ws is not None else None, n.value, _stream(q.device)))
+            window, out.data_ptr(), ws.data_ptr() if ws is not None else None, size, _stream(q.device)))
     return out
 
 

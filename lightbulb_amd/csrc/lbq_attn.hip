@@ -22,7 +22,7 @@ struct Layout {
 // 117.  More rows would be read once per tile of 16; the long form reads 256 (128 above 128 channels) once.
 //
 // Parts: as many as leave every CU one workgroup.  Up to there each part is so much less work in a
-// row; beyond, a second round costs more than it brings (12 tokens at 8000 keys, 96 workgroups: 2
+// row; beyond, a second filling of the CUs costs more than it brings (12 tokens at 8000 keys, 96 workgroups: 2
 // parts 40 us, 3 parts 55; 40 tokens at 4000, 320 workgroups: whole 76, 2 parts 76, 3 parts 80; 1200
 // rows over 4000 keys, 40 tiles: 6 parts 60, 7 parts 82, whole 176).  Parts are joined by a launch of
 // 4 to 5 us, so that short contexts are left whole: in the short form up to 2 steps a wave of 64 keys of 128
