@@ -38,6 +38,7 @@ struct AttnPlan {
     int64_t short_tokens, long_row;
     int short_per;                  // 0: the batch's tokens
     int tiles;                      // tiles of the long form, an upper bound
+    int tiles_per;                  // tiles of each sequence; 0: as many as it has rows for, and at most one more
     int group;                      // query heads per kv head
     int short_rows;                 // rows (queries * group) up to which a sequence takes the short form; 0: none does
 };
@@ -556,11 +557,12 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
     const int H = a.c.kv_heads, P = a.c.page_size, lp = a.c.log2_page;
     // the tiles with most keys (a sequence's last) first
     const int h = group % H, split = group / H % plan.splits_long, tile = plan.tiles - 1 - group / H / plan.splits_long;
-    const int b = find_sequence(a.s.batch, tile, [&](int i) { return (int64_t)a.cu_q[i] * plan.group / ROWS + i; });
+    const int b = plan.tiles_per ? tile / plan.tiles_per
+                                 : find_sequence(a.s.batch, tile, [&](int i) { return (int64_t)a.cu_q[i] * plan.group / ROWS + i; });
     Sequence sq;
     if (!sequence_of(a, b, sq) || sq.n * plan.group <= plan.short_rows) return;
     const int rows = sq.n * plan.group;
-    const int row0 = (int)(tile - (sq.t0 * plan.group / ROWS + b)) * ROWS;
+    const int row0 = (plan.tiles_per ? tile % plan.tiles_per : (int)(tile - (sq.t0 * plan.group / ROWS + b))) * ROWS;
     if (row0 < 0 || row0 >= rows) return;
     const int row = row0 + WAVE_ROWS * wave + n;
     const bool mine = row < rows;

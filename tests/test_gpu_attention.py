@@ -372,6 +372,27 @@ def test_bounds_that_do_not_hold(dev, dtype):
     assert (out[4:44] == 7.0).all() and (out[47:] == 7.0).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 256])
+def test_more_rows_than_the_bound_gives_tiles(dev, dtype, dim):
+    # a bound of 20 new tokens, which one sequence breaks: its rows are right or left as they were, the others' are right
+    new = [20, 90, 7, 20]
+    cache, step, q = setup(dev, "int8", dtype, 16, dim, 2, 4, [300, 20, 100, 0], new, pad=2)
+    out = torch.full(q.shape, 7.0, dtype=dtype, device=dev)
+    at.paged_attention(q, cache, at.Step(step.tables, step.seq_lens, step.cu_new, None, None, page_size=16, num_tokens=139, max_new=20), out=out)
+    left = (out[:137] == 7.0).flatten(1).all(1)
+    assert not left[:20].any() and not left[110:].any()
+    filled = torch.where(left[:, None, None], check(q, cache, step)[:137], out[:137])
+    check(q, cache, step, got=torch.cat([filled, out[137:]]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("batch,new", [(33, 5), (7, 70), (3, 200)])
+def test_sequences_of_one_length(dev, dtype, batch, new):
+    cache, step, q = setup(dev, "e4m3", dtype, 32, 128, 2, 4, [(i * 37) % 150 for i in range(batch)], [new] * batch, pad=0)
+    check(q, cache, at.Step(step.tables, step.seq_lens, step.cu_new, None, None, page_size=32, num_tokens=batch * new, max_new=new))
+
+
 @pytest.mark.parametrize("new", [[1, 3, 2], [70, 3, 50]])
 def test_queries_of_stride_zero(dev, new):
     # one query for all heads, one row for all tokens
