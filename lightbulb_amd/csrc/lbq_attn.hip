@@ -47,10 +47,13 @@ Layout layout(const KvAttention &a) {
     // waves of a workgroup, in either form and also all that a CU holds
     const int waves = a.c.head_dim <= 128 ? 8 : 4;
     const int64_t tile_rows = attn::WAVE_ROWS * waves;
-    // Tiles by the sequences' rows, some of them empty and anywhere among the others; or of a number for
-    // each sequence where that is no more: no empty ones where all have as many rows (32 sequences of 5
-    // tokens at 2000 keys, 256 tiles: 61 us, with 16 empty ones between them 118: workgroups are dealt out to
-    // the shader engines in turn, and one had 9 for its 8 CUs).
+    // Workgroups are dealt out to the shader engines in turn, whatever they do: with idle ones between the
+    // others some engines have too many (32 sequences of 5 tokens at 2000 keys, 256 tiles and 16 empty ones: 118 and 61).  So tiles are a
+    // number for each sequence, where that is no more than by their rows; and where sequences may be idle or
+    // of the other form, up to 256 of them are counted by each workgroup for itself (32 tokens, every
+    // second of 64 sequences: 60 and 45 us, every fourth of 128: 117 and 45; a few more cycles a workgroup).
+    l.plan.listed = a.s.batch > 1 && a.s.batch <= attn::LISTED && !same;
+    l.plan.short_sequences = (int)(l.plan.listed ? std::min<int64_t>(a.s.batch, t) : a.s.batch);
     const int64_t per_sequence = (most * group + tile_rows - 1) / tile_rows, by_rows = t * group / tile_rows + a.s.batch;
     l.plan.tiles_per = a.max_new && per_sequence * a.s.batch <= by_rows ? (int)per_sequence : 0;
     l.plan.tiles = (int)(l.plan.tiles_per ? per_sequence * a.s.batch : by_rows);

@@ -38,7 +38,9 @@ struct AttnPlan {
     int64_t short_tokens, long_row;
     int short_per;                  // 0: the batch's tokens
     int tiles;                      // tiles of the long form, an upper bound
-    int tiles_per;                  // tiles of each sequence; 0: as many as it has rows for, and at most one more
+    int tiles_per;                  // no sequence has more tiles than these; 0: not known
+    int short_sequences;            // no more sequences take the short form
+    int listed;                     // whether sequences and tiles are counted on the device, without those of another form
     int group;                      // query heads per kv head
     int short_rows;                 // rows (queries * group) up to which a sequence takes the short form; 0: none does
 };
@@ -187,6 +189,69 @@ __device__ __forceinline__ bool sequence_of(const KvAttention &a, int b, Sequenc
     return true;
 }
 
+// Item x of a list that holds count(i) items of each sequence i in order, for up to LISTED sequences:
+// its sequence and its place among that one's; or, where `last` is set, the x-th item from the end.  The same
+// x in every lane of a wave; all 64 lanes call it.
+constexpr int LISTED = 256;
+template <class Count>
+__device__ __forceinline__ bool find_item(int batch, int x, bool last, Count count, int &b, int &index) {
+    constexpr int PER = LISTED / 64;
+    const int lane = threadIdx.x & 63;
+    int c[PER], sum = 0;
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+        c[j] = lane * PER + j < batch ? count(lane * PER + j) : 0;
+        sum += c[j];
+    }
+    int upto = sum;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int before = __shfl_up(upto, d);
+        if (lane >= d) upto += before;
+    }
+    const int total = __builtin_amdgcn_readlane(upto, 63);
+    if (x >= total) return false;
+    if (last) x = total - 1 - x;
+    const int at = __popcll(__ballot(upto <= x));  // (sums never fall: the lanes before the item's)
+    index = x - __builtin_amdgcn_readlane(upto - sum, at);
+    b = at * PER;
+    bool found = false;
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+        const int n = __builtin_amdgcn_readlane(c[j], at);
+        found |= index < n;
+        if (!found) index -= n, b++;
+    }
+    return true;
+}
+
+// The same where each sequence holds one item or none: by counting bits alone.
+template <class Has>
+__device__ __forceinline__ bool find_one(int batch, int x, bool last, Has has, int &b) {
+    constexpr int PER = LISTED / 64;
+    const int lane = threadIdx.x & 63;
+    uint64_t mask[PER], in = 0;
+    int total = 0;
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+        mask[j] = __ballot(64 * j + lane < batch && has(64 * j + lane));
+        total += __popcll(mask[j]);
+    }
+    if (x >= total) return false;
+    if (last) x = total - 1 - x;
+    b = 0;
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+        const int n = __popcll(mask[j]);
+        if (in) continue;
+        if (x < n) in = mask[j], b = 64 * j;
+        else x -= n;
+    }
+    const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
+    b += __ffsll((unsigned long long)__ballot((in >> lane & 1) && before == x)) - 1;
+    return true;
+}
+
 // keys [lo, hi) that the query at position pos sees
 __device__ __forceinline__ void seen_range(const KvAttention &a, const Sequence &s, int pos, int &lo, int &hi) {
     hi = a.causal ? max(min(s.len, pos + 1), 0) : s.len;
@@ -244,7 +309,16 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
     float(*const s_l)[SHORT_ROWS] = s_m + WAVES;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, c = lane >> 4;
     const int H = a.c.kv_heads, P = a.c.page_size, lp = a.c.log2_page;
-    const int h = group % H, split = group / H % plan.splits_short, b = group / H / plan.splits_short;
+    const int h = group % H, split = group / H % plan.splits_short;
+    int b = group / H / plan.splits_short;
+    if (plan.listed) {
+        const int most = plan.short_rows / plan.group;
+        const auto mine = [&](int i) {
+            const int n = a.cu_q[i + 1] - a.cu_q[i];
+            return n > 0 && n <= most;
+        };
+        if (!find_one(a.s.batch, b, false, mine, b)) return;
+    }
     Sequence sq;
     if (!sequence_of(a, b, sq) || sq.n * plan.group > plan.short_rows) return;
     const int rows = sq.n * plan.group;
@@ -556,14 +630,32 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, hf = lane >> 5;
     const int H = a.c.kv_heads, P = a.c.page_size, lp = a.c.log2_page;
     // the tiles with most keys (a sequence's last) first
-    const int h = group % H, split = group / H % plan.splits_long, tile = plan.tiles - 1 - group / H / plan.splits_long;
-    const int b = plan.tiles_per ? tile / plan.tiles_per
-                                 : find_sequence(a.s.batch, tile, [&](int i) { return (int64_t)a.cu_q[i] * plan.group / ROWS + i; });
+    const int h = group % H, split = group / H % plan.splits_long;
+    int b, tile;  // (of the sequence)
+    if (plan.listed) {
+        const int least = plan.short_rows / plan.group, most = plan.tiles_per ? plan.tiles_per : plan.tiles, x = group / H / plan.splits_long;
+        const auto new_tokens = [&](int i) { return a.cu_q[i + 1] - a.cu_q[i]; };
+        if (most == 1) {
+            tile = 0;
+            if (!find_one(a.s.batch, x, true, [&](int i) { return new_tokens(i) > least; }, b)) return;
+        } else {
+            const auto tiles = [&](int i) {
+                const int n = new_tokens(i);
+                return n > least ? (int)min(((int64_t)n * plan.group + ROWS - 1) / ROWS, (int64_t)most) : 0;
+            };
+            if (!find_item(a.s.batch, x, true, tiles, b, tile)) return;
+        }
+    } else {
+        tile = plan.tiles - 1 - group / H / plan.splits_long;
+        b = plan.tiles_per ? tile / plan.tiles_per
+                           : find_sequence(a.s.batch, tile, [&](int i) { return (int64_t)a.cu_q[i] * plan.group / ROWS + i; });
+        tile -= plan.tiles_per ? b * plan.tiles_per : (int)((int64_t)a.cu_q[b] * plan.group / ROWS) + b;
+    }
     Sequence sq;
     if (!sequence_of(a, b, sq) || sq.n * plan.group <= plan.short_rows) return;
     const int rows = sq.n * plan.group;
-    const int row0 = (plan.tiles_per ? tile % plan.tiles_per : (int)(tile - (sq.t0 * plan.group / ROWS + b))) * ROWS;
-    if (row0 < 0 || row0 >= rows) return;
+    if (tile < 0 || tile >= (rows + ROWS - 1) / ROWS) return;
+    const int row0 = tile * ROWS;
     const int row = row0 + WAVE_ROWS * wave + n;
     const bool mine = row < rows;
     const int tok = (mine ? row : rows - 1) / plan.group, head = h * plan.group + (mine ? row : rows - 1) % plan.group;
@@ -1031,7 +1123,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_attn_join(KvAttention a, AttnP
 
 template <int D, int KIND, int DT>
 hipError_t launch_typed(const KvAttention &a, const AttnPlan &plan, bool any_short, bool any_long, hipStream_t st) {
-    const int short_groups = any_short ? plan.splits_short * a.c.kv_heads * a.s.batch : 0;
+    const int short_groups = any_short ? plan.splits_short * a.c.kv_heads * plan.short_sequences : 0;
     const auto launch = [&](auto k, int groups, int threads, size_t lds, auto... more) {
         if (lds > 65536) {
             hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);

@@ -302,6 +302,20 @@ def test_batches(dev, batch):
     check(q, cache, step)
 
 
+@pytest.mark.parametrize("batch", [2, 63, 64, 65, 256, 257])
+@pytest.mark.parametrize("most", [1, 3, 150])
+@pytest.mark.parametrize("hinted", [False, True])
+def test_idle_sequences(dev, batch, most, hinted):
+    # few of many sequences have new tokens, the first, the last and some between, of either form
+    rng = random.Random(batch + most)
+    new = [rng.choice((1, most, most)) if i in (0, batch - 1) or rng.random() < 0.15 else 0 for i in range(batch)]
+    cache, step, q = setup(dev, "int8", torch.float32, 16, 64, 1, 4, [rng.randint(0, 60) for _ in new], new)
+    if hinted:
+        step = at.Step(step.tables, step.seq_lens, step.cu_new, None, None, page_size=16, num_tokens=step.num_tokens, max_len=step.seq_lens.max().item(),
+                       max_new=max(new))
+    check(q, cache, step)
+
+
 def test_bad_rows(dev):
     # cu_new that is no list of rows: nothing out of bounds is written
     cache, step, q = setup(dev, "int8", torch.float32, 16, 64, 1, 2, [30, 30], [4, 70], pad=0)
