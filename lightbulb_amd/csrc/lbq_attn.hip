@@ -19,7 +19,12 @@ struct Layout {
 //
 // Forms: a sequence of up to 16 rows (queries of one kv head's group) is one 16-column tile and takes
 // the short form: 32 single tokens at 4000 keys 45 us, in the long form 111; one at 131071 keys 50 and
-// 117.  More rows would be read once per tile of 16; the long form reads 256 (128 above 128 channels) once.
+// 117.  More rows are more tiles, which read the keys again but out of the caches; the long form reads 256
+// rows (128 above 128 channels) once, and has one wave of eight at work for each 32.  Where no sequence has more
+// than 48 rows the short form takes all (5 tokens of 4 heads, 32 sequences at 2000 keys: 41 us and 61, 8 at 4000: 25
+// and 40; 12 tokens: 57 and 65, 31 and 42), or 64 where their tiles fit the CUs at once (16 tokens, 8
+// sequences: 31 and 43; 32, which do not fit: 73 and 65).  Beside longer sequences it takes those of one
+// tile (2 tiles: a prompt of 200 with two tokens at 8000 keys 36 us, one tile 31).
 //
 // Parts: as many as leave every CU one workgroup.  Up to there each part is so much less work in a
 // row; beyond, a second filling of the CUs costs more than it brings (12 tokens at 8000 keys, 96 workgroups: 2
@@ -39,11 +44,16 @@ Layout layout(const KvAttention &a) {
     const int64_t group = a.q_heads / a.c.kv_heads, t = a.s.num_tokens;
     const int64_t most = a.max_new ? std::min<int64_t>(a.max_new, t) : t;
     l.plan.group = (int)group;
-    // where all sequences have more than 16 rows, the long form takes whatever is there
+    // where all sequences have more rows than the short form takes, the long form takes whatever is there
     const bool same = a.max_new && most * a.s.batch == t;
-    l.any_long = most * group > attn::SHORT_ROWS;
-    l.any_short = group <= attn::SHORT_ROWS && !(same && l.any_long);
-    l.plan.short_rows = l.any_short ? attn::SHORT_ROWS : 0;
+    const int64_t cus = num_cus(), heads = (int64_t)a.s.batch * a.c.kv_heads;
+    const int64_t row_tiles = (most * group + attn::SHORT_ROWS - 1) / attn::SHORT_ROWS, limit = 4 * heads <= cus ? 4 : heads <= MAX_GROUPS / 4 ? 3 : 1;
+    const int64_t short_tiles = row_tiles <= limit ? row_tiles : 1;
+    const int64_t short_rows = short_tiles * attn::SHORT_ROWS;
+    l.any_long = most * group > short_rows;
+    l.any_short = group <= short_rows && !(same && l.any_long);
+    l.plan.short_rows = l.any_short ? (int)short_rows : 0;
+    l.plan.short_tiles = (int)short_tiles;
     // waves of a workgroup, in either form and also all that a CU holds
     const int waves = a.c.head_dim <= 128 ? 8 : 4;
     const int64_t tile_rows = attn::WAVE_ROWS * waves;
@@ -53,13 +63,13 @@ Layout layout(const KvAttention &a) {
     // of the other form, up to 256 of them are counted by each workgroup for itself (32 tokens, every
     // second of 64 sequences: 60 and 45 us, every fourth of 128: 117 and 45; a few more cycles a workgroup).
     l.plan.listed = a.s.batch > 1 && a.s.batch <= attn::LISTED && !same;
-    l.plan.short_sequences = (int)(l.plan.listed ? std::min<int64_t>(a.s.batch, t) : a.s.batch);
+    l.plan.short_groups = (int)((l.plan.listed ? std::min<int64_t>(a.s.batch, t) : a.s.batch) * short_tiles);
     const int64_t per_sequence = (most * group + tile_rows - 1) / tile_rows, by_rows = t * group / tile_rows + a.s.batch;
     l.plan.tiles_per = a.max_new && per_sequence * a.s.batch <= by_rows ? (int)per_sequence : 0;
     l.plan.tiles = (int)(l.plan.tiles_per ? per_sequence * a.s.batch : by_rows);
     // keys that any of a sequence's rows sees
     const int64_t seen = a.causal && a.window > 0 ? std::min<int64_t>(a.max_len, a.window + most) : a.max_len;
-    const int64_t cus = num_cus(), steps = (seen + attn::TILE - 1) / attn::TILE;
+    const int64_t steps = (seen + attn::TILE - 1) / attn::TILE;
     const auto splits = [&](int64_t wanted, int64_t least, int64_t launched) {
         return (int)std::max<int64_t>(1, std::min({wanted, steps / least, (int64_t)128, MAX_GROUPS / launched}));
     };
@@ -67,10 +77,10 @@ Layout layout(const KvAttention &a) {
     // (ragged sequences: the last tile of each is half full in the mean)
     const int64_t tiles = (l.plan.tiles_per ? l.plan.tiles : t * group / tile_rows + (sequences + 1) / 2) * a.c.kv_heads;
     l.plan.splits_long = l.any_long && steps >= 8 ? splits(cus / tiles, 2, (int64_t)l.plan.tiles * a.c.kv_heads) : 1;
-    const int64_t groups = sequences * a.c.kv_heads, least = l.any_long ? 2 * waves : 2;
+    const int64_t groups = sequences * a.c.kv_heads * short_tiles, least = l.any_long ? 2 * waves : 2;
     const int64_t wanted = l.any_long ? std::max((cus - tiles) / groups, steps / (16 * waves)) : cus / groups;
-    l.plan.splits_short = l.any_short && steps * a.c.head_dim > 256 * waves ? splits(wanted, least, (int64_t)a.s.batch * a.c.kv_heads) : 1;
-    const int64_t per = attn::SHORT_ROWS / group;
+    l.plan.splits_short = l.any_short && steps * a.c.head_dim > 256 * waves ? splits(wanted, least, (int64_t)l.plan.short_groups * a.c.kv_heads) : 1;
+    const int64_t per = short_rows / group;
     l.plan.short_per = l.any_short && per * a.s.batch < t ? (int)per : 0;
     l.plan.short_tokens = l.plan.short_per ? per * a.s.batch : t;
     l.short_rows = l.plan.short_tokens * a.q_heads;

@@ -39,7 +39,8 @@ struct AttnPlan {
     int short_per;                  // 0: the batch's tokens
     int tiles;                      // tiles of the long form, an upper bound
     int tiles_per;                  // no sequence has more tiles than these; 0: not known
-    int short_sequences;            // no more sequences take the short form
+    int short_groups;               // tiles of the short form (16 rows), an upper bound
+    int short_tiles;                // of each sequence, likewise
     int listed;                     // whether sequences and tiles are counted on the device, without those of another form
     int group;                      // query heads per kv head
     int short_rows;                 // rows (queries * group) up to which a sequence takes the short form; 0: none does
@@ -57,8 +58,7 @@ typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-// rows of one kv head's queries that the short form takes: one 16-column tile
-constexpr int SHORT_ROWS = 16;
+constexpr int SHORT_ROWS = 16;  // rows of one kv head's queries in a tile of the short form
 constexpr int TILE = 64;  // keys per step of either form
 
 // f16 parts of a query value and of a weight.  f16 outputs take weights of two parts too: one
@@ -281,7 +281,7 @@ __device__ __forceinline__ float not_zero(float f) { return f == 0.f ? 0x1p-126f
 __device__ __forceinline__ float part_weight(float m, float l, float top) { return l * exp2_fast(m - base_of(top)); }
 
 // ---------------------------------------------------------------------------
-// Short form: up to 16 query rows of one kv head (a token step: its group of query heads).
+// Short form: tiles of up to 16 query rows of one kv head (a token step: its group of query heads).
 // Bound by reading the cache, 2 head_dim bytes per key: one wave takes 64 keys at a time
 // straight from memory into its operands, the next 64 on their way while it works, with no
 // barrier until the waves' outputs are joined at the end.  32 tokens of 8 heads with ragged contexts
@@ -296,7 +296,7 @@ __device__ __forceinline__ float part_weight(float m, float l, float top) { retu
 template <int D, int WAVES>
 constexpr size_t short_lds() { return sizeof(float) * WAVES * SHORT_ROWS * (D + 4 + 2); }
 
-// group: its place among the form's workgroups (parts * kv heads * sequences); lds: short_lds bytes
+// group: its place among the form's workgroups (parts * kv heads * tiles); lds: short_lds bytes
 template <int D, int KIND, int DT, int WAVES>
 __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan &plan, int group, float *lds) {
     constexpr int NS = QUERY_PARTS<DT>, NW = WEIGHT_PARTS<DT>;
@@ -310,24 +310,26 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, c = lane >> 4;
     const int H = a.c.kv_heads, P = a.c.page_size, lp = a.c.log2_page;
     const int h = group % H, split = group / H % plan.splits_short;
-    int b = group / H / plan.splits_short;
+    const int x = group / H / plan.splits_short;
+    int b = x / plan.short_tiles, tile = x % plan.short_tiles;  // (of the sequence)
     if (plan.listed) {
         const int most = plan.short_rows / plan.group;
-        const auto mine = [&](int i) {
+        const auto tiles = [&](int i) {
             const int n = a.cu_q[i + 1] - a.cu_q[i];
-            return n > 0 && n <= most;
+            return n > 0 && n <= most ? (n * plan.group + SHORT_ROWS - 1) / SHORT_ROWS : 0;
         };
-        if (!find_one(a.s.batch, b, false, mine, b)) return;
+        if (plan.short_tiles == 1 ? !find_one(a.s.batch, x, false, tiles, b) : !find_item(a.s.batch, x, false, tiles, b, tile)) return;
     }
     Sequence sq;
     if (!sequence_of(a, b, sq) || sq.n * plan.group > plan.short_rows) return;
-    const int rows = sq.n * plan.group;
-    const int tok = n / plan.group, head = h * plan.group + n % plan.group;
+    const int row0 = tile * SHORT_ROWS, rows = min(sq.n * plan.group - row0, SHORT_ROWS);
+    if (rows <= 0) return;
     const bool mine = n < rows;
+    const int tok = (row0 + (mine ? n : 0)) / plan.group, head = h * plan.group + (row0 + (mine ? n : 0)) % plan.group;
     int lo, hi, first_lo, first_hi, last_lo, last_hi;
-    seen_range(a, sq, sq.first + (mine ? tok : 0), lo, hi);
-    seen_range(a, sq, sq.first, first_lo, first_hi);
-    seen_range(a, sq, sq.first + sq.n - 1, last_lo, last_hi);
+    seen_range(a, sq, sq.first + tok, lo, hi);
+    seen_range(a, sq, sq.first + row0 / plan.group, first_lo, first_hi);
+    seen_range(a, sq, sq.first + (row0 + rows - 1) / plan.group, last_lo, last_hi);
     if (!mine) hi = 0;
     // this part's steps of 64 keys: every WAVES-th is this wave's
     const int t_lo = first_lo / TILE, t_hi = (last_hi + TILE - 1) / TILE;
@@ -341,7 +343,7 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
     // (the first keys are asked for before the row is looked at: each waits for memory once)
     float raw[STEPS][8];
     {
-        const int64_t at = (sq.t0 + (mine ? tok : 0)) * a.q.token_stride + (int64_t)(mine ? head : h * plan.group) * a.q.head_stride;
+        const int64_t at = (sq.t0 + tok) * a.q.token_stride + (int64_t)head * a.q.head_stride;
 #pragma unroll
         for (int s = 0; s < STEPS; s++)
 #pragma unroll
@@ -562,7 +564,7 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
         }
 #pragma unroll
         for (int j = 0; j < 4; j++) v[j] = sum == 0.f ? 0.f : v[j] / sum;
-        const int tok = row / plan.group, head = h * plan.group + row % plan.group;
+        const int tok = (row0 + row) / plan.group, head = h * plan.group + (row0 + row) % plan.group;
         if (plan.splits_short == 1) {
             store_values4<DT>(a.out, ((int64_t)(sq.t0 + tok) * a.q_heads + head) * D + d, v);
         } else {
@@ -1123,7 +1125,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_attn_join(KvAttention a, AttnP
 
 template <int D, int KIND, int DT>
 hipError_t launch_typed(const KvAttention &a, const AttnPlan &plan, bool any_short, bool any_long, hipStream_t st) {
-    const int short_groups = any_short ? plan.splits_short * a.c.kv_heads * plan.short_sequences : 0;
+    const int short_groups = any_short ? plan.splits_short * a.c.kv_heads * plan.short_groups : 0;
     const auto launch = [&](auto k, int groups, int threads, size_t lds, auto... more) {
         if (lds > 65536) {
             hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);

@@ -316,6 +316,21 @@ def test_idle_sequences(dev, batch, most, hinted):
     check(q, cache, step)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("kv,group,ctx,new", [(1, 7, [5000], [5]), (2, 4, [300, 0, 2000], [16, 16, 3]), (1, 3, [700, 20], [21, 1]), (3, 8, [90] * 9, [5] * 9),
+                                              (1, 17, [4000, 10], [1, 3]), (1, 1, [1500], [64]), (8, 2, [40] * 6, [24] * 6)])
+def test_few_tokens(dev, dtype, kind, kv, group, ctx, new):
+    # up to 64 rows of a kv head: tiles that end inside a token's heads
+    cache, step, q = setup(dev, kind, dtype, 32, 128, kv, group, ctx, new)
+    lens = [c + n for c, n in zip(ctx, new)]
+    hinted = at.Step(step.tables, step.seq_lens, step.cu_new, None, None, page_size=32, num_tokens=step.num_tokens, max_len=max(lens), max_new=max(new))
+    check(q, cache, step)
+    check(q, cache, hinted)
+    check(q, cache, hinted, window=37)
+    check(q, cache, hinted, causal=False)
+
+
 def test_bad_rows(dev):
     # cu_new that is no list of rows: nothing out of bounds is written
     cache, step, q = setup(dev, "int8", torch.float32, 16, 64, 1, 2, [30, 30], [4, 70], pad=0)
