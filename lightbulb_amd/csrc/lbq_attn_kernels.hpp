@@ -1018,8 +1018,9 @@ __device__ __forceinline__ PartRow part_row(const KvAttention &a, const AttnPlan
     r.at = r.row + (r.is_short ? 0 : plan.long_row);
     return r;
 }
-// the batch's token t of a row, given sequence b that begins at or before t; false where no sequence has it in this form
-template <class Find>
+// the batch's token t of a row, given sequence b that begins at or before t; false where no sequence has it in this
+// form, or where it lies behind the tiles that the bound on new tokens gives (its parts are nobody's)
+template <int D, class Find>
 __device__ __forceinline__ bool part_token(const KvAttention &a, const AttnPlan &plan, const PartRow &r, Find find, int64_t &t) {
     t = r.row / a.q_heads;
     const bool own = r.is_short && plan.short_per;
@@ -1027,6 +1028,10 @@ __device__ __forceinline__ bool part_token(const KvAttention &a, const AttnPlan 
     Sequence sq;
     if (!sequence_of(a, b, sq)) return false;
     if (own) t += sq.t0 - (int64_t)b * plan.short_per;
+    if (!r.is_short && plan.tiles_per) {
+        const int64_t row = (t - sq.t0) * plan.group + r.row % a.q_heads % plan.group;
+        if (row >= (int64_t)plan.tiles_per * WAVE_ROWS * LONG_WAVES<D>) return false;
+    }
     return t >= sq.t0 && t < sq.t0 + sq.n && (sq.n * plan.group <= plan.short_rows) == r.is_short;
 }
 
@@ -1049,7 +1054,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_attn_join_row(KvAttention a, A
     for (int z = 0; z < AHEAD; z++)
         x[z] = g < G && g + z * G < r.splits ? *reinterpret_cast<const f32x4 *>(part + (g + z * G) * r.all * D) : f32x4{0.f, 0.f, 0.f, 0.f};
     int64_t t;
-    if (!part_token(a, plan, r, [&](int64_t at) { return find_sequence(a.s.batch, at, [&](int i) { return (int64_t)a.cu_q[i]; }); }, t)) return;
+    if (!part_token<D>(a, plan, r, [&](int64_t at) { return find_sequence(a.s.batch, at, [&](int i) { return (int64_t)a.cu_q[i]; }); }, t)) return;
     float top = m;
 #pragma unroll
     for (int i = 32; i; i /= 2) top = fmaxf(top, __shfl_xor(top, i));
@@ -1103,7 +1108,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_attn_join(KvAttention a, AttnP
         }
         return b;
     };
-    if (!part_token(a, plan, r, find, t)) return;
+    if (!part_token<D>(a, plan, r, find, t)) return;
     const float *const stat = plan.stat + 2 * r.at;
     const float *const part = plan.part + r.at * D + d;
     float top = -INFINITY;
