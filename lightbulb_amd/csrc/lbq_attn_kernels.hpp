@@ -11,11 +11,13 @@
 // accumulator layout of S^T (column = lane mod 16 or 32, rows in registers) is already the operand
 // layout of P^T once the rows of K are taken in the right order.  Weights never leave registers.
 //
-// Weights are exponentials relative to a base that follows the running maximum and is moved only
-// when the maximum is 2^6 above it (moving it multiplies all accumulators).  They carry a factor 2^9,
-// so that they stay below 2^15 and both their f16 parts of those that matter clear of the
-// subnormals; the row's sum carries it too.  Value scales are applied to the weights, inside the
-// exponential, relative to a power of two r that no scale seen so far exceeds.
+// Value scales are applied to the weights, inside the exponential: a weight is 2^(x + s - b), x the logit
+// and 2^s the key's value scale relative to a power of two r that no scale seen so far exceeds.  Its base b
+// follows the row's largest x + s, not its largest x, so that what decides the row's result is held to the
+// same bits whatever other pages' scales are: seen with no weight, or by other rows only.  b is moved only when
+// the maximum is 2^6 above it (moving it multiplies all accumulators).  Weights carry a factor 2^9, so
+// that they stay below 2^15 and both f16 parts of those that matter clear of the subnormals.  The row's sum
+// is that of 2^(x - b) with the same factor.
 #pragma once
 #include "lbq_kv.hpp"
 
@@ -265,12 +267,45 @@ __device__ __forceinline__ float seen_or_not(float x, int j, int from, int to) {
     return __uint_as_float((out & 0xff800000u) | (~out & __float_as_uint(x)));
 }
 
-// The weights' factor for a value scale s, relative to r and in powers of two.  Below 2^-45 a
-// weight of at most 2^15 is less than half the smallest f16 step whatever it is, so that the
-// bound changes nothing, and keeps the inverse finite for a scale of 0.
+// The weights' factor for a value scale s, relative to r and in powers of two.  A scale below 2^-80 r, or of 0,
+// counts as that.  So no logit of a row is more than 86 above b (which is at most 6 behind the logit less 80):
+// a row's sum stays below 2^95 for each key.  And b is no more than the largest logit: a key that matters to
+// the sum, 2^-30 of it say, has a weight of at least 2^(9 - 30 - 80), a normal number.
 // (The last term is 0, or NaN for a scale that is.)
 __device__ __forceinline__ float scale_log(float s, float inv_r) {
-    return fmaf(s, 0.f, fmaxf(__builtin_amdgcn_logf(s * inv_r), -45.f));
+    return fmaf(s, 0.f, fmaxf(__builtin_amdgcn_logf(s * inv_r), -80.f));
+}
+
+// what a row's weights are relative to, in powers of two
+struct Base {
+    float b = -INFINITY;
+    float r = 0.f, inv_r = 1.f;
+
+    // r grows to 2^e and b falls as much, but no lane's part l of the row's sum (the largest: row_l) passes 2^100 by
+    // it: the outputs' factor, 1 (or what the rounding of b leaves) unless the sum keeps b up.  Outputs under
+    // scales of 0 stand for nothing.
+    __device__ __forceinline__ float grow(int e, float &l, float row_l) {
+        const float by = (float)(e + 1 - __builtin_amdgcn_frexp_expf(r)), most = fmaxf((float)(100 - __builtin_amdgcn_frexp_expf(row_l)), 0.f);
+        const float to = b - (r == 0.f ? most : fminf(by, most)), fall = b == -INFINITY ? 0.f : b - to;
+        const float factor = r == 0.f ? 0.f : exp2_fast(fall - by);
+        l *= exp2_fast(fall);
+        b = to;
+        r = ldexpf(1.f, e), inv_r = ldexpf(1.f, -e);
+        return factor;
+    }
+    // the largest logit with its scale is `top`, or it was: the factor of sum and outputs
+    __device__ __forceinline__ float move(float top) {
+        const float to = fmaxf(b, top), factor = exp2_fast(b - base_of(to));
+        b = to;
+        return factor;
+    }
+};
+// a row's sum, whose exponent goes into its base, for joins: at most 1 (m + e is rounded, its difference from m is not)
+__device__ __forceinline__ void settle(float &m, float &l) {
+    if (!(l > 0.f && l < INFINITY)) return;
+    const float to = m + (float)__builtin_amdgcn_frexp_expf(l);
+    l *= exp2_fast(m - to);
+    m = to;
 }
 
 // A logit's factor where products of -infinity stand for keys that are not seen: not 0, which
@@ -352,7 +387,8 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
     f32x4 o[DB];
 #pragma unroll
     for (int i = 0; i < DB; i++) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f, r = 0.f, inv_r = 1.f;
+    float l = 0.f;
+    Base base;
 
     const int32_t *table = a.s.tables + b * a.s.table_stride;
     const int64_t page_bytes = (int64_t)P * D;
@@ -483,21 +519,20 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
         }
         float vmax = fmaxf(vs, __shfl_xor(vs, 16));
         vmax = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(fmaxf(vmax, __shfl_xor(vmax, 32)))));
-        float grown = 1.f;
-        if (vmax > r) {
-            const int e = scale_ceiling(vmax);
-            inv_r = ldexpf(1.f, -e);
-            grown = r * inv_r;
-            r = ldexpf(1.f, e);
+        if (vmax > base.r) {
+            const float row_l = fmaxf(l, __shfl_xor(l, 16));
+            const float g = base.grow(scale_ceiling(vmax), l, fmaxf(row_l, __shfl_xor(row_l, 32)));
+#pragma unroll
+            for (int i = 0; i < DB; i++) o[i] *= g;
         }
-        float f = ks * factor, lv = scale_log(vs, inv_r), back = exp2_fast(-lv);  // f >= 0: the largest product has the largest logit
+        float f = ks * factor, lv = scale_log(vs, base.inv_r);  // f >= 0: the largest product has the largest logit
         if (key < last_lo || key + TILE > first_hi || __any(vp < 0)) {
             // some row does not see some of these keys, or they are not there
             const int from = lo - (key + 16 * c), to = vp >= 0 ? hi - (key + 16 * c) : 0;
 #pragma unroll
             for (int j = 0; j < 16; j++) x[j] = seen_or_not(x[j], j, from, to);
             f = not_zero(f);
-            if (max(from, 0) >= min(to, 16)) f = 1.f, lv = 0.f, back = 1.f;  // none of them, so neither their scales
+            if (max(from, 0) >= min(to, 16)) f = 1.f, lv = 0.f;  // none of them, so neither their scales
             const int keep = vp >= 0 ? min(max(sq.len - (key + 16 * c), 0), 16) : 0;
 #pragma unroll
             for (int i = 0; i < DB; i++) vc[i] = keep_bytes(vc[i], keep);
@@ -505,24 +540,23 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
         float top = larger(x[0], x[1]);
 #pragma unroll
         for (int j = 2; j < 16; j++) top = fmaxf(top, x[j]);
-        top *= f;  // of this lane's keys; the row's only where the base has to move
-        if (grown != 1.f || __any(top > m + LAZY_LOG2)) {
+        top = fmaf(top, f, lv);  // of this lane's keys; the row's only where the base has to move
+        if (__any(top > base.b + LAZY_LOG2)) {
             top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), m);
-            const float alpha = exp2_fast(m - base_of(top)), g = alpha * grown;
-            l *= alpha;
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float g = base.move(top);
+            l *= g;
 #pragma unroll
             for (int i = 0; i < DB; i++) o[i] *= g;
-            m = top;
         }
-        const float base = base_of(m) - WEIGHT_LOG2 - lv;
+        const float at = base_of(base.b) - WEIGHT_LOG2 - lv;
         float w[16], sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 16; j++) {
-            w[j] = exp2_fast(fmaf(x[j], f, -base));
+            w[j] = exp2_fast(fmaf(x[j], f, -at));
             sum += w[j];
         }
-        l = fmaf(sum, back, l);
+        l = fmaf(sum, exp2_fast(-lv), l);
         half8 p[2][NW];
         parts8<NW>(w, p[0]);
         parts8<NW>(w + 8, p[1]);
@@ -544,11 +578,12 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     const float inv = l == 0.f ? 0.f : 1.f / l;  // (apart from r: their quotient can be subnormal)
+    settle(base.b, l);
 #pragma unroll
     for (int i = 0; i < DB; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) s_o[wave][n][16 * i + 4 * c + j] = l == 0.f ? 0.f : o[i][j] * inv * r;
-    if (c == 0) s_m[wave][n] = m, s_l[wave][n] = l;
+        for (int j = 0; j < 4; j++) s_o[wave][n][16 * i + 4 * c + j] = l == 0.f ? 0.f : o[i][j] * inv * base.r;
+    if (c == 0) s_m[wave][n] = base.b, s_l[wave][n] = l;
     __syncthreads();
     for (int i = threadIdx.x; i < rows * (D / 4); i += 64 * WAVES) {
         const int row = i / (D / 4), d = i % (D / 4) * 4;
@@ -709,7 +744,8 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
     for (int i = 0; i < DB; i++)
 #pragma unroll
         for (int j = 0; j < 16; j++) o[i][j] = 0.f;
-    float m = -INFINITY, l = 0.f, r = 0.f, inv_r = 1.f;
+    float l = 0.f;
+    Base base;
 
     // ---- the steps' pages and scales
     _Float16 *const buffers = lds;
@@ -721,8 +757,8 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
     bool missing = false;  // whether a group that a row could see is not there
     const int32_t *const table = a.s.tables + b * a.s.table_stride;
     const int seen_end = min(end * TILE, sq.len);
-    // the entries of steps c0 .. c1 - 1; grown: r's growth, which the accumulators have to follow
-    auto look_up = [&](int c0, int c1, float &grown) {
+    // the entries of steps c0 .. c1 - 1; grown: whether r grew, and the outputs have to be multiplied by `by`
+    auto look_up = [&](int c0, int c1, bool &grown, float &by) {
         const int n = (c1 - c0) * GROUPS;
         float vmax = 0.f;
         bool lacks = false;
@@ -747,14 +783,9 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
 #pragma unroll
         for (int i = 0; i < WAVES; i++) vmax = fmaxf(vmax, s_max[i]), missing |= s_missing[i] != 0;
         missing = __any(missing);
-        grown = 1.f;
-        if (vmax > r) {  // (the same in every thread)
-            const int e = scale_ceiling(vmax);
-            inv_r = ldexpf(1.f, -e);
-            grown = r * inv_r;
-            r = ldexpf(1.f, e);
-        }
-        for (int i = tid; i < n; i += THREADS) s_lv[i] = scale_log(s_lv[i], inv_r);
+        grown = vmax > base.r;  // (the same in every thread)
+        if (grown) by = base.grow(scale_ceiling(vmax), l, fmaxf(l, __shfl_xor(l, 32)));
+        for (int i = tid; i < n; i += THREADS) s_lv[i] = scale_log(s_lv[i], base.inv_r);
         __syncthreads();
     };
 
@@ -892,18 +923,16 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
             float x = larger(s[u / 2][8 * (u % 2)], s[u / 2][8 * (u % 2) + 1]);
 #pragma unroll
             for (int j = 2; j < 8; j++) x = fmaxf(x, s[u / 2][8 * (u % 2) + j]);
-            top = fmaxf(top, x * f[u]);
+            top = fmaxf(top, fmaf(x, f[u], lv[u]));
         }
-        if (__any(top > m + LAZY_LOG2)) {  // (this lane's keys; the row's only where the base has to move)
-            top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), m);
-            const float alpha = exp2_fast(m - base_of(top));
-            l *= alpha;
-            scale_outputs(alpha);
-            m = top;
+        if (__any(top > base.b + LAZY_LOG2)) {  // (this lane's keys; the row's only where the base has to move)
+            const float g = base.move(fmaxf(top, __shfl_xor(top, 32)));
+            l *= g;
+            scale_outputs(g);
         }
     };
     auto weigh = [&](int u) {
-        const float at = base_of(m) - WEIGHT_LOG2 - lv[u];
+        const float at = base_of(base.b) - WEIGHT_LOG2 - lv[u];
         float w[8], sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
@@ -916,9 +945,10 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
 
     for (int c0 = begin; c0 < end; c0 += TABLE_STEPS) {
         const int n = min(end - c0, TABLE_STEPS);
-        float grown;
-        look_up(c0, c0 + n, grown);
-        if (grown != 1.f) scale_outputs(grown);
+        bool grown;
+        float by;
+        look_up(c0, c0 + n, grown, by);
+        if (grown) scale_outputs(by);
         read_places(0);
         load(c0);
         read_places(min(1, n - 1));
@@ -968,14 +998,17 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
     const float inv = l == 0.f ? 0.f : 1.f / l;  // (apart from r: their quotient can be subnormal)
     if (!mine) return;
     const int64_t out = (sq.t0 + tok) * a.q_heads + head, at = plan.long_row + split * a.num_q * a.q_heads + out;
-    if (plan.splits_long > 1 && hf == 0) plan.stat[2 * at] = m, plan.stat[2 * at + 1] = l;
+    if (plan.splits_long > 1) {
+        settle(base.b, l);
+        if (hf == 0) plan.stat[2 * at] = base.b, plan.stat[2 * at + 1] = l;
+    }
 #pragma unroll
     for (int i = 0; i < DB; i++)
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             float v[4];
 #pragma unroll
-            for (int z = 0; z < 4; z++) v[z] = l == 0.f ? 0.f : o[i][4 * j + z] * inv * r;
+            for (int z = 0; z < 4; z++) v[z] = l == 0.f ? 0.f : o[i][4 * j + z] * inv * base.r;
             const int d = 32 * i + 8 * j + 4 * hf;
             if (plan.splits_long == 1) store_values4<DT>(a.out, out * D + d, v);
             else *reinterpret_cast<f32x4 *>(plan.part + at * D + d) = f32x4{v[0], v[1], v[2], v[3]};

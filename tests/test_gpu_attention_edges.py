@@ -1,6 +1,7 @@
 """Attention over the 8-bit cache where calls are allowed and seldom made: bounds that do not hold while the
-keys are cut into parts."""
+keys are cut into parts, and value scales far apart."""
 import ctypes
+import math
 
 import pytest
 import torch
@@ -39,3 +40,129 @@ def test_rows_behind_the_bound_are_not_joined(dev, lbq, dtype, dim, batch):
     filled = out.clone()
     filled[first + served: first + 100] = at.paged_attention(q, cache, step)[first + served: first + 100]
     check(q, cache, step, got=filled)
+
+
+QUERY_STEP = 2.0 ** -24  # of the row's largest: what a query's channel may be off by, at the least
+
+
+def row_bound(q, cache, step, scale, causal=True, window=0):
+    """(out, bound) of f32, f16 or bf16 rows, element by element and from what a row itself sees, in 64 bits.
+
+    A key's logit: its operands are held to 2^-22 and QUERY_STEP of the row's largest, and its running sum is rounded
+    at most 20 times.  The exponent that it enters, with the base and the value scale's logarithm, is rounded at most 6 times,
+    each half a step of the magnitudes in it.  So its weight is off by e = (2^-22 + 20 * 2^-24) sum |q k| scale
+    + QUERY_STEP max |q| sum |k| scale + ln 2 * 6 * 2^-24 (|logit| + |base| + |log scale| + 15) + 16 * 2^-24 for the
+    exponential's last bits, in parts of itself, and the result, to the first order, by sum p e |v| + (sum p e) |out|.
+    Values: one rounding for each 16 keys and each join, 2^-24 each.  f16 parts of a weight are off by half the smallest f16
+    step where the row's largest weight with its value scale is at least 2^9: 2^-34 |code| of the largest p s, for each
+    key; bf16 weights are one f16 part: 2^-11.  A page's scale below 2^-80 of the largest counts as that."""
+    codes, scales = [cache.k.double(), cache.v.double()], [cache.k_scales.double(), cache.v_scales.double()]
+    heads, kv, page, ln2 = q.shape[1], cache.kv_heads, cache.page_size, math.log(2)
+    g, out, bound = heads // kv, torch.zeros(q.shape, dtype=torch.float64, device=q.device), torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    lens, cu = step.seq_lens.tolist(), step.cu_new.tolist()
+    half = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[q.dtype]
+    tiny = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -24, torch.bfloat16: 2.0 ** -133}[q.dtype]
+    for b, n in enumerate(lens):
+        t0, t1 = cu[b], cu[b + 1]
+        pages = step.tables[b, : -(-n // page)].long()
+        j, pos = torch.arange(n, device=q.device), n - (t1 - t0) + torch.arange(t1 - t0, device=q.device)[:, None]
+        seen = (j <= pos) & ((j > pos - window) if window else (j >= 0)) if causal else torch.ones(t1 - t0, n, dtype=torch.bool, device=q.device)
+        for h in range(kv):
+            k = (codes[0][pages, h] * scales[0][pages, h][:, None, None]).reshape(-1, q.shape[2])[:n]
+            c = codes[1][pages, h].transpose(1, 2).reshape(-1, q.shape[2])[:n]
+            s = scales[1][pages, h].repeat_interleave(page)[:n]
+            rows = q[t0:t1, h * g:(h + 1) * g].double()
+            x = (rows @ k.t() * scale).masked_fill(~seen[:, None], -math.inf)
+            p = torch.softmax(x, -1)
+            logs = torch.log2(s.clamp(min=2.0 ** -80 * s.max().item())) - math.log2(s.max().item())
+            base = (x / ln2 + logs).amax(-1, keepdim=True).abs()
+            reach = (rows.abs() @ k.abs().t()) * abs(scale)
+            ends = rows.abs().amax(-1, keepdim=True) * k.abs().sum(-1) * abs(scale)
+            exponent = x.nan_to_num(neginf=0.0).abs() / ln2 + base + logs.abs() + 15
+            e = (2.0 ** -22 + 20 * 2.0 ** -24) * reach + QUERY_STEP * ends + ln2 * 6 * 2.0 ** -24 * exponent + 16 * 2.0 ** -24
+            assert (p * e).max() < 0.01
+            v = c * s[:, None]
+            o, mag = p @ v, p @ v.abs()
+            most, code = (p * s).amax(-1, keepdim=True), 127.0 if cache.kind == "int8" else 448.0
+            off = 1.01 * ((p * e) @ v.abs() + (p * e).sum(-1, keepdim=True) * o.abs())
+            off = off + ((n / 16 + 64) * 2.0 ** -24 + (2.0 ** -11 if q.dtype == torch.bfloat16 else 0.0)) * mag
+            off = off + n * 2.0 ** -34 * code * most + n * 2.0 ** -80 * code * s.max()
+            out[t0:t1, h * g:(h + 1) * g] = o
+            bound[t0:t1, h * g:(h + 1) * g] = off * (1 + half) + half * o.abs() + tiny
+    return out, bound
+
+
+def check_rows(q, cache, step, **kw):
+    got = at.paged_attention(q, cache, step, **kw)
+    want, bound = row_bound(q, cache, step, cache.head_dim ** -0.5, **kw)
+    off = (got.double() - want).abs()
+    assert (off <= bound).all(), f"off by {(off / bound).max().item():.3g} of the bound"
+    return got
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dim,new", [(64, 1), (128, 1), (128, 5), (64, 100), (128, 100), (256, 40)])
+@pytest.mark.parametrize("power", [-60, -40, -20])
+def test_scales_of_pages_without_weight(dev, dtype, kind, dim, new, power):
+    # the page that decides a row has a value scale far below that of pages whose weights are next to nothing: one
+    # before it and one behind it, and short and long contexts, whole and in parts
+    for ctx in (200, 3000):
+        cache, step, q = setup(dev, kind, dtype, 16, dim, 1, 2, [ctx], [new], pad=0)
+        pages = step.tables[0, : -(-(ctx + new) // 16)].long()
+        cache.v_scales[pages] = 2.0 ** (power if dtype != torch.float16 else power / 4 - 8)
+        if dtype == torch.float16:  # (the result has to be a normal number of its type)
+            cache.v_scales[pages] *= 8
+        # keys of the loud pages against the queries: logits lower by 40 and more
+        q[:, :, 0] = 60.0
+        cache.k.view(torch.int8)[pages, :, :, 0] = 0
+        loud = pages[[1, len(pages) // 2, len(pages) - 2 - new // 16]]
+        cache.v_scales[loud] = 1.0
+        cache.k_scales[loud] = 0.25
+        cache.k.view(torch.int8)[loud, :, :, 0] = -127 if kind == "int8" else -2  # (e4m3: -448)
+        got = check_rows(q, cache, step)
+        assert got.float().abs().max() > 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,ctx,new", [(64, 0, 64), (128, 0, 300), (256, 10, 90), (128, 2000, 40)])
+def test_scales_of_pages_of_later_rows(dev, dtype, dim, ctx, new):
+    # value scales that grow from page to page: a causal row is as exact as if the later pages were not there
+    cache, step, q = setup(dev, "int8", dtype, 16, dim, 1, 2, [ctx], [new], pad=0)
+    pages = step.tables[0, : -(-(ctx + new) // 16)].long()
+    low, high = (-20, 6) if dtype == torch.float16 else (-60, 10)
+    cache.v_scales[pages, 0] = torch.exp2(torch.linspace(low, high, len(pages), device=dev))
+    check_rows(q, cache, step)
+    cache.v_scales[pages, 0] = cache.v_scales[pages, 0].flip(0)
+    check_rows(q, cache, step)
+    check_rows(q, cache, step, window=30)
+    check_rows(q, cache, step, causal=False)
+
+
+@pytest.mark.parametrize("new", [1, 90])
+def test_pages_of_zeros_first(dev, new):
+    # pages whose scale is 0 stand for zeros whatever codes they hold, also where all of the first steps' are
+    cache, step, q = setup(dev, "int8", torch.float32, 64, 64, 1, 2, [30000], [new], pad=0)
+    pages = step.tables[0, : -(-(30000 + new) // 64)].long()
+    cache.v_scales[pages] = 0.0
+    assert (at.paged_attention(q, cache, step) == 0).all()
+    cache.v_scales[pages[-3:]] = 2.0 ** -100
+    check_rows(q, cache, step)
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("new", [1, 5, 90])
+def test_scales_that_grow_late(dev, kind, new):
+    # whole pages of large logits under scales of 2^-70 and 0, then a single page of scale 1, which some rows weigh and
+    # others do not, at any place of the steps that are looked up at once
+    for place in (0, 1, 3, 40, 256, 400):
+        cache, step, q = setup(dev, kind, torch.float32, 64, 64, 1, 4, [30000], [new], pad=0)
+        pages = step.tables[0, : -(-(30000 + new) // 64)].long()
+        cache.v_scales[pages] = 2.0 ** -70
+        cache.v_scales[pages[::3]] = 0.0
+        cache.v_scales[pages[place]] = 1.0
+        q[:, :, 0] = torch.linspace(-60, 60, 4, device=dev)  # for the page, or against it, by the head
+        cache.k.view(torch.int8)[pages, :, :, 0] = 0
+        cache.k_scales[pages[place]] = 0.25
+        cache.k.view(torch.int8)[pages[place], :, :, 0] = 127 if kind == "int8" else 0x7e
+        check_rows(q, cache, step)
