@@ -387,7 +387,8 @@ int lbq_kv_append(lbq_ctx *ctx, const lbq_kv_cache *cache, const lbq_kv_step *st
  * Not causal (window 0): every row sees the whole sequence -- cross attention, with cu_new of
  * the decoder's rows and tables and seq_lens of the encoder's states.  A row that sees
  * nothing is zero.  out is [num_tokens][q_heads][head_dim], contiguous, apart from q.
- * Sums and softmax are f32.  Weights go into their product with the values relative to the row's
+ * Sums and softmax are f32.  Queries go into their products off by 2^-22 of themselves or 2^-31 of their row's
+ * largest.  Weights go into their product with the values relative to the row's
  * largest weight with its value scale, as f16 in two parts (f32, f16: off by 2^-22 of themselves or 2^-34 of the
  * largest) or one (bf16: 2^-11); value scales below 2^-80 of the sequence's largest count as that.  f32
  * results are f32's, about 1e-6 of sum_j softmax_j |v_j|.  The work of one sequence is spread over the chip through d_ws:

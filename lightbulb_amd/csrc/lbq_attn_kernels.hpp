@@ -2,7 +2,8 @@
 //
 // The codes of both kinds are f16 numbers, so a code goes into a matrix instruction exactly and
 // its scale, one per 16 or more keys, into the f32 logit or weight.  f32 queries go in as two f16
-// parts of a power-of-two multiple of their row (22 bits); f16 and bf16 queries are one part, exactly.
+// parts of a power-of-two multiple of their row (22 bits, and no less than 2^-40 of the row's largest); f16 and bf16
+// queries are one part, exactly down to 2^-30 of it.  (int8 keys of the short form: attn_short.)
 // Weights go in as two f16 parts, for bf16 as one.  The products of both parts go into one f32 sum:
 // results of f32's accuracy at twice the matrix work.
 //
@@ -150,17 +151,22 @@ __device__ __forceinline__ void parts8(const float *v, half8 *o) {
     }
 }
 
-// Four values as whole numbers of three signed digits to the base of 256: o[i] has digit i of each
-// (256^2 o[2] + 256 o[1] + o[0]).
-constexpr float MOST_DIGITS = 127 * 65536 + 127 * 256 + 127;
+// Four values as whole numbers of four signed digits to the base of 256: o[i] has digit i of each
+// (256^3 o[3] + 256^2 o[2] + 256 o[1] + o[0]).  With the row's largest in 31 bits what is 2^-8 of it still has all
+// the bits of an f32, and nothing is off by more than 2^-31 of it (three digits, 2^-24: a channel a thousand times
+// the others left them 14 bits).
+constexpr float MOST_DIGITS = 0x7f7f7f00;  // the largest f32 up to 127 in each digit
 __device__ __forceinline__ void digits4(const float *v, uint32_t *o) {
     uint32_t w[4];  // the number + 128 in each digit
 #pragma unroll
-    for (int j = 0; j < 4; j++) w[j] = (uint32_t)(int)rintf(v[j]) + 0x808080u;
-    const uint32_t ab = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), cd = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
-    o[0] = __builtin_amdgcn_perm(cd, ab, 0x05040100u) ^ 0x80808080u;
-    o[1] = __builtin_amdgcn_perm(cd, ab, 0x07060302u) ^ 0x80808080u;
-    o[2] = (__builtin_amdgcn_perm(w[1], w[0], 0x0c0c0602u) | __builtin_amdgcn_perm(w[3], w[2], 0x06020c0cu)) ^ 0x80808080u;
+    for (int j = 0; j < 4; j++) w[j] = (uint32_t)(int)rintf(v[j]) + 0x80808080u;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {  // digits 2 i and 2 i + 1
+        const uint32_t pick = i ? 0x07030602u : 0x05010400u;
+        const uint32_t ab = __builtin_amdgcn_perm(w[1], w[0], pick), cd = __builtin_amdgcn_perm(w[3], w[2], pick);
+        o[2 * i] = __builtin_amdgcn_perm(cd, ab, 0x05040100u) ^ 0x80808080u;
+        o[2 * i + 1] = __builtin_amdgcn_perm(cd, ab, 0x07060302u) ^ 0x80808080u;
+    }
 }
 
 // the exponent e with |max| < 2^e for the parts of a query row: values times 2^(15 - e) fit f16
@@ -336,8 +342,8 @@ template <int D, int KIND, int DT, int WAVES>
 __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan &plan, int group, float *lds) {
     constexpr int NS = QUERY_PARTS<DT>, NW = WEIGHT_PARTS<DT>;
     constexpr int STEPS = D / 32, DB = D / 16;
-    // int8 keys need not go to f16: with the row as whole numbers of three digits the products are
-    // whole too, and exact (32 tokens: 45.2 us, with f16 keys 46.3; at 500 keys 9.2 and 9.7)
+    // int8 keys need not go to f16: with the row as whole numbers of four digits the products are
+    // whole too, and exact (32 tokens: 44.9 us, with f16 keys 46.3; at 500 keys 9.6 and 9.7)
     constexpr bool DIGITS = KIND == KV_INT8;
     float(*const s_o)[SHORT_ROWS][D + 4] = reinterpret_cast<float(*)[SHORT_ROWS][D + 4]>(lds);
     float(*const s_m)[SHORT_ROWS] = reinterpret_cast<float(*)[SHORT_ROWS]>(lds + WAVES * SHORT_ROWS * (D + 4));
@@ -443,7 +449,7 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
     }
     // the row's parts or digits, and the factor of its logits (in powers of two)
     half8 q[DIGITS ? 1 : STEPS][NS];
-    uint32_t qd[3][DIGITS ? D / 16 : 1];
+    uint32_t qd[4][DIGITS ? D / 16 : 1];
     float factor;
     {
         uint32_t most = 0;  // (as whole numbers: what is not finite is the largest)
@@ -453,7 +459,7 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
             for (int j = 0; j < 8; j++) most = max(most, __float_as_uint(fabsf(raw[s][j])));
         most = max(most, (uint32_t)__shfl_xor((int)most, 16));
         most = max(most, (uint32_t)__shfl_xor((int)most, 32));
-        constexpr int BITS = DIGITS ? 23 : 15;
+        constexpr int BITS = DIGITS ? 31 : 15;
         int e = row_exponent(__uint_as_float(most));
         if (DIGITS && ldexpf(__uint_as_float(most), BITS - e) > MOST_DIGITS) e++;
 #pragma unroll
@@ -463,16 +469,16 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
             if constexpr (DIGITS) {
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    uint32_t d[3];
+                    uint32_t d[4];
                     digits4(raw[s] + 4 * j, d);
 #pragma unroll
-                    for (int i = 0; i < 3; i++) qd[i][2 * s + j] = d[i];
+                    for (int i = 0; i < 4; i++) qd[i][2 * s + j] = d[i];
                 }
             } else {
                 parts8<NS>(raw[s], q[s]);
             }
         }
-        factor = ldexpf(fabsf(a.scale) * 1.44269504088896340736f, e - BITS);
+        factor = ldexpf(fabsf(a.scale) * 1.44269504088896340736f, e - (DIGITS ? BITS - 8 : BITS));  // (their products count in 2^8)
         if (DIGITS && most >= 0x7f800000u) factor = __uint_as_float(0x7fc00000u);  // (digits cannot say so)
     }
     // (the older wave of a SIMD goes first where both could, and would be done long before the other)
@@ -486,9 +492,9 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             if constexpr (DIGITS) {
-                i32x4 s[3] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
+                i32x4 s[4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
-                for (int u = 0; u < 3; u++) {
+                for (int u = 0; u < 4; u++) {
 #pragma unroll
                     for (int j = 0; j < D / 64; j++)
                         s[u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
@@ -499,7 +505,8 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
                                                                     (i32x4){(int)qd[u][D / 16 - 2], (int)qd[u][D / 16 - 1], 0, 0}, s[u], 0, 0, 0);
                 }
 #pragma unroll
-                for (int j = 0; j < 4; j++) x[4 * i + j] = fmaf((float)s[2][j], 65536.f, (float)(256 * s[1][j] + s[0][j]));
+                for (int j = 0; j < 4; j++)  // 2^-8 of it, each half a whole number below 2^31
+                    x[4 * i + j] = fmaf((float)(256 * s[3][j] + s[2][j]), 256.f, (float)(256 * s[1][j] + s[0][j]) * 0x1p-8f);
             } else {
                 f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll

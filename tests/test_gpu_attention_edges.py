@@ -1,5 +1,5 @@
 """Attention over the 8-bit cache where calls are allowed and seldom made: bounds that do not hold while the
-keys are cut into parts, and value scales far apart."""
+keys are cut into parts, value scales far apart, and queries with one large channel."""
 import ctypes
 import math
 
@@ -42,7 +42,7 @@ def test_rows_behind_the_bound_are_not_joined(dev, lbq, dtype, dim, batch):
     check(q, cache, step, got=filled)
 
 
-QUERY_STEP = 2.0 ** -24  # of the row's largest: what a query's channel may be off by, at the least
+QUERY_STEP = 2.0 ** -31  # of the row's largest: what a query's channel may be off by, at the least
 
 
 def row_bound(q, cache, step, scale, causal=True, window=0):
@@ -166,3 +166,20 @@ def test_scales_that_grow_late(dev, kind, new):
         cache.k_scales[pages[place]] = 0.25
         cache.k.view(torch.int8)[pages[place], :, :, 0] = 127 if kind == "int8" else 0x7e
         check_rows(q, cache, step)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dim,ctx,new", [(64, 300, 1), (96, 40, 3), (128, 3000, 1), (192, 90, 5), (256, 500, 1), (128, 100, 90)])
+@pytest.mark.parametrize("loud", [200.0, 8000.0, 50000.0])
+def test_queries_with_one_large_channel(dev, dtype, kind, dim, ctx, new, loud):
+    # a channel far above the others in which the keys are zero, or a code of 1: the other channels decide, to the same bits
+    cache, step, q = setup(dev, kind, dtype, 16, dim, 2, 2, [ctx, 0, 77], [new] * 3, pad=0)
+    q[:, ::2, 5] = loud
+    q[:, 1::2, dim - 3] = -loud
+    codes = cache.k.view(torch.int8)
+    codes[..., 5] = 0
+    codes[..., dim - 3] = 0
+    check_rows(q, cache, step)
+    codes[::7, :, ::5, 5] = 1  # (e4m3: 2^-9)
+    check_rows(q, cache, step)
