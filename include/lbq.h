@@ -386,7 +386,7 @@ int lbq_kv_append(lbq_ctx *ctx, const lbq_kv_cache *cache, const lbq_kv_step *st
  * seq_len - n + i and sees j <= position, and with a window > 0 only j > position - window.
  * Not causal (window 0): every row sees the whole sequence -- cross attention, with cu_new of
  * the decoder's rows and tables and seq_lens of the encoder's states.  A row that sees
- * nothing is zero.  out is [num_tokens][q_heads][head_dim], contiguous, apart from q.
+ * nothing is zero; one that sees something and whose query is not finite is NaN.  out is [num_tokens][q_heads][head_dim], contiguous, apart from q.
  * Sums and softmax are f32.  Queries go into their products off by 2^-22 of themselves or 2^-31 of their row's
  * largest.  Weights go into their product with the values relative to the row's
  * largest weight with its value scale, as f16 in two parts (f32, f16: off by 2^-22 of themselves or 2^-34 of the

@@ -3,7 +3,7 @@
 // The codes of both kinds are f16 numbers, so a code goes into a matrix instruction exactly and
 // its scale, one per 16 or more keys, into the f32 logit or weight.  f32 queries go in as two f16
 // parts of a power-of-two multiple of their row (22 bits, and no less than 2^-40 of the row's largest); f16 and bf16
-// queries are one part, exactly down to 2^-30 of it.  (int8 keys of the short form: attn_short.)
+// queries are one part, exactly down to 2^-28 of it.  (int8 keys of the short form: attn_short.)
 // Weights go in as two f16 parts, for bf16 as one.  The products of both parts go into one f32 sum:
 // results of f32's accuracy at twice the matrix work.
 //
@@ -479,7 +479,8 @@ __device__ __forceinline__ void attn_short(const KvAttention &a, const AttnPlan 
             }
         }
         factor = ldexpf(fabsf(a.scale) * 1.44269504088896340736f, e - (DIGITS ? BITS - 8 : BITS));  // (their products count in 2^8)
-        if (DIGITS && most >= 0x7f800000u) factor = __uint_as_float(0x7fc00000u);  // (digits cannot say so)
+        // digits cannot say so, and one f16 part would leave a row of which all logits are -infinity as one that sees nothing
+        if (most >= 0x7f800000u) factor = __uint_as_float(0x7fc00000u);
     }
     // (the older wave of a SIMD goes first where both could, and would be done long before the other)
     if (wave >= 4) __builtin_amdgcn_s_setprio(1);
@@ -744,6 +745,7 @@ __device__ __forceinline__ void attn_long(const KvAttention &a, const AttnPlan &
             parts8<NS>(v, q[i]);
         }
         factor = ldexpf(fabsf(a.scale) * 1.44269504088896340736f, e - 15);
+        if (amax == INFINITY) factor = __uint_as_float(0x7fc00000u);  // (as in attn_short; NaN is in the products)
     }
 
     f32x16 o[DB], s[2];

@@ -1,5 +1,6 @@
 """Attention over the 8-bit cache where calls are allowed and seldom made: bounds that do not hold while the
-keys are cut into parts, value scales far apart, and queries with one large channel."""
+keys are cut into parts, value scales far apart, queries with one large channel, and queries that are
+not finite."""
 import ctypes
 import math
 
@@ -183,3 +184,25 @@ def test_queries_with_one_large_channel(dev, dtype, kind, dim, ctx, new, loud):
     check_rows(q, cache, step)
     codes[::7, :, ::5, 5] = 1  # (e4m3: 2^-9)
     check_rows(q, cache, step)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("new", [[1, 1], [5, 2], [66, 5]])
+def test_rows_that_are_not_finite(dev, dtype, kind, new):
+    # NaN whatever the keys' signs: also where all of a row's logits are -infinity, and in every form alike
+    for bad, sign in ((math.inf, 0x80), (-math.inf, 0), (math.inf, 0), (math.nan, 0)):
+        cache, step, q = setup(dev, kind, dtype, 64, 64, 1, 4, [100, 30], new, pad=0)
+        codes = cache.k.view(torch.uint8)
+        codes[..., 9] = (codes[..., 9] & 0x3f | 1) if kind == "e4m3" or not sign else 1
+        if sign:
+            codes[..., 9] = codes[..., 9] | 0x80
+        q *= 0.1  # (so that no other channel's products are infinite)
+        clean = at.paged_attention(q, cache, step)
+        q[0, 2, 9] = bad
+        got = at.paged_attention(q, cache, step)
+        assert torch.isnan(got[0, 2]).all()
+        got[0, 2] = clean[0, 2]
+        assert torch.equal(got, clean)
+        step.seq_lens[0] = 0  # it sees nothing: zero
+        assert (at.paged_attention(q, cache, step)[0] == 0).all()
