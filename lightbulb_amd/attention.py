@@ -51,8 +51,11 @@ class Step:
     new tokens); ``slots`` int64 and ``positions`` int32 [num_tokens] for an append.  ``max_len``
     and ``max_new`` bound the sequences and their new tokens where the caller knows them: work is
     laid out by them, and what lies beyond them is not served.  0 leaves them open.
-    ``granted`` and ``free_count`` are set by ``PageTable.step``.
+    ``granted`` and ``free_count`` are set by ``PageTable.step``; ``crosses`` says that the rows are another
+    step's (``across``).
     """
+
+    crosses = False
 
     def __init__(self, tables: torch.Tensor, seq_lens: torch.Tensor, cu_new: torch.Tensor, slots: torch.Tensor | None,
                  positions: torch.Tensor | None, *, page_size: int, num_tokens: int, max_len: int = 0, max_new: int = 0,
@@ -83,8 +86,10 @@ class Step:
         to an encoder's states, whose lengths and pages are ``source``'s."""
         if source.tables.shape[0] != self.tables.shape[0]:
             raise ValueError(f"{self.tables.shape[0]} sequences across {source.tables.shape[0]}")
-        return Step(source.tables, source.seq_lens, self.cu_new, None, None, page_size=source.page_size, num_tokens=self.num_tokens,
-                    max_len=source.max_len, max_new=self.max_new)
+        s = Step(source.tables, source.seq_lens, self.cu_new, None, None, page_size=source.page_size, num_tokens=self.num_tokens,
+                 max_len=source.max_len, max_new=self.max_new)
+        s.crosses = True
+        return s
 
 
 class PageTable:
@@ -295,19 +300,22 @@ class KvCache:
         return out
 
 
-def paged_attention(q: torch.Tensor, cache: KvCache, step: Step, *, scale: float | None = None, causal: bool = True, window: int = 0,
+def paged_attention(q: torch.Tensor, cache: KvCache, step: Step, *, scale: float | None = None, causal: bool | None = None, window: int = 0,
                     out: torch.Tensor | None = None) -> torch.Tensor:
     """``softmax(scale q k^T) v`` of the step's queries [num_tokens, heads, head_dim] over the cache; each
     ``heads / kv_heads`` query heads share a key/value head.  Causal: row i of a sequence's n new ones is at
     position ``seq_len - n + i`` and sees the tokens up to it, or the last ``window`` of them.  Not causal: all
-    of the sequence (``Step.across`` for cross attention).  A row that sees nothing is zero; rows behind the
-    last sequence are left as they are.  ``scale`` defaults to head_dim ** -0.5."""
+    of the sequence.  ``causal`` defaults to true, and to false for a step ``across`` other sequences: cross
+    attention.  A row that sees nothing is zero; rows behind the last sequence are left as they are.  ``scale``
+    defaults to head_dim ** -0.5."""
     cache._fits(step)
     dim, kv = cache.head_dim, cache.kv_heads
     t = _rows("q", q, None, dim, step)
     heads = q.shape[1]
     if heads < 1 or heads % kv:
         raise ValueError(f"{heads} query heads over {kv} key/value heads")
+    if causal is None:
+        causal = not step.crosses
     if window < 0 or (window and not causal):
         raise ValueError(f"a window of {window} needs a causal mask")
     if out is None:

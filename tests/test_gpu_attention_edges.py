@@ -1,6 +1,6 @@
 """Attention over the 8-bit cache where calls are allowed and seldom made: bounds that do not hold while the
-keys are cut into parts, value scales far apart, queries with one large channel, and queries that are
-not finite."""
+keys are cut into parts, value scales far apart, queries with one large channel, queries that are
+not finite, and the defaults of a step across other sequences."""
 import ctypes
 import math
 
@@ -206,3 +206,18 @@ def test_rows_that_are_not_finite(dev, dtype, kind, new):
         assert torch.equal(got, clean)
         step.seq_lens[0] = 0  # it sees nothing: zero
         assert (at.paged_attention(q, cache, step)[0] == 0).all()
+
+
+@pytest.mark.parametrize("new", [[1, 1], [90, 3]])
+def test_a_step_across_sees_all_of_the_source(dev, new):
+    # without a word about the mask: a decoder's rows over longer and shorter sources
+    cache, source, _ = setup(dev, "int8", torch.float32, 16, 64, 2, 2, [200, 2], [0, 0])
+    t = sum(new)
+    mine = at.Step(torch.zeros(2, 1, dtype=torch.int32, device=dev), i32(new, dev), i32([0, new[0], t], dev), None, None, page_size=64, num_tokens=t)
+    q = torch.randn(t, 4, 64, device=dev)
+    want = at.paged_attention(q, cache, mine.across(source), causal=False)
+    assert torch.equal(at.paged_attention(q, cache, mine.across(source)), want)
+    # (a single row's causal mask is none: it is at the source's last position)
+    assert torch.equal(at.paged_attention(q, cache, mine.across(source), causal=True), want) == (t == 2)
+    with pytest.raises(ValueError, match="window"):
+        at.paged_attention(q, cache, mine.across(source), window=5)
