@@ -43,7 +43,15 @@ def _expect_tables(tables: torch.Tensor) -> None:
         raise ValueError("block tables must be an int32 tensor [sequences, blocks] with contiguous rows")
 
 
-class Step:
+class _Fixed:
+    """What the library is given as addresses and sizes when the object is made: setting such an attribute
+    anew would leave the library with the old ones.  The tensors' contents may change."""
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"a {type(self).__name__}'s {name} is fixed when it is made")
+
+
+class Step(_Fixed):
     """One step's view of the cache: which pages hold the sequences, and which rows are new.
 
     ``tables`` int32 [batch, blocks], ``seq_lens`` int32 [batch] (new tokens included) and
@@ -72,14 +80,12 @@ class Step:
             raise ValueError("num_tokens, max_len and max_new must not be negative")
         if page_size not in PAGE_SIZES:
             raise ValueError(f"page_size {page_size} is none of {PAGE_SIZES}")
-        self.tables, self.seq_lens, self.cu_new, self.slots, self.positions = tables, seq_lens, cu_new, slots, positions
-        self.page_size, self.num_tokens, self.max_len, self.max_new = page_size, num_tokens, max_len, max_new
-        self.granted, self.free_count = granted, free_count
-        self.device = tables.device
-        self._struct = _lib.KvStepStruct(
-            tables.data_ptr(), tables.stride(0), seq_lens.data_ptr(), cu_new.data_ptr(), slots.data_ptr() if slots is not None else None,
-            positions.data_ptr() if positions is not None else None, num_tokens, tables.shape[0], tables.shape[1], max_len, max_new)
-        self._ws: dict = {}  # bytes of workspace by heads and head_dim: every layer asks
+        vars(self).update(
+            tables=tables, seq_lens=seq_lens, cu_new=cu_new, slots=slots, positions=positions, page_size=page_size, num_tokens=num_tokens,
+            max_len=max_len, max_new=max_new, granted=granted, free_count=free_count, device=tables.device, _struct=_lib.KvStepStruct(
+                tables.data_ptr(), tables.stride(0), seq_lens.data_ptr(), cu_new.data_ptr(), slots.data_ptr() if slots is not None else None,
+                positions.data_ptr() if positions is not None else None, num_tokens, tables.shape[0], tables.shape[1], max_len, max_new),
+            _ws={})  # bytes of workspace by heads and head_dim: every layer asks
 
     def across(self, source: "Step") -> "Step":
         """This step's rows over ``source``'s sequences: cross attention of a decoder's queries
@@ -88,11 +94,11 @@ class Step:
             raise ValueError(f"{self.tables.shape[0]} sequences across {source.tables.shape[0]}")
         s = Step(source.tables, source.seq_lens, self.cu_new, None, None, page_size=source.page_size, num_tokens=self.num_tokens,
                  max_len=source.max_len, max_new=self.max_new)
-        s.crosses = True
+        vars(s)["crosses"] = True
         return s
 
 
-class PageTable:
+class PageTable(_Fixed):
     """Block tables of ``max_seqs`` sequences over a pool of ``num_pages`` pages, on the GPU.
 
     ``tables`` int32 [max_seqs, max_blocks] (-1: no page); ``free`` int32 [num_pages], of which the
@@ -121,14 +127,12 @@ class PageTable:
             raise ValueError(f"page_size {page_size} is none of {PAGE_SIZES}")
         _expect("free", free, torch.int32, tables.device)
         _expect("free_count", free_count, torch.int32, tables.device, 1)
-        self.tables, self.free, self.free_count, self.page_size = tables, free, free_count, page_size
-        self.device = tables.device
-        self._ctx = context(self.device)
-        self._ticket = torch.zeros(1, dtype=torch.int32, device=self.device)
-        self._longs = torch.empty(0, dtype=torch.int64, device=self.device)
-        # (what a call would ask the tensors for each time: 2 us of a token step's 12)
-        self._rows, self._blocks = tables.shape
-        self._places = (tables.data_ptr(), tables.stride(0), self._blocks, page_size, free.data_ptr(), free.numel())
+        dev, (rows, blocks) = tables.device, tables.shape
+        vars(self).update(
+            tables=tables, free=free, free_count=free_count, page_size=page_size, device=dev, _ctx=context(dev),
+            _ticket=torch.zeros(1, dtype=torch.int32, device=dev), _longs=torch.empty(0, dtype=torch.int64, device=dev),
+            # (what a call would ask the tensors for each time: 2 us of a token step's 12)
+            _rows=rows, _blocks=blocks, _places=(tables.data_ptr(), tables.stride(0), blocks, page_size, free.data_ptr(), free.numel()))
 
     def step(self, ctx_lens: torch.Tensor, new_lens: torch.Tensor, num_tokens: int, *, commit: bool = True, max_len: int = 0,
              max_new: int = 0) -> Step:
@@ -160,11 +164,11 @@ class PageTable:
             self._ctx, ctx_lens.data_ptr(), new_lens.data_ptr(), b, *self._places, p_count, p_left, self._ticket.data_ptr(), num_tokens,
             p_lens, p_cu, p_granted, p_slots, p_pos, _stream(dev)))
         s = Step.__new__(Step)
-        s.tables, s.seq_lens, s.cu_new, s.slots, s.positions = self.tables if b == self._rows else self.tables[:b], seq_lens, cu, slots, positions
-        s.page_size, s.num_tokens, s.max_len, s.max_new = self.page_size, num_tokens, max_len, max_new
-        s.granted, s.free_count, s.device = granted, left, dev
-        s._struct = _lib.KvStepStruct(self._places[0], self._places[1], p_lens, p_cu, p_slots, p_pos, num_tokens, b, self._blocks, max_len, max_new)
-        s._ws = {}
+        vars(s).update(
+            tables=self.tables if b == self._rows else self.tables[:b], seq_lens=seq_lens, cu_new=cu, slots=slots, positions=positions,
+            page_size=self.page_size, num_tokens=num_tokens, max_len=max_len, max_new=max_new, granted=granted, free_count=left, device=dev,
+            _struct=_lib.KvStepStruct(self._places[0], self._places[1], p_lens, p_cu, p_slots, p_pos, num_tokens, b, self._blocks, max_len, max_new),
+            _ws={})
         return s
 
     def release(self, lens: torch.Tensor, which: torch.Tensor) -> None:
@@ -180,7 +184,7 @@ class PageTable:
                                              _stream(self.device)))
 
 
-class Rotary:
+class Rotary(_Fixed):
     """Rotary position angles: ``cos`` and ``sin`` f32 [max_pos, rot_dim / 2].  Pairs are channels
     (i, i + rot_dim / 2), or neighbours (2 i, 2 i + 1) where ``interleaved`` (candle's ``rope`` and
     ``rope_i``)."""
@@ -190,8 +194,7 @@ class Rotary:
             raise ValueError(f"angles must be two tensors [positions, pairs], got {tuple(cos.shape)} and {tuple(sin.shape)}")
         _expect("cos", cos, torch.float32, cos.device)
         _expect("sin", sin, torch.float32, cos.device)
-        self.cos, self.sin, self.interleaved = cos, sin, bool(interleaved)
-        self.max_pos, self.rot_dim = cos.shape[0], 2 * cos.shape[1]
+        vars(self).update(cos=cos, sin=sin, interleaved=bool(interleaved), max_pos=cos.shape[0], rot_dim=2 * cos.shape[1])
 
     @classmethod
     def from_theta(cls, rot_dim: int, max_pos: int, theta: float = 10000.0, interleaved: bool = False, device="cuda") -> "Rotary":
@@ -216,7 +219,7 @@ def _rows(name: str, x: torch.Tensor, heads: int | None, dim: int, step: Step) -
     return t
 
 
-class KvCache:
+class KvCache(_Fixed):
     """One layer's keys and values: codes ``k`` [pages, kv_heads, page_size, head_dim] and ``v``
     [pages, kv_heads, head_dim, page_size] (values are held transposed), int8 or e4m3, and f32 scales
     ``k_scales`` and ``v_scales`` [pages, kv_heads]; a value is code * scale."""
@@ -252,11 +255,11 @@ class KvCache:
         _expect("v", v, k.dtype, k.device)
         for name, s in (("k_scales", k_scales), ("v_scales", v_scales)):
             _expect(name, s, torch.float32, k.device, pages * heads)
-        self.k, self.v, self.k_scales, self.v_scales = k, v, k_scales, v_scales
-        self.kind, kind = kinds[k.dtype]
-        self.page_size, self.kv_heads, self.head_dim, self.device = page, heads, dim, k.device
-        self._ctx = context(k.device)
-        self._struct = _lib.KvCacheStruct(k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), pages, kind, page, heads, dim)
+        name, kind = kinds[k.dtype]
+        vars(self).update(
+            k=k, v=v, k_scales=k_scales, v_scales=v_scales, kind=name, page_size=page, kv_heads=heads, head_dim=dim, device=k.device,
+            _ctx=context(k.device),
+            _struct=_lib.KvCacheStruct(k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), pages, kind, page, heads, dim))
 
     def _fits(self, step: Step) -> None:
         if step.page_size != self.page_size:
