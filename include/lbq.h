@@ -348,9 +348,12 @@ typedef struct lbq_kv_step {
  * before it need are no more than *d_free_count; the i-th page taken is
  * d_free[*d_free_count - 1 - i] and goes into d_tables, whose other entries stay.  Where it is
  * not granted, granted[b] and seq_lens[b] are 0 and its rows' slots and positions -1.
+ * A sequence of a negative length counts as one of no rows.
  * *d_free_count_out = *d_free_count less the pages taken; the two pointers may be equal
  * (the step is then taken), in which case d_ticket is a word that is zero before the call and
- * after it. */
+ * after it.  Where they are not, the pages stay free: their entries in the tables are a forecast, which holds
+ * until the next call, and nothing may be appended to their slots.  An entry behind the blocks that a sequence's
+ * length needs is of no meaning to any call. */
 int lbq_kv_step_build(lbq_ctx *ctx, const int32_t *d_ctx_lens, const int32_t *d_new_lens, int32_t batch,
                       int32_t *d_tables, int64_t table_stride, int32_t max_blocks, int32_t page_size,
                       const int32_t *d_free, int64_t num_pages, const int32_t *d_free_count, int32_t *d_free_count_out,

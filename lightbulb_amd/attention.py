@@ -59,11 +59,11 @@ class Step(_Fixed):
     new tokens); ``slots`` int64 and ``positions`` int32 [num_tokens] for an append.  ``max_len``
     and ``max_new`` bound the sequences and their new tokens where the caller knows them: work is
     laid out by them, and what lies beyond them is not served.  0 leaves them open.
-    ``granted`` and ``free_count`` are set by ``PageTable.step``; ``crosses`` says that the rows are another
-    step's (``across``).
+    ``granted`` and ``free_count`` are set by ``PageTable.step``; ``taken`` is false for one that took no
+    pages (``commit=False``); ``crosses`` says that the rows are another step's (``across``).
     """
 
-    crosses = False
+    crosses, taken = False, True
 
     def __init__(self, tables: torch.Tensor, seq_lens: torch.Tensor, cu_new: torch.Tensor, slots: torch.Tensor | None,
                  positions: torch.Tensor | None, *, page_size: int, num_tokens: int, max_len: int = 0, max_new: int = 0,
@@ -101,9 +101,9 @@ class Step(_Fixed):
 class PageTable(_Fixed):
     """Block tables of ``max_seqs`` sequences over a pool of ``num_pages`` pages, on the GPU.
 
-    ``tables`` int32 [max_seqs, max_blocks] (-1: no page); ``free`` int32 [num_pages], of which the
-    first ``free_count`` are the free pages, the last of them taken first.  Several layers' caches
-    share one table.
+    ``tables`` int32 [max_seqs, max_blocks] (-1: no page; what stands behind the blocks that a sequence's
+    length needs is of no meaning); ``free`` int32 [num_pages], of which the first ``free_count`` are the
+    free pages, the last of them taken first.  Several layers' caches share one table.
     """
 
     def __init__(self, num_pages: int, page_size: int, max_seqs: int, max_blocks: int, device="cuda"):
@@ -139,8 +139,9 @@ class PageTable(_Fixed):
         """Pages, slots and positions for ``new_lens`` more tokens of sequences that hold ``ctx_lens``
         (int32 [batch] on the GPU; batch row b uses table row b).  Rows 0 .. num_tokens - 1 of q, k
         and v hold the sequences' new tokens in order; what is left over is padding.  A sequence that
-        does not fit the free pages, its table row or ``num_tokens`` has ``granted`` 0 and sees nothing.
-        ``commit=False`` works the step out without taking the pages."""
+        does not fit the free pages, its table row or ``num_tokens`` has ``granted`` 0 and sees nothing; one of a negative
+        length has no rows either.  ``commit=False`` works the step out without taking the pages: they stand in the
+        tables until another step is worked out, but stay free, and nothing can be appended to them."""
         b, dev = ctx_lens.numel(), self.device
         _expect("ctx_lens", ctx_lens, torch.int32, dev)
         _expect("new_lens", new_lens, torch.int32, dev, b)
@@ -166,7 +167,7 @@ class PageTable(_Fixed):
         s = Step.__new__(Step)
         vars(s).update(
             tables=self.tables if b == self._rows else self.tables[:b], seq_lens=seq_lens, cu_new=cu, slots=slots, positions=positions,
-            page_size=self.page_size, num_tokens=num_tokens, max_len=max_len, max_new=max_new, granted=granted, free_count=left, device=dev,
+            page_size=self.page_size, num_tokens=num_tokens, max_len=max_len, max_new=max_new, granted=granted, free_count=left, device=dev, taken=commit,
             _struct=_lib.KvStepStruct(self._places[0], self._places[1], p_lens, p_cu, p_slots, p_pos, num_tokens, b, self._blocks, max_len, max_new),
             _ws={})
         return s
@@ -273,6 +274,8 @@ class KvCache(_Fixed):
         rotated by ``rotary`` first, and gives ``q`` [num_tokens, heads, head_dim] rotated likewise.
         Pages that are not there take nothing, and rows of ``q`` without a position are left unset."""
         self._fits(step)
+        if not step.taken:
+            raise ValueError("the step took no pages (commit=False): they are free, and the next step's")
         t = _rows("k", k, self.kv_heads, self.head_dim, step)
         if _rows("v", v, self.kv_heads, self.head_dim, step) != t:
             raise ValueError(f"k is {k.dtype}, v {v.dtype}")
