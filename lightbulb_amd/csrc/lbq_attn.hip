@@ -38,7 +38,9 @@ struct Layout {
 // the CUs that it leaves, and parts of 2 steps a wave (a prompt of 100 with eight tokens at 3000 keys:
 // 24 us, 3 steps 30; of 200 with two at 8000: 34, 29, without limit 35); and parts of no more than 16
 // steps a wave where it leaves none (a prompt of 4000 with one token at 131071 keys: 279 us,
-// 8 steps 300, 32 286, whole 797).
+// 8 steps 300, 32 286, whole 797), but no more than four workgroups a CU: max_len may be far above
+// the real lengths (a chunk of 512 with 63 tokens at 2000 keys, max_len 131072: 94 us, without limit 258, two a CU 80; with
+// 255 at 1000 keys 160 and 898; with 15 at 2000 and one at 131071 131, 128 and 268).
 Layout layout(const KvAttention &a) {
     Layout l = {};
     const int64_t group = a.q_heads / a.c.kv_heads, t = a.s.num_tokens;
@@ -78,7 +80,7 @@ Layout layout(const KvAttention &a) {
     const int64_t tiles = (l.plan.tiles_per ? l.plan.tiles : t * group / tile_rows + (sequences + 1) / 2) * a.c.kv_heads;
     l.plan.splits_long = l.any_long && steps >= 8 ? splits(cus / tiles, 2, (int64_t)l.plan.tiles * a.c.kv_heads) : 1;
     const int64_t groups = sequences * a.c.kv_heads * short_tiles, least = l.any_long ? 2 * waves : 2;
-    const int64_t wanted = l.any_long ? std::max((cus - tiles) / groups, steps / (16 * waves)) : cus / groups;
+    const int64_t wanted = l.any_long ? std::max((cus - tiles) / groups, std::min(steps / (16 * waves), 4 * cus / groups)) : cus / groups;
     l.plan.splits_short = l.any_short && steps * a.c.head_dim > 256 * waves ? splits(wanted, least, (int64_t)l.plan.short_groups * a.c.kv_heads) : 1;
     const int64_t per = short_rows / group;
     l.plan.short_per = l.any_short && per * a.s.batch < t ? (int)per : 0;

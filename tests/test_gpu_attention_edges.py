@@ -221,3 +221,18 @@ def test_a_step_across_sees_all_of_the_source(dev, new):
     assert torch.equal(at.paged_attention(q, cache, mine.across(source), causal=True), want) == (t == 2)
     with pytest.raises(ValueError, match="window"):
         at.paged_attention(q, cache, mine.across(source), window=5)
+
+
+def test_workspace_is_bounded_beside_a_prompt(dev, lbq):
+    # many single tokens beside a chunk, and a table for far longer sequences: parts for a few workgroups a CU at most,
+    # of 64 rows a sequence and 130 values a row (without limit 16 parts: 68 MB for 64 sequences, 204 MB for 256)
+    for batch in (8, 64, 256):
+        cache, step, _ = setup(dev, "int8", torch.float32, 64, 128, 8, 4, [100] * batch, [512] + [1] * (batch - 1), pad=0)
+        wide = at.Step(step.tables, step.seq_lens, step.cu_new, None, None, page_size=64, num_tokens=step.num_tokens, max_new=512)
+        wide._struct.max_blocks = wide._struct.table_stride = 2048  # sequences of up to 131072 tokens; nothing is read
+        n = ctypes.c_size_t()
+        assert lbq.lbq_kv_attention_workspace(cache._ctx, cache._struct, wide._struct, 32, n) == 0
+        cus = torch.cuda.get_device_properties(dev).multi_processor_count
+        short = max(1, 4 * cus // (batch * 8)) * batch * 4 * 32
+        long = max(1, 256 // ((512 + batch) * 4 // 256 * 8)) * step.num_tokens * 32
+        assert n.value <= (short + long) * 130 * 4
