@@ -29,7 +29,9 @@ struct Layout {
 // Parts: as many as leave every CU one workgroup.  Up to there each part is so much less work in a
 // row; beyond, a second filling of the CUs costs more than it brings (12 tokens at 8000 keys, 96 workgroups: 2
 // parts 40 us, 3 parts 55; 40 tokens at 4000, 320 workgroups: whole 76, 2 parts 76, 3 parts 80; 1200
-// rows over 4000 keys, 40 tiles: 6 parts 60, 7 parts 82, whole 176).  Parts are joined by a launch of
+// rows over 4000 keys, 40 tiles: 6 parts 60, 7 parts 82, whole 176).  Workgroups of the short form are counted by the
+// batch's tokens, not by the most that each sequence could have (12 single tokens at 4000 keys without max_new 26.4
+// us, by the most 31; 12 tokens of 6 sequences at 3000, up to 5 each, 18.8 and 22.9).  Parts are joined by a launch of
 // 4 to 5 us, so that short contexts are left whole: in the short form up to 2 steps a wave of 64 keys of 128
 // channels (1100 keys: whole 13.3 us, parts 11.8 to 12.3; 800: 11.7, 11.8; at 64 channels 1100: 9.5, 11.9), in
 // the long form up to 7 steps (400 rows over 200 keys: whole 20.3, 2 parts 22.8).  A part has at
@@ -79,7 +81,9 @@ Layout layout(const KvAttention &a) {
     // (ragged sequences: the last tile of each is half full in the mean)
     const int64_t tiles = (l.plan.tiles_per ? l.plan.tiles : t * group / tile_rows + (sequences + 1) / 2) * a.c.kv_heads;
     l.plan.splits_long = l.any_long && steps >= 8 ? splits(cus / tiles, 2, (int64_t)l.plan.tiles * a.c.kv_heads) : 1;
-    const int64_t groups = sequences * a.c.kv_heads * short_tiles, least = l.any_long ? 2 * waves : 2;
+    // (of the short form: no sequence has fewer than its first token's, and the others' rows fill theirs)
+    const int64_t first = (group + attn::SHORT_ROWS - 1) / attn::SHORT_ROWS, more = ((t - sequences) * group + attn::SHORT_ROWS - 1) / attn::SHORT_ROWS;
+    const int64_t groups = std::min(sequences * first + more, sequences * short_tiles) * a.c.kv_heads, least = l.any_long ? 2 * waves : 2;
     const int64_t wanted = l.any_long ? std::max((cus - tiles) / groups, std::min(steps / (16 * waves), 4 * cus / groups)) : cus / groups;
     l.plan.splits_short = l.any_short && steps * a.c.head_dim > 256 * waves ? splits(wanted, least, (int64_t)l.plan.short_groups * a.c.kv_heads) : 1;
     const int64_t per = short_rows / group;

@@ -236,3 +236,12 @@ def test_workspace_is_bounded_beside_a_prompt(dev, lbq):
         short = max(1, 4 * cus // (batch * 8)) * batch * 4 * 32
         long = max(1, 256 // ((512 + batch) * 4 // 256 * 8)) * step.num_tokens * 32
         assert n.value <= (short + long) * 130 * 4
+
+
+@pytest.mark.parametrize("kv,group,ctx,new", [(8, 4, [4000] * 12, [1] * 12), (2, 4, [5000, 70], [1, 1]), (8, 4, [3000] * 6, [1, 5, 1, 3, 1, 1]), (1, 17, [9000, 10, 0], [1, 2, 1])])
+def test_parts_without_a_bound_on_new_tokens(dev, lbq, kv, group, ctx, new):
+    # the parts go by the tokens that are there, not by the most that a sequence could have of them
+    cache, step, q = setup(dev, "int8", torch.float32, 64, 128, kv, group, ctx, new, pad=0, slack=0)
+    out = torch.full(q.shape, 7.0, device=dev)
+    assert attend_with_workspace(lbq, q, cache, step, out, math.nan) > 0
+    check(q, cache, step, got=out)
