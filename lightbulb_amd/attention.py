@@ -27,6 +27,8 @@ _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 _KINDS = {"int8": (0, torch.int8), "e4m3": (1, torch.float8_e4m3fn)}
 PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 96, 128, 192, 256)
+#: lengths and counts go to the library in 32 bits; a bound above that is this one
+_MOST = 2 ** 31 - 1
 
 
 def _expect(name: str, t: torch.Tensor, dtype, device, numel: int | None = None) -> None:
@@ -84,7 +86,8 @@ class Step(_Fixed):
             tables=tables, seq_lens=seq_lens, cu_new=cu_new, slots=slots, positions=positions, page_size=page_size, num_tokens=num_tokens,
             max_len=max_len, max_new=max_new, granted=granted, free_count=free_count, device=tables.device, _struct=_lib.KvStepStruct(
                 tables.data_ptr(), tables.stride(0), seq_lens.data_ptr(), cu_new.data_ptr(), slots.data_ptr() if slots is not None else None,
-                positions.data_ptr() if positions is not None else None, num_tokens, tables.shape[0], tables.shape[1], max_len, max_new),
+                positions.data_ptr() if positions is not None else None, num_tokens, tables.shape[0], tables.shape[1],
+                min(max_len, _MOST), min(max_new, _MOST)),
             _ws={})  # bytes of workspace by heads and head_dim: every layer asks
 
     def across(self, source: "Step") -> "Step":
@@ -168,7 +171,8 @@ class PageTable(_Fixed):
         vars(s).update(
             tables=self.tables if b == self._rows else self.tables[:b], seq_lens=seq_lens, cu_new=cu, slots=slots, positions=positions,
             page_size=self.page_size, num_tokens=num_tokens, max_len=max_len, max_new=max_new, granted=granted, free_count=left, device=dev, taken=commit,
-            _struct=_lib.KvStepStruct(self._places[0], self._places[1], p_lens, p_cu, p_slots, p_pos, num_tokens, b, self._blocks, max_len, max_new),
+            _struct=_lib.KvStepStruct(self._places[0], self._places[1], p_lens, p_cu, p_slots, p_pos, num_tokens, b, self._blocks,
+                                      min(max_len, _MOST), min(max_new, _MOST)),
             _ws={})
         return s
 

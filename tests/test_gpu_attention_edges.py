@@ -245,3 +245,13 @@ def test_parts_without_a_bound_on_new_tokens(dev, lbq, kv, group, ctx, new):
     out = torch.full(q.shape, 7.0, device=dev)
     assert attend_with_workspace(lbq, q, cache, step, out, math.nan) > 0
     check(q, cache, step, got=out)
+
+
+def test_bounds_beyond_32_bits(dev):
+    cache, step, q = setup(dev, "int8", torch.float32, 16, 64, 2, 2, [300, 2], [1, 20], pad=0)
+    want = at.paged_attention(q, cache, step)
+    free = at.Step(step.tables, step.seq_lens, step.cu_new, None, None, page_size=16, num_tokens=21, max_len=2 ** 32 + 10, max_new=2 ** 32 + 1)
+    assert torch.equal(at.paged_attention(q, cache, free), want)
+    table = at.PageTable(8, 16, 1, 8, dev)
+    step = table.step(i32([0], dev), i32([100], dev), 100, max_len=2 ** 32 + 10, max_new=2 ** 32 + 1)
+    assert step._struct.max_len == step._struct.max_new == 2 ** 31 - 1

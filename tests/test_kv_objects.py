@@ -1,5 +1,5 @@
 """The cache's objects hold addresses and sizes of the tensors they were made of: attributes that the library would
-not see again are not set anew."""
+not see again are not set anew, and sizes that its fields do not hold are not cut."""
 import pytest
 import torch
 
@@ -34,3 +34,13 @@ def test_attributes_are_fixed(no_device):
                 setattr(obj, name, new)
             assert getattr(obj, name) is kept
     assert step.across(step).crosses and not step.crosses
+
+
+@pytest.mark.parametrize("most", [2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 32 + 5, 10 ** 18])
+def test_bounds_beyond_32_bits_stay_bounds(most):
+    # (their low 32 bits would be another bound, and keys beyond it unseen)
+    step = at.Step(i32(2, 3), i32(2), i32(3), None, None, page_size=16, num_tokens=4, max_len=most, max_new=most)
+    assert step._struct.max_len == step._struct.max_new == 2 ** 31 - 1
+    assert (step.max_len, step.max_new) == (most, most)
+    across = step.across(step)
+    assert across._struct.max_len == across._struct.max_new == 2 ** 31 - 1
