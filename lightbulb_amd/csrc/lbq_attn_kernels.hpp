@@ -65,7 +65,9 @@ constexpr int SHORT_ROWS = 16;  // rows of one kv head's queries in a tile of th
 constexpr int TILE = 64;  // keys per step of either form
 
 // f16 parts of a query value and of a weight.  f16 outputs take weights of two parts too: one
-// part's rounding is as large as the output's own, and would leave it 1.4 times as far off.
+// part's rounding is as large as the output's own, and would leave it 1.4 times as far off.  bf16 outputs
+// take one: their own rounding is 16 times as large (the 8000-token prompt: 471 us and 0.00166 off the definition in 64
+// bits; with two parts 604 us and 0.00165, as 32-bit arithmetic has it; one value in ten is rounded to the neighbour instead).
 template <int DT>
 constexpr int QUERY_PARTS = DT == DT_F32 ? 2 : 1;
 template <int DT>
@@ -330,7 +332,7 @@ __device__ __forceinline__ float part_weight(float m, float l, float top) { retu
 // workgroups of unlike length start and end apart).  131071 keys of one sequence, 268 MB: 51 us, 5.3 TB/s,
 // and 4 to join 32 parts.  One workgroup takes 2.5 us for a step of its eight waves, most of it the
 // values' way to f16 and the weights, and 7 for launch, bounds, pages and the first codes: a short context's
-// time (1000 keys: 11.8 us).  16x16x32 products; in S^T lane
+// time (1000 keys: 12.3 us).  16x16x32 products; in S^T lane
 // (c, n) = (lane / 16, lane % 16) holds keys 16 c .. 16 c + 15 of the 64 for row n, which is
 // what the products with V take, and all of one page: one scale per lane.
 // ---------------------------------------------------------------------------
@@ -631,8 +633,9 @@ __global__ __launch_bounds__(64 * SHORT_WAVES<D>, D <= 128 ? 2 : 1) void k_attn_
 
 // ---------------------------------------------------------------------------
 // Long form: query rows of one kv head (row i * group + head: neighbouring tokens see nearly the
-// same keys), 32 for each wave.  Bound by the matrix cores and by the vector unit's weights
-// (seven instructions each), which hardly run at once within a wave.  64 keys at a
+// same keys), 32 for each wave.  Long prompts are bound by the matrix cores and by the vector unit's weights
+// (seven instructions each), which hardly run at once within a wave; calls of few workgroups, or of unlike ones, by
+// the longest of them, by barriers and by waves without rows.  64 keys at a
 // time are turned into f16 once for all waves and kept in LDS, the next steps' codes on their
 // way from memory meanwhile.  32x32x16 products; rows of K lie in LDS in the order in which lane
 // (half, n) then holds keys 16 u + 8 half + j of its row n, what the products with V take.
@@ -648,10 +651,10 @@ __global__ __launch_bounds__(64 * SHORT_WAVES<D>, D <= 128 ? 2 : 1) void k_attn_
 // weights of 16 keys are formed between the products of the 16 before.
 //
 // A prompt of 8000 tokens in bf16, 32 heads of 128 channels, window 5000, 450.6 GFLOP: 463 to 479 us,
-// 0.94 to 0.97 PFLOP/s (a large library product: 1.14); the matrix cores are busy in 43 % of the cycles, the vector
-// unit in 49 %, at 2.0 GHz: the power limit.  Four chunks of 512 over contexts of 1500 in f32, 38.7 GFLOP and
-// twice the products: 97 us.  220 rows a head over 1500 states of 64 channels in f16: 44 us on 160 CUs, the
-// vector unit's time (per key and row as much as at 128 channels, for half the products).  Measured and no
+// 0.94 to 0.97 PFLOP/s (a large library product: 1.14); the matrix cores are busy in 41 % of the cycles, the vector
+// unit in 47 %, at 2.0 of 2.4 GHz: the power limit, as far as the clock says.  Four chunks of 512 over contexts of 1500
+// in f32, 38.7 GFLOP and twice the products: 98 us, units busy in 31 and 26 %.  220 rows a head over 1500 states of 64
+// channels in f16: 44 us on 160 CUs, where 4 to 7 of 8 waves have rows and the units are busy in 18 and 34 %.  Measured and no
 // better: steps of 128 keys (64 channels: -3 %, causal prompts +2 %), codes two steps ahead, four waves a workgroup
 // (618 us for the prompt), three buffers with the waves half a step apart (665), sums by dot products.
 // ---------------------------------------------------------------------------
