@@ -56,7 +56,7 @@ def row_bound(q, cache, step, scale, causal=True, window=0):
     exponential's last bits, in parts of itself, and the result, to the first order, by sum p e |v| + (sum p e) |out|.
     Values: one rounding for each 16 keys and each join, 2^-24 each.  f16 parts of a weight are off by half the smallest f16
     step where the row's largest weight with its value scale is at least 2^9: 2^-34 |code| of the largest p s, for each
-    key; bf16 weights are one f16 part: 2^-11.  A page's scale below 2^-80 of the largest counts as that."""
+    key; bf16 weights are one f16 part: 2^-11.  The result is rounded once, by half a step of its type at most.  A page's scale below 2^-80 of the largest counts as that."""
     codes, scales = [cache.k.double(), cache.v.double()], [cache.k_scales.double(), cache.v_scales.double()]
     heads, kv, page, ln2 = q.shape[1], cache.kv_heads, cache.page_size, math.log(2)
     g, out, bound = heads // kv, torch.zeros(q.shape, dtype=torch.float64, device=q.device), torch.zeros(q.shape, dtype=torch.float64, device=q.device)
@@ -89,7 +89,8 @@ def row_bound(q, cache, step, scale, causal=True, window=0):
             off = off + ((n / 16 + 64) * 2.0 ** -24 + (2.0 ** -11 if q.dtype == torch.bfloat16 else 0.0)) * mag
             off = off + n * 2.0 ** -34 * code * most + n * 2.0 ** -80 * code * s.max()
             out[t0:t1, h * g:(h + 1) * g] = o
-            bound[t0:t1, h * g:(h + 1) * g] = off * (1 + half) + half * o.abs() + tiny
+            step_half = half * torch.exp2(torch.floor(torch.log2(o.abs() + off)))  # of the result's own binade
+            bound[t0:t1, h * g:(h + 1) * g] = off + step_half.nan_to_num(0.0) + tiny
     return out, bound
 
 
@@ -255,3 +256,13 @@ def test_bounds_beyond_32_bits(dev):
     table = at.PageTable(8, 16, 1, 8, dev)
     step = table.step(i32([0], dev), i32([100], dev), 100, max_len=2 ** 32 + 10, max_new=2 ** 32 + 1)
     assert step._struct.max_len == step._struct.max_new == 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dim,ctx,new", [(64, 700, 1), (128, 90, 1), (128, 3000, 4), (64, 10, 130), (128, 0, 300), (192, 40, 70)])
+def test_rows_by_what_they_see(dev, dtype, kind, dim, ctx, new):
+    # ordinary rows by the narrow bound (f16 results from weights of one f16 part are outside it)
+    cache, step, q = setup(dev, kind, dtype, 32, dim, 2, 2, [ctx, 50], [new, 2], pad=0, spread=1.0)
+    check_rows(q, cache, step)
+    check_rows(q, cache, step, window=40)
