@@ -65,6 +65,8 @@ def row_bound(q, cache, step, scale, causal=True, window=0):
     tiny = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -24, torch.bfloat16: 2.0 ** -133}[q.dtype]
     for b, n in enumerate(lens):
         t0, t1 = cu[b], cu[b + 1]
+        if t0 == t1:
+            continue
         pages = step.tables[b, : -(-n // page)].long()
         j, pos = torch.arange(n, device=q.device), n - (t1 - t0) + torch.arange(t1 - t0, device=q.device)[:, None]
         seen = (j <= pos) & ((j > pos - window) if window else (j >= 0)) if causal else torch.ones(t1 - t0, n, dtype=torch.bool, device=q.device)
