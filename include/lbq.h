@@ -404,6 +404,69 @@ int lbq_kv_attention(lbq_ctx *ctx, const lbq_kv_cache *cache, const lbq_kv_step 
                      int64_t window, void *d_out, void *d_ws, size_t ws_bytes, void *stream);
 
 /* ---------------------------------------------------------------------------
+ * Linears in 8-bit integers with a scale for each token and channel, and the norms between
+ * them.  A token's values x[k] become int8 codes and one f32 scale:
+ *   scale = max_j |x[j]| / 127 rounded to f32, at least 2^-126; 0 where all values are 0
+ *   code  = x / scale to the nearest whole number, ties to even, as if the quotient were exact
+ * A token with a value that is not finite has the scale NaN and codes 0: its products are NaN.
+ * A weight has int8 codes [n][k] and one f32 scale for each of its n channels.  An output is
+ *   y[i][j] = scale[i] * channel_scale[j] * sum_k code[i][k] weight_code[j][k] + bias[j]
+ * with the sum exact (k is at most 131071, codes may be -128) and two roundings to f32 after it, in the
+ * last of which the bias goes in; where a scale is outside 2^-60 to 2^44, 0 too, it is formed in 64
+ * bits.  The same bits come out whatever m is and wherever the row stands.
+ * Rows of codes, of tokens and weights alike, are LBQ_I8_ROW(k) bytes apart and zero from k on, 16-byte
+ * aligned.  Types are LBQ_TYPE_F32, _F16 or _BF16; rows of values may have any stride (in elements).
+ * All calls run on the context's device and use none of its memory: calls on different streams need
+ * no order among themselves but that of their own buffers.
+ * ------------------------------------------------------------------------- */
+#define LBQ_I8_ROW(k) (((int64_t)(k) + 127) / 128 * 128)
+
+typedef struct lbq_i8_weight {
+    const int8_t *d_codes;  /* [n][LBQ_I8_ROW(k)] */
+    const float *d_scales;  /* [n] */
+    const float *d_bias;    /* [n], or NULL */
+    int64_t n;
+} lbq_i8_weight;
+
+/* x[m][k] -> codes [m][LBQ_I8_ROW(k)] and scales [m].  Weights' rows are quantised by the same call. */
+int lbq_i8_quantize(lbq_ctx *ctx, uint32_t type, const void *d_x, int64_t row_stride, int64_t m, int64_t k,
+                    int8_t *d_codes, float *d_scales, void *stream);
+
+/* d_ys[i][m][n_i] of `count` weights (up to LBQ_GROUP_MAX) on one set of tokens: q, k and v, say.  d_x NULL:
+ * d_codes and d_scales hold the tokens.  Else x[m][k] of x_type is quantised first, into d_codes and
+ * d_scales, whose contents then are not the caller's. */
+int lbq_i8_linear(lbq_ctx *ctx, uint32_t x_type, const void *d_x, int64_t x_stride, int8_t *d_codes, float *d_scales,
+                  int64_t m, int64_t k, const lbq_i8_weight *const *ws, int count, uint32_t out_type, void *const *d_ys,
+                  void *stream);
+
+/* d_y[m][n] = silu(g) * u of the two weights' products g and u (f32, biases included), silu(v) =
+ * v / (1 + exp(-v)): mlp_wrapper.rs:190-194 over such weights, which have the same n and k. */
+int lbq_i8_gate_up_silu(lbq_ctx *ctx, uint32_t x_type, const void *d_x, int64_t x_stride, int8_t *d_codes,
+                        float *d_scales, int64_t m, int64_t k, const lbq_i8_weight *gate, const lbq_i8_weight *up,
+                        uint32_t out_type, void *d_y, void *stream);
+
+/* The residual stream's update by a block's output x[m][k] and the norm in front of the next block:
+ *   r = residual + scale * gate * post(x)        y = norm(r)
+ * residual, gate and the norms may each be NULL (nothing is added; no gate; no norm).  A norm is
+ *   LBQ_NORM_RMS    u / sqrt(mean(u^2) + eps) * (weight + offset) + bias
+ *   LBQ_NORM_LAYER  the same of u - mean(u)
+ * with f32 weight and bias (may be NULL) of k values.  The gate is of x's type, gate_stride elements from row to
+ * row, 0: one for all.  r [m][k] is of residual_type and y [m][k] of x's, both contiguous; with d_codes and
+ * d_scales y becomes codes, of its values rounded to f32, and d_y is NULL.  d_r may be NULL, or d_residual
+ * itself where its rows are contiguous.  A row is worked out in 64 bits and rounded where it is stored; y is
+ * the norm of r before its rounding.  k is at most 32768. */
+enum lbq_norm_kind { LBQ_NORM_RMS = 0, LBQ_NORM_LAYER = 1 };
+typedef struct lbq_norm {
+    int32_t kind; /* lbq_norm_kind */
+    float eps, offset;
+    const float *d_weight, *d_bias;
+} lbq_norm;
+int lbq_residual_norm(lbq_ctx *ctx, uint32_t type, const void *d_x, int64_t x_stride, uint32_t residual_type,
+                      const void *d_residual, int64_t residual_stride, const lbq_norm *post, const void *d_gate,
+                      int64_t gate_stride, float scale, const lbq_norm *norm, int64_t m, int64_t k, void *d_r, void *d_y,
+                      int8_t *d_codes, float *d_scales, void *stream);
+
+/* ---------------------------------------------------------------------------
  * GGUF container (v3, little-endian) and the direct GGUF -> device upload.
  * lbq_gguf_open maps the file and parses it as the reference's parse_gguf does
  * (/root/reference/src/gguf/parser.rs:136-213, reached from Content::read,

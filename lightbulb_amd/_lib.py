@@ -43,6 +43,17 @@ class KvStepStruct(ctypes.Structure):
                 ("max_new", _I32)]
 
 
+class I8WeightStruct(ctypes.Structure):
+    """``lbq_i8_weight``"""
+    _fields_ = [("d_codes", _VP), ("d_scales", _VP), ("d_bias", _VP), ("n", _I64)]
+
+
+class NormStruct(ctypes.Structure):
+    """``lbq_norm``"""
+    _fields_ = [("kind", _I32), ("eps", _c.c_float), ("offset", _c.c_float), ("d_weight", _VP), ("d_bias", _VP)]
+
+
+_I8W, _NORM = _c.POINTER(I8WeightStruct), _c.POINTER(NormStruct)
 _CACHE, _STEP = _c.POINTER(KvCacheStruct), _c.POINTER(KvStepStruct)
 SIGNATURES = {
     "lbq_last_error": (_c.c_char_p, []),
@@ -82,6 +93,11 @@ SIGNATURES = {
     "lbq_kv_attention_workspace": (_c.c_int, [_VP, _CACHE, _STEP, _I32, _c.POINTER(_SZ)]),
     "lbq_kv_attention": (_c.c_int, [_VP, _CACHE, _STEP, _U32, _VP, _I64, _I64, _I32, _c.c_float, _I32, _I64, _VP, _VP, _SZ,
                                     _VP]),
+    "lbq_i8_quantize": (_c.c_int, [_VP, _U32, _VP, _I64, _I64, _I64, _VP, _VP, _VP]),
+    "lbq_i8_linear": (_c.c_int, [_VP, _U32, _VP, _I64, _VP, _VP, _I64, _I64, _c.POINTER(_VP), _c.c_int, _U32, _c.POINTER(_VP), _VP]),
+    "lbq_i8_gate_up_silu": (_c.c_int, [_VP, _U32, _VP, _I64, _VP, _VP, _I64, _I64, _I8W, _I8W, _U32, _VP, _VP]),
+    "lbq_residual_norm": (_c.c_int, [_VP, _U32, _VP, _I64, _U32, _VP, _I64, _NORM, _VP, _I64, _c.c_float, _NORM, _I64, _I64, _VP, _VP,
+                                     _VP, _VP, _VP]),
     "lbq_gguf_open": (_c.c_int, [_c.c_char_p, _c.POINTER(_VP)]),
     "lbq_gguf_close": (_c.c_int, [_VP]),
     "lbq_gguf_header": (_c.c_int, [_VP, _c.POINTER(_U32), _c.POINTER(_I64), _c.POINTER(_I64), _c.POINTER(_c.c_uint64),

@@ -1,0 +1,144 @@
+"""The residual stream's update and the norms before and after a block against their definition in 64 bits."""
+import math
+
+import pytest
+import torch
+
+import int8_ref as ref
+from lightbulb_amd import int8
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def values(gen, m, k, dtype, dev, spread=1.0):
+    return (torch.randn(m, k, generator=gen) * spread).to(dtype).to(dev)
+
+
+def make_norm(gen, k, kind, dev, bias=None, offset=0.0, eps=1e-5):
+    """(Norm, its plain form), or (None, None)."""
+    if not kind:
+        return None, None
+    w = 1 + 0.3 * torch.randn(k, generator=gen) - offset
+    b = torch.randn(k, generator=gen) if (kind == "layer" if bias is None else bias) else None
+    return (int8.Norm(w.to(dev), eps, bias=None if b is None else b.to(dev), kind=kind, offset=offset),
+            {"kind": kind, "weight": w, "bias": b, "eps": torch.tensor(eps, dtype=torch.float32).item(), "offset": torch.tensor(offset, dtype=torch.float32).item()})
+
+
+def check(x, residual, gate, scale, post, pre, quantize=False, **kw):
+    """One call against its definition: 64-bit arithmetic leaves about 1e-13 of the terms, then one rounding (f32), or two."""
+    r, y = int8.residual_norm(x, residual, post=post[0], gate=gate, scale=scale, norm=pre[0], quantize=quantize)
+    rw, yw = ref.residual_norm(x, residual, post[1], gate, torch.tensor(scale, dtype=torch.float32).double().item(), pre[1])
+    if residual is None and gate is None and post[0] is None and scale == 1.0:
+        assert r is x
+    else:
+        rt = x.dtype if residual is None else residual.dtype
+        assert r.dtype == rt and r.shape == x.shape
+        size = rw.abs() + (0 if residual is None else residual.cpu().double().abs())
+        ref.close(r, rw, ref.stored(rw, ref.U * rw.abs() + 1e-13 * size + ref.least(torch.float32), rt))
+    if pre[0] is None:
+        assert y is None
+        return
+    if quantize:
+        c, s = ref.codes(yw.float())
+        assert torch.equal(y.codes.cpu().double(), c) and torch.equal(torch.nan_to_num(y.scales.cpu(), nan=-1.0), torch.nan_to_num(s, nan=-1.0))
+        assert not y._rows.cpu()[:, x.shape[-1]:].any()
+    else:
+        assert y.dtype == x.dtype and y.shape == x.shape
+        far = 1e-12 * (1 + yw.abs())
+        if pre[1]["kind"] == "layer":
+            # a mean of at most 32 additions in a row on either side, each off by 2^-53 of the largest value, over the spread
+            spread = (rw.var(-1, unbiased=False, keepdim=True) + pre[1]["eps"]).sqrt()
+            far = far + 64 * 2.0 ** -53 * rw.abs().amax(-1, keepdim=True) / spread * (pre[1]["weight"].double() + pre[1]["offset"]).abs()
+        ref.close(y, yw, ref.stored(yw, ref.U * yw.abs() + far, x.dtype))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("quantize", [False, True])
+@pytest.mark.parametrize("m,k", [(1, 1), (3, 8), (1, 100), (5, 512), (2, 513), (9, 1000), (1, 2048), (4, 2049), (1, 4096), (6, 5000), (2, 8192),
+                                 (3, 8200), (1, 16384), (2, 16385), (1, 32768)])
+def test_widths(dev, dtype, quantize, m, k):
+    gen = torch.Generator().manual_seed(m + k)
+    x, res = values(gen, m, k, dtype, dev), values(gen, m, k, torch.float32, dev, 2.0)
+    check(x, res, None, 1.0, make_norm(gen, k, "rms", dev), make_norm(gen, k, "rms", dev), quantize)
+    check(x, None, None, 1.0, (None, None), make_norm(gen, k, "layer", dev), quantize)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("stream", DTYPES)
+@pytest.mark.parametrize("post", ["", "rms", "layer"])
+@pytest.mark.parametrize("pre", ["", "rms", "layer"])
+def test_forms(dev, dtype, stream, post, pre):
+    gen = torch.Generator().manual_seed(len(post) + 3 * len(pre))
+    m, k = 7, 700
+    x, res = values(gen, m, k, dtype, dev), values(gen, m, k, stream, dev)
+    gates = [None, values(gen, 1, k, dtype, dev)[0], values(gen, m, k, dtype, dev)]
+    for gate in gates:
+        for scale in (1.0, 0.22):
+            for offset in (0.0, 1.0):
+                ps, pr = make_norm(gen, k, post, dev, offset=offset), make_norm(gen, k, pre, dev, bias=offset == 0.0, offset=offset)
+                for residual in (res, None):
+                    check(x, residual, gate, scale, ps, pr)
+                if pre:
+                    check(x, res, gate, scale, ps, pr, quantize=True)
+
+
+@pytest.mark.parametrize("quantize", [False, True])
+def test_layer_norm_of_shifted_rows(dev, quantize):
+    # a mean a million times the spread: the sums hold it
+    gen = torch.Generator().manual_seed(1)
+    x = values(gen, 4, 1500, torch.float32, dev) + torch.tensor([1e6, -3e5, 0.0, 1e3], device=dev)[:, None]
+    check(x, None, None, 1.0, (None, None), make_norm(gen, 1500, "layer", dev), quantize)
+    check(x, values(gen, 4, 1500, torch.float32, dev), None, 0.5, (None, None), make_norm(gen, 1500, "layer", dev), quantize)
+
+
+def test_rows_of_odd_values(dev):
+    gen = torch.Generator().manual_seed(2)
+    k = 600
+    x = torch.randn(9, k, generator=gen)
+    x[0] = 0.0
+    x[1] *= 1e30   # squares beyond f32
+    x[2] *= 1e-30  # under eps
+    x[3, 5] = math.nan
+    x[4, 599] = math.inf
+    x[5] = 1.0
+    x[6] = torch.randn(k, generator=gen) * 1e-42  # subnormal
+    x = x.to(dev)
+    rms, layer = make_norm(gen, k, "rms", dev), make_norm(gen, k, "layer", dev)
+    for pre in (rms, layer):
+        for quantize in (False, True):
+            check(x, None, None, 1.0, (None, None), pre, quantize)
+    r, y = int8.residual_norm(x, torch.ones_like(x), norm=rms[0])
+    assert torch.isnan(y[3]).all() and torch.isfinite(y[[0, 1, 2, 5, 6, 7, 8]]).all() and torch.isnan(r[3, 5]) and torch.isfinite(r[3, 6])
+
+
+def test_no_eps(dev):
+    # a zero row over eps = 0 is 0 / 0, by the formula; others are as they are
+    gen = torch.Generator().manual_seed(3)
+    x = values(gen, 3, 130, torch.float32, dev)
+    x[1] = 0.0
+    for quantize in (False, True):
+        check(x, None, None, 1.0, (None, None), make_norm(gen, 130, "rms", dev, eps=0.0), quantize)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_strided_inputs(dev, dtype):
+    gen = torch.Generator().manual_seed(4)
+    base = values(gen, 24, 900, dtype, dev)
+    rms = make_norm(gen, 301, "rms", dev)
+    x, res, gate = base[:8, 1:302], base[8:24:2, 300:601], base[3:4, 7:308].expand(8, 301)
+    check(x, res, gate, 0.5, make_norm(gen, 301, "layer", dev), rms)
+    check(x, res, None, 1.0, (None, None), rms, quantize=True)
+    x3 = base.view(4, 6, 900)[:, :1, 2:303]
+    r, y = int8.residual_norm(x3, x3, norm=rms[0])
+    assert r.shape == y.shape == (4, 1, 301)
+    rw, yw = ref.residual_norm(x3, x3, None, None, 1.0, rms[1])
+    ref.close(y, yw, ref.stored(yw, ref.U * yw.abs() + 1e-12, dtype))
+
+
+def test_no_rows(dev):
+    n = int8.Norm(torch.ones(64, device=dev), 1e-5)
+    r, y = int8.residual_norm(torch.empty(0, 64, device=dev), torch.empty(0, 64, device=dev), norm=n)
+    assert r.shape == y.shape == (0, 64)
+    r, y = int8.residual_norm(torch.empty(2, 0, 64, device=dev), norm=n, quantize=True)
+    assert y.shape == (2, 0, 64) and y.scales.shape == (2, 0)
