@@ -44,16 +44,15 @@ class KvStepStruct(ctypes.Structure):
 
 
 class I8WeightStruct(ctypes.Structure):
-    """``lbq_i8_weight``"""
+    """``lbq_i8_weight``, passed by its address"""
     _fields_ = [("d_codes", _VP), ("d_scales", _VP), ("d_bias", _VP), ("n", _I64)]
 
 
 class NormStruct(ctypes.Structure):
-    """``lbq_norm``"""
+    """``lbq_norm``, passed by its address"""
     _fields_ = [("kind", _I32), ("eps", _c.c_float), ("offset", _c.c_float), ("d_weight", _VP), ("d_bias", _VP)]
 
 
-_I8W, _NORM = _c.POINTER(I8WeightStruct), _c.POINTER(NormStruct)
 _CACHE, _STEP = _c.POINTER(KvCacheStruct), _c.POINTER(KvStepStruct)
 SIGNATURES = {
     "lbq_last_error": (_c.c_char_p, []),
@@ -95,8 +94,8 @@ SIGNATURES = {
                                     _VP]),
     "lbq_i8_quantize": (_c.c_int, [_VP, _U32, _VP, _I64, _I64, _I64, _VP, _VP, _VP]),
     "lbq_i8_linear": (_c.c_int, [_VP, _U32, _VP, _I64, _VP, _VP, _I64, _I64, _c.POINTER(_VP), _c.c_int, _U32, _c.POINTER(_VP), _VP]),
-    "lbq_i8_gate_up_silu": (_c.c_int, [_VP, _U32, _VP, _I64, _VP, _VP, _I64, _I64, _I8W, _I8W, _U32, _VP, _VP]),
-    "lbq_residual_norm": (_c.c_int, [_VP, _U32, _VP, _I64, _U32, _VP, _I64, _NORM, _VP, _I64, _c.c_float, _NORM, _I64, _I64, _VP, _VP,
+    "lbq_i8_gate_up_silu": (_c.c_int, [_VP, _U32, _VP, _I64, _VP, _VP, _I64, _I64, _VP, _VP, _U32, _VP, _VP]),
+    "lbq_residual_norm": (_c.c_int, [_VP, _U32, _VP, _I64, _U32, _VP, _I64, _VP, _VP, _I64, _c.c_float, _VP, _I64, _I64, _VP, _VP,
                                      _VP, _VP, _VP]),
     "lbq_gguf_open": (_c.c_int, [_c.c_char_p, _c.POINTER(_VP)]),
     "lbq_gguf_close": (_c.c_int, [_VP]),

@@ -41,7 +41,7 @@ SOURCES = ["lbq_act.hip", "lbq_gemv.hip", "lbq_gemv_q4k.hip", "lbq_gemv_q5k.hip"
            "lbq_gemm_q6k.hip", "lbq_gemm_q8_0.hip", "lbq_gemm_q4_0.hip", "lbq_gemm_q5_0.hip",
            "lbq_gemm_k23.hip", "lbq_gemm_b32.hip", "lbq_dense.hip", "lbq_wquant.hip",
            "lbq_kv.hip", "lbq_attn.hip", "lbq_attn_d64.hip", "lbq_attn_d96.hip", "lbq_attn_d128.hip",
-           "lbq_attn_d192.hip", "lbq_attn_d256.hip", "lbq_i8.hip", "lbq_i8_gemm.hip",
+           "lbq_attn_d192.hip", "lbq_attn_d256.hip", "lbq_i8.hip", "lbq_i8_gemv.hip", "lbq_i8_gemm.hip",
            "lbq_api.cpp", "lbq_kv_api.cpp", "lbq_i8_api.cpp", "lbq_gguf.cpp"]
 
 

@@ -16,6 +16,7 @@ enum : int { I8_F32 = 0, I8_F16 = 1, I8_BF16 = 2 };
 constexpr int I8_GROUP = 4;
 constexpr int64_t I8_MAX_K = 131071, I8_MAX_N = (int64_t)1 << 24, I8_MAX_M = (int64_t)1 << 24;
 constexpr int64_t NORM_MAX_K = 32768;
+constexpr int I8_FUSED_ROWS = 4, I8_FUSED_CODES = 16384;
 inline int64_t i8_kp(int64_t k) { return (k + 127) / 128 * 128; }
 
 // rows of values [m][k], `stride` elements apart
@@ -43,8 +44,12 @@ struct I8Linear {
     const float *t[I8_GROUP], *bias[I8_GROUP];
     void *y[I8_GROUP];  // [m][n]
     int n[I8_GROUP];
-    I8Rows x;  // values that codes and scales are of (x.p nullptr: they are there)
+    I8Rows x;  // values that the kernel quantises itself (x.p nullptr: codes and scales are there)
 };
+// whether the product's kernel quantises m rows of values itself
+bool i8_quantizes_in_kernel(int64_t m, int64_t k);
+bool i8_streams(const I8Linear &a);  // the kernel for few tokens
+hipError_t launch_i8_stream(const I8Linear &a, hipStream_t st);
 hipError_t launch_i8_linear(const I8Linear &a, hipStream_t st);
 
 struct NormArgs {
@@ -169,13 +174,20 @@ __device__ __forceinline__ float i8_result(int acc, float s, float t, float b) {
 __device__ __forceinline__ float i8_result_wide(int acc, float s, float t, float b) {
     return i8_usual(s) && i8_usual(t) ? i8_result(acc, s, t, b) : (float)((double)acc * (double)s * (double)t + (double)b);
 }
-// g / (1 + exp(-g)) u.  exp as 2^(h + l) with h + l = -g log2(e) to 48 bits: a plain product would be
-// off by |g| 2^-24 of the result.
+// g / (1 + exp(-g)) u, for an output of type OUT.  F32: exp as 2^(h + l) with h + l = -g log2(e) to 48 bits, where a
+// plain product would be off by |g| 2^-24 of the result; what l adds is kept beside 1, so that an h beyond the
+// exponent's range leaves no inf - inf.
+template <int OUT>
 __device__ __forceinline__ float i8_silu_mul(float g, float u) {
-    constexpr float L = 1.44269502f, LO = 1.92596303e-8f;  // log2(e), and what L leaves of it
-    const float h = -g * L, l = fabsf(h) <= 126.f ? fmaf(-g, L, -h) - g * LO : 0.f;
-    const float e = __builtin_amdgcn_exp2f(h);
-    const float d = h > 126.f ? INFINITY : 1.f + fmaf(e, l * 0.693147182f, e);
+    constexpr float L = 1.44269502f, LO = 1.92596303e-8f, LN2 = 0.693147182f;  // log2(e), and what L leaves of it
+    const float h = -g * L;
+    float d;
+    if constexpr (OUT == I8_F32) {
+        const float l = fmaf(-g, LO * LN2, fmaf(fmaf(-g, L, -h), LN2, 1.f));
+        d = fmaf(__builtin_amdgcn_exp2f(h), __builtin_amdgcn_fmed3f(l, 0.9f, 1.1f), 1.f);
+    } else {
+        d = 1.f + __builtin_amdgcn_exp2f(h);
+    }
     return g * __builtin_amdgcn_rcpf(d) * u;
 }
 #endif

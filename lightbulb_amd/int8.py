@@ -22,13 +22,15 @@ import ctypes
 import torch
 
 from . import _lib
-from .quantized import GROUP_MAX, _stream, context
+from .quantized import GROUP_MAX, _ctxs, _stream, context
 
 #: element types of values -> the library's type ids
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
+_VP1 = ctypes.c_void_p * 1
 _KINDS = {"rms": 0, "layer": 1}
 MAX_K = 131071  # sums of 2^14 k stay below 2^31
 NORM_MAX_K = 32768
+_FUSED_ROWS, _FUSED_CODES = 4, 16384  # LBQ_I8_FUSED_ROWS, LBQ_I8_FUSED_CODES
 
 
 def _row(k: int) -> int:
@@ -41,26 +43,28 @@ def _values(name: str, xs: torch.Tensor) -> tuple[int, int, int]:
     t = _DTYPES.get(xs.dtype)
     if t is None:
         raise ValueError(f"{name} must be f32, f16 or bf16, got {xs.dtype}")
-    shape, strides = xs.shape, xs.stride()
+    shape = xs.shape
     if len(shape) < 2:
         raise ValueError(f"{name} has only one dimension {tuple(shape)}")
     k = shape[-1]
-    if len(shape) == 2:
-        m, stride = shape[0], strides[0]
-    elif xs.is_contiguous():
-        m, stride = xs.numel() // k if k else 0, k
-    else:
-        m, stride, step = 1, 0, None
-        for n, s in zip(reversed(shape[:-1]), reversed(strides[:-1])):
-            if n != 1:
-                if step is not None and s != step:
-                    raise ValueError(f"{name} {tuple(shape)} of strides {strides}: rows must be evenly apart")
-                stride = s if step is None else stride
-                step = s * n
-            m *= n
+    if xs.is_contiguous():
+        return t, shape[0] if len(shape) == 2 else xs.numel() // max(k, 1), k
+    strides = xs.stride()
+    m, stride, step = 1, 0, None
+    for n, s in zip(reversed(shape[:-1]), reversed(strides[:-1])):
+        if n != 1:
+            if step is not None and s != step:
+                raise ValueError(f"{name} {tuple(shape)} of strides {strides}: rows must be evenly apart")
+            stride = s if step is None else stride
+            step = s * n
+        m *= n
     if k > 1 and strides[-1] != 1:
         raise ValueError(f"{name} {tuple(shape)} of strides {strides}: rows must be contiguous")
     return t, m, stride
+
+
+def _context(dev: torch.device) -> int:
+    return _ctxs.get(dev.index) or context(dev)
 
 
 def _vector(name: str, t: torch.Tensor, n: int, device) -> None:
@@ -85,8 +89,8 @@ class Int8Tokens(_Fixed):
     """Tokens as ``codes`` int8 [.., k] and ``scales`` f32 [..]: a value is code * scale.  Made by
     ``quantize_tokens`` and ``residual_norm``; ``dtype`` is that of the values they stand for."""
 
-    def __init__(self, rows: torch.Tensor, scales: torch.Tensor, shape: tuple[int, ...], dtype: torch.dtype):
-        vars(self).update(_rows=rows, scales=scales, shape=torch.Size(shape), dtype=dtype, device=rows.device)
+    def __init__(self, rows: torch.Tensor, scales: torch.Tensor, shape: torch.Size, dtype: torch.dtype):
+        vars(self).update(_rows=rows, scales=scales, shape=shape, dtype=dtype, device=rows.device)
 
     @property
     def codes(self) -> torch.Tensor:
@@ -109,10 +113,10 @@ def quantize_tokens(xs: torch.Tensor) -> Int8Tokens:
     """Each row of ``xs`` [.., k] as int8 codes and one scale, its largest magnitude / 127; codes are the nearest,
     ties to even.  A row with a value that is not finite has the scale NaN and codes 0."""
     t, m, stride = _values("xs", xs)
-    rows, scales = _empty_tokens(xs.shape, m, xs.device)
-    _lib.check(_lib.lib().lbq_i8_quantize(context(xs.device), t, xs.data_ptr(), stride, m, xs.shape[-1], rows.data_ptr(), scales.data_ptr(),
-                                          _stream(xs.device)))
-    return Int8Tokens(rows, scales, xs.shape, xs.dtype)
+    shape, dev = xs.shape, xs.device
+    rows, scales = _empty_tokens(shape, m, dev)
+    _lib.check(_lib.lib().lbq_i8_quantize(_context(dev), t, xs.data_ptr(), stride, m, shape[-1], rows.data_ptr(), scales.data_ptr(), _stream(dev)))
+    return Int8Tokens(rows, scales, shape, xs.dtype)
 
 
 class Int8Weight(_Fixed):
@@ -168,11 +172,16 @@ class Int8Linear(_Fixed):
             _vector("bias", bias, n, weight.device)
         struct = _lib.I8WeightStruct(weight._rows.data_ptr(), weight.scales.data_ptr(), bias.data_ptr() if bias is not None else None, n)
         vars(self).update(weight=weight, bias=bias, device=weight.device, _n=n, _k=k, _struct=struct, _at=ctypes.addressof(struct),
-                          _ctx=context(weight.device))
+                          _ptr=_VP1(ctypes.addressof(struct)), _ctx=context(weight.device))
 
     def forward(self, xs: "torch.Tensor | Int8Tokens", dtype: torch.dtype | None = None) -> torch.Tensor:
         """``xs`` [.., k], values or tokens quantised before; the output is of ``dtype``, by default that of the values."""
-        return int8_linear_group((self,), xs, dtype)[0]
+        dev = self.device
+        t, x, stride, codes, scales, m, out, dtype, _held = _input(xs, self._k, dev, dtype)
+        y = torch.empty((*xs.shape[:-1], self._n), dtype=dtype, device=dev)
+        if m:
+            _lib.check(_lib.lib().lbq_i8_linear(self._ctx, t, x, stride, codes, scales, m, self._k, self._ptr, 1, out, _VP1(y.data_ptr()), _stream(dev)))
+        return y
 
     __call__ = forward
 
@@ -183,17 +192,21 @@ class Int8Linear(_Fixed):
 def _input(xs, k: int, device, dtype):
     """(type id, values, stride, codes, scales, rows, out type id, out dtype, what keeps the codes' memory) of a product's
     input."""
-    if xs.shape[-1:] != (k,):
-        raise ValueError(f"input {tuple(xs.shape)} incompatible with k = {k}")
+    shape, own = xs.shape, xs.dtype
+    if not shape or shape[-1] != k:
+        raise ValueError(f"input {tuple(shape)} incompatible with k = {k}")
     if xs.device != device:
         raise ValueError(f"input on {xs.device}, weights on {device}")
-    dtype = xs.dtype if dtype is None else dtype
+    if dtype is None:
+        dtype = own
     out = _DTYPES.get(dtype)
     if out is None:
         raise ValueError(f"outputs must be f32, f16 or bf16, got {dtype}")
     if isinstance(xs, Int8Tokens):
         return 0, None, 0, xs._rows.data_ptr(), xs.scales.data_ptr(), xs._rows.shape[0], out, dtype, xs
     t, m, stride = _values("the input", xs)
+    if m <= _FUSED_ROWS and (m if m < 3 else 4) * _row(k) <= _FUSED_CODES:
+        return t, xs.data_ptr(), stride, None, None, m, out, dtype, None
     # codes and, behind them, scales
     codes = torch.empty(m * (_row(k) + 4), dtype=torch.int8, device=device)
     at = codes.data_ptr()
@@ -214,10 +227,11 @@ def int8_linear_group(linears, xs: "torch.Tensor | Int8Tokens", dtype: torch.dty
             raise ValueError(f"grouped linears must share k and device: {lin._k} on {lin.device}, {k} on {dev}")
     t, x, stride, codes, scales, m, out, dtype, _held = _input(xs, k, dev, dtype)
     lead = xs.shape[:-1]
-    ys = [torch.empty(*lead, lin._n, dtype=dtype, device=dev) for lin in linears]
+    ys = [torch.empty((*lead, lin._n), dtype=dtype, device=dev) for lin in linears]
     if m:
-        _lib.check(_lib.lib().lbq_i8_linear(first._ctx, t, x, stride, codes, scales, m, k, (ctypes.c_void_p * count)(*[lin._at for lin in linears]),
-                                            count, out, (ctypes.c_void_p * count)(*[y.data_ptr() for y in ys]), _stream(dev)))
+        array = ctypes.c_void_p * count
+        _lib.check(_lib.lib().lbq_i8_linear(first._ctx, t, x, stride, codes, scales, m, k, array(*[lin._at for lin in linears]), count, out,
+                                            array(*[y.data_ptr() for y in ys]), _stream(dev)))
     return ys
 
 
@@ -228,10 +242,9 @@ def int8_gate_up_silu(gate: Int8Linear, up: Int8Linear, xs: "torch.Tensor | Int8
     if up._k != k or up._n != gate._n or up.device != dev:
         raise ValueError(f"gate {gate.weight.shape()} on {dev} and up {up.weight.shape()} on {up.device} must share shape and device")
     t, x, stride, codes, scales, m, out, dtype, _held = _input(xs, k, dev, dtype)
-    y = torch.empty(*xs.shape[:-1], gate._n, dtype=dtype, device=dev)
+    y = torch.empty((*xs.shape[:-1], gate._n), dtype=dtype, device=dev)
     if m:
-        _lib.check(_lib.lib().lbq_i8_gate_up_silu(gate._ctx, t, x, stride, codes, scales, m, k, gate._struct, up._struct, out, y.data_ptr(),
-                                                  _stream(dev)))
+        _lib.check(_lib.lib().lbq_i8_gate_up_silu(gate._ctx, t, x, stride, codes, scales, m, k, gate._at, up._at, out, y.data_ptr(), _stream(dev)))
     return y
 
 
@@ -253,8 +266,9 @@ class Norm(_Fixed):
             _vector("the norm's bias", bias, k, weight.device)
         if not eps >= 0:
             raise ValueError(f"eps = {eps}")
-        vars(self).update(weight=weight, eps=float(eps), bias=bias, kind=kind, offset=float(offset), device=weight.device, _k=k,
-                          _struct=_lib.NormStruct(_KINDS[kind], eps, offset, weight.data_ptr(), bias.data_ptr() if bias is not None else None))
+        struct = _lib.NormStruct(_KINDS[kind], eps, offset, weight.data_ptr(), bias.data_ptr() if bias is not None else None)
+        vars(self).update(weight=weight, eps=float(eps), bias=bias, kind=kind, offset=float(offset), device=weight.device, _k=k, _struct=struct,
+                          _at=ctypes.addressof(struct))
 
 
 def residual_norm(xs: torch.Tensor, residual: torch.Tensor | None = None, *, post: Norm | None = None, gate: torch.Tensor | None = None,
@@ -267,38 +281,42 @@ def residual_norm(xs: torch.Tensor, residual: torch.Tensor | None = None, *, pos
     ``Int8Tokens`` with ``quantize``, None without ``norm``.  Rows are worked out in 64 bits; y is the norm of r before r
     is rounded to its type."""
     t, m, stride = _values("xs", xs)
-    shape, dev, k = xs.shape, xs.device, xs.shape[-1]
+    shape, dev, dtype = xs.shape, xs.device, xs.dtype
+    k = shape[-1]
     for n in (post, norm):
         if n is not None and (n._k != k or n.device != dev):
             raise ValueError(f"a norm over {n._k} values on {n.device}, input {tuple(shape)} on {dev}")
     if quantize and norm is None:
         raise ValueError("codes are the norm's result: quantize needs a norm")
-    rt, rp, rs, gp, gs = t, None, 0, None, 0
+    r, rt, rp, rs, gp, gs = xs, t, None, 0, None, 0
+    changed = True
     if residual is not None:
         if residual.shape != shape or residual.device != dev:
             raise ValueError(f"residual {tuple(residual.shape)} on {residual.device}, input {tuple(shape)} on {dev}")
         rt, _, rs = _values("the residual", residual)
         rp = residual.data_ptr()
+    else:
+        changed = gate is not None or post is not None or scale != 1.0
     if gate is not None:
-        if gate.dtype != xs.dtype or gate.device != dev:
-            raise ValueError(f"gate of {gate.dtype} on {gate.device}, input {xs.dtype} on {dev}")
+        if gate.dtype != dtype or gate.device != dev:
+            raise ValueError(f"gate of {gate.dtype} on {gate.device}, input {dtype} on {dev}")
         if gate.shape == shape:
             _, _, gs = _values("the gate", gate)
         elif gate.shape != shape[-1:] or not gate.is_contiguous():
             raise ValueError(f"gate {tuple(gate.shape)} for input {tuple(shape)}: one contiguous row, or the input's shape")
         gp = gate.data_ptr()
-    changed = residual is not None or gate is not None or post is not None or scale != 1.0
-    r = torch.empty(shape, dtype=xs.dtype if residual is None else residual.dtype, device=dev) if changed else xs
-    y = rows = scales = None
+    if changed:
+        like = xs if residual is None else residual
+        r = torch.empty_like(like, memory_format=torch.contiguous_format)
+    y = yp = cp = sp = None
     if quantize:
         rows, scales = _empty_tokens(shape, m, dev)
-        y = Int8Tokens(rows, scales, shape, xs.dtype)
+        y, cp, sp = Int8Tokens(rows, scales, shape, dtype), rows.data_ptr(), scales.data_ptr()
     elif norm is not None:
-        y = torch.empty(shape, dtype=xs.dtype, device=dev)
+        y = torch.empty_like(xs, memory_format=torch.contiguous_format)
+        yp = y.data_ptr()
     if m and (changed or norm is not None):
         _lib.check(_lib.lib().lbq_residual_norm(
-            context(dev), t, xs.data_ptr(), stride, rt, rp, rs, post._struct if post is not None else None, gp, gs, scale,
-            norm._struct if norm is not None else None, m, k, r.data_ptr() if changed else None,
-            y.data_ptr() if y is not None and not quantize else None, rows.data_ptr() if quantize else None,
-            scales.data_ptr() if quantize else None, _stream(dev)))
+            _context(dev), t, xs.data_ptr(), stride, rt, rp, rs, None if post is None else post._at, gp, gs, scale,
+            None if norm is None else norm._at, m, k, r.data_ptr() if changed else None, yp, cp, sp, _stream(dev)))
     return r, y

@@ -13,6 +13,10 @@ FAR = 1 << 40
 INVALID, TYPE, SHAPE, LIMIT = -1, -2, -3, -6
 
 
+def at(struct):
+    return None if struct is None else ctypes.addressof(struct)
+
+
 def weight(**kw):
     f = dict(d_codes=D, d_scales=D, d_bias=None, n=64)
     f.update(kw)
@@ -23,15 +27,16 @@ def quantize(lbq, ctx=D, type=0, x=D, stride=100, m=3, k=100, codes=FAR, scales=
     return lbq.lbq_i8_quantize(ctx, type, x, stride, m, k, codes, scales, None)
 
 
-def linear(lbq, ws=None, ctx=D, type=0, x=D, stride=100, codes=FAR, scales=2 * FAR, m=3, k=100, count=None, out=0, ys=None):
+def linear(lbq, ws=None, ctx=D, type=0, x=D, stride=100, codes=FAR, scales=2 * FAR, m=5, k=100, count=None, out=0, ys=None):
     ws = [weight()] if ws is None else ws
-    at = (ctypes.c_void_p * 8)(*[w if w is None else ctypes.addressof(w) for w in ws])
+    array = (ctypes.c_void_p * 8)(*[at(w) for w in ws])
     ys = (ctypes.c_void_p * 8)(*(ys or [3 * FAR] * 8))
-    return lbq.lbq_i8_linear(ctx, type, x, stride, codes, scales, m, k, at, len(ws) if count is None else count, out, ys, None)
+    return lbq.lbq_i8_linear(ctx, type, x, stride, codes, scales, m, k, array, len(ws) if count is None else count, out, ys, None)
 
 
-def gate_up(lbq, gate=None, up=None, ctx=D, type=0, x=D, stride=100, codes=FAR, scales=2 * FAR, m=3, k=100, out=0, y=3 * FAR):
-    return lbq.lbq_i8_gate_up_silu(ctx, type, x, stride, codes, scales, m, k, gate or weight(), up or weight(), out, y, None)
+def gate_up(lbq, gate=None, up=None, ctx=D, type=0, x=D, stride=100, codes=FAR, scales=2 * FAR, m=5, k=100, out=0, y=3 * FAR):
+    gate, up = gate or weight(), up or weight()
+    return lbq.lbq_i8_gate_up_silu(ctx, type, x, stride, codes, scales, m, k, at(gate), at(up), out, y, None)
 
 
 def norm(**kw):
@@ -42,7 +47,8 @@ def norm(**kw):
 
 def residual_norm(lbq, ctx=D, type=0, x=D, stride=100, rt=0, res=FAR, res_stride=100, post=None, gate=None, gate_stride=0, pre=True, m=3, k=100,
                   r=2 * FAR, y=3 * FAR, codes=None, scales=None):
-    return lbq.lbq_residual_norm(ctx, type, x, stride, rt, res, res_stride, post, gate, gate_stride, 1.0, norm() if pre is True else pre, m, k, r, y,
+    pre = norm() if pre is True else pre
+    return lbq.lbq_residual_norm(ctx, type, x, stride, rt, res, res_stride, at(post), gate, gate_stride, 1.0, at(pre), m, k, r, y,
                                  codes, scales, None)
 
 
@@ -80,7 +86,7 @@ def test_outputs(lbq):
     assert linear(lbq, [weight(), None], ) == INVALID
     assert linear(lbq, ys=[None]) == INVALID and linear(lbq, ys=[3 * FAR + 2]) == INVALID
     assert linear(lbq, [weight(), weight()], ys=[3 * FAR, None]) == INVALID
-    assert linear(lbq, ys=[D + 1196]) == INVALID  # the last of x's rows
+    assert linear(lbq, ys=[D + 1996]) == INVALID  # the last of x's rows
     assert linear(lbq, x=None, ys=[FAR + 128]) == INVALID and linear(lbq, x=None, ys=[2 * FAR + 8]) == INVALID
     assert gate_up(lbq, y=None) == INVALID and gate_up(lbq, y=D) == INVALID
     assert gate_up(lbq, weight(n=32)) == SHAPE
