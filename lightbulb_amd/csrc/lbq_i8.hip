@@ -2,7 +2,7 @@
 // before and after a block.
 #include "lbq_i8.hpp"
 
-#include <algorithm>
+#include "lbq_device.hpp"
 
 namespace lbq {
 namespace {
@@ -11,13 +11,39 @@ namespace {
 // workgroup, or 256 / TPR of them.
 template <int TPR>
 struct RowShape {
-    static constexpr int THREADS = TPR < 256 ? 256 : TPR, ROWS = THREADS / TPR, WAVES = TPR / 64;
+    static constexpr int THREADS = TPR < 128 ? 256 : TPR, ROWS = THREADS / TPR, WAVES = TPR / 64;
 };
 
+// the same lanes of a value's words elsewhere in the wave
+template <int CTRL, typename V>
+__device__ __forceinline__ V dpp_words(V v) {
+    if constexpr (sizeof(V) == 4) {
+        return __builtin_bit_cast(V, dpp_u32<CTRL>(__builtin_bit_cast(uint32_t, v)));
+    } else {
+        const uint64_t w = __builtin_bit_cast(uint64_t, v);
+        return __builtin_bit_cast(V, (uint64_t)dpp_u32<CTRL>((uint32_t)w) | (uint64_t)dpp_u32<CTRL>((uint32_t)(w >> 32)) << 32);
+    }
+}
+// v of all lanes in every lane: within rows of 16 by DPP, between them by swaps of rows and halves
 template <typename V, typename F>
 __device__ __forceinline__ V wave_all(V v, F f) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v = f(v, __shfl_xor(v, d));
+    v = f(v, dpp_words<0xB1>(v));   // quad_perm [1,0,3,2]
+    v = f(v, dpp_words<0x4E>(v));   // quad_perm [2,3,0,1]
+    v = f(v, dpp_words<0x124>(v));  // row_ror:4
+    v = f(v, dpp_words<0x128>(v));  // row_ror:8
+    auto both = [&](auto swap) {
+        if constexpr (sizeof(V) == 4) {
+            const auto r = swap(__builtin_bit_cast(uint32_t, v));
+            v = f(__builtin_bit_cast(V, (uint32_t)r[0]), __builtin_bit_cast(V, (uint32_t)r[1]));
+        } else {
+            const uint64_t w = __builtin_bit_cast(uint64_t, v);
+            const auto lo = swap((uint32_t)w), hi = swap((uint32_t)(w >> 32));
+            v = f(__builtin_bit_cast(V, (uint64_t)(uint32_t)lo[0] | (uint64_t)(uint32_t)hi[0] << 32),
+                  __builtin_bit_cast(V, (uint64_t)(uint32_t)lo[1] | (uint64_t)(uint32_t)hi[1] << 32));
+        }
+    };
+    both([](uint32_t u) { return __builtin_amdgcn_permlane16_swap(u, u, false, false); });
+    both([](uint32_t u) { return __builtin_amdgcn_permlane32_swap(u, u, false, false); });
     return v;
 }
 // over the row's threads, in one order; `part` is this reduction's own
@@ -27,9 +53,9 @@ __device__ __forceinline__ V row_all(V v, V *part, F f) {
     if constexpr (WAVES > 1) {
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
         __syncthreads();
-        v = part[0];
+        v = part[threadIdx.x / 64 / WAVES * WAVES];
 #pragma unroll
-        for (int w = 1; w < WAVES; w++) v = f(v, part[w]);
+        for (int w = 1; w < WAVES; w++) v = f(v, part[threadIdx.x / 64 / WAVES * WAVES + w]);
     }
     return v;
 }
@@ -85,118 +111,171 @@ __global__ __launch_bounds__(RowShape<TPR>::THREADS) void k_i8_quantize(const vo
     }
 }
 
+// The sums that a norm needs of a row u, about a value c near it: sum of u - c and of its square.
+struct Moments {
+    double a, b;
+};
+template <int WAVES>
+__device__ __forceinline__ Moments row_all(Moments v, Moments *part) {
+    v.a = wave_all(v.a, Sum{}), v.b = wave_all(v.b, Sum{});
+    if constexpr (WAVES > 1) {
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = part[0];
+#pragma unroll
+        for (int w = 1; w < WAVES; w++) v = {v.a + part[w].a, v.b + part[w].b};
+    }
+    return v;
+}
+
+// a mean in F and what F leaves of it
+template <typename F>
+struct Mean {
+    F hi = 0, lo = 0;
+    __device__ __forceinline__ void set(double m) { hi = (F)m, lo = sizeof(F) == 4 ? (F)(m - (double)hi) : (F)0; }
+    __device__ __forceinline__ F off(F u) const { return sizeof(F) == 4 ? (u - hi) - lo : u - hi; }  // u - mean, off by two roundings of itself
+};
+
 // r = residual + scale gate post(x), y = pre(r), of a row: with u a row,
 //   root mean square   u / sqrt(mean(u^2) + eps) (w + offset) + b
 //   layer              (u - mean(u)) / sqrt(mean((u - mean(u))^2) + eps) (w + offset) + b
-// in 64 bits throughout, which this machine has at the rate of 32: a value is rounded once, where it is
-// stored, r as pre sees it not at all, and a code does not go by the order of a sum.  y as codes is
-// rounded to f32 first.  Every value of a row is read before one is written.
-template <int DX, int DR, int TPR, int NV>
+// Sums are in 64 bits.  Values are in F: 32 bits where y is a value, 64 where it becomes a code, which so does not go by the order
+// of a sum (f32's last bits would turn one code in 10^5), rounded to f32 before it does.  A variance is formed in one pass, about the
+// row's first value c: as the row holds c, (c - mean)^2 is at most k times the variance, and the difference of the sums loses no
+// more than k 2^-53.  The row stays in registers as it was read, and r is formed anew for each pass over it: held in 64 bits it
+// would take twice the registers, and with them go the rows that a CU has on the way.  Every value of a row is read before one
+// is written (r may lie where residual does).
+template <int DX, int DR, int TPR, int NV, typename F>
 __global__ __launch_bounds__(RowShape<TPR>::THREADS) void k_residual_norm(ResidualNorm a) {
     using S = RowShape<TPR>;
-    __shared__ double sums[4][S::THREADS / 64];
-    __shared__ uint32_t part[S::THREADS / 64];
+    static_assert(S::ROWS == 1 || S::WAVES == 1, "barriers of one row");
+    __shared__ Moments sums[2][S::WAVES];
+    __shared__ uint32_t part[S::WAVES];
     const int t = threadIdx.x % TPR, k = a.k;
     const int64_t row = (int64_t)blockIdx.x * S::ROWS + threadIdx.x / TPR;
     if (S::ROWS > 1 && row >= a.m) return;  // (a whole wave, and no barrier follows)
-    double v[NV][8];
-    auto each = [&](auto f) {
+    const char *xr = static_cast<const char *>(a.x.p) + row * a.x.stride * SIZE<DX>;
+    const char *gr = a.gate.p ? static_cast<const char *>(a.gate.p) + row * a.gate.stride * SIZE<DX> : nullptr;
+    const char *rr = a.residual.p ? static_cast<const char *>(a.residual.p) + row * a.residual.stride * SIZE<DR> : nullptr;
+    I8Piece<DX> x[NV];
+    I8Piece<DR> res[NV];
 #pragma unroll
-        for (int j = 0; j < NV; j++) f(8 * (t + j * TPR), v[j]);
-    };
-    auto normed = [&](const NormArgs &n, int at) {
-        if (!n.kind) return;
-        double mean = 0, ss = 0;
-        if (n.kind == 2) {
-            each([&](int, const double *u) {
-#pragma unroll
-                for (int e = 0; e < 8; e++) mean += u[e];  // (zero behind the row's end)
-            });
-            mean = row_all<S::WAVES>(mean, sums[at], Sum{}) / k;
+    for (int j = 0; j < NV; j++) {
+        const int i = 8 * (t + j * TPR);
+        if (i < k) {
+            x[j] = i8_piece<DX>(xr, i, k);
+            if (rr) res[j] = i8_piece<DR>(rr, i, k);
         }
-        each([&](int i, double *u) {
+    }
+    // (the row's first values, for c)
+    const bool layer = a.post.kind == 2 || a.pre.kind == 2;
+    const I8Piece<DX> x0 = layer ? i8_piece<DX>(xr, 0, 1) : I8Piece<DX>{};
+    const I8Piece<DR> r0 = layer && rr ? i8_piece<DR>(rr, 0, 1) : I8Piece<DR>{};
+
+    auto statistics = [&](const NormArgs &n, double c, Moments *at, Mean<F> &mean, F &inv, auto values) {
+        Moments s = {0, 0};
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            const int i = 8 * (t + j * TPR);
+            if (i >= k) continue;
+            F u[8];
+            values(j, i, u);
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                u[e] = i + e < k ? u[e] - mean : 0.0;
-                ss = fma(u[e], u[e], ss);
+                const double d = i + e < k ? (double)u[e] - c : 0.0;
+                s.a += d, s.b = fma(d, d, s.b);
             }
-        });
-        const double inv = 1.0 / sqrt(row_all<S::WAVES>(ss, sums[at + 1], Sum{}) / k + (double)n.eps);
-        each([&](int i, double *u) {
-            if (i >= k) return;
-            float w[8], b[8] = {};
-            i8_load8<I8_F32>(n.w, i, k, w);
-            if (n.b) i8_load8<I8_F32>(n.b, i, k, b);
-#pragma unroll
-            for (int e = 0; e < 8; e++) u[e] = fma(u[e] * inv, (double)w[e] + (double)n.offset, (double)b[e]);
-        });
+        }
+        s = row_all<S::WAVES>(s, at);
+        const double off = n.kind == 2 ? s.a / k : 0.0;
+        if (n.kind == 2) mean.set(c + off);
+        const double var = fma(-off, off, s.b / k);
+        inv = (F)(1.0 / sqrt((var < 0 ? 0.0 : var) + (double)n.eps));  // (a NaN stays one)
     };
-    const char *xr = static_cast<const char *>(a.x.p) + row * a.x.stride * SIZE<DX>;
-    float f[8];
-    each([&](int i, double *u) {
-        i8_load8<DX>(xr, i, k, f);
+    // u -> (u - mean) inv (w + offset) + b
+    auto scaled = [&](const NormArgs &n, const Mean<F> &mean, F inv, int i, F *u) {
+        const I8Piece<I8_F32> w = i8_piece<I8_F32>(n.w, i, k);
 #pragma unroll
-        for (int e = 0; e < 8; e++) u[e] = f[e];
-    });
-    normed(a.post, 0);
-    if (a.gate.p) {
-        const char *gr = static_cast<const char *>(a.gate.p) + row * a.gate.stride * SIZE<DX>;
-        each([&](int i, double *u) {
-            i8_load8<DX>(gr, i, k, f);
+        for (int e = 0; e < 8; e++) u[e] = mean.off(u[e]) * inv * ((F)w[e] + (F)n.offset);
+        if (n.b) {
+            const I8Piece<I8_F32> b = i8_piece<I8_F32>(n.b, i, k);
 #pragma unroll
-            for (int e = 0; e < 8; e++) u[e] *= f[e];
+            for (int e = 0; e < 8; e++) u[e] += (F)b[e];
+        }
+    };
+    Mean<F> post_mean, pre_mean;
+    F post_inv = 1, pre_inv = 1;
+    auto stream = [&](const I8Piece<DX> &xv, const I8Piece<DR> &rv, int i, F *u) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) u[e] = xv[e];
+        if (a.post.kind) scaled(a.post, post_mean, post_inv, i, u);
+        if (gr) {
+            const I8Piece<DX> g = i8_piece<DX>(gr, i, k);
+#pragma unroll
+            for (int e = 0; e < 8; e++) u[e] *= (F)g[e];
+        }
+        if (rr) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) u[e] = __builtin_elementwise_fma(u[e], (F)a.scale, (F)rv[e]);
+        } else if (a.scale != 1.f) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) u[e] *= (F)a.scale;
+        }
+    };
+    if (a.post.kind) {
+        statistics(a.post, a.post.kind == 2 ? (double)x0[0] : 0.0, sums[0], post_mean, post_inv, [&](int j, int, F *u) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) u[e] = x[j][e];
         });
     }
-    if (a.residual.p) {
-        const char *rr = static_cast<const char *>(a.residual.p) + row * a.residual.stride * SIZE<DR>;
-        each([&](int i, double *u) {
-            i8_load8<DR>(rr, i, k, f);
-#pragma unroll
-            for (int e = 0; e < 8; e++) u[e] = fma(u[e], (double)a.scale, (double)f[e]);
-        });
-    } else if (a.scale != 1.f) {
-        each([&](int, double *u) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) u[e] *= (double)a.scale;
-        });
+    if (a.pre.kind) {
+        double c = 0;
+        if (a.pre.kind == 2) {
+            F u[8];
+            stream(x0, r0, 0, u);
+            c = u[0];
+        }
+        statistics(a.pre, c, sums[1], pre_mean, pre_inv, [&](int j, int i, F *u) { stream(x[j], res[j], i, u); });
     }
-    if (a.r) {
-        char *out = static_cast<char *>(a.r) + row * k * SIZE<DR>;
-        each([&](int i, const double *u) {
-            if (i >= k) return;
+    const int kp = (k + 127) / 128 * 128;
+    uint32_t top = 0;
+    float y[NV][8];
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const int i = 8 * (t + j * TPR);
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[j][e] = 0.f;
+        if (i >= k) continue;
+        F u[8];
+        stream(x[j], res[j], i, u);
+        if (a.r) {
+            float f[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) f[e] = (float)u[e];
-            i8_store8<DR>(out, i, k, f);
-        });
+            i8_store8<DR>(static_cast<char *>(a.r) + row * k * SIZE<DR>, i, k, f);
+        }
+        if (!a.pre.kind) continue;
+        scaled(a.pre, pre_mean, pre_inv, i, u);
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[j][e] = i + e < k ? (float)u[e] : 0.f;
+        if constexpr (sizeof(F) == 4) {
+            i8_store8<DX>(static_cast<char *>(a.y) + row * k * SIZE<DX>, i, k, y[j]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) top = max(top, i8_magnitude(y[j][e]));
+        }
     }
-    if (!a.pre.kind) return;
-    normed(a.pre, 2);
-    if (a.y) {
-        char *out = static_cast<char *>(a.y) + row * k * SIZE<DX>;
-        each([&](int i, const double *u) {
-            if (i >= k) return;
-#pragma unroll
-            for (int e = 0; e < 8; e++) f[e] = (float)u[e];
-            i8_store8<DX>(out, i, k, f);
-        });
-    } else {
-        const int kp = (k + 127) / 128 * 128;
-        uint32_t top = 0;
-        each([&](int i, const double *u) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) top = max(top, i + e < k ? i8_magnitude((float)u[e]) : 0u);
-        });
-        const float s = i8_scale(__uint_as_float(row_all<S::WAVES>(top, part, Max{}))), inv = 1.f / s;
+    if constexpr (sizeof(F) == 8) {
+        const float s = i8_scale(__uint_as_float(row_all<S::WAVES>(top, part, Max{}))), is = 1.f / s;
         if (t == 0) a.codes.scales[row] = s;
         int8_t *cr = a.codes.codes + row * kp;
-        each([&](int i, const double *u) {
-            if (i >= kp) return;
-            uint32_t c[2];
 #pragma unroll
-            for (int e = 0; e < 8; e++) f[e] = i + e < k ? (float)u[e] : 0.f;
-            i8_codes8(f, s, inv, s > 0.f, c);
-            *reinterpret_cast<uint2 *>(cr + i) = make_uint2(c[0], c[1]);
-        });
+        for (int j = 0; j < NV; j++) {
+            const int i = 8 * (t + j * TPR);
+            uint32_t c[2];
+            i8_codes8(y[j], s, is, s > 0.f, c);
+            if (i < kp) *reinterpret_cast<uint2 *>(cr + i) = make_uint2(c[0], c[1]);
+        }
     }
 }
 
@@ -221,7 +300,9 @@ hipError_t quantize_rows(const I8Rows &x, int64_t m, int k, const I8Tokens &t, h
 template <int DX, int DR, int TPR, int NV>
 hipError_t norm(const ResidualNorm &a, hipStream_t st) {
     using S = RowShape<TPR>;
-    k_residual_norm<DX, DR, TPR, NV><<<(unsigned)((a.m + S::ROWS - 1) / S::ROWS), S::THREADS, 0, st>>>(a);
+    const unsigned blocks = (unsigned)((a.m + S::ROWS - 1) / S::ROWS);
+    if (a.codes.codes) k_residual_norm<DX, DR, TPR, NV, double><<<blocks, S::THREADS, 0, st>>>(a);
+    else k_residual_norm<DX, DR, TPR, NV, float><<<blocks, S::THREADS, 0, st>>>(a);
     return hipGetLastError();
 }
 template <int DX, int DR>
@@ -229,6 +310,8 @@ hipError_t norm_rows(const ResidualNorm &a, hipStream_t st) {
     const int kp = (int)i8_kp(a.k);
     if (kp <= 512) return norm<DX, DR, 64, 1>(a, st);
     if (kp <= 2048) return norm<DX, DR, 256, 1>(a, st);
+    if (kp <= 4096) return norm<DX, DR, 512, 1>(a, st);
+    if (kp <= 6144) return norm<DX, DR, 256, 3>(a, st);
     if (kp <= 8192) return norm<DX, DR, 512, 2>(a, st);
     if (kp <= 16384) return norm<DX, DR, 1024, 2>(a, st);
     return norm<DX, DR, 1024, 4>(a, st);

@@ -72,37 +72,48 @@ hipError_t launch_residual_norm(const ResidualNorm &a, hipStream_t st);
 // eight values from element i on of a row of k, zero behind its end; rows need no more than their
 // elements' alignment
 template <int DT>
-__device__ __forceinline__ void i8_load8(const void *row, int i, int k, float v[8]) {
+struct I8Piece {
+    uint32_t u[DT == I8_F32 ? 8 : 4];
+    __device__ __forceinline__ float operator[](int e) const {
+        if constexpr (DT == I8_F32) return __uint_as_float(u[e]);
+        const uint32_t b = e & 1 ? u[e >> 1] >> 16 : u[e >> 1] & 0xffffu;
+        return DT == I8_BF16 ? __uint_as_float(b << 16) : __half2float(__ushort_as_half((unsigned short)b));
+    }
+};
+template <int DT>
+__device__ __forceinline__ I8Piece<DT> i8_piece(const void *row, int i, int k) {
+    I8Piece<DT> v;
     if constexpr (DT == I8_F32) {
-        struct __attribute__((packed, aligned(4))) V { float f[8]; };
-        const float *p = static_cast<const float *>(row) + i;
+        struct __attribute__((packed, aligned(4))) V { uint32_t u[8]; };
+        const uint32_t *p = static_cast<const uint32_t *>(row) + i;
         if (i + 8 <= k) {
-            const V u = *reinterpret_cast<const V *>(p);
+            const V w = *reinterpret_cast<const V *>(p);
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = u.f[e];
+            for (int e = 0; e < 8; e++) v.u[e] = w.u[e];
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = i + e < k ? p[e] : 0.f;
+            for (int e = 0; e < 8; e++) v.u[e] = i + e < k ? p[e] : 0u;
         }
     } else {
         typedef uint32_t u32x4a2 __attribute__((ext_vector_type(4), aligned(2)));
         const uint16_t *p = static_cast<const uint16_t *>(row) + i;
-        uint32_t u[4];
         if (i + 8 <= k) {
             const u32x4a2 w = *reinterpret_cast<const u32x4a2 *>(p);
 #pragma unroll
-            for (int e = 0; e < 4; e++) u[e] = w[e];
+            for (int e = 0; e < 4; e++) v.u[e] = w[e];
         } else {
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                u[e] = (i + 2 * e < k ? p[2 * e] : 0u) | (i + 2 * e + 1 < k ? (uint32_t)p[2 * e + 1] << 16 : 0u);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const uint32_t b = e & 1 ? u[e >> 1] >> 16 : u[e >> 1] & 0xffffu;
-            v[e] = DT == I8_BF16 ? __uint_as_float(b << 16) : __half2float(__ushort_as_half((unsigned short)b));
+                v.u[e] = (i + 2 * e < k ? p[2 * e] : 0u) | (i + 2 * e + 1 < k ? (uint32_t)p[2 * e + 1] << 16 : 0u);
         }
     }
+    return v;
+}
+template <int DT>
+__device__ __forceinline__ void i8_load8(const void *row, int i, int k, float v[8]) {
+    const I8Piece<DT> p = i8_piece<DT>(row, i, k);
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = p[e];
 }
 
 // rounded once, to nearest even

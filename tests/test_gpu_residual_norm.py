@@ -25,17 +25,45 @@ def make_norm(gen, k, kind, dev, bias=None, offset=0.0, eps=1e-5):
             {"kind": kind, "weight": w, "bias": b, "eps": torch.tensor(eps, dtype=torch.float32).item(), "offset": torch.tensor(offset, dtype=torch.float32).item()})
 
 
+def spread_of(u, n):
+    """sqrt(mean + eps) of a norm's rows, and the values over it."""
+    d = u - u.mean(-1, keepdim=True) if n["kind"] == "layer" else u
+    s = ((d * d).mean(-1, keepdim=True) + n["eps"]).sqrt()
+    return s, d / s
+
+
+def norm_bound(u, du, n):
+    """How far a norm of rows within du of u may be in f32: 8 roundings of the scaled value (two of the distance from the mean,
+    of 1 / spread, of weight + offset, two products, and two more for the spread's own), the bias's, and what du does by itself, through the mean and
+    through the spread.  Subnormal: a half step of the first product, times the weight, and one of the second."""
+    w = (n["weight"].double() + n["offset"]).abs()
+    s, v = spread_of(u, n)
+    y = ref.normed(u, n)
+    most = du.amax(-1, keepdim=True) / s.clamp(min=1e-300)
+    return 8 * ref.U * (v * w).abs() + ref.U * y.abs() + most * w * (2 + v.abs()) + ref.least(torch.float32) * (1 + w)
+
+
 def check(x, residual, gate, scale, post, pre, quantize=False, **kw):
-    """One call against its definition: 64-bit arithmetic leaves about 1e-13 of the terms, then one rounding (f32), or two."""
+    """One call against its definition.  Codes: 64 bits, which leave about 1e-13 of the terms, then the roundings of what is stored.
+    Values: f32 with the bounds above."""
     r, y = int8.residual_norm(x, residual, post=post[0], gate=gate, scale=scale, norm=pre[0], quantize=quantize)
-    rw, yw = ref.residual_norm(x, residual, post[1], gate, torch.tensor(scale, dtype=torch.float32).double().item(), pre[1])
+    scale = torch.tensor(scale, dtype=torch.float32).double().item()
+    rw, yw = ref.residual_norm(x, residual, post[1], gate, scale, pre[1])
+    # f32: the first norm, the gate, the scale with the residual
+    u = x.cpu().double()
+    du = norm_bound(u, torch.zeros_like(u), post[1]) if post[1] else torch.zeros_like(u)
+    g = gate.cpu().double().abs() if gate is not None else 1.0
+    u = ref.normed(u, post[1]).abs() * g
+    dr = abs(scale) * (du * g + (ref.U * u if gate is not None else 0.0)) + ref.U * rw.abs() + ref.least(torch.float32)
+    if quantize:
+        dr = ref.U * rw.abs() + 1e-13 * (rw.abs() + (0 if residual is None else residual.cpu().double().abs())) + ref.least(torch.float32)
     if residual is None and gate is None and post[0] is None and scale == 1.0:
         assert r is x
+        dr = torch.zeros_like(dr)
     else:
         rt = x.dtype if residual is None else residual.dtype
         assert r.dtype == rt and r.shape == x.shape
-        size = rw.abs() + (0 if residual is None else residual.cpu().double().abs())
-        ref.close(r, rw, ref.stored(rw, ref.U * rw.abs() + 1e-13 * size + ref.least(torch.float32), rt))
+        ref.close(r, rw, ref.stored(rw, dr, rt))
     if pre[0] is None:
         assert y is None
         return
@@ -45,12 +73,7 @@ def check(x, residual, gate, scale, post, pre, quantize=False, **kw):
         assert not y._rows.cpu()[:, x.shape[-1]:].any()
     else:
         assert y.dtype == x.dtype and y.shape == x.shape
-        far = 1e-12 * (1 + yw.abs())
-        if pre[1]["kind"] == "layer":
-            # a mean of at most 32 additions in a row on either side, each off by 2^-53 of the largest value, over the spread
-            spread = (rw.var(-1, unbiased=False, keepdim=True) + pre[1]["eps"]).sqrt()
-            far = far + 64 * 2.0 ** -53 * rw.abs().amax(-1, keepdim=True) / spread * (pre[1]["weight"].double() + pre[1]["offset"]).abs()
-        ref.close(y, yw, ref.stored(yw, ref.U * yw.abs() + far, x.dtype))
+        ref.close(y, yw, ref.stored(yw, norm_bound(rw, dr, pre[1]), x.dtype))
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -85,7 +108,7 @@ def test_forms(dev, dtype, stream, post, pre):
 
 @pytest.mark.parametrize("quantize", [False, True])
 def test_layer_norm_of_shifted_rows(dev, quantize):
-    # a mean a million times the spread: the sums hold it
+    # a mean a million times the spread: the sums hold it, and what f32 rows lose is r's own rounding
     gen = torch.Generator().manual_seed(1)
     x = values(gen, 4, 1500, torch.float32, dev) + torch.tensor([1e6, -3e5, 0.0, 1e3], device=dev)[:, None]
     check(x, None, None, 1.0, (None, None), make_norm(gen, 1500, "layer", dev), quantize)
@@ -133,7 +156,7 @@ def test_strided_inputs(dev, dtype):
     r, y = int8.residual_norm(x3, x3, norm=rms[0])
     assert r.shape == y.shape == (4, 1, 301)
     rw, yw = ref.residual_norm(x3, x3, None, None, 1.0, rms[1])
-    ref.close(y, yw, ref.stored(yw, ref.U * yw.abs() + 1e-12, dtype))
+    ref.close(y, yw, ref.stored(yw, norm_bound(rw, ref.U * rw.abs(), rms[1]), dtype))
 
 
 def test_no_rows(dev):
