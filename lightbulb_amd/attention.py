@@ -20,7 +20,8 @@ import ctypes
 import torch
 
 from . import _lib
-from .quantized import GROUP_MAX, QuantizableLinear, _stream, context, qmatmul_group
+from .int8 import int8_linear_group
+from .quantized import GROUP_MAX, QuantizableLinear, _expect_values, _stream, context, qmatmul_group
 
 #: element types of queries, keys, values and outputs -> the library's type ids
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
@@ -360,21 +361,27 @@ class Attention:
         self.rotary, self.scale, self.window = rotary, scale, window
 
     def _project(self, xs: torch.Tensor) -> list[torch.Tensor]:
-        """q, k and v; quantized projections of one type in one call."""
+        """q, k and v; quantized projections of one type, or 8-bit integer ones, in one call."""
         projs = (self.q_proj, self.k_proj, self.v_proj)
         groups: dict = {}
         for i, p in enumerate(projs):
-            groups.setdefault(p.inner.qtensor().dtype() if p.is_quantized() else ("dense", i), []).append(i)
+            groups.setdefault(p.inner.qtensor().dtype() if p.is_quantized() else "int8" if p.is_int8() else ("dense", i), []).append(i)
         out: list = [None] * 3
-        for at in groups.values():
-            ys = qmatmul_group([projs[i].inner for i in at], xs) if 1 < len(at) <= GROUP_MAX else [projs[at[0]].forward(xs)]
+        for kind, at in groups.items():
+            if not 1 < len(at) <= GROUP_MAX:
+                ys = [projs[at[0]].forward(xs)]
+            elif kind == "int8":
+                ys = int8_linear_group([projs[i].inner for i in at], xs)
+            else:
+                _expect_values(xs)
+                ys = qmatmul_group([projs[i].inner for i in at], xs)
             for i, y in zip(at, ys):
                 out[i] = y
         return out
 
     def forward(self, xs: torch.Tensor, cache: KvCache, step: Step) -> torch.Tensor:
-        """``xs`` [.., hidden], ``step.num_tokens`` rows: the step's new tokens in order.  Rows behind the
-        last sequence's come out unset."""
+        """``xs`` [.., hidden], ``step.num_tokens`` rows: the step's new tokens in order, as values or, over 8-bit
+        integer projections, as ``int8.Int8Tokens``.  Rows behind the last sequence's come out unset."""
         n = step.num_tokens
         q, k, v = (y.view(n, h, self.head_dim) for y, h in zip(self._project(xs), (self.heads, self.kv_heads, self.kv_heads)))
         if self.rotary is None:

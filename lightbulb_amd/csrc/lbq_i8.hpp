@@ -14,7 +14,7 @@ namespace lbq {
 
 enum : int { I8_F32 = 0, I8_F16 = 1, I8_BF16 = 2 };
 constexpr int I8_GROUP = 4;
-constexpr int64_t I8_MAX_K = 131071, I8_MAX_N = (int64_t)1 << 24, I8_MAX_M = (int64_t)1 << 24;
+constexpr int64_t I8_MAX_K = 131071, I8_MAX_N = (int64_t)1 << 24, I8_MAX_M = ((int64_t)1 << 22) - 1;  // (workgroups of up to 1024 threads: below 2^32)
 constexpr int64_t NORM_MAX_K = 32768;
 constexpr int I8_FUSED_ROWS = 4, I8_FUSED_CODES = 16384;
 inline int64_t i8_kp(int64_t k) { return (k + 127) / 128 * 128; }
@@ -116,9 +116,16 @@ __device__ __forceinline__ void i8_load8(const void *row, int i, int k, float v[
     for (int e = 0; e < 8; e++) v[e] = p[e];
 }
 
-// rounded once, to nearest even
+// an f32 value as it is: without this the compiler forms some F16 results from the product itself, in one rounding for
+// two, and the same output would go by the kernel that it comes from
+__device__ __forceinline__ float i8_f32(float v) {
+    asm("" : "+v"(v));
+    return v;
+}
+// rounded to nearest even
 template <int DT>
 __device__ __forceinline__ uint32_t i8_bits16(float v) {
+    if constexpr (DT == I8_F16) v = i8_f32(v);
     if constexpr (DT == I8_F16) return __half_as_ushort(__float2half_rn(v));
     return __builtin_bit_cast(uint16_t, (__bf16)v);
 }

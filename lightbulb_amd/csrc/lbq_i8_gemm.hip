@@ -51,7 +51,7 @@ template <int OUT>
 __device__ __forceinline__ uint32_t i8_pack(float a, float b) {
     if constexpr (OUT == I8_F16) {
         typedef _Float16 half2 __attribute__((ext_vector_type(2)));
-        return __builtin_bit_cast(uint32_t, half2{(_Float16)a, (_Float16)b});
+        return __builtin_bit_cast(uint32_t, half2{(_Float16)i8_f32(a), (_Float16)i8_f32(b)});
     } else {
         typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
         return __builtin_bit_cast(uint32_t, bf2{(__bf16)a, (__bf16)b});

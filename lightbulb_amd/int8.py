@@ -11,7 +11,7 @@ exact:
                           the next block, as values or straight as the next products' codes
 
 They stand beside ``quantized.QMatMul``: ``QuantizableLinear.from_int8`` puts an ``Int8Linear`` into
-``quantized.Mlp`` and ``attention.Attention``, the projections of the reference's blocks
+``quantized.Mlp``, ``attention.Attention`` and ``block.Block``, the projections of the reference's blocks
 (src/model/custom_transformer_block.rs, mlp_wrapper.rs:190-195, custom_attention.rs:265-267, :671).
 The arithmetic runs in liblbq's HIP kernels; torch provides memory and the current stream.
 """

@@ -409,7 +409,8 @@ def rmsnorm_gate_up_silu(gate: "QMatMul", up: "QMatMul", xs: torch.Tensor, weigh
 class Mlp:
     """``Mlp`` (src/model/mlp_wrapper.rs): ``down_proj(silu(gate_proj(x)) * up_proj(x))``
     over ``QuantizableLinear`` projections; quantized gate/up pairs take the fused
-    ``gate_up_silu`` path."""
+    ``gate_up_silu`` path, 8-bit integer ones ``int8.int8_gate_up_silu`` (x as values or as
+    ``int8.Int8Tokens``)."""
 
     def __init__(self, gate_proj: "QuantizableLinear", up_proj: "QuantizableLinear", down_proj: "QuantizableLinear"):
         self.gate_proj, self.up_proj, self.down_proj = gate_proj, up_proj, down_proj
@@ -418,7 +419,11 @@ class Mlp:
         g, u = self.gate_proj, self.up_proj
         if (g.is_quantized() and u.is_quantized() and g.inner.qtensor().dtype() == u.inner.qtensor().dtype()
                 and g.inner.qtensor().shape() == u.inner.qtensor().shape()):
+            _expect_values(xs)
             h = gate_up_silu(g.inner, u.inner, xs)
+        elif g.is_int8() and u.is_int8() and g.inner.weight.shape() == u.inner.weight.shape():
+            from .int8 import int8_gate_up_silu
+            h = int8_gate_up_silu(g.inner, u.inner, xs)
         else:
             h = torch.nn.functional.silu(g.forward(xs)) * u.forward(xs)
         return self.down_proj.forward(h)
@@ -489,8 +494,13 @@ class QEmbedding:
 # ---------------------------------------------------------------------------
 # QuantizableLinear (src/model/quantizable_linear.rs)
 # ---------------------------------------------------------------------------
+def _expect_values(xs) -> None:
+    if not isinstance(xs, torch.Tensor):
+        raise ValueError(f"{type(xs).__name__} go to 8-bit integer linears only")
+
+
 class QuantizableLinear:
-    """Either ``Regular`` (dense f32 weight [n, k], optional bias) or ``Quantized(QMatMul)``."""
+    """``Regular`` (dense f32 weight [n, k], optional bias), ``Quantized(QMatMul)`` or ``Int8`` (``int8.Int8Linear``)."""
 
     def __init__(self, kind: str, inner):
         self.kind = kind
@@ -504,10 +514,21 @@ class QuantizableLinear:
     def from_qmatmul(cls, qmatmul: QMatMul) -> "QuantizableLinear":
         return cls("Quantized", qmatmul)
 
+    @classmethod
+    def from_int8(cls, linear) -> "QuantizableLinear":
+        """Over an ``int8.Int8Linear``: the output is of the input's type."""
+        return cls("Int8", linear)
+
     def is_quantized(self) -> bool:
         return self.kind == "Quantized"
 
+    def is_int8(self) -> bool:
+        return self.kind == "Int8"
+
     def forward(self, xs: torch.Tensor) -> torch.Tensor:
+        if self.kind == "Int8":
+            return self.inner.forward(xs)
+        _expect_values(xs)
         if self.kind == "Quantized":
             return self.inner.forward(xs)
         w, b = self.inner
