@@ -2,8 +2,6 @@
 // before and after a block.
 #include "lbq_i8.hpp"
 
-#include "lbq_device.hpp"
-
 namespace lbq {
 namespace {
 
@@ -14,42 +12,10 @@ struct RowShape {
     static constexpr int THREADS = TPR < 128 ? 256 : TPR, ROWS = THREADS / TPR, WAVES = TPR / 64;
 };
 
-// the same lanes of a value's words elsewhere in the wave
-template <int CTRL, typename V>
-__device__ __forceinline__ V dpp_words(V v) {
-    if constexpr (sizeof(V) == 4) {
-        return __builtin_bit_cast(V, dpp_u32<CTRL>(__builtin_bit_cast(uint32_t, v)));
-    } else {
-        const uint64_t w = __builtin_bit_cast(uint64_t, v);
-        return __builtin_bit_cast(V, (uint64_t)dpp_u32<CTRL>((uint32_t)w) | (uint64_t)dpp_u32<CTRL>((uint32_t)(w >> 32)) << 32);
-    }
-}
-// v of all lanes in every lane: within rows of 16 by DPP, between them by swaps of rows and halves
-template <typename V, typename F>
-__device__ __forceinline__ V wave_all(V v, F f) {
-    v = f(v, dpp_words<0xB1>(v));   // quad_perm [1,0,3,2]
-    v = f(v, dpp_words<0x4E>(v));   // quad_perm [2,3,0,1]
-    v = f(v, dpp_words<0x124>(v));  // row_ror:4
-    v = f(v, dpp_words<0x128>(v));  // row_ror:8
-    auto both = [&](auto swap) {
-        if constexpr (sizeof(V) == 4) {
-            const auto r = swap(__builtin_bit_cast(uint32_t, v));
-            v = f(__builtin_bit_cast(V, (uint32_t)r[0]), __builtin_bit_cast(V, (uint32_t)r[1]));
-        } else {
-            const uint64_t w = __builtin_bit_cast(uint64_t, v);
-            const auto lo = swap((uint32_t)w), hi = swap((uint32_t)(w >> 32));
-            v = f(__builtin_bit_cast(V, (uint64_t)(uint32_t)lo[0] | (uint64_t)(uint32_t)hi[0] << 32),
-                  __builtin_bit_cast(V, (uint64_t)(uint32_t)lo[1] | (uint64_t)(uint32_t)hi[1] << 32));
-        }
-    };
-    both([](uint32_t u) { return __builtin_amdgcn_permlane16_swap(u, u, false, false); });
-    both([](uint32_t u) { return __builtin_amdgcn_permlane32_swap(u, u, false, false); });
-    return v;
-}
 // over the row's threads, in one order; `part` is this reduction's own
 template <int WAVES, typename V, typename F>
 __device__ __forceinline__ V row_all(V v, V *part, F f) {
-    v = wave_all(v, f);
+    v = i8_wave_all(v, f);
     if constexpr (WAVES > 1) {
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
         __syncthreads();
@@ -59,13 +25,6 @@ __device__ __forceinline__ V row_all(V v, V *part, F f) {
     }
     return v;
 }
-struct Sum {
-    __device__ double operator()(double a, double b) const { return a + b; }
-};
-struct Max {
-    __device__ uint32_t operator()(uint32_t a, uint32_t b) const { return a > b ? a : b; }
-};
-
 template <int DT>
 constexpr int SIZE = DT == I8_F32 ? 4 : 2;
 
@@ -100,7 +59,7 @@ __global__ __launch_bounds__(RowShape<TPR>::THREADS) void k_i8_quantize(const vo
     } else {
         for (int i = 8 * t; i < k; i += 8 * TPR) i8_load8<DT>(xr, i, k, v[0]), look(v[0]);
     }
-    const float s = i8_scale(__uint_as_float(row_all<S::WAVES>(top, part, Max{}))), inv = 1.f / s;
+    const float s = i8_scale(__uint_as_float(row_all<S::WAVES>(top, part, I8Max{}))), inv = 1.f / s;
     if (t == 0) scales[row] = s;
     if constexpr (NV) {
 #pragma unroll
@@ -117,7 +76,7 @@ struct Moments {
 };
 template <int WAVES>
 __device__ __forceinline__ Moments row_all(Moments v, Moments *part) {
-    v.a = wave_all(v.a, Sum{}), v.b = wave_all(v.b, Sum{});
+    v.a = i8_wave_all(v.a, I8Sum{}), v.b = i8_wave_all(v.b, I8Sum{});
     if constexpr (WAVES > 1) {
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
         __syncthreads();
@@ -266,7 +225,7 @@ __global__ __launch_bounds__(RowShape<TPR>::THREADS) void k_residual_norm(Residu
         }
     }
     if constexpr (sizeof(F) == 8) {
-        const float s = i8_scale(__uint_as_float(row_all<S::WAVES>(top, part, Max{}))), is = 1.f / s;
+        const float s = i8_scale(__uint_as_float(row_all<S::WAVES>(top, part, I8Max{}))), is = 1.f / s;
         if (t == 0) a.codes.scales[row] = s;
         int8_t *cr = a.codes.codes + row * kp;
 #pragma unroll
@@ -290,9 +249,10 @@ hipError_t quantize_rows(const I8Rows &x, int64_t m, int k, const I8Tokens &t, h
     const int kp = (int)i8_kp(k);
     if (kp <= 512) return quantize<DT, 64, 1>(x, m, k, kp, t, st);
     if (kp <= 2048) return quantize<DT, 256, 1>(x, m, k, kp, t, st);
-    if (kp <= 4096) return quantize<DT, 256, 2>(x, m, k, kp, t, st);
-    if (kp <= 8192) return quantize<DT, 256, 4>(x, m, k, kp, t, st);
-    if (kp <= 16384) return quantize<DT, 1024, 2>(x, m, k, kp, t, st);
+    if (kp <= 4096) return quantize<DT, 512, 1>(x, m, k, kp, t, st);
+    if (kp <= 8192) return quantize<DT, 512, 2>(x, m, k, kp, t, st);
+    // (14336 bf16 values: 16 rows 3.8 us, with 512 threads 4.3; 4096 rows 35.4 and 32.9)
+    if (kp <= 16384) return m <= 512 ? quantize<DT, 1024, 2>(x, m, k, kp, t, st) : quantize<DT, 512, 4>(x, m, k, kp, t, st);
     if (kp <= 65536) return quantize<DT, 1024, 8>(x, m, k, kp, t, st);
     return quantize<DT, 1024, 0>(x, m, k, kp, t, st);
 }

@@ -170,6 +170,49 @@ __device__ __forceinline__ uint32_t i8_code(float x, float s, float inv) {
     const bool move = fabsf(left) > most || (fabsf(left) == most && (i & 1));
     return (uint32_t)(move ? left > 0.f ? i + 1 : i - 1 : i) & 0xffu;
 }
+template <int CTRL>
+__device__ __forceinline__ uint32_t i8_dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false);
+}
+// the same lanes of a value's words elsewhere in the wave
+template <int CTRL, typename V>
+__device__ __forceinline__ V i8_dpp_words(V v) {
+    if constexpr (sizeof(V) == 4) {
+        return __builtin_bit_cast(V, i8_dpp<CTRL>(__builtin_bit_cast(uint32_t, v)));
+    } else {
+        const uint64_t w = __builtin_bit_cast(uint64_t, v);
+        return __builtin_bit_cast(V, (uint64_t)i8_dpp<CTRL>((uint32_t)w) | (uint64_t)i8_dpp<CTRL>((uint32_t)(w >> 32)) << 32);
+    }
+}
+// v of all lanes in every lane: within rows of 16 by DPP, between them by swaps of rows and halves
+template <typename V, typename F>
+__device__ __forceinline__ V i8_wave_all(V v, F f) {
+    v = f(v, i8_dpp_words<0xB1>(v));   // quad_perm [1,0,3,2]
+    v = f(v, i8_dpp_words<0x4E>(v));   // quad_perm [2,3,0,1]
+    v = f(v, i8_dpp_words<0x124>(v));  // row_ror:4
+    v = f(v, i8_dpp_words<0x128>(v));  // row_ror:8
+    auto both = [&](auto swap) {
+        if constexpr (sizeof(V) == 4) {
+            const auto r = swap(__builtin_bit_cast(uint32_t, v));
+            v = f(__builtin_bit_cast(V, (uint32_t)r[0]), __builtin_bit_cast(V, (uint32_t)r[1]));
+        } else {
+            const uint64_t w = __builtin_bit_cast(uint64_t, v);
+            const auto lo = swap((uint32_t)w), hi = swap((uint32_t)(w >> 32));
+            v = f(__builtin_bit_cast(V, (uint64_t)(uint32_t)lo[0] | (uint64_t)(uint32_t)hi[0] << 32),
+                  __builtin_bit_cast(V, (uint64_t)(uint32_t)lo[1] | (uint64_t)(uint32_t)hi[1] << 32));
+        }
+    };
+    both([](uint32_t u) { return __builtin_amdgcn_permlane16_swap(u, u, false, false); });
+    both([](uint32_t u) { return __builtin_amdgcn_permlane32_swap(u, u, false, false); });
+    return v;
+}
+struct I8Sum {
+    __device__ double operator()(double a, double b) const { return a + b; }
+};
+struct I8Max {
+    __device__ uint32_t operator()(uint32_t a, uint32_t b) const { return a > b ? a : b; }
+};
+
 // magnitudes as the bits of their absolute values: their order is the magnitudes', infinity and NaN
 // above all of them
 __device__ __forceinline__ uint32_t i8_magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }

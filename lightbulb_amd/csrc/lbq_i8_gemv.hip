@@ -41,14 +41,17 @@ __global__ __launch_bounds__(64 * I8_WAVES) void k_i8_gemv(I8Linear a, I8Stream 
     const int N = a.n[wi], n0 = tile * 16 * R, m = (int)a.m;
     const int blocks = a.kp / 128, b0 = blocks * share / g.ks, b1 = blocks * (share + 1) / g.ks, last = max(b1 - 1, 0);
 
-    // (rows behind the last repeat it)
-    const int8_t *wp[NB], *xp[MT];
+    // the tile's first row, and a lane's offset from it (rows behind the last repeat it)
+    const int8_t *w0[NB];
+    uint32_t wo[NB], xo[MT];
 #pragma unroll
-    for (int i = 0; i < NB; i++) wp[i] = a.w[PAIR ? i & 1 : wi] + min(n0 + 16 * (PAIR ? i >> 1 : i) + lr, N - 1) * kp + 16 * lg;
-    const int xstep = (int)kp + 16;  // FUSED: rows of codes in LDS, on different banks
+    for (int i = 0; i < NB; i++) {
+        w0[i] = a.w[PAIR ? i & 1 : wi] + n0 * kp;
+        wo[i] = (uint32_t)(min(16 * (PAIR ? i >> 1 : i) + lr, N - 1 - n0) * a.kp + 16 * lg);
+    }
+    const int xstep = FUSED ? a.kp + 16 : a.kp;  // FUSED: rows of codes in LDS, on different banks
 #pragma unroll
-    for (int i = 0; i < MT; i++)
-        xp[i] = FUSED ? xs + min(lr, m - 1) * xstep + 16 * lg : a.codes + min(16 * i + lr, m - 1) * kp + 16 * lg;
+    for (int i = 0; i < MT; i++) xo[i] = (uint32_t)(min(16 * i + lr, m - 1) * xstep + 16 * lg);
 
     intx4 w[2][U][NB][2], x[2][U][MT][2];
     auto load_w = [&](int r, int b) __attribute__((always_inline)) {
@@ -57,7 +60,7 @@ __global__ __launch_bounds__(64 * I8_WAVES) void k_i8_gemv(I8Linear a, I8Stream 
 #pragma unroll
             for (int i = 0; i < NB; i++)
 #pragma unroll
-                for (int h = 0; h < 2; h++) w[r][u][i][h] = *reinterpret_cast<const intx4 *>(wp[i] + 128 * min(b + u, last) + 64 * h);
+                for (int h = 0; h < 2; h++) w[r][u][i][h] = *reinterpret_cast<const intx4 *>(w0[i] + 128 * min(b + u, last) + 64 * h + wo[i]);
     };
     auto load_x = [&](int r, int b) __attribute__((always_inline)) {
         if constexpr (!FUSED)
@@ -66,21 +69,25 @@ __global__ __launch_bounds__(64 * I8_WAVES) void k_i8_gemv(I8Linear a, I8Stream 
 #pragma unroll
                 for (int i = 0; i < MT; i++)
 #pragma unroll
-                    for (int h = 0; h < 2; h++) x[r][u][i][h] = *reinterpret_cast<const intx4 *>(xp[i] + 128 * min(b + u, last) + 64 * h);
+                    for (int h = 0; h < 2; h++) x[r][u][i][h] = *reinterpret_cast<const intx4 *>(a.codes + 128 * min(b + u, last) + 64 * h + xo[i]);
     };
-    // scales and biases of the outputs, asked for early
+    // scales and biases of the outputs, asked for early where that leaves registers for two workgroups a CU
+    constexpr bool EARLY = NV < 4;
     float tc[NB], bc[NB], sc[MT][4];
+    auto vectors = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < NB; j++) {
-        const int wj = PAIR ? j & 1 : wi, n = min(n0 + 16 * (PAIR ? j >> 1 : j) + lr, N - 1);
-        tc[j] = a.t[wj][n];
-        bc[j] = a.bias[wj] ? a.bias[wj][n] : 0.f;
-    }
-    if constexpr (!FUSED)
+        for (int j = 0; j < NB; j++) {
+            const int wj = PAIR ? j & 1 : wi, n = min(n0 + 16 * (PAIR ? j >> 1 : j) + lr, N - 1);
+            tc[j] = a.t[wj][n];
+            bc[j] = a.bias[wj] ? a.bias[wj][n] : 0.f;
+        }
 #pragma unroll
         for (int i = 0; i < MT; i++)
 #pragma unroll
-            for (int v = 0; v < 4; v++) sc[i][v] = a.scales[min(16 * i + 4 * lg + v, m - 1)];
+            for (int v = 0; v < 4; v++)
+                if constexpr (!FUSED) sc[i][v] = a.scales[min(16 * i + 4 * lg + v, m - 1)];
+    };
+    if constexpr (EARLY) vectors();
     intx4 acc[MT][NB] = {};
     auto multiply = [&](int r, int b) __attribute__((always_inline)) {
 #pragma unroll
@@ -90,9 +97,9 @@ __global__ __launch_bounds__(64 * I8_WAVES) void k_i8_gemv(I8Linear a, I8Stream 
             for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int i = 0; i < MT; i++) {
-                    const intx4 xo = FUSED ? *reinterpret_cast<const intx4 *>(xp[i] + 128 * (b + u) + 64 * h) : x[r][u][i][h];
+                    const intx4 xv = FUSED ? *reinterpret_cast<const intx4 *>(xs + 128 * (b + u) + 64 * h + xo[i]) : x[r][u][i][h];
 #pragma unroll
-                    for (int j = 0; j < NB; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xo, w[r][u][j][h], acc[i][j], 0, 0, 0);
+                    for (int j = 0; j < NB; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xv, w[r][u][j][h], acc[i][j], 0, 0, 0);
                 }
         }
     };
@@ -107,14 +114,13 @@ __global__ __launch_bounds__(64 * I8_WAVES) void k_i8_gemv(I8Linear a, I8Stream 
 #pragma unroll
         for (int j = 0; j < P; j++)
             if (j < np) i8_load8<DX>(xr, 8 * (tr + j * lanes), a.k, v[j]);
-        load_w(0, b0);
+        load_w(0, b0), load_w(1, b0 + U);
 #pragma unroll
         for (int j = 0; j < P; j++)
             if (j < np)
 #pragma unroll
                 for (int e = 0; e < 8; e++) top = max(top, i8_magnitude(v[j][e]));
-#pragma unroll
-        for (int d = 32; d; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+        top = i8_wave_all(top, I8Max{});
         if (lane == 0) part[wave] = top;
         __syncthreads();
         const int first = t / lanes * (lanes / 64);
@@ -137,21 +143,22 @@ __global__ __launch_bounds__(64 * I8_WAVES) void k_i8_gemv(I8Linear a, I8Stream 
 #pragma unroll
         for (int v = 0; v < 4; v++) sc[0][v] = sx[min(4 * lg + v, m - 1)];
     } else {
-        load_x(0, b0), load_w(0, b0);
+        load_x(0, b0), load_w(0, b0), load_x(1, b0 + U), load_w(1, b0 + U);
     }
     int b = b0;
-    for (; b + 2 * U < b1; b += 2 * U) {
-        load_x(1, b + U), load_w(1, b + U);
+    for (; b + 3 * U < b1; b += 2 * U) {
         multiply(0, b);
         load_x(0, b + 2 * U), load_w(0, b + 2 * U);
         multiply(1, b + U);
+        load_x(1, b + 3 * U), load_w(1, b + 3 * U);
     }
-    if (b + U < b1) {
-        load_x(1, b + U), load_w(1, b + U);
-        multiply(0, b);
+    multiply(0, b);
+    if (b + 2 * U < b1) {
+        load_x(0, b + 2 * U), load_w(0, b + 2 * U);
         multiply(1, b + U);
+        multiply(0, b + 2 * U);
     } else {
-        multiply(0, b);
+        multiply(1, b + U);
     }
 
     if (g.ks > 1) {
@@ -161,9 +168,10 @@ __global__ __launch_bounds__(64 * I8_WAVES) void k_i8_gemv(I8Linear a, I8Stream 
             for (int j = 0; j < NB; j++) *reinterpret_cast<intx4 *>(sums[wave][i * NB + j][lane]) = acc[i][j];
         __syncthreads();
     }
+    if constexpr (!EARLY) vectors();
     if (at >= all) return;
     // lane: channel lr of a 16 x 16 tile, its tokens 4 lg + v; value (i, j, v) goes to one of the tile's waves
-    const int w0 = wave - share;
+    const int lead = wave - share;
     void *y = a.y[PAIR ? 0 : wi];
 #pragma unroll
     for (int i = 0; i < MT; i++)
@@ -180,7 +188,7 @@ __global__ __launch_bounds__(64 * I8_WAVES) void k_i8_gemv(I8Linear a, I8Stream 
                     c[p] = acc[i][q][v];
                     if (g.ks > 1) {
                         c[p] = 0;
-                        for (int s = 0; s < g.ks; s++) c[p] += sums[w0 + s][i * NB + q][lane][v];
+                        for (int s = 0; s < g.ks; s++) c[p] += sums[lead + s][i * NB + q][lane][v];
                     }
                 }
                 if (n >= N || tok >= m) continue;
@@ -205,6 +213,9 @@ hipError_t run(const I8Linear &a, hipStream_t st) {
     I8Stream g = {};
     const int tiles = tiles16<R>(a, g.tile_end), blocks = a.kp / 128;
     g.ks = blocks >= 8 ? 8 : blocks >= 4 ? 4 : blocks >= 2 ? 2 : 1;
+    // longer shares where that still leaves the CUs a workgroup (a pair of 14336, 16 tokens: 29.7 us in eighths of k, 24.9 in
+    // quarters; single weights 16.0 and 15.5, 128256 channels 92.7 and 96.3)
+    if (PAIR && R == 2 && tiles / 2 >= num_cus() * 3 / 4) g.ks = std::min(g.ks, 4);
     const unsigned groups = (unsigned)((tiles + I8_WAVES / g.ks - 1) / (I8_WAVES / g.ks));
     if (a.out == I8_F32) k_i8_gemv<MT, R, U, PAIR, FUSED, DX, I8_F32><<<groups, 64 * I8_WAVES, 0, st>>>(a, g);
     else if (a.out == I8_F16) k_i8_gemv<MT, R, U, PAIR, FUSED, DX, I8_F16><<<groups, 64 * I8_WAVES, 0, st>>>(a, g);
@@ -221,12 +232,12 @@ template <bool PAIR>
 hipError_t stream(const I8Linear &a, hipStream_t st) {
     int end[I8_GROUP];
     // Two tiles of 16 channels a wave where there are more of them than CUs, so that each token operand is used twice.  us at
-    // k = 4096, one tile and two: 4096 channels 5.8 and 7.0, 6144 8.4 and 7.9, 128256 (8 tokens) 113 and 101, a pair of
-    // 14336 (16 tokens) 32.6 and 27.5.
+    // k = 4096, one tile and two: 4096 channels 6.2 and 7.0, 6144 8.6 and 7.9, 14336 (16 tokens) 18.9 and 16.0, 128256 (8 tokens)
+    // 102 and 93.  A fused kernel's registers take two blocks at once (6144: 8.9 us for 9.3), a pair's of two tiles do not.
     const bool two = tiles16<1>(a, end) > num_cus();
-    if (a.x.p) return two ? fused<2, 1, PAIR>(a, st) : fused<1, 2, PAIR>(a, st);
+    if (a.x.p) return two ? fused<2, PAIR ? 1 : 2, PAIR>(a, st) : fused<1, 2, PAIR>(a, st);
     if (a.m > 16) return run<2, 1, 1, PAIR, false, I8_F32>(a, st);
-    return two ? run<1, 2, 1, PAIR, false, I8_F32>(a, st) : run<1, 1, 2, PAIR, false, I8_F32>(a, st);
+    return two ? run<1, 2, 1, PAIR, false, I8_F32>(a, st) : run<1, 1, 1, PAIR, false, I8_F32>(a, st);
 }
 
 }  // namespace
