@@ -435,10 +435,11 @@ int lbq_i8_quantize(lbq_ctx *ctx, uint32_t type, const void *d_x, int64_t row_st
 /* d_ys[i][m][n_i] of `count` weights (up to LBQ_GROUP_MAX) on one set of tokens: q, k and v, say.  d_x NULL:
  * d_codes and d_scales hold the tokens.  Else x[m][k] of x_type is quantised first, into d_codes and
  * d_scales, whose contents then are not the caller's; up to LBQ_I8_FUSED_ROWS tokens of together at most
- * LBQ_I8_FUSED_CODES bytes of codes (m rounded up to a power of two) are quantised by the product's kernel, and
- * d_codes and d_scales may be NULL. */
+ * LBQ_I8_FUSED_CODES bytes of codes (m rounded up to a power of two) are quantised by the product's kernel where
+ * the weights have at most LBQ_I8_FUSED_CHANNELS channels in all, and d_codes and d_scales may be NULL. */
 #define LBQ_I8_FUSED_ROWS 4
 #define LBQ_I8_FUSED_CODES 16384
+#define LBQ_I8_FUSED_CHANNELS 16384
 int lbq_i8_linear(lbq_ctx *ctx, uint32_t x_type, const void *d_x, int64_t x_stride, int8_t *d_codes, float *d_scales,
                   int64_t m, int64_t k, const lbq_i8_weight *const *ws, int count, uint32_t out_type, void *const *d_ys,
                   void *stream);

@@ -93,7 +93,7 @@ SIGNATURES = {
     "lbq_kv_attention": (_c.c_int, [_VP, _CACHE, _STEP, _U32, _VP, _I64, _I64, _I32, _c.c_float, _I32, _I64, _VP, _VP, _SZ,
                                     _VP]),
     "lbq_i8_quantize": (_c.c_int, [_VP, _U32, _VP, _I64, _I64, _I64, _VP, _VP, _VP]),
-    "lbq_i8_linear": (_c.c_int, [_VP, _U32, _VP, _I64, _VP, _VP, _I64, _I64, _c.POINTER(_VP), _c.c_int, _U32, _c.POINTER(_VP), _VP]),
+    "lbq_i8_linear": (_c.c_int, [_VP, _U32, _VP, _I64, _VP, _VP, _I64, _I64, _VP, _c.c_int, _U32, _VP, _VP]),
     "lbq_i8_gate_up_silu": (_c.c_int, [_VP, _U32, _VP, _I64, _VP, _VP, _I64, _I64, _VP, _VP, _U32, _VP, _VP]),
     "lbq_residual_norm": (_c.c_int, [_VP, _U32, _VP, _I64, _U32, _VP, _I64, _VP, _VP, _I64, _c.c_float, _VP, _I64, _I64, _VP, _VP,
                                      _VP, _VP, _VP]),

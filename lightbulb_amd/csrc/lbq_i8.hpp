@@ -16,7 +16,7 @@ enum : int { I8_F32 = 0, I8_F16 = 1, I8_BF16 = 2 };
 constexpr int I8_GROUP = 4;
 constexpr int64_t I8_MAX_K = 131071, I8_MAX_N = (int64_t)1 << 24, I8_MAX_M = ((int64_t)1 << 22) - 1;  // (workgroups of up to 1024 threads: below 2^32)
 constexpr int64_t NORM_MAX_K = 32768;
-constexpr int I8_FUSED_ROWS = 4, I8_FUSED_CODES = 16384;
+constexpr int I8_FUSED_ROWS = 4, I8_FUSED_CODES = 16384, I8_FUSED_CHANNELS = 16384;
 inline int64_t i8_kp(int64_t k) { return (k + 127) / 128 * 128; }
 
 // rows of values [m][k], `stride` elements apart
@@ -46,8 +46,8 @@ struct I8Linear {
     int n[I8_GROUP];
     I8Rows x;  // values that the kernel quantises itself (x.p nullptr: codes and scales are there)
 };
-// whether the product's kernel quantises m rows of values itself
-bool i8_quantizes_in_kernel(int64_t m, int64_t k);
+// whether the product's kernel quantises m rows of values itself; channels: of all its weights
+bool i8_quantizes_in_kernel(int64_t m, int64_t k, int64_t channels);
 bool i8_streams(const I8Linear &a);  // the kernel for few tokens
 hipError_t launch_i8_stream(const I8Linear &a, hipStream_t st);
 hipError_t launch_i8_linear(const I8Linear &a, hipStream_t st);

@@ -113,7 +113,7 @@ int linear_args(uint32_t x_type, const void *d_x, int64_t x_stride, void *d_code
         int dt;
         if (int e = check_type("x", x_type, &dt)) return e;
         if (int e = check_rows("x", d_x, x_stride, k, dt, &a->x)) return e;
-        *quantize = !lbq::i8_quantizes_in_kernel(m, k);
+        *quantize = !lbq::i8_quantizes_in_kernel(m, k, rows);
     }
     if (!d_x || *quantize)
         if (int e = check_tokens(d_codes, d_scales, &t)) return e;

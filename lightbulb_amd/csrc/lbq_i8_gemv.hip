@@ -106,7 +106,8 @@ __global__ __launch_bounds__(64 * I8_WAVES) void k_i8_gemv(I8Linear a, I8Stream 
 
     if constexpr (FUSED) {
         // rows of 512, 256 or 128 threads; x is asked for before the weights, whose loads it would wait for
-        const int lanes = 64 * I8_WAVES >> (m > 2 ? 2 : m - 1), row = min(t / lanes, m - 1), tr = t % lanes, np = (a.kp / 8 + lanes - 1) / lanes;
+        const int lanes = 64 * I8_WAVES >> (m > 2 ? 2 : m - 1), row = min(t / lanes, m - 1), tr = t % lanes;
+        const int np = (a.kp / 8 + lanes - 1) / lanes;
         constexpr int P = I8_FUSED_CODES / 8 / (64 * I8_WAVES);
         const char *xr = static_cast<const char *>(a.x.p) + row * a.x.stride * (DX == I8_F32 ? 4 : 2);
         float v[P][8];
@@ -242,8 +243,11 @@ hipError_t stream(const I8Linear &a, hipStream_t st) {
 
 }  // namespace
 
-bool i8_quantizes_in_kernel(int64_t m, int64_t k) {
-    return m <= I8_FUSED_ROWS && (m > 2 ? 4 : m) * i8_kp(k) <= I8_FUSED_CODES;
+// Every workgroup quantises the tokens for itself, which saves a launch and its gap (1 token, 4096 channels of 4096: 6.6 us a call for
+// 10.1) while the CUs' workgroups are all at work at once; over more channels it costs more than it saves (4 tokens, pair
+// of 14336: 28.7 us for 27.1; 128256 channels 101 for 91), and so do more tokens (8: 13.6 for 10.1).
+bool i8_quantizes_in_kernel(int64_t m, int64_t k, int64_t channels) {
+    return m <= I8_FUSED_ROWS && (m > 2 ? 4 : m) * i8_kp(k) <= I8_FUSED_CODES && channels <= I8_FUSED_CHANNELS;
 }
 
 // Up to 16 tokens; up to 32 where a tile of 16 channels a CU is enough: us of this kernel and of the tiles' at k = 4096, 32 tokens,

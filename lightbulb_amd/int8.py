@@ -18,6 +18,7 @@ The arithmetic runs in liblbq's HIP kernels; torch provides memory and the curre
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -26,11 +27,12 @@ from .quantized import GROUP_MAX, _ctxs, _stream, context
 
 #: element types of values -> the library's type ids
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
-_VP1 = ctypes.c_void_p * 1
+#: addresses as the library takes a list of them
+_ADDRESSES = [struct.Struct(f"={n}Q").pack for n in range(GROUP_MAX + 1)]
 _KINDS = {"rms": 0, "layer": 1}
 MAX_K = 131071  # sums of 2^14 k stay below 2^31
 NORM_MAX_K = 32768
-_FUSED_ROWS, _FUSED_CODES = 4, 16384  # LBQ_I8_FUSED_ROWS, LBQ_I8_FUSED_CODES
+_FUSED_ROWS, _FUSED_CODES, _FUSED_CHANNELS = 4, 16384, 16384  # LBQ_I8_FUSED_ROWS, .._CODES, .._CHANNELS
 
 
 def _row(k: int) -> int:
@@ -85,16 +87,22 @@ class _Fixed:
 # ---------------------------------------------------------------------------
 # codes
 # ---------------------------------------------------------------------------
-class Int8Tokens(_Fixed):
+class Int8Tokens:
     """Tokens as ``codes`` int8 [.., k] and ``scales`` f32 [..]: a value is code * scale.  Made by
     ``quantize_tokens`` and ``residual_norm``; ``dtype`` is that of the values they stand for."""
 
-    def __init__(self, rows: torch.Tensor, scales: torch.Tensor, shape: torch.Size, dtype: torch.dtype):
-        vars(self).update(_rows=rows, scales=scales, shape=shape, dtype=dtype, device=rows.device)
+    __slots__ = ("_rows", "scales", "shape", "dtype", "device")
+
+    def __init__(self, rows: torch.Tensor, scales: torch.Tensor, shape: torch.Size, dtype: torch.dtype, device: torch.device):
+        self._rows, self.scales, self.shape, self.dtype, self.device = rows, scales, shape, dtype, device
 
     @property
     def codes(self) -> torch.Tensor:
-        return self._rows[:, :self.shape[-1]].unflatten(0, self.shape[:-1])
+        rows, shape = self._rows, self.shape
+        if rows.shape == shape:
+            return rows
+        rows = rows.narrow(1, 0, shape[-1])
+        return rows if len(shape) == 2 else rows.unflatten(0, shape[:-1])
 
     def dequantize(self) -> torch.Tensor:
         """The values that the codes stand for, f32."""
@@ -105,8 +113,9 @@ class Int8Tokens(_Fixed):
 
 
 def _empty_tokens(shape, m: int, device) -> tuple[torch.Tensor, torch.Tensor]:
-    return (torch.empty(m, _row(shape[-1]), dtype=torch.int8, device=device),
-            torch.empty(shape[:-1], dtype=torch.float32, device=device))
+    # (sizes one by one: 1.3 us each where a tuple of them takes 1.7)
+    return (torch.empty(m, (shape[-1] + 127) // 128 * 128, dtype=torch.int8, device=device),
+            torch.empty(*shape[:-1], dtype=torch.float32, device=device))
 
 
 def quantize_tokens(xs: torch.Tensor) -> Int8Tokens:
@@ -116,7 +125,7 @@ def quantize_tokens(xs: torch.Tensor) -> Int8Tokens:
     shape, dev = xs.shape, xs.device
     rows, scales = _empty_tokens(shape, m, dev)
     _lib.check(_lib.lib().lbq_i8_quantize(_context(dev), t, xs.data_ptr(), stride, m, shape[-1], rows.data_ptr(), scales.data_ptr(), _stream(dev)))
-    return Int8Tokens(rows, scales, shape, xs.dtype)
+    return Int8Tokens(rows, scales, shape, xs.dtype, dev)
 
 
 class Int8Weight(_Fixed):
@@ -170,17 +179,19 @@ class Int8Linear(_Fixed):
         n, k = weight.shape()
         if bias is not None:
             _vector("bias", bias, n, weight.device)
-        struct = _lib.I8WeightStruct(weight._rows.data_ptr(), weight.scales.data_ptr(), bias.data_ptr() if bias is not None else None, n)
-        vars(self).update(weight=weight, bias=bias, device=weight.device, _n=n, _k=k, _struct=struct, _at=ctypes.addressof(struct),
-                          _ptr=_VP1(ctypes.addressof(struct)), _ctx=context(weight.device))
+        arg = _lib.I8WeightStruct(weight._rows.data_ptr(), weight.scales.data_ptr(), bias.data_ptr() if bias is not None else None, n)
+        at = ctypes.addressof(arg)
+        vars(self).update(weight=weight, bias=bias, device=weight.device, _n=n, _k=k, _arg=arg, _at=at, _list=_ADDRESSES[1](at),
+                          _ctx=context(weight.device))
 
     def forward(self, xs: "torch.Tensor | Int8Tokens", dtype: torch.dtype | None = None) -> torch.Tensor:
         """``xs`` [.., k], values or tokens quantised before; the output is of ``dtype``, by default that of the values."""
         dev = self.device
-        t, x, stride, codes, scales, m, out, dtype, _held = _input(xs, self._k, dev, dtype)
-        y = torch.empty((*xs.shape[:-1], self._n), dtype=dtype, device=dev)
+        t, x, stride, codes, scales, m, out, dtype, _held = _input(xs, self._k, self._n, dev, dtype)
+        y = torch.empty(*xs.shape[:-1], self._n, dtype=dtype, device=dev)
         if m:
-            _lib.check(_lib.lib().lbq_i8_linear(self._ctx, t, x, stride, codes, scales, m, self._k, self._ptr, 1, out, _VP1(y.data_ptr()), _stream(dev)))
+            _lib.check(_lib.lib().lbq_i8_linear(self._ctx, t, x, stride, codes, scales, m, self._k, self._list, 1, out,
+                                                _ADDRESSES[1](y.data_ptr()), _stream(dev)))
         return y
 
     __call__ = forward
@@ -189,7 +200,7 @@ class Int8Linear(_Fixed):
         return f"Int8Linear({self.weight!r}, bias={self.bias is not None})"
 
 
-def _input(xs, k: int, device, dtype):
+def _input(xs, k: int, channels: int, device, dtype):
     """(type id, values, stride, codes, scales, rows, out type id, out dtype, what keeps the codes' memory) of a product's
     input."""
     shape, own = xs.shape, xs.dtype
@@ -205,7 +216,7 @@ def _input(xs, k: int, device, dtype):
     if isinstance(xs, Int8Tokens):
         return 0, None, 0, xs._rows.data_ptr(), xs.scales.data_ptr(), xs._rows.shape[0], out, dtype, xs
     t, m, stride = _values("the input", xs)
-    if m <= _FUSED_ROWS and (m if m < 3 else 4) * _row(k) <= _FUSED_CODES:
+    if m <= _FUSED_ROWS and (m if m < 3 else 4) * _row(k) <= _FUSED_CODES and channels <= _FUSED_CHANNELS:
         return t, xs.data_ptr(), stride, None, None, m, out, dtype, None
     # codes and, behind them, scales
     codes = torch.empty(m * (_row(k) + 4), dtype=torch.int8, device=device)
@@ -225,13 +236,13 @@ def int8_linear_group(linears, xs: "torch.Tensor | Int8Tokens", dtype: torch.dty
     for lin in linears:
         if lin._k != k or lin.device != dev:
             raise ValueError(f"grouped linears must share k and device: {lin._k} on {lin.device}, {k} on {dev}")
-    t, x, stride, codes, scales, m, out, dtype, _held = _input(xs, k, dev, dtype)
+    t, x, stride, codes, scales, m, out, dtype, _held = _input(xs, k, sum([lin._n for lin in linears]), dev, dtype)
     lead = xs.shape[:-1]
-    ys = [torch.empty((*lead, lin._n), dtype=dtype, device=dev) for lin in linears]
+    ys = [torch.empty(*lead, lin._n, dtype=dtype, device=dev) for lin in linears]
     if m:
-        array = ctypes.c_void_p * count
-        _lib.check(_lib.lib().lbq_i8_linear(first._ctx, t, x, stride, codes, scales, m, k, array(*[lin._at for lin in linears]), count, out,
-                                            array(*[y.data_ptr() for y in ys]), _stream(dev)))
+        pack = _ADDRESSES[count]
+        _lib.check(_lib.lib().lbq_i8_linear(first._ctx, t, x, stride, codes, scales, m, k, pack(*[lin._at for lin in linears]), count, out,
+                                            pack(*[y.data_ptr() for y in ys]), _stream(dev)))
     return ys
 
 
@@ -241,8 +252,8 @@ def int8_gate_up_silu(gate: Int8Linear, up: Int8Linear, xs: "torch.Tensor | Int8
     k, dev = gate._k, gate.device
     if up._k != k or up._n != gate._n or up.device != dev:
         raise ValueError(f"gate {gate.weight.shape()} on {dev} and up {up.weight.shape()} on {up.device} must share shape and device")
-    t, x, stride, codes, scales, m, out, dtype, _held = _input(xs, k, dev, dtype)
-    y = torch.empty((*xs.shape[:-1], gate._n), dtype=dtype, device=dev)
+    t, x, stride, codes, scales, m, out, dtype, _held = _input(xs, k, 2 * gate._n, dev, dtype)
+    y = torch.empty(*xs.shape[:-1], gate._n, dtype=dtype, device=dev)
     if m:
         _lib.check(_lib.lib().lbq_i8_gate_up_silu(gate._ctx, t, x, stride, codes, scales, m, k, gate._at, up._at, out, y.data_ptr(), _stream(dev)))
     return y
@@ -266,9 +277,9 @@ class Norm(_Fixed):
             _vector("the norm's bias", bias, k, weight.device)
         if not eps >= 0:
             raise ValueError(f"eps = {eps}")
-        struct = _lib.NormStruct(_KINDS[kind], eps, offset, weight.data_ptr(), bias.data_ptr() if bias is not None else None)
-        vars(self).update(weight=weight, eps=float(eps), bias=bias, kind=kind, offset=float(offset), device=weight.device, _k=k, _struct=struct,
-                          _at=ctypes.addressof(struct))
+        arg = _lib.NormStruct(_KINDS[kind], eps, offset, weight.data_ptr(), bias.data_ptr() if bias is not None else None)
+        vars(self).update(weight=weight, eps=float(eps), bias=bias, kind=kind, offset=float(offset), device=weight.device, _k=k, _arg=arg,
+                          _at=ctypes.addressof(arg))
 
 
 def residual_norm(xs: torch.Tensor, residual: torch.Tensor | None = None, *, post: Norm | None = None, gate: torch.Tensor | None = None,
@@ -306,14 +317,14 @@ def residual_norm(xs: torch.Tensor, residual: torch.Tensor | None = None, *, pos
             raise ValueError(f"gate {tuple(gate.shape)} for input {tuple(shape)}: one contiguous row, or the input's shape")
         gp = gate.data_ptr()
     if changed:
-        like = xs if residual is None else residual
-        r = torch.empty_like(like, memory_format=torch.contiguous_format)
+        like, apart = (xs, stride) if residual is None else (residual, rs)
+        r = torch.empty_like(like) if apart == k else torch.empty(*shape, dtype=like.dtype, device=dev)
     y = yp = cp = sp = None
     if quantize:
         rows, scales = _empty_tokens(shape, m, dev)
-        y, cp, sp = Int8Tokens(rows, scales, shape, dtype), rows.data_ptr(), scales.data_ptr()
+        y, cp, sp = Int8Tokens(rows, scales, shape, dtype, dev), rows.data_ptr(), scales.data_ptr()
     elif norm is not None:
-        y = torch.empty_like(xs, memory_format=torch.contiguous_format)
+        y = torch.empty_like(xs) if stride == k else torch.empty(*shape, dtype=dtype, device=dev)
         yp = y.data_ptr()
     if m and (changed or norm is not None):
         _lib.check(_lib.lib().lbq_residual_norm(

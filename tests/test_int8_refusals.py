@@ -129,7 +129,7 @@ def fake_linear(n, k, device="cpu"):
     """A linear without a device's context."""
     lin = int8.Int8Linear.__new__(int8.Int8Linear)
     w = int8.Int8Weight(torch.zeros(n, k, dtype=torch.int8), torch.ones(n))
-    vars(lin).update(weight=w, bias=None, device=torch.device(device), _n=n, _k=k, _struct=None, _at=D, _ctx=D)
+    vars(lin).update(weight=w, bias=None, device=torch.device(device), _n=n, _k=k, _at=D, _ctx=D)
     return lin
 
 
