@@ -87,12 +87,20 @@ __device__ __forceinline__ Moments row_all(Moments v, Moments *part) {
     return v;
 }
 
-// a mean in F and what F leaves of it
+// What a norm takes of a row: the mean in F and what F leaves of it, and 1 / sqrt(..).  In 32 bits a row of values whose
+// inverse is near the ends of the range is lifted by a power of two first, and mean and inverse are those of the lifted row.
 template <typename F>
-struct Mean {
-    F hi = 0, lo = 0;
-    __device__ __forceinline__ void set(double m) { hi = (F)m, lo = sizeof(F) == 4 ? (F)(m - (double)hi) : (F)0; }
-    __device__ __forceinline__ F off(F u) const { return sizeof(F) == 4 ? (u - hi) - lo : u - hi; }  // u - mean, off by two roundings of itself
+struct NormOf {
+    F mean = 0, left = 0, inv = 1, lift = 1;
+    __device__ __forceinline__ void set(double m, double i) {
+        if constexpr (sizeof(F) == 4) {
+            lift = i > 0x1p100 ? 0x1p60f : i < 0x1p-100 ? 0x1p-60f : 1.f;
+            lift = __uint_as_float((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(lift)));
+            m *= (double)lift, i /= (double)lift;
+        }
+        mean = (F)m, left = sizeof(F) == 4 ? (F)(m - (double)mean) : (F)0, inv = (F)i;
+    }
+    __device__ __forceinline__ F off(F u) const { return sizeof(F) == 4 ? (u - mean) - left : u - mean; }  // u - mean, off by two roundings of itself
 };
 
 // r = residual + scale gate post(x), y = pre(r), of a row: with u a row,
@@ -131,7 +139,7 @@ __global__ __launch_bounds__(RowShape<TPR>::THREADS) void k_residual_norm(Residu
     const I8Piece<DX> x0 = layer ? i8_piece<DX>(xr, 0, 1) : I8Piece<DX>{};
     const I8Piece<DR> r0 = layer && rr ? i8_piece<DR>(rr, 0, 1) : I8Piece<DR>{};
 
-    auto statistics = [&](const NormArgs &n, double c, Moments *at, Mean<F> &mean, F &inv, auto values) {
+    auto statistics = [&](const NormArgs &n, double c, Moments *at, NormOf<F> &of, auto values) {
         Moments s = {0, 0};
 #pragma unroll
         for (int j = 0; j < NV; j++) {
@@ -147,27 +155,29 @@ __global__ __launch_bounds__(RowShape<TPR>::THREADS) void k_residual_norm(Residu
         }
         s = row_all<S::WAVES>(s, at);
         const double off = n.kind == 2 ? s.a / k : 0.0;
-        if (n.kind == 2) mean.set(c + off);
         const double var = fma(-off, off, s.b / k);
-        inv = (F)(1.0 / sqrt((var < 0 ? 0.0 : var) + (double)n.eps));  // (a NaN stays one)
+        of.set(n.kind == 2 ? c + off : 0.0, 1.0 / sqrt((var < 0 ? 0.0 : var) + (double)n.eps));  // (a NaN stays one)
     };
     // u -> (u - mean) inv (w + offset) + b
-    auto scaled = [&](const NormArgs &n, const Mean<F> &mean, F inv, int i, F *u) {
+    auto scaled = [&](const NormArgs &n, const NormOf<F> &of, int i, F *u) {
         const I8Piece<I8_F32> w = i8_piece<I8_F32>(n.w, i, k);
+        if (sizeof(F) == 4 && of.lift != 1) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) u[e] = mean.off(u[e]) * inv * ((F)w[e] + (F)n.offset);
+            for (int e = 0; e < 8; e++) u[e] *= of.lift;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) u[e] = of.off(u[e]) * of.inv * ((F)w[e] + (F)n.offset);
         if (n.b) {
             const I8Piece<I8_F32> b = i8_piece<I8_F32>(n.b, i, k);
 #pragma unroll
             for (int e = 0; e < 8; e++) u[e] += (F)b[e];
         }
     };
-    Mean<F> post_mean, pre_mean;
-    F post_inv = 1, pre_inv = 1;
+    NormOf<F> post, pre;
     auto stream = [&](const I8Piece<DX> &xv, const I8Piece<DR> &rv, int i, F *u) {
 #pragma unroll
         for (int e = 0; e < 8; e++) u[e] = xv[e];
-        if (a.post.kind) scaled(a.post, post_mean, post_inv, i, u);
+        if (a.post.kind) scaled(a.post, post, i, u);
         if (gr) {
             const I8Piece<DX> g = i8_piece<DX>(gr, i, k);
 #pragma unroll
@@ -182,7 +192,7 @@ __global__ __launch_bounds__(RowShape<TPR>::THREADS) void k_residual_norm(Residu
         }
     };
     if (a.post.kind) {
-        statistics(a.post, a.post.kind == 2 ? (double)x0[0] : 0.0, sums[0], post_mean, post_inv, [&](int j, int, F *u) {
+        statistics(a.post, a.post.kind == 2 ? (double)x0[0] : 0.0, sums[0], post, [&](int j, int, F *u) {
 #pragma unroll
             for (int e = 0; e < 8; e++) u[e] = x[j][e];
         });
@@ -194,7 +204,7 @@ __global__ __launch_bounds__(RowShape<TPR>::THREADS) void k_residual_norm(Residu
             stream(x0, r0, 0, u);
             c = u[0];
         }
-        statistics(a.pre, c, sums[1], pre_mean, pre_inv, [&](int j, int i, F *u) { stream(x[j], res[j], i, u); });
+        statistics(a.pre, c, sums[1], pre, [&](int j, int i, F *u) { stream(x[j], res[j], i, u); });
     }
     const int kp = (k + 127) / 128 * 128;
     uint32_t top = 0;
@@ -214,7 +224,7 @@ __global__ __launch_bounds__(RowShape<TPR>::THREADS) void k_residual_norm(Residu
             i8_store8<DR>(static_cast<char *>(a.r) + row * k * SIZE<DR>, i, k, f);
         }
         if (!a.pre.kind) continue;
-        scaled(a.pre, pre_mean, pre_inv, i, u);
+        scaled(a.pre, pre, i, u);
 #pragma unroll
         for (int e = 0; e < 8; e++) y[j][e] = i + e < k ? (float)u[e] : 0.f;
         if constexpr (sizeof(F) == 4) {

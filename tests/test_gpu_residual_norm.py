@@ -144,6 +144,20 @@ def test_no_eps(dev):
         check(x, None, None, 1.0, (None, None), make_norm(gen, 130, "rms", dev, eps=0.0), quantize)
 
 
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+def test_rows_at_the_ends_of_the_range(dev, kind):
+    # no eps: 1 / spread of these is itself beyond f32 or subnormal; the norms' values are ordinary
+    gen = torch.Generator().manual_seed(7)
+    x = torch.randn(8, 700, generator=gen).clamp(-3, 3) * torch.tensor([1e-44, 1e-40, 1e-37, 1e-31, 1e29, 1e32, 1e36, 1e38])[:, None]
+    x[7] = torch.where(x[7] < 0, -3.4e38, 3.4e38)
+    x = x.to(dev)
+    for eps in (0.0, 1e-30):
+        n = make_norm(gen, 700, kind, dev, eps=eps)
+        for quantize in (False, True):
+            check(x, None, None, 1.0, (None, None), n, quantize)
+        check(x, None, None, 1.0, n, make_norm(gen, 700, kind, dev))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_strided_inputs(dev, dtype):
     gen = torch.Generator().manual_seed(4)
