@@ -67,16 +67,17 @@ int check_sizes(int64_t m, int64_t k, int64_t most_k) {
 int check_rows(const char *what, const void *p, int64_t stride, int64_t k, int dt, lbq::I8Rows *rows) {
     if (!p) return fail(LBQ_ERR_INVALID_ARG, "null %s", what);
     if (!aligned(p, size_of(dt))) return fail(LBQ_ERR_INVALID_ARG, "%s must be aligned to its elements", what);
-    if (stride < 0 || stride > (int64_t)1 << 40) return fail(LBQ_ERR_SHAPE, "rows of %s %lld values apart", what, (long long)stride);
+    if (stride < 0 || stride > (int64_t)1 << 38) return fail(LBQ_ERR_SHAPE, "rows of %s %lld values apart", what, (long long)stride);
     *rows = {p, stride, dt};
     return LBQ_OK;
 }
 int64_t bytes_of(const lbq::I8Rows &r, int64_t m, int64_t k) { return r.p ? ((m - 1) * r.stride + k) * size_of(r.dtype) : 0; }
 
-int check_tokens(const void *codes, const void *scales, lbq::I8Tokens *t) {
+int check_tokens(const void *codes, const void *scales, int64_t m, int64_t k, lbq::I8Tokens *t) {
     if (!codes || !scales) return fail(LBQ_ERR_INVALID_ARG, "null codes or scales of the tokens");
     if (!aligned(codes, 16)) return fail(LBQ_ERR_INVALID_ARG, "the tokens' codes must be 16-byte aligned");
     if (!aligned(scales, 4)) return fail(LBQ_ERR_INVALID_ARG, "the tokens' scales must be 4-byte aligned");
+    if (overlap(codes, m * lbq::i8_kp(k), scales, m * 4)) return fail(LBQ_ERR_INVALID_ARG, "the tokens' codes and scales must not overlap");
     *t = {static_cast<int8_t *>(const_cast<void *>(codes)), static_cast<float *>(const_cast<void *>(scales))};
     return LBQ_OK;
 }
@@ -116,7 +117,7 @@ int linear_args(uint32_t x_type, const void *d_x, int64_t x_stride, void *d_code
         *quantize = !lbq::i8_quantizes_in_kernel(m, k, rows);
     }
     if (!d_x || *quantize)
-        if (int e = check_tokens(d_codes, d_scales, &t)) return e;
+        if (int e = check_tokens(d_codes, d_scales, m, k, &t)) return e;
     if (*quantize && (overlap(d_x, bytes_of(a->x, m, k), t.codes, m * a->kp) || overlap(d_x, bytes_of(a->x, m, k), t.scales, m * 4)))
         return fail(LBQ_ERR_INVALID_ARG, "the codes' memory must not overlap x");
     a->codes = t.codes, a->scales = t.scales;
@@ -130,6 +131,8 @@ int check_output(void *y, int i, int64_t n, lbq::I8Linear *a) {
     const int64_t bytes = a->m * n * size;
     if (overlap(y, bytes, a->codes, a->m * a->kp) || overlap(y, bytes, a->scales, a->m * 4) || overlap(y, bytes, a->x.p, bytes_of(a->x, a->m, a->k)))
         return fail(LBQ_ERR_INVALID_ARG, "an output must not overlap the input");
+    for (int j = 0; j < i; j++)
+        if (overlap(y, bytes, a->y[j], a->m * a->n[j] * size)) return fail(LBQ_ERR_INVALID_ARG, "the outputs must not overlap");
     a->y[i] = y;
     return LBQ_OK;
 }
@@ -172,7 +175,7 @@ int lbq_i8_quantize(lbq_ctx *ctx, uint32_t type, const void *d_x, int64_t row_st
     if (int e = check_sizes(m, k, lbq::I8_MAX_K)) return e;
     if (m == 0) return LBQ_OK;
     if (int e = check_rows("x", d_x, row_stride, k, dt, &x)) return e;
-    if (int e = check_tokens(d_codes, d_scales, &t)) return e;
+    if (int e = check_tokens(d_codes, d_scales, m, k, &t)) return e;
     if (overlap(d_x, bytes_of(x, m, k), d_codes, m * lbq::i8_kp(k)) || overlap(d_x, bytes_of(x, m, k), d_scales, m * 4))
         return fail(LBQ_ERR_INVALID_ARG, "the codes' memory must not overlap x");
     return launched(ctx, "quantise launch", [&] { return lbq::launch_i8_quantize(x, m, k, t, static_cast<hipStream_t>(stream)); });
@@ -225,7 +228,7 @@ int lbq_residual_norm(lbq_ctx *ctx, uint32_t type, const void *d_x, int64_t x_st
         if (int e = check_rows("the gate", d_gate, gate_stride, k, dt, &a.gate)) return e;
     if (d_codes || d_scales) {
         if (d_y || !norm) return fail(LBQ_ERR_INVALID_ARG, "codes are the second norm's result in the place of y");
-        if (int e = check_tokens(d_codes, d_scales, &a.codes)) return e;
+        if (int e = check_tokens(d_codes, d_scales, m, k, &a.codes)) return e;
     } else if (!!norm != !!d_y) {
         return fail(LBQ_ERR_INVALID_ARG, "a second norm and its result go together");
     }

@@ -117,6 +117,18 @@ def test_norms(lbq, kw, status):
     assert residual_norm(lbq, pre=norm(**kw)) == status and residual_norm(lbq, post=norm(**kw)) == status
 
 
+def test_results_in_one_place(lbq):
+    # outputs of one call, and tokens' codes and scales, must lie apart
+    ws = [weight(n=40), weight(n=40)]
+    assert linear(lbq, ws, ys=[3 * FAR, 3 * FAR]) == INVALID
+    assert linear(lbq, ws, ys=[3 * FAR, 3 * FAR + 5 * 40 * 4 - 4]) == INVALID
+    assert linear(lbq, ws, ys=[3 * FAR + 5 * 40 * 4 - 4, 3 * FAR]) == INVALID
+    assert linear(lbq, [weight()], scales=FAR + 4 * 128) == INVALID and linear(lbq, [weight()], x=None, scales=FAR) == INVALID
+    assert quantize(lbq, scales=FAR + 2 * 128) == INVALID and gate_up(lbq, scales=FAR + 4 * 128) == INVALID
+    assert residual_norm(lbq, y=None, codes=4 * FAR, scales=4 * FAR + 128) == INVALID
+    assert quantize(lbq, stride=(1 << 38) + 1) == SHAPE
+
+
 # ---------------------------------------------------------------------------
 # Python
 # ---------------------------------------------------------------------------
