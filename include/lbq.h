@@ -411,11 +411,13 @@ int lbq_kv_attention(lbq_ctx *ctx, const lbq_kv_cache *cache, const lbq_kv_step 
  * A token with a value that is not finite has the scale NaN and codes 0: its products are NaN.
  * A weight has int8 codes [n][k] and one f32 scale for each of its n channels.  An output is
  *   y[i][j] = scale[i] * channel_scale[j] * sum_k code[i][k] weight_code[j][k] + bias[j]
- * with the sum exact (k is at most 131071, codes may be -128) and two roundings to f32 after it, in the
- * last of which the bias goes in; where a scale is outside 2^-60 to 2^44, 0 too, it is formed in 64
- * bits.  The same bits come out whatever m is and wherever the row stands.
+ * with the sum exact (k is at most 131071, codes may be -128); the sum and the scales' product are rounded to
+ * f32, and their product with the bias added is rounded once.  Where a scale is outside 2^-60 to 2^44, 0 too,
+ * all is formed in 64 bits.  The same bits come out whatever m is and wherever the row stands.
  * Rows of codes, of tokens and weights alike, are LBQ_I8_ROW(k) bytes apart and zero from k on, 16-byte
- * aligned.  Types are LBQ_TYPE_F32, _F16 or _BF16; rows of values may have any stride (in elements).
+ * aligned.  Types are LBQ_TYPE_F32, _F16 or _BF16; rows of values may have any stride (in elements).  Up to
+ * 2^22 - 1 tokens and 2^24 channels a weight, tokens times channels of a call below 2^35.  Results lie apart from
+ * the inputs and from each other.
  * All calls run on the context's device and use none of its memory: calls on different streams need
  * no order among themselves but that of their own buffers.
  * ------------------------------------------------------------------------- */
@@ -458,8 +460,8 @@ int lbq_i8_gate_up_silu(lbq_ctx *ctx, uint32_t x_type, const void *d_x, int64_t 
  * with f32 weight and bias (may be NULL) of k values.  The gate is of x's type, gate_stride elements from row to
  * row, 0: one for all.  r [m][k] is of residual_type and y [m][k] of x's, both contiguous; with d_codes and
  * d_scales y becomes codes, of its values rounded to f32, and d_y is NULL.  d_r may be NULL, or d_residual
- * itself where its rows are contiguous.  A row is worked out in 64 bits and rounded where it is stored; y is
- * the norm of r before its rounding.  k is at most 32768. */
+ * itself where its rows are contiguous.  Sums over a row are in 64 bits, values in 32, or 64 where y becomes
+ * codes; y is the norm of r before r is rounded to its type.  k is at most 32768. */
 enum lbq_norm_kind { LBQ_NORM_RMS = 0, LBQ_NORM_LAYER = 1 };
 typedef struct lbq_norm {
     int32_t kind; /* lbq_norm_kind */

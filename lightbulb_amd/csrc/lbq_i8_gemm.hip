@@ -79,6 +79,10 @@ struct Tile {
 // the 16 lanes that read at once fall on different banks.  Where a k-step of 32 has more than two products a
 // wave, the next one's operands are read under them, and the loads go out one behind each; where it has fewer, a
 // whole stage's operands are read ahead.
+// 4096 x 14336 -> 4096 188 us, 2.55 POP/s; 2048 tokens, gate and up of 14336 x 4096 216 us, 2.23.  Bound by the card's power: the
+// matrix pipes are busy 60 to 70 % of cycles at 1.8 GHz, and on codes of zeros, which take less of it, the rate is 3.0.  512 tokens over
+// 6144 channels of 4096 20.6 us, by the lines that a CU takes in (below).  Stages of 64 bytes in 3 to 5 slots took 214 to 228 us
+// for 190 to 199, four waves of 128 x 128 each 307 (registers spill).
 template <class T, int OUT>
 __device__ __forceinline__ void i8_tile(const I8Linear &a, int64_t m0, int n0, int wi, uint8_t *lds_base) {
     constexpr int TM = T::TM, TN = T::TN, D = T::D, NW = T::NW, RA = T::RA, RL = T::RL, BM = T::BM, BO = T::BO;

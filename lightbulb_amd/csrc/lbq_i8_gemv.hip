@@ -22,6 +22,8 @@ constexpr int I8_WAVES = 8, I8_LDS = I8_FUSED_CODES + 16 * I8_FUSED_ROWS;
 // other's are multiplied.  Bound by memory: each weight is read once by one wave; the tokens come out of the
 // L2, or (FUSED: values quantised by the workgroup, codes and scales as the other kernel's) out of LDS.  Shares
 // of k meet in LDS; whole numbers, so that their order does not matter.
+// 8 tokens over 128256 channels of 4096 93 us, 5.7 TB/s; 16 tokens, gate and up of 14336 25 us, 4.7 TB/s; one token over 6144 8.5 us,
+// of which about 3 are the launch, its values' quantisation and the join.
 template <int MT, int R, int U, bool PAIR, bool FUSED, int DX, int OUT>
 __global__ __launch_bounds__(64 * I8_WAVES) void k_i8_gemv(I8Linear a, I8Stream g) {
     constexpr int NB = R * (PAIR ? 2 : 1), NV = MT * NB;

@@ -289,8 +289,8 @@ def residual_norm(xs: torch.Tensor, residual: torch.Tensor | None = None, *, pos
 
     ``residual`` has the shape of ``xs`` [.., k] and any of the types (its own is r's); ``gate`` is [k] or of the shape of
     ``xs``, and of its type.  What is None is left out; r is ``xs`` itself where nothing is done to it.  y is of ``xs``'s type,
-    ``Int8Tokens`` with ``quantize``, None without ``norm``.  Rows are worked out in 64 bits; y is the norm of r before r
-    is rounded to its type."""
+    ``Int8Tokens`` with ``quantize``, None without ``norm``.  Sums over a row are in 64 bits, values in 32, or 64 with
+    ``quantize``; y is the norm of r before r is rounded to its type."""
     t, m, stride = _values("xs", xs)
     shape, dev, dtype = xs.shape, xs.device, xs.dtype
     k = shape[-1]
