@@ -88,6 +88,15 @@ def test_widths(dev, dtype, quantize, m, k):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("quantize", [False, True])
+@pytest.mark.parametrize("k", [8200, 10001, 12289, 14336])
+def test_many_wide_rows(dev, dtype, quantize, k):
+    gen = torch.Generator().manual_seed(k)
+    x, res = values(gen, 258, k, dtype, dev, 2.0), values(gen, 258, k, torch.float32, dev)
+    check(x, res, None, 1.0, make_norm(gen, k, "rms", dev), make_norm(gen, k, "layer", dev), quantize)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("stream", DTYPES)
 @pytest.mark.parametrize("post", ["", "rms", "layer"])
 @pytest.mark.parametrize("pre", ["", "rms", "layer"])
