@@ -81,7 +81,7 @@ struct Tile {
 // whole stage's operands are read ahead.
 // 4096 x 14336 -> 4096 188 us, 2.55 POP/s; 2048 tokens, gate and up of 14336 x 4096 216 us, 2.23.  Bound by the card's power: the
 // matrix pipes are busy 60 to 70 % of cycles at 1.8 GHz, and on codes of zeros, which take less of it, the rate is 3.0.  512 tokens over
-// 6144 channels of 4096 20.6 us, by the lines that a CU takes in (below).  Stages of 64 bytes in 3 to 5 slots took 214 to 228 us
+// 6144 channels of 4096 20 us, by the lines that a CU takes in (below).  Stages of 64 bytes in 3 to 5 slots took 214 to 228 us
 // for 190 to 199, four waves of 128 x 128 each 307 (registers spill).
 template <class T, int OUT>
 __device__ __forceinline__ void i8_tile(const I8Linear &a, int64_t m0, int n0, int wi, uint8_t *lds_base) {
@@ -360,7 +360,8 @@ template <bool PAIR>
 hipError_t tiles(const I8Linear &a, hipStream_t st) {
     using Big = Tile<2, 4, 4, 2, 2, PAIR>;     // 256 x 256
     using Half = Tile<2, 4, 2, 2, 3, PAIR>;    // 128 x 256
-    using Square = Tile<4, 2, 1, 2, 4, PAIR>;  // 128 x 128
+    // 128 x 128 (waves of 64 x 32 where a pair does not need two columns: 512 x 4096 -> 6144 22.2 to 22.6 us for 23.8 of 32 x 64)
+    using Square = std::conditional_t<PAIR, Tile<4, 2, 1, 2, 4, true>, Tile<2, 4, 2, 1, 4, false>>;
     using Tall = std::conditional_t<PAIR, Square, Tile<4, 2, 1, 1, 4, false>>;                         // 128 x 64
     using Small = std::conditional_t<PAIR, Tile<2, 2, 1, 2, 4, true>, Tile<2, 2, 1, 1, 4, false>>;     // 64 x 128 or 64 x 64
     using Least = std::conditional_t<PAIR, Small, Tile<1, 2, 1, 1, 6, false>>;                         // 32 x 64
