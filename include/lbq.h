@@ -447,7 +447,8 @@ int lbq_i8_linear(lbq_ctx *ctx, uint32_t x_type, const void *d_x, int64_t x_stri
                   void *stream);
 
 /* d_y[m][n] = silu(g) * u of the two weights' products g and u (f32, biases included), silu(v) =
- * v / (1 + exp(-v)): mlp_wrapper.rs:190-194 over such weights, which have the same n and k. */
+ * v / (1 + exp(-v)), as an f32 value down to its least one: mlp_wrapper.rs:190-194 over such weights, which have
+ * the same n and k. */
 int lbq_i8_gate_up_silu(lbq_ctx *ctx, uint32_t x_type, const void *d_x, int64_t x_stride, int8_t *d_codes,
                         float *d_scales, int64_t m, int64_t k, const lbq_i8_weight *gate, const lbq_i8_weight *up,
                         uint32_t out_type, void *d_y, void *stream);
