@@ -184,13 +184,15 @@ __device__ __forceinline__ V i8_dpp_words(V v) {
         return __builtin_bit_cast(V, (uint64_t)i8_dpp<CTRL>((uint32_t)w) | (uint64_t)i8_dpp<CTRL>((uint32_t)(w >> 32)) << 32);
     }
 }
-// v of all lanes in every lane: within rows of 16 by DPP, between them by swaps of rows and halves
+// v of all lanes in every lane: within rows of 16 by DPP, between them by swaps of rows and halves.  Each step joins the
+// same two parts in all lanes that hold them, so that a sum rounds alike in every lane (a rotation by 4 joins a quad with the
+// one before it in some lanes and the one behind it in others).
 template <typename V, typename F>
 __device__ __forceinline__ V i8_wave_all(V v, F f) {
     v = f(v, i8_dpp_words<0xB1>(v));   // quad_perm [1,0,3,2]
     v = f(v, i8_dpp_words<0x4E>(v));   // quad_perm [2,3,0,1]
-    v = f(v, i8_dpp_words<0x124>(v));  // row_ror:4
-    v = f(v, i8_dpp_words<0x128>(v));  // row_ror:8
+    v = f(v, i8_dpp_words<0x141>(v));  // row_half_mirror
+    v = f(v, i8_dpp_words<0x140>(v));  // row_mirror
     auto both = [&](auto swap) {
         if constexpr (sizeof(V) == 4) {
             const auto r = swap(__builtin_bit_cast(uint32_t, v));

@@ -26,3 +26,18 @@ def test_silu_of_far_gates_over_large_values(dev, dtype, m):
         y = g.double() * torch.sigmoid(g.double()) * u
         bound = (8 * ref.U + (0 if dtype == torch.float32 else 2 * ref.U * g.abs())) * y.abs() + ref.least(torch.float32) * (1 + abs(u))
         ref.close(int8.int8_gate_up_silu(gate, up, x), y.expand(m, -1), ref.stored(y, bound, dtype).expand(m, -1))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("k", [128, 512, 513])
+@pytest.mark.parametrize("where", [(8, 104), (40, 8), (64, 16)])
+def test_equal_values_of_a_row_stay_equal(dev, dtype, k, where):
+    # 2^100 and -2^100 in different quads of a row's lanes, ones elsewhere: what the mean comes to goes by the order of the sum, but
+    # one row has one mean, so that its equal values have one result (up to (1 - 0) 2^-96 here, far above f32's least)
+    x = torch.ones(3, k)
+    x[:, 0], x[:, where[0]], x[:, where[1]] = 0.0, 2.0 ** 100, -(2.0 ** 100)
+    x = x.to(dtype).to(dev)
+    ones = (x[0] == 1).nonzero()[:, 0]
+    n = int8.Norm(torch.ones(k, device=dev), 0.0, kind="layer")
+    for y in (int8.residual_norm(x, norm=n)[1], int8.residual_norm(x, post=n)[0]):
+        assert torch.isfinite(y).all() and torch.equal(y[:, ones], y[:, ones[:1]].expand(3, ones.numel()))
