@@ -15,6 +15,7 @@ namespace lbq {
 enum : int { I8_F32 = 0, I8_F16 = 1, I8_BF16 = 2 };
 constexpr int I8_GROUP = 4;
 constexpr int64_t I8_MAX_K = 131071, I8_MAX_N = (int64_t)1 << 24, I8_MAX_M = ((int64_t)1 << 22) - 1;  // (workgroups of up to 1024 threads: below 2^32)
+constexpr int64_t I8_MAX_OUTPUTS = (int64_t)1 << 35;  // tokens times channels of a call stay below
 constexpr int64_t NORM_MAX_K = 32768;
 constexpr int I8_FUSED_ROWS = 4, I8_FUSED_CODES = 16384, I8_FUSED_CHANNELS = 16384;
 inline int64_t i8_kp(int64_t k) { return (k + 127) / 128 * 128; }

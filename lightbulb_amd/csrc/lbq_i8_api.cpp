@@ -102,8 +102,9 @@ int linear_args(uint32_t x_type, const void *d_x, int64_t x_stride, void *d_code
         if (int e = check_weight(ws[i], i, a)) return e;
         rows += ws[i]->n;
     }
-    // (tiles of at least 64 tokens by 32 channels for 256 threads: a launch stays below 2^32 of them)
-    if ((m / 64 + 1) * (rows / 32 + lbq::I8_GROUP) >= (int64_t)1 << 24)
+    // (tiles take a thread for 16 outputs at most, streams of few tokens 32 threads a channel: with each weight's last tiles, which
+    // need not be full, a launch stays below 2^32 threads)
+    if (m * rows >= lbq::I8_MAX_OUTPUTS)
         return fail(LBQ_ERR_LIMIT, "%lld tokens by %lld channels in one call", (long long)m, (long long)rows);
     if (int e = check_type("the outputs", out_type, &a->out)) return e;
     a->m = m, a->k = (int)k, a->kp = (int)lbq::i8_kp(k), a->count = count;
