@@ -417,7 +417,7 @@ int lbq_kv_attention(lbq_ctx *ctx, const lbq_kv_cache *cache, const lbq_kv_step 
  * Rows of codes, of tokens and weights alike, are LBQ_I8_ROW(k) bytes apart and zero from k on, 16-byte
  * aligned.  Types are LBQ_TYPE_F32, _F16 or _BF16; rows of values may have any stride (in elements).  Up to
  * 2^22 - 1 tokens and 2^24 channels a weight, tokens times channels of a call below 2^35.  Results lie apart from
- * the inputs and from each other.
+ * the inputs (weights, biases and norms' vectors among them) and from each other; others are refused.
  * All calls run on the context's device and use none of its memory: calls on different streams need
  * no order among themselves but that of their own buffers.
  * ------------------------------------------------------------------------- */

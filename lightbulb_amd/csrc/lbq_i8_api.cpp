@@ -92,6 +92,14 @@ int check_weight(const lbq_i8_weight *w, int i, lbq::I8Linear *a) {
     return LBQ_OK;
 }
 
+// whether [p, p + bytes) meets a weight's memory
+bool over_weights(const void *p, int64_t bytes, const lbq::I8Linear &a) {
+    for (int i = 0; i < a.count; i++)
+        if (overlap(p, bytes, a.w[i], (int64_t)a.n[i] * a.kp) || overlap(p, bytes, a.t[i], (int64_t)a.n[i] * 4) || overlap(p, bytes, a.bias[i], (int64_t)a.n[i] * 4))
+            return true;
+    return false;
+}
+
 // everything but the outputs; *quantize: the values need a launch of their own
 int linear_args(uint32_t x_type, const void *d_x, int64_t x_stride, void *d_codes, float *d_scales, int64_t m, int64_t k,
                 const lbq_i8_weight *const *ws, int count, uint32_t out_type, lbq::I8Linear *a, bool *quantize) {
@@ -121,6 +129,8 @@ int linear_args(uint32_t x_type, const void *d_x, int64_t x_stride, void *d_code
         if (int e = check_tokens(d_codes, d_scales, m, k, &t)) return e;
     if (*quantize && (overlap(d_x, bytes_of(a->x, m, k), t.codes, m * a->kp) || overlap(d_x, bytes_of(a->x, m, k), t.scales, m * 4)))
         return fail(LBQ_ERR_INVALID_ARG, "the codes' memory must not overlap x");
+    if (*quantize && (over_weights(t.codes, m * a->kp, *a) || over_weights(t.scales, m * 4, *a)))
+        return fail(LBQ_ERR_INVALID_ARG, "the codes' memory must not overlap a weight");
     a->codes = t.codes, a->scales = t.scales;
     return LBQ_OK;
 }
@@ -132,6 +142,7 @@ int check_output(void *y, int i, int64_t n, lbq::I8Linear *a) {
     const int64_t bytes = a->m * n * size;
     if (overlap(y, bytes, a->codes, a->m * a->kp) || overlap(y, bytes, a->scales, a->m * 4) || overlap(y, bytes, a->x.p, bytes_of(a->x, a->m, a->k)))
         return fail(LBQ_ERR_INVALID_ARG, "an output must not overlap the input");
+    if (over_weights(y, bytes, *a)) return fail(LBQ_ERR_INVALID_ARG, "an output must not overlap a weight");
     for (int j = 0; j < i; j++)
         if (overlap(y, bytes, a->y[j], a->m * a->n[j] * size)) return fail(LBQ_ERR_INVALID_ARG, "the outputs must not overlap");
     a->y[i] = y;
@@ -242,6 +253,9 @@ int lbq_residual_norm(lbq_ctx *ctx, uint32_t type, const void *d_x, int64_t x_st
         if (overlap(out[i].p, out[i].n, d_x, bytes_of(a.x, m, k)) || overlap(out[i].p, out[i].n, d_gate, bytes_of(a.gate, m, k)) ||
             (!(i == 0 && in_place) && overlap(out[i].p, out[i].n, d_residual, bytes_of(a.residual, m, k))))
             return fail(LBQ_ERR_INVALID_ARG, "the results must not overlap the inputs");
+        for (const lbq::NormArgs *n : {&a.post, &a.pre})
+            if (overlap(out[i].p, out[i].n, n->w, k * 4) || overlap(out[i].p, out[i].n, n->b, k * 4))
+                return fail(LBQ_ERR_INVALID_ARG, "the results must not overlap a norm's weight or bias");
         for (int j = 0; j < i; j++)
             if (overlap(out[i].p, out[i].n, out[j].p, out[j].n)) return fail(LBQ_ERR_INVALID_ARG, "the results must not overlap");
     }

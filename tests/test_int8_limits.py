@@ -28,3 +28,28 @@ def test_sizes_beyond_the_limit(lbq, m, ns):
     assert linear(lbq, [far(n, i) for i, n in enumerate(ns)], ys=[None] * 8, **kw) == LIMIT and b"in one call" in lbq.lbq_last_error()
     if 2 * ns[0] * m >= 1 << 35:
         assert gate_up(lbq, far(ns[0], 0), far(ns[0], 1), y=None, **kw) == LIMIT
+
+
+def test_outputs_over_what_is_read(lbq):
+    # 5 tokens over 64 channels of 100 values: 1280 bytes of outputs
+    w = weight(d_codes=16 * FAR, d_scales=17 * FAR, d_bias=18 * FAR)
+    for y in (16 * FAR, 16 * FAR + 64 * 128 - 4, 16 * FAR - 1276, 17 * FAR + 252, 18 * FAR - 4):
+        assert linear(lbq, [w], ys=[y]) == INVALID and b"weight" in lbq.lbq_last_error(), hex(y)
+        assert linear(lbq, [weight(), w], ys=[3 * FAR, y]) == INVALID and linear(lbq, [weight(), w], ys=[y, 3 * FAR]) == INVALID
+        assert gate_up(lbq, w, y=y) == INVALID and gate_up(lbq, None, w, y=y) == INVALID
+    # the tokens' codes, where the call writes them
+    for kw in (dict(codes=16 * FAR + 128), dict(scales=17 * FAR), dict(scales=18 * FAR - 16)):
+        assert linear(lbq, [weight(), w], **kw) == INVALID and b"weight" in lbq.lbq_last_error()
+        assert gate_up(lbq, w, **kw) == INVALID and gate_up(lbq, None, w, **kw) == INVALID
+    # beside it, and codes that are read only (the null output is looked at last)
+    for y in (16 * FAR + 64 * 128, 16 * FAR - 1280, 17 * FAR + 256):
+        assert linear(lbq, [w, w], ys=[y, None]) == INVALID and b"null output" in lbq.lbq_last_error()
+    assert linear(lbq, [w], x=None, codes=16 * FAR, scales=17 * FAR, ys=[None]) == INVALID and b"null output" in lbq.lbq_last_error()
+
+
+def test_norms_results_over_their_vectors(lbq):
+    n = norm(d_weight=16 * FAR, d_bias=17 * FAR)
+    for kw in (dict(r=16 * FAR), dict(y=16 * FAR + 396), dict(r=17 * FAR - 1196), dict(y=17 * FAR), dict(y=None, codes=16 * FAR + 112, scales=5 * FAR),
+               dict(y=None, codes=4 * FAR, scales=17 * FAR + 396)):
+        assert residual_norm(lbq, pre=n, **kw) == INVALID and b"norm" in lbq.lbq_last_error(), kw
+        assert residual_norm(lbq, post=n, **kw) == INVALID and b"norm" in lbq.lbq_last_error(), kw
