@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import ctypes
 import struct
+from operator import attrgetter
 
 import torch
 
@@ -91,10 +92,12 @@ class Int8Tokens:
     """Tokens as ``codes`` int8 [.., k] and ``scales`` f32 [..]: a value is code * scale.  Made by
     ``quantize_tokens`` and ``residual_norm``; ``dtype`` is that of the values they stand for."""
 
-    __slots__ = ("_rows", "scales", "shape", "dtype", "device")
+    # (what the products take by address goes together: the attributes cannot be set, the tensors' contents may change)
+    __slots__ = ("_rows", "_scales", "_shape", "_dtype", "_device")
+    scales, shape, dtype, device = (property(attrgetter(name)) for name in __slots__[1:])
 
     def __init__(self, rows: torch.Tensor, scales: torch.Tensor, shape: torch.Size, dtype: torch.dtype, device: torch.device):
-        self._rows, self.scales, self.shape, self.dtype, self.device = rows, scales, shape, dtype, device
+        self._rows, self._scales, self._shape, self._dtype, self._device = rows, scales, shape, dtype, device
 
     @property
     def codes(self) -> torch.Tensor:

@@ -1,7 +1,9 @@
-"""The integer linears' and norms' stated limits, and results laid over what a call reads, without a device: the C entry points check
-before any HIP call."""
+"""The integer linears' and norms' stated limits, results laid over what a call reads, and tokens' attributes, without a device: the C
+entry points check before any HIP call."""
 import pytest
+import torch
 
+from lightbulb_amd import int8
 from test_int8_refusals import D, FAR, INVALID, LIMIT, gate_up, linear, norm, residual_norm, weight
 
 MOST = (1 << 22) - 1  # tokens
@@ -53,3 +55,15 @@ def test_norms_results_over_their_vectors(lbq):
                dict(y=None, codes=4 * FAR, scales=17 * FAR + 396)):
         assert residual_norm(lbq, pre=n, **kw) == INVALID and b"norm" in lbq.lbq_last_error(), kw
         assert residual_norm(lbq, post=n, **kw) == INVALID and b"norm" in lbq.lbq_last_error(), kw
+
+
+def test_tokens_keep_what_they_were_made_with():
+    # a scale for every row of codes, as the products read them: other tensors cannot take their places
+    t = int8.Int8Tokens(torch.ones(2, 128, dtype=torch.int8), torch.full((2,), 0.5), torch.Size((2, 100)), torch.bfloat16, torch.device("cpu"))
+    assert t.shape == (2, 100) and t.dtype == torch.bfloat16 and t.device == torch.device("cpu") and t.codes.shape == (2, 100)
+    for name, value in dict(scales=torch.ones(1), codes=torch.ones(1, 100, dtype=torch.int8), shape=torch.Size((4, 100)), dtype=torch.float32,
+                            device=torch.device("meta")).items():
+        with pytest.raises(AttributeError):
+            setattr(t, name, value)
+    t.scales.mul_(2)
+    assert torch.equal(t.dequantize(), torch.ones(2, 100)) and "(2, 100)" in repr(t)
