@@ -25,13 +25,18 @@ class Block:
         self.attention, self.mlp = attention, mlp
         self.input_norm, self.mlp_norm, self.attn_post, self.mlp_post = input_norm, mlp_norm, attn_post, mlp_post
         self.attn_gate, self.mlp_gate, self.scale = attn_gate, mlp_gate, scale
-        # codes straight from the norm where every product behind it takes them
-        self._attn_codes = all(p.is_int8() for p in (attention.q_proj, attention.k_proj, attention.v_proj))
-        self._mlp_codes = mlp.gate_proj.is_int8() and mlp.up_proj.is_int8()
+
+    # codes straight from the norm where every product behind it takes them
+    def _attn_codes(self) -> bool:
+        a = self.attention
+        return a.q_proj.is_int8() and a.k_proj.is_int8() and a.v_proj.is_int8()
+
+    def _mlp_codes(self) -> bool:
+        return self.mlp.gate_proj.is_int8() and self.mlp.up_proj.is_int8()
 
     def normed(self, xs: torch.Tensor) -> "torch.Tensor | Int8Tokens":
         """``input_norm(xs)`` as the attention takes it."""
-        return residual_norm(xs, norm=self.input_norm, quantize=self._attn_codes)[1]
+        return residual_norm(xs, norm=self.input_norm, quantize=self._attn_codes())[1]
 
     def forward(self, xs: torch.Tensor, cache: KvCache, step: Step, normed: "torch.Tensor | Int8Tokens | None" = None,
                 next: "Block | None" = None) -> tuple[torch.Tensor, "torch.Tensor | Int8Tokens | None"]:
@@ -39,9 +44,9 @@ class Block:
         as ``normed``: its norm is formed with this block's last update.  ``normed`` None: the input norm is formed
         here.  Rows behind the last sequence's come out unset."""
         a = self.attention(self.normed(xs) if normed is None else normed, cache, step)
-        h, b = residual_norm(a, xs, post=self.attn_post, gate=self.attn_gate, scale=self.scale, norm=self.mlp_norm, quantize=self._mlp_codes)
+        h, b = residual_norm(a, xs, post=self.attn_post, gate=self.attn_gate, scale=self.scale, norm=self.mlp_norm, quantize=self._mlp_codes())
         y = self.mlp(b)
-        after, codes = (None, False) if next is None else (next.input_norm, next._attn_codes)
+        after, codes = (None, False) if next is None else (next.input_norm, next._attn_codes())
         return residual_norm(y, h, post=self.mlp_post, gate=self.mlp_gate, scale=self.scale, norm=after, quantize=codes)
 
     __call__ = forward
