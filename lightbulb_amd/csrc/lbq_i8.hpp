@@ -240,13 +240,15 @@ __device__ __forceinline__ float i8_result_wide(int acc, float s, float t, float
 }
 // g / (1 + exp(-g)) u, for an output of type OUT.  F32: exp as 2^(h + l) with h + l = -g log2(e) to 48 bits, where a
 // plain product would be off by |g| 2^-24 of the result; what l adds is kept beside 1, so that an h beyond the
-// exponent's range leaves no inf - inf.  Gates far below zero take 1 + exp(-g) and g by 2^-64: neither the sum nor its
-// reciprocal, which is never subnormal, leaves the range before g / (1 + exp(-g)) itself is below f32's least value.
-template <int OUT>
+// exponent's range leaves no inf - inf.  FAR: gates below I8_FAR take 1 + exp(-g) and g by 2^-64, and neither the sum nor
+// its reciprocal, which is never subnormal, leaves the range before g / (1 + exp(-g)) itself is below f32's least value.
+// Others have the same bits with and without.
+constexpr float I8_FAR = -80.f;
+template <int OUT, bool FAR = true>
 __device__ __forceinline__ float i8_silu_mul(float g, float u) {
     constexpr float L = 1.44269502f, LO = 1.92596303e-8f, LN2 = 0.693147182f;  // log2(e), and what L leaves of it
     const float h = i8_f32(-g * L);  // (as rounded: what the rounding left is l's)
-    const bool far = h > 100.f;
+    const bool far = FAR && g < I8_FAR;
     const float one = far ? 0x1p-64f : 1.f, e = __builtin_amdgcn_exp2f(far ? h - 64.f : h);
     float d;
     if constexpr (OUT == I8_F32) {

@@ -101,7 +101,7 @@ class Int8Tokens:
 
     @property
     def codes(self) -> torch.Tensor:
-        rows, shape = self._rows, self.shape
+        rows, shape = self._rows, self._shape
         if rows.shape == shape:
             return rows
         rows = rows.narrow(1, 0, shape[-1])
