@@ -292,7 +292,8 @@ hipError_t norm_rows(const ResidualNorm &a, hipStream_t st) {
     if (kp <= 6144) return norm<DX, DR, 256, 3>(a, st);
     if (kp <= 8192) return norm<DX, DR, 512, 2>(a, st);
     // (16-bit values of 14336 with codes: 64 rows 14.7 us, with 512 threads 15.8; 1400 rows 53.9 and 48.0, with a first norm 93.7 and
-    // 75.5; 2048 of 10000 58.8 and 47.8.  f32, whose pieces are twice the registers, 79.6 and 85.5)
+    // 75.5; 2048 of 10000 58.8 and 47.8.  f32, whose pieces are twice the registers, 79.6 and 85.5.  With the threads the order of a
+    // row's sums changes: a value's last bit may go by whether m is above 256 there)
     if constexpr (DX != I8_F32) {
         if (kp <= 12288 && a.m > 256) return norm<DX, DR, 512, 3>(a, st);
         if (kp <= 16384 && a.m > 256) return norm<DX, DR, 512, 4>(a, st);

@@ -80,8 +80,10 @@ struct Tile {
 // wave, the next one's operands are read under them, and the loads go out one behind each; where it has fewer, a
 // whole stage's operands are read ahead.
 // 4096 x 14336 -> 4096 188 us, 2.55 POP/s; 2048 tokens, gate and up of 14336 x 4096 216 us, 2.23.  Bound by the card's power: the
-// matrix pipes are busy 60 to 70 % of cycles at 1.8 GHz, and on codes of zeros, which take less of it, the rate is 3.0.  512 tokens over
-// 6144 channels of 4096 20 us, by the lines that a CU takes in (below).  Stages of 64 bytes in 3 to 5 slots took 214 to 228 us
+// matrix pipes are busy 55 to 70 % of cycles at 1.8 GHz, and on codes of zeros, which take less of it, the rate is 3.0.  512 tokens over
+// 6144 channels of 4096 (192 tiles of 128 x 128, a call on codes made before) 19.0 us, 22.4 where the weights come out of memory: 5.4 of
+// a launch's start and end, and 0.40 or 0.52 a stage, of which the matrix instructions are 0.21; over k of 512 to 8192 alike, so that it is
+// not the lines missing in an L2.  All CUs take in 16 TB/s together there (256 tiles of 128 x 64: 20 to 25).  Stages of 64 bytes in 3 to 5 slots took 214 to 228 us
 // for 190 to 199, four waves of 128 x 128 each 307 (registers spill).
 template <class T, int OUT>
 __device__ __forceinline__ void i8_tile(const I8Linear &a, int64_t m0, int n0, int wi, uint8_t *lds_base) {
@@ -365,9 +367,9 @@ hipError_t run(const I8Linear &a, int wide, hipStream_t st) {
     return hipGetLastError();
 }
 
-// A CU takes in about 50 GB/s of lines that are not in its XCD's L2, whatever is in flight, so that a round of
-// tiles, one a CU, costs by the rows and channels of a tile, and large tiles pay only where they fill the CUs.  us of the first round
-// and of each further one at k = 4096 (measured; other k by their length alike).
+// A stage's time goes by what is taken in, the rows and channels of a tile, so that large tiles pay only where they fill the
+// CUs.  us of the first round of tiles, one a CU, and of each further one at k = 4096 (measured, weights out of memory; other k by
+// their length alike).
 template <class T>
 float cost(const I8Linear &a, float first, float next) {
     int end[I8_GROUP];
@@ -378,7 +380,8 @@ template <bool PAIR>
 hipError_t tiles(const I8Linear &a, hipStream_t st) {
     using Big = Tile<2, 4, 4, 2, 2, PAIR>;     // 256 x 256
     using Half = Tile<2, 4, 2, 2, 3, PAIR>;    // 128 x 256
-    // 128 x 128 (waves of 64 x 32 where a pair does not need two columns: 512 x 4096 -> 6144 22.2 to 22.6 us for 23.8 of 32 x 64)
+    // 128 x 128 (waves of 64 x 32 where a pair does not need two columns: 512 x 4096 -> 6144 a call on codes made before 22.2 to
+    // 22.6 us, weights out of memory, for 23.8 of 32 x 64)
     using Square = std::conditional_t<PAIR, Tile<4, 2, 1, 2, 4, true>, Tile<2, 4, 2, 1, 4, false>>;
     using Tall = std::conditional_t<PAIR, Square, Tile<4, 2, 1, 1, 4, false>>;                         // 128 x 64
     using Small = std::conditional_t<PAIR, Tile<2, 2, 1, 2, 4, true>, Tile<2, 2, 1, 1, 4, false>>;     // 64 x 128 or 64 x 64

@@ -216,8 +216,10 @@ hipError_t run(const I8Linear &a, hipStream_t st) {
     I8Stream g = {};
     const int tiles = tiles16<R>(a, g.tile_end), blocks = a.kp / 128;
     g.ks = blocks >= 8 ? 8 : blocks >= 4 ? 4 : blocks >= 2 ? 2 : 1;
-    // longer shares where that still leaves the CUs a workgroup (a pair of 14336, 16 tokens: 29.7 us in eighths of k, 24.9 in
-    // quarters; single weights 16.0 and 15.5, 128256 channels 92.7 and 96.3)
+    // longer shares where that leaves three quarters of the CUs a workgroup or more.  us in eighths and quarters of k = 4096, a
+    // pair, 16 tokens: 8192 channels 17.7 and 23.4, 10240 28.1 and 23.8, 12288 (the first to take quarters) 29.0 and 24.7, 14336 32.0
+    // and 25.1, 16384 33.9 and 27.0, 20480 44.2 and 46.5, 28672 57.7 and 50.0; k = 8192: 12288 51.5 and 43.4, 16384 52.1 and 50.4.
+    // (Single weights 16.0 and 15.5, 128256 channels 92.7 and 96.3.)
     if (PAIR && R == 2 && tiles / 2 >= num_cus() * 3 / 4) g.ks = std::min(g.ks, 4);
     const unsigned groups = (unsigned)((tiles + I8_WAVES / g.ks - 1) / (I8_WAVES / g.ks));
     if (a.out == I8_F32) k_i8_gemv<MT, R, U, PAIR, FUSED, DX, I8_F32><<<groups, 64 * I8_WAVES, 0, st>>>(a, g);
